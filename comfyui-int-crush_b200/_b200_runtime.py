@@ -694,8 +694,270 @@ def unpack_int4_to_float16(packed: torch.Tensor, scale: torch.Tensor, K: int,
     return out
 
 
+# ── attention-side operators ─────────────────────────────────────────────────
+
+_MASKS = {torch.bool: L.IC_MASK_BOOL, torch.float16: L.IC_MASK_F16, torch.bfloat16: L.IC_MASK_BF16,
+          torch.float32: L.IC_MASK_F32}
+_ROPE = {"interleaved": L.IC_ROPE_INTERLEAVED, "half": L.IC_ROPE_HALF}
+_S3 = ctypes.c_int64 * 12
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """``t`` ([batch, tokens, heads, D]) as the kernels read it: elements
+    contiguous, 16-byte aligned rows; a copy where it is not."""
+    b, l, h, d = t.stride()
+    if d == 1 and not ((b | l | h) & 7 or t.data_ptr() & 15):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _out_heads(what: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    b, l, h, d = out.stride() if out.dim() == 4 else (0, 0, 0, 0)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"{what}: out must be {like.dtype} {tuple(like.shape)}, got {out.dtype} {tuple(out.shape)}")
+    if d != 1 or (b | l | h) & 7 or out.data_ptr() & 15 or any(
+            s == 0 and n > 1 for s, n in zip((b, l, h), out.shape)):
+        raise ValueError(f"{what}: out must have contiguous elements, strides that are multiples of 8 and a 16-byte "
+                         f"aligned start, got strides {out.stride()}")
+    return out
+
+
+def _index(t: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        if t.dtype.is_floating_point or t.dtype == torch.bool:
+            raise TypeError(f"an index tensor must hold integers, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t.contiguous()
+
+
+def _gamma16(what: str, t: torch.Tensor | None, D: int) -> torch.Tensor | None:
+    if t is None:
+        return None
+    g = _f32c(t.reshape(-1))
+    if g.numel() != D:
+        raise ValueError(f"{what}: gamma has {g.numel()} entries, expected {D}")
+    return g.clone() if g.data_ptr() & 15 else g
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor | None = None,
+    *,
+    q_gamma: torch.Tensor | None = None,
+    k_gamma: torch.Tensor | None = None,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    layout: str = "interleaved",
+    positions: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+):
+    """RMS norm of every query and key head and the position rotation, one pass.
+
+    ``q`` [B, L, H, D] and ``k`` [B, L, Hk, D] (fp16 / bf16, D a multiple of 8
+    up to 256) may be strided views, e.g. of a fused QKV projection's output.
+    Each head becomes ``x * rsqrt(mean(x^2) + eps) * gamma`` (gammas [D], None
+    = ones) in fp32; then its first ``2 * cos.shape[-1]`` elements turn by the
+    angles whose cosines and sines are in row ``positions[b, l]`` (default:
+    ``l``) of the tables ``cos`` / ``sin`` [rows, rot / 2]: pairs
+    ``(2i, 2i + 1)`` (``layout="interleaved"``) or ``(i, i + rot / 2)``
+    (``"half"``).  Without tables only the norm is applied.
+
+    A position outside the tables gives NaN for its token and sets the
+    library's device error word.  Returns ``(q, k)`` normalised, or only ``q``
+    without a ``k``; ``q_out`` / ``k_out`` may be the inputs themselves.
+    """
+    _need_cuda("qk_norm_rope", q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"qk_norm_rope: q must be float16/bfloat16, got {q.dtype}")
+    if q.dim() != 4:
+        raise ValueError(f"qk_norm_rope: q must be [batch, tokens, heads, D], got {tuple(q.shape)}")
+    if layout not in _ROPE:
+        raise ValueError(f"qk_norm_rope: layout must be 'interleaved' or 'half', got {layout!r}")
+    B, T, H, D = q.shape
+    rot = rows = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("qk_norm_rope: cos and sin come together")
+    if cos is not None:
+        if cos.shape != sin.shape or cos.dim() != 2:
+            raise ValueError(f"qk_norm_rope: tables must be [rows, rot / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        cos, sin = _f32c(cos), _f32c(sin)
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    if positions is not None:
+        if positions.shape != (B, T):
+            raise ValueError(f"qk_norm_rope: positions must be [{B}, {T}], got {tuple(positions.shape)}")
+        positions = _index(positions)
+    gq = _gamma16("qk_norm_rope", q_gamma, D)
+    x = _heads(q)
+    y = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device) if q_out is None else _out_heads("qk_norm_rope", q_out, q)
+    if k is None:
+        if k_gamma is not None or k_out is not None:
+            raise ValueError("qk_norm_rope: k_gamma / k_out without a k")
+        Hk, xk, yk, gk = 0, None, None, None
+        strides = _S3(*x.stride()[:3], *y.stride()[:3])
+    else:
+        if k.dim() != 4 or k.dtype != q.dtype or k.shape[:2] != (B, T) or k.shape[3] != D:
+            raise ValueError(f"qk_norm_rope: k must be {q.dtype} [{B}, {T}, heads, {D}], got {k.dtype} {tuple(k.shape)}")
+        Hk = k.shape[2]
+        gk = _gamma16("qk_norm_rope", k_gamma, D)
+        xk = _heads(k)
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else _out_heads("qk_norm_rope", k_out, k)
+        strides = _S3(*x.stride()[:3], *y.stride()[:3], *xk.stride()[:3], *yk.stride()[:3])
+    st = L.lib().ic_qk_norm_rope(
+        _p(x), _p(y), H, _p(xk), _p(yk), Hk, _DT[q.dtype], B, T, D, strides, _p(gq), _p(gk), float(eps), _ROPE[layout],
+        rot, _p(cos) if rot else None, _p(sin) if rot else None, rows, _p(positions), _stream(q))
+    L.check(st, "ic_qk_norm_rope")
+    return y if k is None else (y, yk)
+
+
+def cross_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    kv_lens: torch.Tensor | None = None,
+    key_mask: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of ``q`` [B, Lq, H, D] to an encoder's states ``k`` / ``v``
+    [B, Lk, Hk, D] (fp16 / bf16, D a multiple of 8 up to 128, H a multiple of
+    Hk: query heads ``h`` share key head ``h // (H // Hk)``):
+    ``softmax(scale * q k^T + mask) v`` with ``scale`` 1/sqrt(D) by default.
+
+    ``kv_lens`` [B] (integers on the device): sample b sees keys below
+    ``kv_lens[b]``.  ``key_mask`` [B, Lk] or [Lk]: bool (False = not seen) or
+    float (added to the scores, -inf = not seen).  What ``k`` and ``v`` hold at
+    keys that are not seen does not matter; a sample that sees none gets
+    zeros.  All may be strided views.  Returns [B, Lq, H, D].
+    """
+    _need_cuda("cross_attention", q, k, v, kv_lens, key_mask, out)
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"cross_attention: q, k and v must share one dtype, float16 or bfloat16, got {q.dtype}, "
+                        f"{k.dtype}, {v.dtype}")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"cross_attention: q must be [B, Lq, H, D], k and v [B, Lk, Hk, D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    if kv_lens is not None:
+        if kv_lens.shape != (B,):
+            raise ValueError(f"cross_attention: kv_lens must be [{B}], got {tuple(kv_lens.shape)}")
+        kv_lens = _index(kv_lens)
+    kind = ld = 0
+    if key_mask is not None:
+        kind = _MASKS.get(key_mask.dtype, 0)
+        if not kind:
+            raise TypeError(f"cross_attention: key_mask must be bool, float16, bfloat16 or float32, got {key_mask.dtype}")
+        if key_mask.shape not in ((B, Lk), (Lk,)):
+            raise ValueError(f"cross_attention: key_mask must be [{B}, {Lk}] or [{Lk}], got {tuple(key_mask.shape)}")
+        if key_mask.stride(-1) != 1:
+            key_mask = key_mask.contiguous()
+        ld = key_mask.stride(0) if key_mask.dim() == 2 and B > 1 else 0
+        if 0 < ld < Lk:
+            key_mask = key_mask.contiguous()
+            ld = Lk
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    y = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device) if out is None else _out_heads("cross_attention", out, q)
+    lib = L.lib()
+    n = lib.ic_cross_attention_workspace(B, Lq, Lk, H, Hk, D, kind)
+    if n < 0:
+        L.check(L.IC_ERR_ARG, "ic_cross_attention")
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    st = lib.ic_cross_attention(
+        _p(q), _p(k), _p(v), _p(y), _DT[q.dtype], B, Lq, Lk, H, Hk, D,
+        _S3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3]),
+        float(D ** -0.5 if scale is None else scale), _p(kv_lens), _p(key_mask), kind, ld, _p(ws), n, _stream(q))
+    L.check(st, "ic_cross_attention")
+    return y
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """``t`` as a [rows, width] matrix with contiguous rows."""
+    t = t.reshape(-1, width)
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
+
+
+def lora_batched(
+    x: torch.Tensor,
+    down: torch.Tensor,
+    up: torch.Tensor,
+    ids: torch.Tensor,
+    scales: torch.Tensor | None = None,
+    *,
+    base: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``base + scales[a] * (x @ down[a]^T) @ up[a]^T`` with an adapter ``a`` of
+    its own for every request (``a < 0``: none), fp32 sums, one rounding.
+
+    ``x`` [..., K] (fp16 / bf16), ``down`` [n, R, K] and ``up`` [n, N, R] the
+    adapters (smaller ranks padded with zeros, R up to 256), ``ids`` integers
+    on the device: one per row of x, or fewer, each for an equal run of rows
+    (one per sample of a batch).  ``base`` [..., N] is the shared projection's
+    output (None: zeros); ``out`` [..., N] may be ``base``.  An id that names
+    no adapter gives NaN for its rows and sets the library's device error
+    word.  (One adapter for all rows: :func:`lowrank_down` /
+    :func:`lowrank_add`, ``_ops.py:236-244``.)
+    """
+    _need_cuda("lora_batched", x, down, up, ids, scales, base, out)
+    dt = x.dtype
+    if dt not in (torch.float16, torch.bfloat16) or down.dtype != dt or up.dtype != dt:
+        raise TypeError(f"lora_batched: x, down and up must share one dtype, float16 or bfloat16, got {dt}, {down.dtype}, "
+                        f"{up.dtype}")
+    if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2]:
+        raise ValueError(f"lora_batched: down must be [n, R, K] and up [n, N, R], got {tuple(down.shape)}, {tuple(up.shape)}")
+    n, R, K = down.shape
+    N = up.shape[1]
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"lora_batched: x has {tuple(x.shape)[-1:]} columns, expected {K}")
+    lead = x.shape[:-1]
+    x2 = _rows(x, K)
+    M = x2.shape[0]
+    S = ids.numel()
+    if (S == 0) != (M == 0) or (S and M % S):
+        raise ValueError(f"lora_batched: {S} adapter ids do not divide {M} rows")
+    ids = _index(ids.reshape(-1))
+    if scales is not None:
+        scales = _f32c(scales.reshape(-1))
+        if scales.numel() != n:
+            raise ValueError(f"lora_batched: {scales.numel()} scales for {n} adapters")
+    b2 = None
+    if base is not None:
+        if base.dtype != dt or base.shape != (*lead, N):
+            raise ValueError(f"lora_batched: base must be {dt} {(*lead, N)}, got {base.dtype} {tuple(base.shape)}")
+        b2 = _rows(base, N)
+    if out is None:
+        out = torch.empty((*lead, N), dtype=dt, device=x.device)
+        o2 = out.view(-1, N) if M else out
+    else:
+        if out.dtype != dt or out.shape != (*lead, N):
+            raise ValueError(f"lora_batched: out must be {dt} {(*lead, N)}, got {out.dtype} {tuple(out.shape)}")
+        o2 = out.view(-1, N)   # raises where the leading dimensions do not fold
+        if o2.stride(1) != 1 or (M > 1 and o2.stride(0) < N):
+            raise ValueError(f"lora_batched: out must be row-major, got strides {out.stride()}")
+    if M == 0 or N == 0:
+        return out
+    lib = L.lib()
+    need = lib.ic_lora_batched_workspace(M, K, N, R, n)
+    if need < 0:
+        L.check(L.IC_ERR_ARG, "ic_lora_batched")
+    ws = torch.empty(need, dtype=torch.float32, device=x.device)
+    down, up = down.contiguous(), up.contiguous()
+    ldx, ldo, ldb = x2.stride(0), o2.stride(0), 0 if b2 is None else b2.stride(0)
+    if M == 1:   # a lone row's stride says nothing
+        ldx, ldo, ldb = K, N, N
+    st = lib.ic_lora_batched(
+        _p(x2), _DT[dt], M, K, ldx, _p(down), _p(up), R, n, _p(ids), M // S, _p(scales), _p(b2), ldb, _p(o2), N, ldo,
+        _p(ws), need, _stream(x))
+    L.check(st, "ic_lora_batched")
+    return out
+
+
 def device_error(clear: bool = True) -> int:
-    """Device error word of the library (1 = a bounded wait timed out)."""
+    """Device error word of the library (1 = a bounded wait timed out, 2 = a
+    position or adapter id out of its range)."""
     return L.read_device_error(clear)
 
 
@@ -708,4 +970,5 @@ __all__ = [
     "fused_w4a8_gemm_dequant", "unpack_int4_to_int8", "unpack_int4_to_float16",
     "prep_quantize", "gemm_a8", "gemm_w4a16", "repack_int4", "lowrank_down", "lowrank_add", "device_error",
     "fused_layernorm_quantize", "fused_rmsnorm_quantize",
+    "qk_norm_rope", "cross_attention", "lora_batched",
 ]

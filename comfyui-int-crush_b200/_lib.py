@@ -28,13 +28,23 @@ IC_W_INT4 = 1
 IC_W_INT4R = 2
 
 IC_DEV_ERR_TIMEOUT = 1
+IC_DEV_ERR_INDEX = 2
+
+IC_ROPE_INTERLEAVED = 0
+IC_ROPE_HALF = 1
+
+IC_MASK_NONE = 0
+IC_MASK_BOOL = 1
+IC_MASK_F16 = 2
+IC_MASK_BF16 = 3
+IC_MASK_F32 = 4
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
 
-# name -> argument types (all return int status except where noted)
+# name -> argument types (all return int status except those in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "ic_version": [],
     "ic_last_error": [],
@@ -61,7 +71,13 @@ SIGNATURES: dict[str, list] = {
     "ic_unpack_int4_to_int8": [_P, _L, _L, _L, _P, _P],
     "ic_selftest_wait_timeout": [_L, _P],
     "ic_unpack_int4_to_f16": [_P, _L, _L, _L, _P, _I, _L, _L, _P, _P],
+    "ic_qk_norm_rope": [_P, _P, _L, _P, _P, _L, _I, _L, _L, _L, _P, _P, _P, _F, _I, _L, _P, _P, _L, _P, _P],
+    "ic_cross_attention": [_P, _P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _P, _F, _P, _P, _I, _L, _P, _L, _P],
+    "ic_cross_attention_workspace": [_L, _L, _L, _L, _L, _L, _I],
+    "ic_lora_batched": [_P, _I, _L, _L, _L, _P, _P, _L, _L, _P, _L, _P, _P, _L, _P, _L, _L, _P, _L, _P],
+    "ic_lora_batched_workspace": [_L, _L, _L, _L, _L],
 }
+_RESTYPES = {"ic_last_error": ctypes.c_char_p, "ic_cross_attention_workspace": _L, "ic_lora_batched_workspace": _L}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -86,7 +102,7 @@ def lib() -> ctypes.CDLL:
             for name, args in SIGNATURES.items():
                 fn = getattr(L, name)
                 fn.argtypes = args
-                fn.restype = ctypes.c_char_p if name == "ic_last_error" else ctypes.c_int
+                fn.restype = _RESTYPES.get(name, ctypes.c_int)
             _lib = L
     return _lib
 

@@ -14,7 +14,15 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libintcrush_b200.so")
-SOURCES = ["intcrush_b200.cu", "ic_common.cuh", "prep_common.cuh", "prep.cu", "prep_tile.cu", "gemm_tc.cu", "skinny.cu", "weights.cu", "abi.cu"]
+# translation unit -> the sources it includes
+UNITS = {
+    "intcrush_b200.cu": ["ic_common.cuh", "prep_common.cuh", "prep.cu", "prep_tile.cu", "gemm_tc.cu", "skinny.cu",
+                         "weights.cu", "abi.cu"],
+    "attention_b200.cu": ["ic_common.cuh", "qk_norm_rope.cu", "lora_batched.cu", "cross_attention.cuh",
+                          "cross_attention.cu", "abi_attention.cu"],
+}
+FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+         "-diag-suppress", "20044"]
 
 
 def _nvcc() -> str:
@@ -22,26 +30,44 @@ def _nvcc() -> str:
     return cand if os.path.exists(cand) else "nvcc"
 
 
-def needs_build() -> bool:
-    if not os.path.exists(LIB):
+def _object(unit: str) -> str:
+    return os.path.join(HERE, "_build", unit.replace(".cu", ".o"))
+
+
+def _stale(target: str, unit: str) -> bool:
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, s) for s in SOURCES]
-    deps.append(os.path.join(HERE, "..", "include", "intcrush_b200.h"))
+    t = os.path.getmtime(target)
+    deps = [os.path.join(CSRC, s) for s in [unit, *UNITS[unit]]]
+    deps += [os.path.join(HERE, "..", "include", "intcrush_b200.h"), os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def needs_build() -> bool:
+    return any(_stale(LIB, u) for u in UNITS)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile the units that changed (side by side) and link the library."""
     if not force and not needs_build():
         return LIB
-    cmd = [
-        _nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-        "--shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-diag-suppress", "20044",
-        "-o", LIB + ".tmp", os.path.join(CSRC, "intcrush_b200.cu"),
-    ]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True)
+    os.makedirs(os.path.join(HERE, "_build"), exist_ok=True)
+    running = []
+    for unit in UNITS:
+        obj = _object(unit)
+        if not force and not _stale(obj, unit):
+            continue
+        cmd = [_nvcc(), *FLAGS, "-c", "-o", obj + ".tmp", os.path.join(CSRC, unit)]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        running.append((subprocess.Popen(cmd), cmd, obj))
+    failed = [(p.returncode, cmd) for p, cmd, _ in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(*failed[0])
+    for _, _, obj in running:
+        os.replace(obj + ".tmp", obj)
+    subprocess.run([_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "--shared", "-cudart", "static", "-o",
+                    LIB + ".tmp", *map(_object, UNITS)], check=True)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

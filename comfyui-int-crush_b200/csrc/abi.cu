@@ -46,6 +46,20 @@ double sylvester_entry(int n) {
 
 }  // namespace
 
+namespace ic {
+
+int set_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+void clear_error() { g_err[0] = 0; }
+
+}  // namespace ic
+
 extern "C" {
 
 int ic_version(void) { return (1 << 16) | 0; }
@@ -93,7 +107,10 @@ int ic_read_device_error(int clear, int* code_out) {
     e = cudaMemcpyToSymbol(g_ic_dev_error, &z, sizeof(int));
     if (e != cudaSuccess) return cuda_status(e, "clearing the device error word");
   }
-  if (code_out) *code_out = v;
+  int w = 0;
+  e = ic::attention_device_error(clear, &w);
+  if (e != cudaSuccess) return cuda_status(e, "reading the device error word");
+  if (code_out) *code_out = v ? v : w;
   return IC_OK;
 }
 

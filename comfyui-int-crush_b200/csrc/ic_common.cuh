@@ -23,12 +23,23 @@
 #define IC_WAIT_NS 2000000000ull   // 2 s per wait, far above any legitimate wait
 #endif
 
-// Device-side error word (IC_DEV_ERR_* codes of include/intcrush_b200.h).
-// The library is compiled as one translation unit (intcrush_b200.cu), so
-// this is its only definition.
-__device__ int g_ic_dev_error = 0;
+// Device-side error word (IC_DEV_ERR_* codes of include/intcrush_b200.h), one
+// per translation unit (intcrush_b200.cu, attention_b200.cu);
+// ic_read_device_error reads both.
+static __device__ int g_ic_dev_error = 0;
 
 namespace ic {
+
+// Shared by the translation units (defined in abi.cu and gemm_tc.cu).
+int set_error(int code, const char* fmt, ...);      // records ic_last_error's text, returns code
+void clear_error();
+cudaError_t attention_device_error(int clear, int* code);   // abi_attention.cu
+int num_sms();
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn();   // cuTensorMapEncodeTiled, NULL without a driver
 
 // Raise a kernel's dynamic shared-memory limit once per device (host side),
 // and with carveout >= 0 its preferred shared-memory carveout (percent of

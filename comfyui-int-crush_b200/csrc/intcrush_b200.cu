@@ -1,5 +1,6 @@
-// Single translation unit of libintcrush_b200.so: the kernels share one
-// device error word and are linked without relocatable device code.
+// Translation unit of the quantised-linear kernels (the other one is
+// attention_b200.cu): its kernels share one device error word and are linked
+// without relocatable device code.
 #include "ic_common.cuh"
 #include "prep.cu"
 #include "gemm_tc.cu"

@@ -30,8 +30,6 @@ struct PrepArgs {
   float eps;
 };
 
-int num_sms();   // gemm_tc.cu
-
 template <typename T> struct MidBits;
 template <> struct MidBits<__half> {          // 10-bit mantissa: 13 fp32 bits below it
   static constexpr uint32_t MASK = 0x1FFFu, MID = 0x1000u;

@@ -29,6 +29,7 @@ extern "C" {
 /* device-side error word (ic_read_device_error) */
 #define IC_DEV_ERR_NONE 0
 #define IC_DEV_ERR_TIMEOUT 1  /* a bounded mbarrier wait expired          */
+#define IC_DEV_ERR_INDEX 2    /* a position or adapter id out of its range */
 
 /* element type codes */
 #define IC_DTYPE_F16 0
@@ -289,6 +290,97 @@ int ic_lowrank_add_ex(void* out, int dtype, int64_t M, int64_t N, int64_t ldo, c
 /* ic_lowrank_add_ex with dtype IC_DTYPE_F16. */
 int ic_lowrank_add(void* out, int64_t M, int64_t N, int64_t ldo, const void* mid,
                    const void* up, int64_t R, float scale, void* stream);
+
+/*
+ * Attention-side operators (no counterpart in the reference, whose blocks
+ * leave them to the host framework): what runs between the quantised
+ * projections of a conditioned transformer block.
+ */
+
+/* rotation layouts */
+#define IC_ROPE_INTERLEAVED 0  /* pairs (2i, 2i + 1)                        */
+#define IC_ROPE_HALF 1         /* pairs (i, i + rot / 2)                    */
+
+/* key mask kinds of ic_cross_attention */
+#define IC_MASK_NONE 0
+#define IC_MASK_BOOL 1         /* uint8 / bool, 0 = key not seen            */
+#define IC_MASK_F16 2          /* added to the scaled scores, -inf = key    */
+#define IC_MASK_BF16 3         /* not seen                                  */
+#define IC_MASK_F32 4
+
+/* RMS norm of every query and key head, then the position rotation, in one
+ * pass: y = x / sqrt(mean(x^2) + eps) * gamma in fp32, then for i < rot / 2
+ * the pair (a, b) of y becomes (a cos - b sin, b cos + a sin) with the
+ * angles' cosines and sines from row `position` of the tables; elements past
+ * rot stay y.  One rounding.
+ *   q, q_out  [B, L, H, D], k, k_out [B, L, Hk, D] in dtype (f16 / bf16);
+ *             either may be absent (its head count 0); the output may be
+ *             the input (same strides)
+ *   strides   12 element strides, batch / token / head of q, q_out, k, k_out;
+ *             multiples of 8, tensors 16-byte aligned, elements contiguous
+ *   D         a multiple of 8, up to 256
+ *   gammas    fp32 [D], 16-byte aligned, or NULL (ones)
+ *   rot       even, 0 (no rotation) .. D
+ *   tables    fp32 [table_rows, rot / 2]
+ *   positions int32 [B, L] contiguous, or NULL (the token's index in its
+ *             sample; table_rows >= L); a position outside the tables sets
+ *             IC_DEV_ERR_INDEX and gives NaN for its token */
+int ic_qk_norm_rope(const void* q, void* q_out, int64_t H, const void* k, void* k_out, int64_t Hk, int dtype,
+                    int64_t B, int64_t L, int64_t D, const int64_t* strides, const float* q_gamma,
+                    const float* k_gamma, float eps, int layout, int64_t rot, const float* cos_table,
+                    const float* sin_table, int64_t table_rows, const int32_t* positions, void* stream);
+
+/* Cross attention to an encoder's states of another length:
+ *   out[b, l, h] = softmax_j(scale * q[b, l, h] . k[b, j, hk] + mask[b, j]) v[b, j, hk],
+ * hk = h / (H / Hk), over the keys that sample b sees: j < kv_lens[b] (int32
+ * [B] or NULL, clamped to [0, Lk]) and mask not 0 (bool) or -inf (additive).
+ * The k and v of a key that is not seen may hold anything; a sample that
+ * sees no key gets zeros.  A constant in an additive mask changes nothing,
+ * whatever its size (a sample whose seen keys all hold a type's lowest value
+ * gets the softmax of its scores).  Scores, softmax and sums in fp32; the weights are
+ * rounded to dtype for the product with v.
+ *   q, out  [B, Lq, H, D], k, v [B, Lk, Hk, D] in dtype (f16 / bf16), D a
+ *           multiple of 8 up to 128, H a multiple of Hk
+ *   strides 12 element strides, batch / token / head of q, k, v, out;
+ *           multiples of 8, tensors 16-byte aligned, elements contiguous
+ *   mask    [B, Lk] rows of ld_mask elements (0: one row for all samples), or
+ *           NULL with IC_MASK_NONE
+ *   workspace  ic_cross_attention_workspace(...) floats, 16-byte aligned,
+ *           contents arbitrary, in use until the call's work has run
+ * The sums' order depends on the sizes only: same inputs, same bits. */
+int ic_cross_attention(const void* q, const void* k, const void* v, void* out, int dtype, int64_t B, int64_t Lq,
+                       int64_t Lk, int64_t H, int64_t Hk, int64_t D, const int64_t* strides, float scale,
+                       const int32_t* kv_lens, const void* mask, int mask_kind, int64_t ld_mask, float* workspace,
+                       int64_t workspace_elems, void* stream);
+/* Floats of workspace for these sizes (0: none needed); -1 and an error
+ * message for sizes that ic_cross_attention refuses. */
+int64_t ic_cross_attention_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D,
+                                     int mask_kind);
+
+/* Low-rank adapters of many requests at once, beside a shared projection:
+ *   out[m] = T(base[m] + scales[a] * (x[m] @ down[a]^T) @ up[a]^T),
+ *   a = ids[m / rows_per_id]
+ * with fp32 sums and one rounding; rows with ids < 0 have no adapter (out =
+ * base).  One adapter for all rows is ic_lowrank_down / ic_lowrank_add
+ * (_ops.py:236-244), which round in between.
+ *   x     [M, K] (ldx), base [M, N] (ldb) or NULL (zeros), out [M, N] (ldo),
+ *         all in dtype (f16 / bf16); out may be base
+ *   down  [n, R, K], up [n, N, R] in dtype; smaller adapters are padded with
+ *         zeros to the common rank R (1..256)
+ *   ids   int32, one per rows_per_id rows (rows_per_id 1: one per row); an
+ *         id >= n sets IC_DEV_ERR_INDEX and gives NaN for its rows
+ *   scales fp32 [n] or NULL (ones)
+ *   workspace  ic_lora_batched_workspace(...) floats, 16-byte aligned,
+ *         contents arbitrary, in use until the call's work has run
+ * Any alignment works; 16-byte aligned rows (K, N and strides multiples of 8,
+ * R a multiple of 4) are faster.  The sums' order depends on the sizes only. */
+int ic_lora_batched(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* down, const void* up,
+                    int64_t R, int64_t n, const int32_t* ids, int64_t rows_per_id, const float* scales,
+                    const void* base, int64_t ldb, void* out, int64_t N, int64_t ldo, float* workspace,
+                    int64_t workspace_elems, void* stream);
+/* Floats of workspace for these sizes; -1 and an error message for sizes
+ * that ic_lora_batched refuses. */
+int64_t ic_lora_batched_workspace(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n);
 
 /* Self-test of the kernels' bounded waits (no counterpart in the
  * reference; failure detection): launches one thread that waits on an
