@@ -706,7 +706,7 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     """``t`` ([batch, tokens, heads, D]) as the kernels read it: elements
     contiguous, 16-byte aligned rows; a copy where it is not."""
     b, l, h, d = t.stride()
-    if d == 1 and not ((b | l | h) & 7 or t.data_ptr() & 15):
+    if d == 1 and not ((b | l | h) & 7 or t.data_ptr() & 15) and (l or t.shape[1] <= 1):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 

@@ -168,6 +168,13 @@ int ic_cross_attention(const void* q, const void* k, const void* v, void* out, i
   if (!head_layout_ok(q, strides) || !head_layout_ok(out, strides + 9) ||
       (Lk && (!head_layout_ok(k, strides + 3) || !head_layout_ok(v, strides + 6))))
     return set_error(IC_ERR_ARG, "%s: tensors must be 16-byte aligned, strides multiples of 8", me);
+  for (int i = 0; i < 12; ++i) {
+    const int64_t tokens = i < 3 || i >= 9 ? Lq : Lk;
+    if (strides[i] < 0 || strides[i] >= (1LL << 38))
+      return set_error(IC_ERR_ARG, "%s: strides must be in [0, 2^38)", me);
+    if (i % 3 == 1 && strides[i] == 0 && tokens > 1)
+      return set_error(IC_ERR_ARG, "%s: a token stride of 0 with more than one token", me);
+  }
   const XattnPlan p = xattn_plan(B, Lq, Lk, (int)H, (int)Hk, (int)D, mask_kind);
   if (p.floats && (!workspace || !at16(workspace) || workspace_elems < p.floats))
     return set_error(IC_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld floats, got %lld", me,

@@ -3,5 +3,6 @@
 #include "ic_common.cuh"
 #include "qk_norm_rope.cu"
 #include "lora_batched.cu"
+#include "cross_attention_tc.cu"
 #include "cross_attention.cu"
 #include "abi_attention.cu"

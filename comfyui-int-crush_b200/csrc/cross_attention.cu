@@ -320,9 +320,26 @@ static int rows_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk) {
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
+// Splits and slots of the tcgen05 kernel: two query tiles per CTA share K and
+// V; with too few tiles for that to fill the SMs, one, and then the keys are
+// split with two tiles of 128 at least in a part.
+static int tc_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int* slots) {
+  const int64_t sms = num_sms();
+  const int64_t tiles = H / Hk * ((Lq + 127) / 128);
+  *slots = B * Hk * tiles <= sms ? 1 : 2;
+  const int64_t items = B * Hk * ((tiles + *slots - 1) / *slots);
+  int64_t s = sms / items;
+  const int64_t most = ((Lk + 127) / 128 + 1) / 2;
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
 XattnPlan xattn_plan(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int D, int mask_kind) {
   XattnPlan p;
-  p.splits = rows_splits(B, Lq, Lk, H, Hk);
+  p.slots = 0;
+  if (Lk == 0) p.splits = 1;
+  else if (Lq > 48) p.splits = tc_splits(B, Lq, Lk, H, Hk, &p.slots);
+  else p.splits = rows_splits(B, Lq, Lk, H, Hk);
   p.Lkp = mask_kind ? (Lk + 127) / 128 * 128 : 0;
   const int64_t rows = B * Lq * H;
   p.part_floats = p.splits > 1 ? ((int64_t)p.splits * rows * (D + 2) + 3) / 4 * 4 : 0;
@@ -341,8 +358,9 @@ static cudaError_t launch_rows(const XattnArgs& a, cudaStream_t st) {
 }
 
 template <typename T>
-static cudaError_t launch_xattn_t(const XattnArgs& a, cudaStream_t st) {
-  cudaError_t e = a.bias ? launch_rows<T, true>(a, st) : launch_rows<T, false>(a, st);
+static cudaError_t launch_xattn_t(const XattnArgs& a, int slots, cudaStream_t st) {
+  cudaError_t e = slots ? launch_xattn_tc<T>(a, slots, st)
+                        : a.bias ? launch_rows<T, true>(a, st) : launch_rows<T, false>(a, st);
   if (e != cudaSuccess || a.splits == 1) return e;
   const int64_t n = a.B * a.Lq * a.H * (a.D / 8);
   xattn_join_kernel<T><<<(unsigned)((n + 127) / 128), 128, 0, st>>>(a);
@@ -379,7 +397,7 @@ cudaError_t launch_cross_attention(XattnArgs a, int dtype, const void* mask, int
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  return dtype == IC_DTYPE_BF16 ? launch_xattn_t<__nv_bfloat16>(a, st) : launch_xattn_t<__half>(a, st);
+  return dtype == IC_DTYPE_BF16 ? launch_xattn_t<__nv_bfloat16>(a, p.slots, st) : launch_xattn_t<__half>(a, p.slots, st);
 }
 
 }  // namespace ic

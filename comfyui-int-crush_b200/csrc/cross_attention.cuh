@@ -29,12 +29,15 @@ struct XattnArgs {
 };
 
 struct XattnPlan {
+  int slots;                   // 0: few-rows kernel, else query tiles per item of the tcgen05 one
   int splits;
   int64_t Lkp;
   int64_t part_floats;
   int64_t floats;              // workspace
 };
 
+template <typename T>
+cudaError_t launch_xattn_tc(const XattnArgs& a, int slots, cudaStream_t st);   // cross_attention_tc.cu
 XattnPlan xattn_plan(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int D, int mask_kind);
 
 // 1 + the last key that sample b may see

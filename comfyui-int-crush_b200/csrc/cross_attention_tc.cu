@@ -1,0 +1,558 @@
+// Cross attention for many query rows on tcgen05 (kind::f16).
+//
+// Persistent, one CTA per SM, 12 warps.  A work item is one key head of one
+// sample with one or two tiles of 128 query rows ("slots"; the slots share the
+// K and V tiles), over the item's part of the keys in tiles of 128:
+//   S_s = Q_s K^T            128 x 128, both operands in shared memory
+//   P_s = 2^(S_s c - m)      registers, written back over S_s as 16-bit pairs
+//   O_s += P_s V             A operand from tensor memory, V as it lies in
+//                            memory (rows = keys: the MN-major B operand)
+// Tensor memory: S_0 | S_1 | O_0 | O_1, 128 columns each.
+//
+// Warps 0-3 / 4-7: softmax of slot 0 / 1, one row per thread (no shuffles).
+// Warp 8: TMA producer (Q slots, a ring of K and V tiles).  Warp 9: MMA
+// issuer.  Warp 10: zeroes the V rows of keys that are not seen (P is 0 there,
+// but 0 * NaN is not) when there are lengths or a mask.
+// The MMAs of one slot run while the other slot's softmax does, and the next
+// item's first S is issued behind the last P V, so that the epilogue of one
+// slot overlaps with MMAs too.
+//
+// S, the running maximum, the row sum and O are fp32.  The maximum moves only
+// when it grows by more than 2^8 (P stays below 2^8 and the sums exact), so O
+// is rescaled in tensor memory on few tiles; P V of the tile before is
+// complete then, because S of this tile was issued behind it.  P is rounded
+// to the activation type (the MMA's operand type), the row sum is not.
+#include "cross_attention.cuh"
+
+#include <type_traits>
+
+namespace ic {
+
+template <int DP>
+struct XtCfg {
+  static constexpr int PANELS = DP / 64;            // 64-element panels of 128 rows, 128B-swizzled
+  static constexpr int TILE = PANELS * 16384;
+  static constexpr int NST = DP == 128 ? 5 : 8;     // ring stages (K and V tiles in turn)
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_KV + NST * TILE;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024; // + alignment of the base
+  static constexpr int THREADS = 384;
+};
+
+struct XtArgs {
+  XattnArgs x;
+  int slots;          // query tiles of an item: 1 or 2
+  int tiles_per_head; // ceil(Lq / 128)
+  int items;
+  int qm[2], km[2], vm[2];   // 0 where the batch / head stride is 0 (coordinate 0), else 1
+};
+
+struct XtItem {
+  int64_t b;
+  int hk, split, tile0, nslots, end, key0, nt;
+};
+
+__device__ __forceinline__ XtItem xt_item(const XtArgs& a, int i) {
+  XtItem t;
+  const int group = a.x.H / a.x.Hk;
+  const int tiles = group * a.tiles_per_head;
+  const int per_head = (tiles + a.slots - 1) / a.slots;
+  t.split = i % a.x.splits;
+  i /= a.x.splits;
+  const int bh = i / per_head;
+  t.tile0 = (i - bh * per_head) * a.slots;
+  t.nslots = min(a.slots, tiles - t.tile0);
+  t.b = bh / a.x.Hk;
+  t.hk = bh - (int)t.b * a.x.Hk;
+  t.end = xattn_end(a.x, t.b);
+  const int kt = (t.end + 127) / 128;
+  const int per = (kt + a.x.splits - 1) / a.x.splits;
+  const int t0 = min(t.split * per, kt);
+  t.nt = min(t0 + per, kt) - t0;
+  t.key0 = t0 * 128;
+  return t;
+}
+// head and first row of slot s
+__device__ __forceinline__ void xt_slot(const XtArgs& a, const XtItem& t, int s, int& h, int& l0) {
+  const int q = t.tile0 + s;
+  const int sub = q / a.tiles_per_head;
+  h = t.hk * (a.x.H / a.x.Hk) + sub;
+  l0 = (q - sub * a.tiles_per_head) * 128;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// MN-major operand in the 128-byte-swizzled layout: 64 contiguous elements
+// per row, 8-row groups 1024 bytes apart (stride offset), panels of 64
+// elements 16384 bytes apart (leading offset).
+__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(16384u >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+
+// The registers of a tcgen05.ld are valid after the wait: tie them to it.
+__device__ __forceinline__ void tie32(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+
+__device__ __forceinline__ bool all_lanes(bool ok) { return __all_sync(0xffffffffu, ok); }
+
+template <typename T, int DP, bool BIAS>
+__global__ void __launch_bounds__(XtCfg<DP>::THREADS, 1)
+xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const XtArgs a) {
+  using C = XtCfg<DP>;
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int NST = C::NST;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [2] TMA -> MMA
+  uint64_t* q_empty = q_full + 2;       // [2] the item's last S is done -> TMA
+  uint64_t* s_full = q_empty + 2;       // [2] S is done -> softmax
+  uint64_t* p_full = s_full + 2;        // [2] P is written, O rescaled -> MMA (4 warps)
+  uint64_t* o_full = p_full + 2;        // [2] the item's last P V is done -> epilogue
+  uint64_t* o_empty = o_full + 2;       // [2] O is read -> MMA (4 warps)
+  uint64_t* kv_full = o_empty + 2;      // [NST] TMA -> MMA, cleaner
+  uint64_t* kv_empty = kv_full + NST;   // [NST] MMA -> TMA
+  uint64_t* ready = kv_empty + NST;     // [NST] cleaner -> MMA
+  uint64_t* drain = ready + NST;        // all MMAs are done, at the end
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_full + i, 1);
+      mbar_init(o_empty + i, 4);
+    }
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+      mbar_init(ready + i, 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const bool clean = BIAS || a.x.kv_lens != nullptr;
+  const uint32_t kv_base = smem_u32(smem) + C::OFF_KV;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      uint32_t use = 0, qn[2] = {0, 0};
+      bool ok = true;
+      const auto load_kv = [&](const CUtensorMap* tm, const XtItem& t, const int* mul, int key) {
+        const uint32_t st = use % NST;
+        if (!mbar_wait(kv_empty + st, ((use / NST) & 1u) ^ 1u, abort_flag)) return false;
+        mbar_arrive_expect_tx(kv_full + st, C::TILE);
+#pragma unroll
+        for (int p = 0; p < C::PANELS; ++p)
+          tma_load_4d(kv_base + st * C::TILE + p * 16384, tm, kv_full + st, 64 * p, t.hk * mul[1], key,
+                      (int)t.b * mul[0]);
+        ++use;
+        return true;
+      };
+      const auto load_q = [&](const XtItem& t, int s) {
+        if (!mbar_wait(q_empty + s, (qn[s] & 1u) ^ 1u, abort_flag)) return false;
+        int h, l0;
+        xt_slot(a, t, s, h, l0);
+        mbar_arrive_expect_tx(q_full + s, C::TILE);
+#pragma unroll
+        for (int p = 0; p < C::PANELS; ++p)
+          tma_load_4d(smem_u32(smem) + s * C::TILE + p * 16384, &tm_q, q_full + s, 64 * p, h * a.qm[1], l0,
+                      (int)t.b * a.qm[0]);
+        ++qn[s];
+        return true;
+      };
+      for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
+        const XtItem t = xt_item(a, i);
+        if (t.nt == 0) continue;
+        ok = load_q(t, 0) && load_kv(&tm_k, t, a.km, t.key0) && (t.nslots < 2 || load_q(t, 1)) &&
+             load_kv(&tm_v, t, a.vm, t.key0);
+        for (int j = 1; ok && j < t.nt; ++j)
+          ok = load_kv(&tm_k, t, a.km, t.key0 + 128 * j) && load_kv(&tm_v, t, a.vm, t.key0 + 128 * j);
+      }
+      if (!ok) {
+        // given up: every copy issued lands before the CTA may leave
+        volatile int never = 0;
+        for (uint32_t u = use > NST ? use - NST : 0; u < use; ++u)
+          mbar_wait(kv_full + u % NST, (u / NST) & 1u, &never);
+        for (int s = 0; s < 2; ++s)
+          if (qn[s]) mbar_wait(q_full + s, (qn[s] - 1) & 1u, &never);
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      const int ksteps = (a.x.D + 15) / 16;
+      const uint32_t i_pv = idesc_f16(128, ksteps * 16, BF) | (1u << 16);   // B is MN-major
+      uint32_t use = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
+      const auto tile_wait = [&](uint32_t u) {
+        return mbar_wait((clean ? ready : kv_full) + u % NST, (u / NST) & 1u, abort_flag);
+      };
+      // keys of tile j of an item, rounded to the MMA's step
+      const auto width = [&](const XtItem& t, int j) { return min(128, (t.end - t.key0 - 128 * j + 15) / 16 * 16); };
+      const auto issue_s = [&](int s, uint32_t u, int n, bool last) {
+        const uint32_t qa = smem_u32(smem) + s * C::TILE, kb = kv_base + (u % NST) * C::TILE;
+        const uint32_t idesc = idesc_f16(128, n, BF);
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+          mma_f16(tmem + s * 128, smem_desc_sw128(qa + off), smem_desc_sw128(kb + off), idesc, k > 0);
+        }
+        mma_commit(s_full + s);
+        if (last) mma_commit(q_empty + s);
+      };
+      const auto next_item = [&](int& i, XtItem& t) {
+        for (; i < a.items; i += gridDim.x) {
+          t = xt_item(a, i);
+          if (t.nt) return true;
+        }
+        return false;
+      };
+      int i = blockIdx.x;
+      XtItem t, nx;
+      bool have = next_item(i, t), ok = true;
+      if (have) {
+        ok = tile_wait(use);
+        for (int s = 0; ok && s < t.nslots; ++s) {
+          ok = mbar_wait(q_full + s, qn[s]++ & 1u, abort_flag);
+          if (ok) issue_s(s, use, width(t, 0), t.nt == 1);
+        }
+        if (ok) mma_commit(kv_empty + use % NST);
+        ++use;   // now at V of tile 0
+      }
+      while (have && ok) {
+        i += gridDim.x;
+        const bool more = next_item(i, nx);
+        for (int j = 0; ok && j < t.nt; ++j) {
+          const bool last = j == t.nt - 1;
+          const uint32_t uv = use, uk = use + 1;   // V of this tile, the K tile after it
+          const int n = last ? (more ? width(nx, 0) : 0) : width(t, j + 1);
+          const int nslots = last && more ? nx.nslots : t.nslots;
+          const int pv_steps = width(t, j) / 16;
+          bool k_seen = false;
+          ok = tile_wait(uv);
+          for (int s = 0; ok && s < max(t.nslots, last && more ? nx.nslots : 0); ++s) {
+            if (s < t.nslots) {
+              ok = mbar_wait(p_full + s, pn[s]++ & 1u, abort_flag);
+              if (ok && j == 0) ok = mbar_wait(o_empty + s, (on[s]++ & 1u) ^ 1u, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t vb = kv_base + (uv % NST) * C::TILE;
+              for (int k = 0; k < pv_steps; ++k)
+                mma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, smem_desc_mn128(vb + k * 2048), i_pv,
+                           (j | k) > 0);
+              if (last) mma_commit(o_full + s);
+            }
+            if (n && s < nslots) {
+              if (!k_seen) ok = tile_wait(uk);
+              k_seen = true;
+              if (ok && last) ok = mbar_wait(q_full + s, qn[s]++ & 1u, abort_flag);
+              if (ok) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
+            }
+          }
+          if (!ok) break;
+          mma_commit(kv_empty + uv % NST);
+          if (n) mma_commit(kv_empty + uk % NST);
+          use += 2;
+        }
+        t = nx;
+        have = more;
+      }
+      // MMAs in flight and their arrivals end before tensor memory is freed
+      // and the CTA leaves
+      volatile int never = 0;
+      mma_commit(drain);
+      mbar_wait(drain, 0, &never);
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------- cleaner
+    if (clean) {
+      uint32_t use = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
+        const XtItem t = xt_item(a, i);
+        for (int j = 0; ok && j < 2 * t.nt; ++j, ++use) {
+          const uint32_t st = use % NST;
+          ok = all_lanes(mbar_wait(kv_full + st, (use / NST) & 1u, abort_flag));
+          if (!ok) break;
+          if (j & 1) {   // a V tile
+            const int k0 = t.key0 + 64 * (j & ~1);
+            const int rows = min(128, (t.end - k0 + 15) / 16 * 16);   // rows that the MMA reads
+            unsigned hide[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int key = k0 + 32 * q + lane;
+              bool no = key >= t.end;
+              if constexpr (BIAS) no = no || __ldg(a.x.bias + t.b * a.x.Lkp + key) == -INFINITY;
+              hide[q] = __ballot_sync(0xffffffffu, no && 32 * q + lane < rows);
+            }
+            if (hide[0] | hide[1] | hide[2] | hide[3]) {
+              uint8_t* tile = smem + C::OFF_KV + st * C::TILE;
+              // lane: 16-byte chunk of a row; 8 chunks per panel
+              const int sub = lane / (8 * C::PANELS), ch = lane % (8 * C::PANELS);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (hide[q])
+                  for (int r = sub; r < 32; r += 32 / (8 * C::PANELS))
+                    if ((hide[q] >> r) & 1u)
+                      *reinterpret_cast<uint4*>(tile + (ch >> 3) * 16384 + (32 * q + r) * 128 + (ch & 7) * 16) =
+                          make_uint4(0u, 0u, 0u, 0u);
+              fence_proxy_async_smem();
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ready + st);
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------- softmax and epilogue
+    const int s = warp >> 2, w = warp & 3;
+    const uint32_t lane_base = (uint32_t)(w * 32) << 16;
+    const uint32_t ts = tmem + s * 128 + lane_base, to = tmem + 256 + s * 128 + lane_base;
+    // scores in units of log2: S * c; a scale that is not positive is taken
+    // out of S first, so that the maximum and -inf for hidden keys stay right
+    const float c = a.x.scale == 0.f ? 1.f : fabsf(a.x.scale) * kLog2e;
+    const bool odd_scale = !(a.x.scale > 0.f);
+    const float sign = a.x.scale < 0.f ? -1.f : 0.f;
+    uint32_t sn = 0, on = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
+      const XtItem t = xt_item(a, i);
+      if (s >= t.nslots) continue;
+      int h, l0;
+      xt_slot(a, t, s, h, l0);
+      const int64_t l = l0 + w * 32 + lane;
+      const bool row_on = l < a.x.Lq;
+      float m = -INFINITY, sum = 0.f;
+      for (int j = 0; j < t.nt; ++j) {
+        const int k0 = t.key0 + 128 * j;
+        const int rem = t.end - k0;          // keys of this tile (>= 128: all)
+        ok = all_lanes(mbar_wait(s_full + s, sn & 1u, abort_flag));
+        if (!ok) break;
+        ++sn;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (32 * q < rem) tmem_ld32(ts + 32 * q, r[q]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tie32(r[q]);
+        if (odd_scale) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) * sign);
+        }
+        if (rem < 128) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * q + e >= rem) r[q][e] = 0xff800000u;   // -inf
+        }
+        float mx;
+        if constexpr (BIAS) {
+          const float4* bias = reinterpret_cast<const float4*>(a.x.bias + t.b * a.x.Lkp + k0);
+          mx = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 b4 = __ldg(bias + 8 * q + e / 4);
+              const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                const float x = bb[f] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(r[q][e + f]), c, bb[f]);
+                r[q][e + f] = __float_as_uint(x);
+                mx = fmaxf(mx, x);
+              }
+            }
+        } else {
+          float m4[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            m4[q] = __uint_as_float(r[q][0]);
+#pragma unroll
+            for (int e = 1; e < 32; ++e) m4[q] = fmaxf(m4[q], __uint_as_float(r[q][e]));
+          }
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+        }
+        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+          const float nm = mx > m + 8.f ? mx : m;
+          const float f = nm == m ? 1.f : ex2(m - nm);
+          m = nm;
+          sum *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int q = 0; q < DP / 32; ++q) {
+              if (32 * q < a.x.D) {
+                uint32_t o[32];
+                tmem_ld32(to + 32 * q, o);
+                tmem_wait_ld();
+                tie32(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st32(to + 32 * q, o);
+              }
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (32 * q < rem) {
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float x0 = __uint_as_float(r[q][e]), x1 = __uint_as_float(r[q][e + 1]);
+              float p0, p1;
+              if constexpr (BIAS) {
+                p0 = ex2(x0 - ref);
+                p1 = ex2(x1 - ref);
+              } else {
+                p0 = ex2(fmaf(x0, c, -ref));
+                p1 = ex2(fmaf(x1, c, -ref));
+              }
+              add[(e >> 1) & 3] += p0 + p1;
+              p[e / 2] = pack16<T>(p0, p1);
+            }
+            tmem_st16(ts + 16 * q, p);
+          }
+        }
+        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + s);
+      }
+      if (!ok) break;
+      if (t.nt) {
+        ok = all_lanes(mbar_wait(o_full + s, on & 1u, abort_flag));
+        if (!ok) break;
+        ++on;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int q = 0; q < DP / 32; ++q) {
+        if (32 * q >= a.x.D) continue;
+        uint32_t o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0u;
+        if (t.nt) {
+          tmem_ld32(to + 32 * q, o);
+          tmem_wait_ld();
+          tie32(o);
+        }
+        if (row_on) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (32 * q + e < a.x.D) {
+              float v[8];
+#pragma unroll
+              for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
+              xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
+            }
+          }
+        }
+      }
+      if (t.nt) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_empty + s);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+// [elements, heads, tokens, batch] of a strided tensor.  A stride of 0 is one
+// entry that every coordinate maps to; a dimension of one entry takes any
+// stride.
+static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, int64_t D, int64_t heads, int64_t tokens,
+                   int64_t batch, int* mul) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  mul[0] = st[0] == 0 ? 0 : 1;
+  mul[1] = st[2] == 0 ? 0 : 1;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)(mul[1] ? heads : 1), (cuuint64_t)tokens,
+                        (cuuint64_t)(mul[0] ? batch : 1)};
+  const int64_t el[3] = {st[2], st[1], st[0]};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 * ((cuuint64_t)D / 8) : (cuuint64_t)el[i] * 2;
+  cuuint32_t box[4] = {64, 1, 128, 1};
+  cuuint32_t one[4] = {1, 1, 1, 1};
+  return fn(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), dims,
+            strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP, bool BIAS>
+static cudaError_t launch_xt(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const XtArgs& a,
+                             cudaStream_t st) {
+  auto kern = xattn_tc_kernel<T, DP, BIAS>;
+  const cudaError_t e = set_smem_once(kern, XtCfg<DP>::SMEM);
+  if (e != cudaSuccess) return e;
+  const int grid = a.items < num_sms() ? a.items : num_sms();
+  kern<<<grid, XtCfg<DP>::THREADS, XtCfg<DP>::SMEM, st>>>(q, k, v, a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_xattn_tc(const XattnArgs& x, int slots, cudaStream_t st) {
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  XtArgs a;
+  a.x = x;
+  a.slots = slots;
+  a.tiles_per_head = (int)((x.Lq + 127) / 128);
+  const int64_t tiles = (int64_t)(x.H / x.Hk) * a.tiles_per_head;
+  const int64_t items = x.B * x.Hk * ((tiles + slots - 1) / slots) * x.splits;
+  if (items > 0x3fffffff) return cudaErrorInvalidValue;
+  a.items = (int)items;
+  CUtensorMap q, k, v;
+  if (!xt_map(&q, BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, a.qm) || !xt_map(&k, BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, a.km) ||
+      !xt_map(&v, BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, a.vm))
+    return cudaErrorInvalidValue;
+  if (x.D <= 64) return x.bias ? launch_xt<T, 64, true>(q, k, v, a, st) : launch_xt<T, 64, false>(q, k, v, a, st);
+  return x.bias ? launch_xt<T, 128, true>(q, k, v, a, st) : launch_xt<T, 128, false>(q, k, v, a, st);
+}
+
+}  // namespace ic

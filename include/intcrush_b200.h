@@ -342,7 +342,8 @@ int ic_qk_norm_rope(const void* q, void* q_out, int64_t H, const void* k, void* 
  *   q, out  [B, Lq, H, D], k, v [B, Lk, Hk, D] in dtype (f16 / bf16), D a
  *           multiple of 8 up to 128, H a multiple of Hk
  *   strides 12 element strides, batch / token / head of q, k, v, out;
- *           multiples of 8, tensors 16-byte aligned, elements contiguous
+ *           multiples of 8, tensors 16-byte aligned, elements contiguous;
+ *           0 for a batch or head dimension of k or v repeats it
  *   mask    [B, Lk] rows of ld_mask elements (0: one row for all samples), or
  *           NULL with IC_MASK_NONE
  *   workspace  ic_cross_attention_workspace(...) floats, 16-byte aligned,
