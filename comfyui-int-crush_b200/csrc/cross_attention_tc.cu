@@ -32,9 +32,10 @@ template <int DP>
 struct XtCfg {
   static constexpr int PANELS = DP / 64;            // 64-element panels of 128 rows, 128B-swizzled
   static constexpr int TILE = PANELS * 16384;
-  static constexpr int NST = DP == 128 ? 5 : 8;     // ring stages (K and V tiles in turn)
+  static constexpr int NST = DP == 128 ? 4 : 6;     // ring stages (K and V tiles in turn)
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_BAR = OFF_KV + NST * TILE;
+  static constexpr int OFF_STG = OFF_KV + NST * TILE;   // 8 warps x 32 output rows x 64 elements
+  static constexpr int OFF_BAR = OFF_STG + 32768;
   static constexpr int SMEM = OFF_BAR + 512 + 1024; // + alignment of the base
   static constexpr int THREADS = 384;
 };
@@ -107,12 +108,76 @@ __device__ __forceinline__ void tie32(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31]));
 }
 
+// The MMA warp stays converged, so that descriptors live in uniform registers;
+// only the issue itself is one lane's (`on`).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on;
+}
+__device__ __forceinline__ void mma_f16_on(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts_on(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                              uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_on(uint32_t on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(on)
+      : "memory");
+}
+
+// Box store shared -> global, clipped at the tensor's edges.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(m)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void untwo(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ bool all_lanes(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(XtCfg<DP>::THREADS, 1)
 xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const XtArgs a) {
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const XtArgs a) {
   using C = XtCfg<DP>;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NST = C::NST;
@@ -131,7 +196,9 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 2);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // values that are the same in all lanes, said so by the broadcast: the role
+  // branches and the MMA warp's descriptors then compile as warp-uniform
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
@@ -158,14 +225,19 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
+    prefetch_tmap(&tm_o);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const bool clean = BIAS || a.x.kv_lens != nullptr;
   const uint32_t kv_base = smem_u32(smem) + C::OFF_KV;
 
+  // registers: 384 threads x 168 = 128 x 88 here + 256 x 208 below, where a
+  // thread holds a row of S
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -197,7 +269,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
         const XtItem t = xt_item(a, i);
         if (t.nt == 0) continue;
-        ok = load_q(t, 0) && load_kv(&tm_k, t, a.km, t.key0) && (t.nslots < 2 || load_q(t, 1)) &&
+        // K first: its stage frees before the Q slots of the item before
+        ok = load_kv(&tm_k, t, a.km, t.key0) && load_q(t, 0) && (t.nslots < 2 || load_q(t, 1)) &&
              load_kv(&tm_v, t, a.vm, t.key0);
         for (int j = 1; ok && j < t.nt; ++j)
           ok = load_kv(&tm_k, t, a.km, t.key0 + 128 * j) && load_kv(&tm_v, t, a.vm, t.key0 + 128 * j);
@@ -213,88 +286,114 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      const int ksteps = (a.x.D + 15) / 16;
-      const uint32_t i_pv = idesc_f16(128, ksteps * 16, BF) | (1u << 16);   // B is MN-major
-      uint32_t use = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
-      const auto tile_wait = [&](uint32_t u) {
-        return mbar_wait((clean ? ready : kv_full) + u % NST, (u / NST) & 1u, abort_flag);
+    const uint32_t on = elect_one();
+    const int ksteps = (a.x.D + 15) / 16;
+    const uint32_t i_pv = idesc_f16(128, ksteps * 16, BF) | (1u << 16);   // B is MN-major
+    uint32_t use = 0, qph = 0, pph = 0, oph = 3;   // a phase bit per slot
+    const auto tile_wait = [&](uint32_t u) {
+      return all_lanes(mbar_wait((clean ? ready : kv_full) + u % NST, (u / NST) & 1u, abort_flag));
+    };
+    const auto slot_wait = [&](uint64_t* bar, uint32_t& ph, int s) {
+      const uint32_t parity = (ph >> s) & 1u;
+      ph ^= 1u << s;
+      return all_lanes(mbar_wait(bar + s, parity, abort_flag));
+    };
+    // keys of tile j of an item, rounded to the MMA's step
+    const auto width = [&](const XtItem& t, int j) { return min(128, (t.end - t.key0 - 128 * j + 15) / 16 * 16); };
+    const auto issue_s = [&](int s, uint32_t u, int n, bool last) {
+      const uint64_t dq = smem_desc_sw128(smem_u32(smem) + s * C::TILE);
+      const uint64_t dk = smem_desc_sw128(kv_base + (u % NST) * C::TILE);
+      const uint32_t idesc = idesc_f16(128, n, BF);
+      const auto step = [&](int k) {   // offsets in descriptor units (16 bytes)
+        const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4);
+        mma_f16_on(on, tmem + s * 128, dq + off, dk + off, idesc, k > 0);
       };
-      // keys of tile j of an item, rounded to the MMA's step
-      const auto width = [&](const XtItem& t, int j) { return min(128, (t.end - t.key0 - 128 * j + 15) / 16 * 16); };
-      const auto issue_s = [&](int s, uint32_t u, int n, bool last) {
-        const uint32_t qa = smem_u32(smem) + s * C::TILE, kb = kv_base + (u % NST) * C::TILE;
-        const uint32_t idesc = idesc_f16(128, n, BF);
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          mma_f16(tmem + s * 128, smem_desc_sw128(qa + off), smem_desc_sw128(kb + off), idesc, k > 0);
-        }
-        mma_commit(s_full + s);
-        if (last) mma_commit(q_empty + s);
-      };
-      const auto next_item = [&](int& i, XtItem& t) {
-        for (; i < a.items; i += gridDim.x) {
-          t = xt_item(a, i);
-          if (t.nt) return true;
-        }
-        return false;
-      };
-      int i = blockIdx.x;
-      XtItem t, nx;
-      bool have = next_item(i, t), ok = true;
-      if (have) {
-        ok = tile_wait(use);
-        for (int s = 0; ok && s < t.nslots; ++s) {
-          ok = mbar_wait(q_full + s, qn[s]++ & 1u, abort_flag);
-          if (ok) issue_s(s, use, width(t, 0), t.nt == 1);
-        }
-        if (ok) mma_commit(kv_empty + use % NST);
-        ++use;   // now at V of tile 0
+      if (ksteps == DP / 16) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) step(k);
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < ksteps; ++k) step(k);
       }
-      while (have && ok) {
-        i += gridDim.x;
-        const bool more = next_item(i, nx);
-        for (int j = 0; ok && j < t.nt; ++j) {
-          const bool last = j == t.nt - 1;
-          const uint32_t uv = use, uk = use + 1;   // V of this tile, the K tile after it
-          const int n = last ? (more ? width(nx, 0) : 0) : width(t, j + 1);
-          const int nslots = last && more ? nx.nslots : t.nslots;
-          const int pv_steps = width(t, j) / 16;
-          bool k_seen = false;
-          ok = tile_wait(uv);
-          for (int s = 0; ok && s < max(t.nslots, last && more ? nx.nslots : 0); ++s) {
-            if (s < t.nslots) {
-              ok = mbar_wait(p_full + s, pn[s]++ & 1u, abort_flag);
-              if (ok && j == 0) ok = mbar_wait(o_empty + s, (on[s]++ & 1u) ^ 1u, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t vb = kv_base + (uv % NST) * C::TILE;
-              for (int k = 0; k < pv_steps; ++k)
-                mma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, smem_desc_mn128(vb + k * 2048), i_pv,
-                           (j | k) > 0);
-              if (last) mma_commit(o_full + s);
-            }
-            if (n && s < nslots) {
-              if (!k_seen) ok = tile_wait(uk);
-              k_seen = true;
-              if (ok && last) ok = mbar_wait(q_full + s, qn[s]++ & 1u, abort_flag);
-              if (ok) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
-            }
-          }
-          if (!ok) break;
-          mma_commit(kv_empty + uv % NST);
-          if (n) mma_commit(kv_empty + uk % NST);
-          use += 2;
-        }
-        t = nx;
-        have = more;
+      mma_commit_on(on, s_full + s);
+      if (last) mma_commit_on(on, q_empty + s);
+    };
+    const auto issue_pv = [&](int s, uint32_t u, int steps, uint32_t accumulate) {
+      const uint64_t dv = smem_desc_mn128(kv_base + (u % NST) * C::TILE);
+      const auto step = [&](int k) {
+        mma_f16_ts_on(on, tmem + 256 + s * 128, tmem + s * 128 + k * 8, dv + k * (2048 >> 4), i_pv,
+                      k > 0 ? 1u : accumulate);
+      };
+      if (steps == 8) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) step(k);
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < steps; ++k) step(k);
       }
-      // MMAs in flight and their arrivals end before tensor memory is freed
-      // and the CTA leaves
-      volatile int never = 0;
-      mma_commit(drain);
-      mbar_wait(drain, 0, &never);
+    };
+    const auto next_item = [&](int& i, XtItem& t) {
+      for (; i < a.items; i += gridDim.x) {
+        t = xt_item(a, i);
+        t.end = uniform(t.end);
+        t.nt = uniform(t.nt);
+        t.key0 = uniform(t.key0);
+        if (t.nt) return true;
+      }
+      return false;
+    };
+    int i = blockIdx.x;
+    XtItem t, nx;
+    bool have = next_item(i, t), ok = true;
+    if (have) {
+      ok = tile_wait(use);
+      for (int s = 0; ok && s < t.nslots; ++s) {
+        ok = slot_wait(q_full, qph, s);
+        if (ok) issue_s(s, use, width(t, 0), t.nt == 1);
+      }
+      if (ok) mma_commit_on(on, kv_empty + use % NST);
+      ++use;   // now at V of tile 0
     }
+    while (have && ok) {
+      i += gridDim.x;
+      const bool more = next_item(i, nx);
+      for (int j = 0; ok && j < t.nt; ++j) {
+        const bool last = j == t.nt - 1;
+        const uint32_t uv = use, uk = use + 1;   // V of this tile, the K tile after it
+        const int n = last ? (more ? width(nx, 0) : 0) : width(t, j + 1);
+        const int nslots = last && more ? nx.nslots : t.nslots;   // slots whose next S uses uk
+        const int pv_steps = width(t, j) / 16;
+        bool k_seen = false;
+        ok = tile_wait(uv);
+        for (int s = 0; ok && s < max(t.nslots, n ? nslots : 0); ++s) {
+          if (s < t.nslots) {
+            ok = slot_wait(p_full, pph, s);
+            if (ok && j == 0) ok = slot_wait(o_empty, oph, s);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(s, uv, pv_steps, j > 0);
+            if (last) mma_commit_on(on, o_full + s);
+          }
+          if (n && s < nslots) {
+            if (!k_seen) ok = tile_wait(uk);
+            k_seen = true;
+            if (ok && last) ok = slot_wait(q_full, qph, s);
+            if (ok) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
+          }
+        }
+        if (!ok) break;
+        mma_commit_on(on, kv_empty + uv % NST);
+        if (n) mma_commit_on(on, kv_empty + uk % NST);
+        use += 2;
+      }
+      t = nx;
+      have = more;
+    }
+    // MMAs in flight and their arrivals end before tensor memory is freed and
+    // the CTA leaves
+    volatile int never = 0;
+    mma_commit_on(on, drain);
+    mbar_wait(drain, 0, &never);
   } else if (warp == 10) {
     // ------------------------------------------------------------- cleaner
     if (clean) {
@@ -336,7 +435,9 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
     }
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------- softmax and epilogue
     const int s = warp >> 2, w = warp & 3;
     const uint32_t lane_base = (uint32_t)(w * 32) << 16;
@@ -346,6 +447,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const float c = a.x.scale == 0.f ? 1.f : fabsf(a.x.scale) * kLog2e;
     const bool odd_scale = !(a.x.scale > 0.f);
     const float sign = a.x.scale < 0.f ? -1.f : 0.f;
+    uint8_t* stage = smem + C::OFF_STG + warp * 4096 + lane * 128;   // this row's 64 elements, 128B-swizzled
     uint32_t sn = 0, on = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
@@ -406,7 +508,9 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int q = 0; q < 4; ++q) {
             m4[q] = __uint_as_float(r[q][0]);
 #pragma unroll
-            for (int e = 1; e < 32; ++e) m4[q] = fmaxf(m4[q], __uint_as_float(r[q][e]));
+            for (int e = 1; e < 31; e += 2)
+              m4[q] = fmaxf(fmaxf(m4[q], __uint_as_float(r[q][e])), __uint_as_float(r[q][e + 1]));
+            m4[q] = fmaxf(m4[q], __uint_as_float(r[q][31]));
           }
           mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
         }
@@ -431,29 +535,28 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float add[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t cc = two(BIAS ? 1.f : c, BIAS ? 1.f : c), rr = two(-ref, -ref);
+        uint64_t add[2] = {two(sum, 0.f), two(0.f, 0.f)};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (32 * q < rem) {
             uint32_t p[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float x0 = __uint_as_float(r[q][e]), x1 = __uint_as_float(r[q][e + 1]);
+              const uint64_t x = fma2(two(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1])), cc, rr);
               float p0, p1;
-              if constexpr (BIAS) {
-                p0 = ex2(x0 - ref);
-                p1 = ex2(x1 - ref);
-              } else {
-                p0 = ex2(fmaf(x0, c, -ref));
-                p1 = ex2(fmaf(x1, c, -ref));
-              }
-              add[(e >> 1) & 3] += p0 + p1;
+              untwo(x, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              add[(e >> 1) & 1] = add2(add[(e >> 1) & 1], two(p0, p1));
               p[e / 2] = pack16<T>(p0, p1);
             }
             tmem_st16(ts + 16 * q, p);
           }
         }
-        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        float s0, s1;
+        untwo(add2(add[0], add[1]), s0, s1);
+        sum = s0 + s1;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -466,27 +569,56 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         ++on;
         tc_fence_after();
       }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const uint64_t ii = two(inv, inv);
 #pragma unroll
-      for (int q = 0; q < DP / 32; ++q) {
-        if (32 * q >= a.x.D) continue;
-        uint32_t o[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0u;
-        if (t.nt) {
-          tmem_ld32(to + 32 * q, o);
-          tmem_wait_ld();
-          tie32(o);
+      for (int p = 0; p < C::PANELS; ++p) {
+        if (64 * p >= a.x.D) continue;
+        if (a.x.splits == 1) {
+          // this warp's staging rows are free again (its last store has read them)
+          if (lane == 0) bulk_wait_read0();
+          __syncwarp();
         }
-        if (row_on) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (32 * q + e < a.x.D) {
-              float v[8];
+        for (int q = 0; q < 2; ++q) {
+          uint32_t o[32];
 #pragma unroll
-              for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
-              xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+          if (t.nt) {
+            tmem_ld32(to + 64 * p + 32 * q, o);
+            tmem_wait_ld();
+            tie32(o);
+          }
+          if (a.x.splits == 1) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t v[4];
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                float lo, hi;
+                untwo(mul2(two(__uint_as_float(o[e + 2 * f]), __uint_as_float(o[e + 2 * f + 1])), ii), lo, hi);
+                v[f] = pack16<T>(lo, hi);
+              }
+              *reinterpret_cast<uint4*>(stage + ((4 * q + e / 8) ^ (lane & 7)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          } else if (row_on) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              if (64 * p + 32 * q + e < a.x.D) {
+                float v[8];
+#pragma unroll
+                for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
+                xattn_put<T>(a.x, t.b, l, h, t.split, 64 * p + 32 * q + e, v, m, sum);
+              }
             }
           }
+        }
+        if (a.x.splits == 1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && l0 + 32 * w < a.x.Lq)
+            tma_store_4d(&tm_o, smem_u32(smem) + C::OFF_STG + warp * 4096, 64 * p, h, l0 + 32 * w, (int)t.b);
+          if (lane == 0) bulk_commit();
         }
       }
       if (t.nt) {
@@ -495,6 +627,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (lane == 0) mbar_arrive(o_empty + s);
       }
     }
+    if (lane == 0) bulk_wait0();   // the stores are done before the CTA leaves
   }
   __syncthreads();
   if (warp == 9) {
@@ -508,7 +641,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // entry that every coordinate maps to; a dimension of one entry takes any
 // stride.
 static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, int64_t D, int64_t heads, int64_t tokens,
-                   int64_t batch, int* mul) {
+                   int64_t batch, uint32_t rows, int* mul) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   mul[0] = st[0] == 0 ? 0 : 1;
@@ -518,7 +651,7 @@ static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, in
   const int64_t el[3] = {st[2], st[1], st[0]};
   cuuint64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 * ((cuuint64_t)D / 8) : (cuuint64_t)el[i] * 2;
-  cuuint32_t box[4] = {64, 1, 128, 1};
+  cuuint32_t box[4] = {64, 1, rows, 1};
   cuuint32_t one[4] = {1, 1, 1, 1};
   return fn(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), dims,
             strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -526,13 +659,12 @@ static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, in
 }
 
 template <typename T, int DP, bool BIAS>
-static cudaError_t launch_xt(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const XtArgs& a,
-                             cudaStream_t st) {
+static cudaError_t launch_xt(const CUtensorMap (&m)[4], const XtArgs& a, cudaStream_t st) {
   auto kern = xattn_tc_kernel<T, DP, BIAS>;
   const cudaError_t e = set_smem_once(kern, XtCfg<DP>::SMEM);
   if (e != cudaSuccess) return e;
   const int grid = a.items < num_sms() ? a.items : num_sms();
-  kern<<<grid, XtCfg<DP>::THREADS, XtCfg<DP>::SMEM, st>>>(q, k, v, a);
+  kern<<<grid, XtCfg<DP>::THREADS, XtCfg<DP>::SMEM, st>>>(m[0], m[1], m[2], m[3], a);
   return cudaGetLastError();
 }
 
@@ -547,12 +679,15 @@ cudaError_t launch_xattn_tc(const XattnArgs& x, int slots, cudaStream_t st) {
   const int64_t items = x.B * x.Hk * ((tiles + slots - 1) / slots) * x.splits;
   if (items > 0x3fffffff) return cudaErrorInvalidValue;
   a.items = (int)items;
-  CUtensorMap q, k, v;
-  if (!xt_map(&q, BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, a.qm) || !xt_map(&k, BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, a.km) ||
-      !xt_map(&v, BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, a.vm))
+  CUtensorMap m[4];
+  int om[2];
+  if (!xt_map(&m[0], BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, 128, a.qm) ||
+      !xt_map(&m[1], BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, 128, a.km) ||
+      !xt_map(&m[2], BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, 128, a.vm) ||
+      !xt_map(&m[3], BF, x.o, x.os, x.D, x.H, x.Lq, x.B, 32, om))
     return cudaErrorInvalidValue;
-  if (x.D <= 64) return x.bias ? launch_xt<T, 64, true>(q, k, v, a, st) : launch_xt<T, 64, false>(q, k, v, a, st);
-  return x.bias ? launch_xt<T, 128, true>(q, k, v, a, st) : launch_xt<T, 128, false>(q, k, v, a, st);
+  if (x.D <= 64) return x.bias ? launch_xt<T, 64, true>(m, a, st) : launch_xt<T, 64, false>(m, a, st);
+  return x.bias ? launch_xt<T, 128, true>(m, a, st) : launch_xt<T, 128, false>(m, a, st);
 }
 
 }  // namespace ic
