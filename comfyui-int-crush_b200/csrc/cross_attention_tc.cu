@@ -1,6 +1,6 @@
 // Cross attention for many query rows on tcgen05 (kind::f16).
 //
-// Persistent, one CTA per SM, 12 warps.  A work item is one key head of one
+// Persistent, one CTA per SM, 16 warps.  A work item is one key head of one
 // sample with one or two tiles of 128 query rows ("slots"; the slots share the
 // K and V tiles), over the item's part of the keys in tiles of 128:
 //   S_s = Q_s K^T            128 x 128, both operands in shared memory
@@ -12,10 +12,11 @@
 // Warps 0-3 / 4-7: softmax of slot 0 / 1, one row per thread (no shuffles).
 // Warp 8: TMA producer (Q slots, a ring of K and V tiles).  Warp 9: MMA
 // issuer.  Warp 10: zeroes the V rows of keys that are not seen (P is 0 there,
-// but 0 * NaN is not) when there are lengths or a mask.
-// The MMAs of one slot run while the other slot's softmax does, and the next
-// item's first S is issued behind the last P V, so that the epilogue of one
-// slot overlaps with MMAs too.
+// but 0 * NaN is not) when there are lengths or a mask.  Warps 12-15: O out of
+// tensor memory, over the row sums, through shared memory to a TMA store.
+// The MMAs of one slot run while the other slot's softmax does; P V starts when
+// half of P is written; the next item's first S is issued behind the last P V,
+// so that nothing drains between items.
 //
 // S, the running maximum, the row sum and O are fp32.  The maximum moves only
 // when it grows by more than 2^8 (P stays below 2^8 and the sums exact), so O
@@ -32,18 +33,34 @@ template <int DP>
 struct XtCfg {
   static constexpr int PANELS = DP / 64;            // 64-element panels of 128 rows, 128B-swizzled
   static constexpr int TILE = PANELS * 16384;
-  static constexpr int NST = DP == 128 ? 4 : 6;     // ring stages (K and V tiles in turn)
+  static constexpr int NST = DP == 128 ? 4 : 8;     // ring stages (K and V tiles in turn)
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_STG = OFF_KV + NST * TILE;   // 8 warps x 32 output rows x 64 elements
-  static constexpr int OFF_BAR = OFF_STG + 32768;
-  static constexpr int SMEM = OFF_BAR + 512 + 1024; // + alignment of the base
-  static constexpr int THREADS = 384;
+  static constexpr int OFF_STG = OFF_KV + NST * TILE;   // 128 output rows in panels of 64 elements
+  static constexpr int OFF_ML = OFF_STG + TILE;         // row maxima and sums, [2 slots][128] float2
+  static constexpr int OFF_BAR = OFF_ML + 2048;
+  static constexpr int SMEM = OFF_BAR + 512;
+  static constexpr int THREADS = 512;
 };
+
+// n / d for 0 <= n < 2^30 by a multiplication: m = ceil(2^(30 + l) / d) with
+// 2^l >= d is exact there (Granlund & Montgomery, "Division by invariant
+// integers using multiplication", 1994).
+struct XtDiv {
+  uint32_t d, m, shift;
+};
+static XtDiv xt_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((1u << l) < d) ++l;
+  return {d, (uint32_t)((((uint64_t)1 << (30 + l)) + d - 1) / d), 30 + l};
+}
+__device__ __forceinline__ int xt_quot(const XtDiv& v, int n) { return (int)(((uint64_t)(uint32_t)n * v.m) >> v.shift); }
 
 struct XtArgs {
   XattnArgs x;
+  XtDiv by_split, by_head, by_hk, by_tiles;   // splits, items of a key head, key heads, query tiles of a head
   int slots;          // query tiles of an item: 1 or 2
   int tiles_per_head; // ceil(Lq / 128)
+  int group, tiles;   // query heads, query tiles of a key head
   int items;
   int qm[2], km[2], vm[2];   // 0 where the batch / head stride is 0 (coordinate 0), else 1
 };
@@ -55,19 +72,18 @@ struct XtItem {
 
 __device__ __forceinline__ XtItem xt_item(const XtArgs& a, int i) {
   XtItem t;
-  const int group = a.x.H / a.x.Hk;
-  const int tiles = group * a.tiles_per_head;
-  const int per_head = (tiles + a.slots - 1) / a.slots;
-  t.split = i % a.x.splits;
-  i /= a.x.splits;
-  const int bh = i / per_head;
-  t.tile0 = (i - bh * per_head) * a.slots;
+  const int tiles = a.tiles;
+  const int i0 = xt_quot(a.by_split, i);
+  t.split = i - i0 * (int)a.by_split.d;
+  const int bh = xt_quot(a.by_head, i0);
+  t.tile0 = (i0 - bh * (int)a.by_head.d) * a.slots;
   t.nslots = min(a.slots, tiles - t.tile0);
-  t.b = bh / a.x.Hk;
-  t.hk = bh - (int)t.b * a.x.Hk;
+  const int b = xt_quot(a.by_hk, bh);
+  t.hk = bh - b * a.x.Hk;
+  t.b = b;
   t.end = xattn_end(a.x, t.b);
   const int kt = (t.end + 127) / 128;
-  const int per = (kt + a.x.splits - 1) / a.x.splits;
+  const int per = xt_quot(a.by_split, kt + a.x.splits - 1);
   const int t0 = min(t.split * per, kt);
   t.nt = min(t0 + per, kt) - t0;
   t.key0 = t0 * 128;
@@ -76,8 +92,8 @@ __device__ __forceinline__ XtItem xt_item(const XtArgs& a, int i) {
 // head and first row of slot s
 __device__ __forceinline__ void xt_slot(const XtArgs& a, const XtItem& t, int s, int& h, int& l0) {
   const int q = t.tile0 + s;
-  const int sub = q / a.tiles_per_head;
-  h = t.hk * (a.x.H / a.x.Hk) + sub;
+  const int sub = xt_quot(a.by_tiles, q);
+  h = t.hk * a.group + sub;
   l0 = (q - sub * a.tiles_per_head) * 128;
 }
 
@@ -171,6 +187,31 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return v;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+  return v;
+}
+// 2^x of two values, x <= 9 or so, on the fp32 pipe: x = n + f with n the
+// nearest integer (read out of the sum with 1.5 * 2^23), 2^f on [-1/2, 1/2] by
+// a degree-4 polynomial of least maximal relative error (2.6e-6, fitted by
+// Lawson's reweighted least squares), times 2^n built from its bits.  Below
+// -126 it stays 2^-126; NaN stays NaN.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  float a, b;
+  untwo(x, a, b);
+  x = two(max_nan(a, -126.f), max_nan(b, -126.f));
+  const uint64_t t = add2(x, two(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, two(-12582912.f, -12582912.f)), two(-1.f, -1.f), x);
+  uint64_t p = two(0.009570102207362652f, 0.009570102207362652f);
+  p = fma2(p, f, two(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
+  untwo(t, a, b);
+  return mul2(p, two(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u),
+                     __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
+}
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ bool all_lanes(bool ok) { return __all_sync(0xffffffffu, ok); }
 
@@ -182,14 +223,17 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NST = C::NST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw;   // no static shared memory: the declared alignment holds
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [2] TMA -> MMA
   uint64_t* q_empty = q_full + 2;       // [2] the item's last S is done -> TMA
   uint64_t* s_full = q_empty + 2;       // [2] S is done -> softmax
-  uint64_t* p_full = s_full + 2;        // [2] P is written, O rescaled -> MMA (4 warps)
+  uint64_t* p_half = s_full + 2;        // [2] P's first 64 keys are written, O rescaled -> MMA (4 warps)
+  uint64_t* p_full = p_half + 2;        // [2] all of P is written -> MMA (4 warps)
   uint64_t* o_full = p_full + 2;        // [2] the item's last P V is done -> epilogue
   uint64_t* o_empty = o_full + 2;       // [2] O is read -> MMA (4 warps)
-  uint64_t* kv_full = o_empty + 2;      // [NST] TMA -> MMA, cleaner
+  uint64_t* l_full = o_empty + 2;       // [2] row maxima and sums are there -> epilogue (4 warps)
+  uint64_t* l_empty = l_full + 2;       // [2] and read -> softmax (4 warps)
+  uint64_t* kv_full = l_empty + 2;      // [NST] TMA -> MMA, cleaner
   uint64_t* kv_empty = kv_full + NST;   // [NST] MMA -> TMA
   uint64_t* ready = kv_empty + NST;     // [NST] cleaner -> MMA
   uint64_t* drain = ready + NST;        // all MMAs are done, at the end
@@ -204,7 +248,10 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
       mbar_init(s_full + i, 1);
+      mbar_init(p_half + i, 4);
       mbar_init(p_full + i, 4);
+      mbar_init(l_full + i, 4);
+      mbar_init(l_empty + i, 4);
       mbar_init(o_full + i, 1);
       mbar_init(o_empty + i, 4);
     }
@@ -233,11 +280,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const uint32_t tmem = uniform(*tmem_slot);
   const bool clean = BIAS || a.x.kv_lens != nullptr;
   const uint32_t kv_base = smem_u32(smem) + C::OFF_KV;
+  float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
 
-  // registers: 384 threads x 168 = 128 x 88 here + 256 x 208 below, where a
-  // thread holds a row of S
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -289,7 +333,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t on = elect_one();
     const int ksteps = (a.x.D + 15) / 16;
     const uint32_t i_pv = idesc_f16(128, ksteps * 16, BF) | (1u << 16);   // B is MN-major
-    uint32_t use = 0, qph = 0, pph = 0, oph = 3;   // a phase bit per slot
+    uint32_t use = 0, qph = 0, hph = 0, pph = 0, oph = 3;   // a phase bit per slot
     const auto tile_wait = [&](uint32_t u) {
       return all_lanes(mbar_wait((clean ? ready : kv_full) + u % NST, (u / NST) & 1u, abort_flag));
     };
@@ -318,18 +362,19 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mma_commit_on(on, s_full + s);
       if (last) mma_commit_on(on, q_empty + s);
     };
-    const auto issue_pv = [&](int s, uint32_t u, int steps, uint32_t accumulate) {
-      const uint64_t dv = smem_desc_mn128(kv_base + (u % NST) * C::TILE);
+    // P V over the steps [k0, k1) of 16 keys: a half of the tile
+    const auto issue_pv = [&](int s, uint32_t u, int k0, int k1, uint32_t accumulate) {
+      const uint64_t dv = smem_desc_mn128(kv_base + (u % NST) * C::TILE) + k0 * (2048 >> 4);
+      const uint32_t pa = tmem + s * 128 + k0 * 8;
       const auto step = [&](int k) {
-        mma_f16_ts_on(on, tmem + 256 + s * 128, tmem + s * 128 + k * 8, dv + k * (2048 >> 4), i_pv,
-                      k > 0 ? 1u : accumulate);
+        mma_f16_ts_on(on, tmem + 256 + s * 128, pa + k * 8, dv + k * (2048 >> 4), i_pv, k > 0 ? 1u : accumulate);
       };
-      if (steps == 8) {
+      if (k1 - k0 == 4) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) step(k);
+        for (int k = 0; k < 4; ++k) step(k);
       } else {
 #pragma unroll 1
-        for (int k = 0; k < steps; ++k) step(k);
+        for (int k = 0; k < k1 - k0; ++k) step(k);
       }
     };
     const auto next_item = [&](int& i, XtItem& t) {
@@ -367,11 +412,15 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         ok = tile_wait(uv);
         for (int s = 0; ok && s < max(t.nslots, n ? nslots : 0); ++s) {
           if (s < t.nslots) {
-            ok = slot_wait(p_full, pph, s);
-            if (ok && j == 0) ok = slot_wait(o_empty, oph, s);
+            if (j == 0) ok = slot_wait(o_empty, oph, s);
+            ok = ok && slot_wait(p_half, hph, s);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(s, uv, pv_steps, j > 0);
+            issue_pv(s, uv, 0, min(pv_steps, 4), j > 0);
+            ok = slot_wait(p_full, pph, s);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(s, uv, 4, pv_steps, 1u);
             if (last) mma_commit_on(on, o_full + s);
           }
           if (n && s < nslots) {
@@ -435,10 +484,95 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
     }
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    // ------------------------------------------------- softmax and epilogue
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------ epilogue
+    const int w = warp & 3;
+    const uint32_t lane_base = (uint32_t)(w * 32) << 16;
+    const bool split = a.x.splits > 1;
+    // this row's 64 elements of a panel, 128B-swizzled; a warp's panels are
+    // 32 rows, one TMA box, each
+    const uint32_t stage_w = smem_u32(smem) + C::OFF_STG + w * 4096;
+    uint8_t* stage = smem + C::OFF_STG + w * 4096 + lane * 128;
+    uint32_t ph[2] = {0, 0};
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
+      const XtItem t = xt_item(a, i);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s >= t.nslots || !ok) continue;
+        int h, l0;
+        xt_slot(a, t, s, h, l0);
+        const int64_t l = l0 + w * 32 + lane;
+        float m = -INFINITY, sum = 0.f;
+        if (t.nt) {
+          ok = all_lanes(mbar_wait(l_full + s, ph[s], abort_flag));
+          if (!ok) continue;
+          const float2 v = ml[s * 128 + w * 32 + lane];
+          m = v.x;
+          sum = v.y;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(l_empty + s);
+          ok = all_lanes(mbar_wait(o_full + s, ph[s], abort_flag));
+          if (!ok) continue;
+          ph[s] ^= 1u;
+          tc_fence_after();
+        }
+        if (!split) {
+          // the last slot's stores have read the staging rows
+          if (lane == 0) bulk_wait_read0();
+          __syncwarp();
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const uint64_t ii = two(inv, inv);
+#pragma unroll 1
+        for (int q = 0; 32 * q < a.x.D; ++q) {
+          uint32_t o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+          if (t.nt) {
+            tmem_ld32(tmem + 256 + s * 128 + lane_base + 32 * q, o);
+            tmem_wait_ld();
+            tie32(o);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (!split) {
+              uint32_t v[4];
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                float lo, hi;
+                untwo(mul2(two(__uint_as_float(o[e + 2 * f]), __uint_as_float(o[e + 2 * f + 1])), ii), lo, hi);
+                v[f] = pack16<T>(lo, hi);
+              }
+              *reinterpret_cast<uint4*>(stage + (q >> 1) * 16384 + ((4 * (q & 1) + e / 8) ^ (lane & 7)) * 16) =
+                  make_uint4(v[0], v[1], v[2], v[3]);
+            } else if (l < a.x.Lq && 32 * q + e < a.x.D) {
+              float v[8];
+#pragma unroll
+              for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
+              xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
+            }
+          }
+        }
+        if (t.nt) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_empty + s);
+        }
+        if (!split) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && l0 + 32 * w < a.x.Lq) {
+            for (int p = 0; 64 * p < a.x.D; ++p)
+              tma_store_4d(&tm_o, stage_w + p * 16384, 64 * p, h, l0 + 32 * w, (int)t.b);
+            bulk_commit();
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait0();   // the stores are done before the CTA leaves
+  } else if (warp < 8) {
+    // ------------------------------------------------------------- softmax
     const int s = warp >> 2, w = warp & 3;
     const uint32_t lane_base = (uint32_t)(w * 32) << 16;
     const uint32_t ts = tmem + s * 128 + lane_base, to = tmem + 256 + s * 128 + lane_base;
@@ -447,16 +581,11 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const float c = a.x.scale == 0.f ? 1.f : fabsf(a.x.scale) * kLog2e;
     const bool odd_scale = !(a.x.scale > 0.f);
     const float sign = a.x.scale < 0.f ? -1.f : 0.f;
-    uint8_t* stage = smem + C::OFF_STG + warp * 4096 + lane * 128;   // this row's 64 elements, 128B-swizzled
-    uint32_t sn = 0, on = 0;
+    uint32_t sn = 0, ln = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
       const XtItem t = xt_item(a, i);
-      if (s >= t.nslots) continue;
-      int h, l0;
-      xt_slot(a, t, s, h, l0);
-      const int64_t l = l0 + w * 32 + lane;
-      const bool row_on = l < a.x.Lq;
+      if (s >= t.nslots || t.nt == 0) continue;
       float m = -INFINITY, sum = 0.f;
       for (int j = 0; j < t.nt; ++j) {
         const int k0 = t.key0 + 128 * j;
@@ -465,169 +594,124 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (!ok) break;
         ++sn;
         tc_fence_after();
-        uint32_t r[4][32];
+        // 64 scores of this row, hidden keys at -inf; with a mask they are
+        // scaled and have their bias already
+        uint32_t r[2][32];
+        const auto load_half = [&](int half) {
+          tmem_ld32(ts + 64 * half, r[0]);
+          tmem_ld32(ts + 64 * half + 32, r[1]);
+          tmem_wait_ld();
+          tie32(r[0]);
+          tie32(r[1]);
+          if (odd_scale) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (32 * q < rem) tmem_ld32(ts + 32 * q, r[q]);
-        tmem_wait_ld();
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tie32(r[q]);
-        if (odd_scale) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) * sign);
-        }
-        if (rem < 128) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * q + e >= rem) r[q][e] = 0xff800000u;   // -inf
-        }
-        float mx;
-        if constexpr (BIAS) {
-          const float4* bias = reinterpret_cast<const float4*>(a.x.bias + t.b * a.x.Lkp + k0);
-          mx = -INFINITY;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 b4 = __ldg(bias + 8 * q + e / 4);
-              const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                const float x = bb[f] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(r[q][e + f]), c, bb[f]);
-                r[q][e + f] = __float_as_uint(x);
-                mx = fmaxf(mx, x);
-              }
-            }
-        } else {
-          float m4[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            m4[q] = __uint_as_float(r[q][0]);
-#pragma unroll
-            for (int e = 1; e < 31; e += 2)
-              m4[q] = fmaxf(fmaxf(m4[q], __uint_as_float(r[q][e])), __uint_as_float(r[q][e + 1]));
-            m4[q] = fmaxf(m4[q], __uint_as_float(r[q][31]));
+              for (int e = 0; e < 32; ++e) r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) * sign);
           }
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+          if (rem < 64 * half + 64) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (32 * q + e >= rem - 64 * half) r[q][e] = 0xff800000u;   // -inf
+          }
+          if constexpr (BIAS) {
+            const float4* bias = reinterpret_cast<const float4*>(a.x.bias + t.b * a.x.Lkp + k0 + 64 * half);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 b4 = __ldg(bias + 8 * q + e / 4);
+                const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                  r[q][e + f] = __float_as_uint(
+                      bb[f] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(r[q][e + f]), c, bb[f]));
+              }
+          }
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (64 * half >= rem) break;
+          load_half(half);
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            m4[0] = fmaxf(fmaxf(m4[0], __uint_as_float(r[0][e])), __uint_as_float(r[0][e + 1]));
+            m4[1] = fmaxf(fmaxf(m4[1], __uint_as_float(r[0][e + 2])), __uint_as_float(r[0][e + 3]));
+            m4[2] = fmaxf(fmaxf(m4[2], __uint_as_float(r[1][e])), __uint_as_float(r[1][e + 1]));
+            m4[3] = fmaxf(fmaxf(m4[3], __uint_as_float(r[1][e + 2])), __uint_as_float(r[1][e + 3]));
+          }
+          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
         }
+        if constexpr (!BIAS) mx *= c;
         if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float nm = mx > m + 8.f ? mx : m;
           const float f = nm == m ? 1.f : ex2(m - nm);
           m = nm;
           sum *= f;
           if (j > 0) {
+#pragma unroll 1
+            for (int q = 0; 32 * q < a.x.D; ++q) {
+              tmem_ld32(to + 32 * q, r[0]);
+              tmem_wait_ld();
+              tie32(r[0]);
 #pragma unroll
-            for (int q = 0; q < DP / 32; ++q) {
-              if (32 * q < a.x.D) {
-                uint32_t o[32];
-                tmem_ld32(to + 32 * q, o);
-                tmem_wait_ld();
-                tie32(o);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(to + 32 * q, o);
-              }
+              for (int e = 0; e < 32; ++e) r[0][e] = __float_as_uint(__uint_as_float(r[0][e]) * f);
+              tmem_st32(to + 32 * q, r[0]);
             }
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
         const uint64_t cc = two(BIAS ? 1.f : c, BIAS ? 1.f : c), rr = two(-ref, -ref);
         uint64_t add[2] = {two(sum, 0.f), two(0.f, 0.f)};
+        // (P of half h covers columns that S's half 0 held: read by then)
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (64 * half < rem) {
+            load_half(half);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (32 * q < rem) {
-            uint32_t p[16];
+            for (int q = 0; q < 2; ++q) {
+              uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const uint64_t x = fma2(two(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1])), cc, rr);
-              float p0, p1;
-              untwo(x, p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
-              add[(e >> 1) & 1] = add2(add[(e >> 1) & 1], two(p0, p1));
-              p[e / 2] = pack16<T>(p0, p1);
+              for (int e = 0; e < 32; e += 2) {
+                uint64_t x = fma2(two(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1])), cc, rr);
+                float p0, p1;
+                // the exponentials would bound this loop (16 a clock per SM):
+                // three of eight pairs go over the fp32 pipe instead
+                if ((e / 2) % 8 == 1 || (e / 2) % 8 == 4 || (e / 2) % 8 == 6) {
+                  x = ex2_poly2(x);
+                  untwo(x, p0, p1);
+                } else {
+                  untwo(x, p0, p1);
+                  p0 = ex2(p0);
+                  p1 = ex2(p1);
+                }
+                add[(e >> 1) & 1] = add2(add[(e >> 1) & 1], two(p0, p1));
+                p[e / 2] = pack16<T>(p0, p1);
+              }
+              tmem_st16(ts + 32 * half + 16 * q, p);
             }
-            tmem_st16(ts + 16 * q, p);
           }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive((half ? p_full : p_half) + s);
         }
         float s0, s1;
         untwo(add2(add[0], add[1]), s0, s1);
         sum = s0 + s1;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + s);
       }
       if (!ok) break;
-      if (t.nt) {
-        ok = all_lanes(mbar_wait(o_full + s, on & 1u, abort_flag));
-        if (!ok) break;
-        ++on;
-        tc_fence_after();
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const uint64_t ii = two(inv, inv);
-#pragma unroll
-      for (int p = 0; p < C::PANELS; ++p) {
-        if (64 * p >= a.x.D) continue;
-        if (a.x.splits == 1) {
-          // this warp's staging rows are free again (its last store has read them)
-          if (lane == 0) bulk_wait_read0();
-          __syncwarp();
-        }
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t o[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-          if (t.nt) {
-            tmem_ld32(to + 64 * p + 32 * q, o);
-            tmem_wait_ld();
-            tie32(o);
-          }
-          if (a.x.splits == 1) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t v[4];
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                float lo, hi;
-                untwo(mul2(two(__uint_as_float(o[e + 2 * f]), __uint_as_float(o[e + 2 * f + 1])), ii), lo, hi);
-                v[f] = pack16<T>(lo, hi);
-              }
-              *reinterpret_cast<uint4*>(stage + ((4 * q + e / 8) ^ (lane & 7)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-          } else if (row_on) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              if (64 * p + 32 * q + e < a.x.D) {
-                float v[8];
-#pragma unroll
-                for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
-                xattn_put<T>(a.x, t.b, l, h, t.split, 64 * p + 32 * q + e, v, m, sum);
-              }
-            }
-          }
-        }
-        if (a.x.splits == 1) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && l0 + 32 * w < a.x.Lq)
-            tma_store_4d(&tm_o, smem_u32(smem) + C::OFF_STG + warp * 4096, 64 * p, h, l0 + 32 * w, (int)t.b);
-          if (lane == 0) bulk_commit();
-        }
-      }
-      if (t.nt) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(o_empty + s);
-      }
+      ok = all_lanes(mbar_wait(l_empty + s, (ln & 1u) ^ 1u, abort_flag));
+      if (!ok) break;
+      ++ln;
+      ml[s * 128 + w * 32 + lane] = make_float2(m, sum);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(l_full + s);
     }
-    if (lane == 0) bulk_wait0();   // the stores are done before the CTA leaves
   }
   __syncthreads();
   if (warp == 9) {
@@ -675,10 +759,17 @@ cudaError_t launch_xattn_tc(const XattnArgs& x, int slots, cudaStream_t st) {
   a.x = x;
   a.slots = slots;
   a.tiles_per_head = (int)((x.Lq + 127) / 128);
-  const int64_t tiles = (int64_t)(x.H / x.Hk) * a.tiles_per_head;
-  const int64_t items = x.B * x.Hk * ((tiles + slots - 1) / slots) * x.splits;
-  if (items > 0x3fffffff) return cudaErrorInvalidValue;
+  a.group = x.H / x.Hk;
+  const int64_t tiles = (int64_t)a.group * a.tiles_per_head;
+  const int64_t per_head = (tiles + slots - 1) / slots;
+  const int64_t items = x.B * x.Hk * per_head * x.splits;
+  if (items + num_sms() >= (1 << 30) || tiles >= (1 << 30)) return cudaErrorInvalidValue;
+  a.tiles = (int)tiles;
   a.items = (int)items;
+  a.by_split = xt_div((uint32_t)x.splits);
+  a.by_head = xt_div((uint32_t)per_head);
+  a.by_hk = xt_div((uint32_t)x.Hk);
+  a.by_tiles = xt_div((uint32_t)a.tiles_per_head);
   CUtensorMap m[4];
   int om[2];
   if (!xt_map(&m[0], BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, 128, a.qm) ||
