@@ -21,6 +21,7 @@ low-rank residual fused), ``lowrank_down`` / ``lowrank_add``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import logging
 import os
 
@@ -699,7 +700,29 @@ def unpack_int4_to_float16(packed: torch.Tensor, scale: torch.Tensor, K: int,
 _MASKS = {torch.bool: L.IC_MASK_BOOL, torch.float16: L.IC_MASK_F16, torch.bfloat16: L.IC_MASK_BF16,
           torch.float32: L.IC_MASK_F32}
 _ROPE = {"interleaved": L.IC_ROPE_INTERLEAVED, "half": L.IC_ROPE_HALF}
-_S3 = ctypes.c_int64 * 12
+_HALF = {torch.float16: L.IC_DTYPE_F16, torch.bfloat16: L.IC_DTYPE_BF16}
+
+# These calls are short on the device, so their host side is kept short too:
+# plain integers for pointers, the raw stream handle, one ctypes array per set
+# of strides.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides12(*strides):
+    return (ctypes.c_int64 * 12)(*strides)
+
+
+def _same_device(what: str, index: int, *ts: torch.Tensor | None) -> None:
+    """All of ``ts`` on CUDA device ``index`` (as ``_need_cuda``)."""
+    if index < 0 or not B200_LIBRARY_LOADED:
+        _need_cuda(what, *ts)
+        raise RuntimeError(f"{what}: intcrush_b200 ops run on CUDA tensors only")
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            _need_cuda(what, *ts)
+            raise RuntimeError(f"{what}: tensors on different devices")
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -723,19 +746,23 @@ def _out_heads(what: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor
 
 
 def _index(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         if t.dtype.is_floating_point or t.dtype == torch.bool:
             raise TypeError(f"an index tensor must hold integers, got {t.dtype}")
         t = t.to(torch.int32)
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _gamma16(what: str, t: torch.Tensor | None, D: int) -> torch.Tensor | None:
     if t is None:
         return None
-    g = _f32c(t.reshape(-1))
-    if g.numel() != D:
-        raise ValueError(f"{what}: gamma has {g.numel()} entries, expected {D}")
+    if t.numel() != D:
+        raise ValueError(f"{what}: gamma has {t.numel()} entries, expected {D}")
+    g = _fp32(t)
     return g.clone() if g.data_ptr() & 15 else g
 
 
@@ -768,12 +795,15 @@ def qk_norm_rope(
     library's device error word.  Returns ``(q, k)`` normalised, or only ``q``
     without a ``k``; ``q_out`` / ``k_out`` may be the inputs themselves.
     """
-    _need_cuda("qk_norm_rope", q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out)
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    index = q.get_device()
+    _same_device("qk_norm_rope", index, q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out)
+    dtype = _HALF.get(q.dtype)
+    if dtype is None:
         raise TypeError(f"qk_norm_rope: q must be float16/bfloat16, got {q.dtype}")
     if q.dim() != 4:
         raise ValueError(f"qk_norm_rope: q must be [batch, tokens, heads, D], got {tuple(q.shape)}")
-    if layout not in _ROPE:
+    form = _ROPE.get(layout)
+    if form is None:
         raise ValueError(f"qk_norm_rope: layout must be 'interleaved' or 'half', got {layout!r}")
     B, T, H, D = q.shape
     rot = rows = 0
@@ -782,32 +812,36 @@ def qk_norm_rope(
     if cos is not None:
         if cos.shape != sin.shape or cos.dim() != 2:
             raise ValueError(f"qk_norm_rope: tables must be [rows, rot / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        cos, sin = _f32c(cos), _f32c(sin)
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
+        cos, sin = _fp32(cos), _fp32(sin)
+        rows, rot = cos.shape
+        rot *= 2
     if positions is not None:
         if positions.shape != (B, T):
             raise ValueError(f"qk_norm_rope: positions must be [{B}, {T}], got {tuple(positions.shape)}")
         positions = _index(positions)
     gq = _gamma16("qk_norm_rope", q_gamma, D)
     x = _heads(q)
-    y = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device) if q_out is None else _out_heads("qk_norm_rope", q_out, q)
+    y = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else _out_heads("qk_norm_rope", q_out, q)
     if k is None:
         if k_gamma is not None or k_out is not None:
             raise ValueError("qk_norm_rope: k_gamma / k_out without a k")
         Hk, xk, yk, gk = 0, None, None, None
-        strides = _S3(*x.stride()[:3], *y.stride()[:3])
+        strides = _strides12(*x.stride()[:3], *y.stride()[:3], 0, 0, 0, 0, 0, 0)
     else:
         if k.dim() != 4 or k.dtype != q.dtype or k.shape[:2] != (B, T) or k.shape[3] != D:
             raise ValueError(f"qk_norm_rope: k must be {q.dtype} [{B}, {T}, heads, {D}], got {k.dtype} {tuple(k.shape)}")
         Hk = k.shape[2]
         gk = _gamma16("qk_norm_rope", k_gamma, D)
         xk = _heads(k)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else _out_heads("qk_norm_rope", k_out, k)
-        strides = _S3(*x.stride()[:3], *y.stride()[:3], *xk.stride()[:3], *yk.stride()[:3])
+        yk = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else _out_heads("qk_norm_rope", k_out, k)
+        strides = _strides12(*x.stride()[:3], *y.stride()[:3], *xk.stride()[:3], *yk.stride()[:3])
     st = L.lib().ic_qk_norm_rope(
-        _p(x), _p(y), H, _p(xk), _p(yk), Hk, _DT[q.dtype], B, T, D, strides, _p(gq), _p(gk), float(eps), _ROPE[layout],
-        rot, _p(cos) if rot else None, _p(sin) if rot else None, rows, _p(positions), _stream(q))
-    L.check(st, "ic_qk_norm_rope")
+        x.data_ptr(), y.data_ptr(), H, None if xk is None else xk.data_ptr(), None if yk is None else yk.data_ptr(), Hk,
+        dtype, B, T, D, strides, None if gq is None else gq.data_ptr(), None if gk is None else gk.data_ptr(), eps, form,
+        rot, cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, rows,
+        None if positions is None else positions.data_ptr(), _raw_stream(index))
+    if st:
+        L.check(st, "ic_qk_norm_rope")
     return y if k is None else (y, yk)
 
 
@@ -832,15 +866,17 @@ def cross_attention(
     keys that are not seen does not matter; a sample that sees none gets
     zeros.  All may be strided views.  Returns [B, Lq, H, D].
     """
-    _need_cuda("cross_attention", q, k, v, kv_lens, key_mask, out)
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    index = q.get_device()
+    _same_device("cross_attention", index, q, k, v, kv_lens, key_mask, out)
+    dtype = _HALF.get(q.dtype)
+    if dtype is None or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"cross_attention: q, k and v must share one dtype, float16 or bfloat16, got {q.dtype}, "
                         f"{k.dtype}, {v.dtype}")
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError(f"cross_attention: q must be [B, Lq, H, D], k and v [B, Lk, Hk, D], got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1], k.shape[2]
+    _, Lk, Hk, _ = k.shape
     if kv_lens is not None:
         if kv_lens.shape != (B,):
             raise ValueError(f"cross_attention: kv_lens must be [{B}], got {tuple(kv_lens.shape)}")
@@ -858,24 +894,28 @@ def cross_attention(
         if 0 < ld < Lk:
             key_mask = key_mask.contiguous()
             ld = Lk
+    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _out_heads("cross_attention", out, q)
     q, k, v = _heads(q), _heads(k), _heads(v)
-    y = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device) if out is None else _out_heads("cross_attention", out, q)
     lib = L.lib()
     n = lib.ic_cross_attention_workspace(B, Lq, Lk, H, Hk, D, kind)
     if n < 0:
         L.check(L.IC_ERR_ARG, "ic_cross_attention")
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     st = lib.ic_cross_attention(
-        _p(q), _p(k), _p(v), _p(y), _DT[q.dtype], B, Lq, Lk, H, Hk, D,
-        _S3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3]),
-        float(D ** -0.5 if scale is None else scale), _p(kv_lens), _p(key_mask), kind, ld, _p(ws), n, _stream(q))
-    L.check(st, "ic_cross_attention")
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dtype, B, Lq, Lk, H, Hk, D,
+        _strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3]),
+        D ** -0.5 if scale is None else scale, None if kv_lens is None else kv_lens.data_ptr(),
+        None if key_mask is None else key_mask.data_ptr(), kind, ld, None if ws is None else ws.data_ptr(), n,
+        _raw_stream(index))
+    if st:
+        L.check(st, "ic_cross_attention")
     return y
 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """``t`` as a [rows, width] matrix with contiguous rows."""
-    t = t.reshape(-1, width)
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
     return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
 
 
@@ -901,9 +941,11 @@ def lora_batched(
     word.  (One adapter for all rows: :func:`lowrank_down` /
     :func:`lowrank_add`, ``_ops.py:236-244``.)
     """
-    _need_cuda("lora_batched", x, down, up, ids, scales, base, out)
+    index = x.get_device()
+    _same_device("lora_batched", index, x, down, up, ids, scales, base, out)
     dt = x.dtype
-    if dt not in (torch.float16, torch.bfloat16) or down.dtype != dt or up.dtype != dt:
+    dtype = _HALF.get(dt)
+    if dtype is None or down.dtype != dt or up.dtype != dt:
         raise TypeError(f"lora_batched: x, down and up must share one dtype, float16 or bfloat16, got {dt}, {down.dtype}, "
                         f"{up.dtype}")
     if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2]:
@@ -912,30 +954,31 @@ def lora_batched(
     N = up.shape[1]
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"lora_batched: x has {tuple(x.shape)[-1:]} columns, expected {K}")
-    lead = x.shape[:-1]
+    full = (*x.shape[:-1], N)
     x2 = _rows(x, K)
     M = x2.shape[0]
     S = ids.numel()
     if (S == 0) != (M == 0) or (S and M % S):
         raise ValueError(f"lora_batched: {S} adapter ids do not divide {M} rows")
-    ids = _index(ids.reshape(-1))
+    ids = _index(ids)
     if scales is not None:
-        scales = _f32c(scales.reshape(-1))
         if scales.numel() != n:
             raise ValueError(f"lora_batched: {scales.numel()} scales for {n} adapters")
+        scales = _fp32(scales)
     b2 = None
     if base is not None:
-        if base.dtype != dt or base.shape != (*lead, N):
-            raise ValueError(f"lora_batched: base must be {dt} {(*lead, N)}, got {base.dtype} {tuple(base.shape)}")
+        if base.dtype != dt or base.shape != full:
+            raise ValueError(f"lora_batched: base must be {dt} {full}, got {base.dtype} {tuple(base.shape)}")
         b2 = _rows(base, N)
     if out is None:
-        out = torch.empty((*lead, N), dtype=dt, device=x.device)
-        o2 = out.view(-1, N) if M else out
+        out = torch.empty(full, dtype=dt, device=x.device)
+        ldo = N
     else:
-        if out.dtype != dt or out.shape != (*lead, N):
-            raise ValueError(f"lora_batched: out must be {dt} {(*lead, N)}, got {out.dtype} {tuple(out.shape)}")
-        o2 = out.view(-1, N)   # raises where the leading dimensions do not fold
-        if o2.stride(1) != 1 or (M > 1 and o2.stride(0) < N):
+        if out.dtype != dt or out.shape != full:
+            raise ValueError(f"lora_batched: out must be {dt} {full}, got {out.dtype} {tuple(out.shape)}")
+        o2 = out.view(-1, N) if M and N else out   # raises where the leading dimensions do not fold
+        ldo = o2.stride(0) if M > 1 else N
+        if N and (o2.stride(1) != 1 or ldo < N):
             raise ValueError(f"lora_batched: out must be row-major, got strides {out.stride()}")
     if M == 0 or N == 0:
         return out
@@ -944,14 +987,16 @@ def lora_batched(
     if need < 0:
         L.check(L.IC_ERR_ARG, "ic_lora_batched")
     ws = torch.empty(need, dtype=torch.float32, device=x.device)
-    down, up = down.contiguous(), up.contiguous()
-    ldx, ldo, ldb = x2.stride(0), o2.stride(0), 0 if b2 is None else b2.stride(0)
-    if M == 1:   # a lone row's stride says nothing
-        ldx, ldo, ldb = K, N, N
+    if not down.is_contiguous():
+        down = down.contiguous()
+    if not up.is_contiguous():
+        up = up.contiguous()
     st = lib.ic_lora_batched(
-        _p(x2), _DT[dt], M, K, ldx, _p(down), _p(up), R, n, _p(ids), M // S, _p(scales), _p(b2), ldb, _p(o2), N, ldo,
-        _p(ws), need, _stream(x))
-    L.check(st, "ic_lora_batched")
+        x2.data_ptr(), dtype, M, K, x2.stride(0) if M > 1 else K, down.data_ptr(), up.data_ptr(), R, n, ids.data_ptr(),
+        M // S, None if scales is None else scales.data_ptr(), None if b2 is None else b2.data_ptr(),
+        N if b2 is None or M == 1 else b2.stride(0), out.data_ptr(), N, ldo, ws.data_ptr(), need, _raw_stream(index))
+    if st:
+        L.check(st, "ic_lora_batched")
     return out
 
 

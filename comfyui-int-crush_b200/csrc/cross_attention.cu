@@ -370,7 +370,10 @@ static cudaError_t launch_xattn_t(const XattnArgs& a, int slots, cudaStream_t st
 cudaError_t launch_cross_attention(XattnArgs a, int dtype, const void* mask, int mask_kind, int64_t ld_mask,
                                    float* workspace, cudaStream_t st) {
   if (a.B == 0 || a.Lq == 0) return cudaSuccess;
-  const XattnPlan p = xattn_plan(a.B, a.Lq, a.Lk, a.H, a.Hk, a.D, mask_kind);
+  XattnPlan p = xattn_plan(a.B, a.Lq, a.Lk, a.H, a.Hk, a.D, mask_kind);
+  // the tcgen05 kernel takes row maxima before the scale: only with a positive
+  // one.  Others are nobody's ordinary call: the few-rows kernel, unsplit.
+  if (p.slots && !(a.scale > 0.f)) p.slots = 0, p.splits = 1;
   a.splits = p.splits;
   a.Lkp = p.Lkp;
   a.part_o = workspace;

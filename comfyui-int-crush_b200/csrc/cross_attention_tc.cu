@@ -3,7 +3,7 @@
 // Persistent, one CTA per SM, 16 warps.  A work item is one key head of one
 // sample with one or two tiles of 128 query rows ("slots"; the slots share the
 // K and V tiles), over the item's part of the keys in tiles of 128:
-//   S_s = Q_s K^T            128 x 128, both operands in shared memory
+//   S_s = Q_s K^T            128 x 128 into tensor memory
 //   P_s = 2^(S_s c - m)      registers, written back over S_s as 16-bit pairs
 //   O_s += P_s V             A operand from tensor memory, V as it lies in
 //                            memory (rows = keys: the MN-major B operand)
@@ -13,16 +13,15 @@
 // Warp 8: TMA producer (Q slots, a ring of K and V tiles).  Warp 9: MMA
 // issuer.  Warp 10: zeroes the V rows of keys that are not seen (P is 0 there,
 // but 0 * NaN is not) when there are lengths or a mask.  Warps 12-15: O out of
-// tensor memory, over the row sums, through shared memory to a TMA store.
+// tensor memory, over the row sums, to global memory.
 // The MMAs of one slot run while the other slot's softmax does; P V starts when
-// half of P is written; the next item's first S is issued behind the last P V,
-// so that nothing drains between items.
+// three quarters of P are written; the next item's first S is issued behind the
+// last P V, so that nothing drains between items.
 //
 // S, the running maximum, the row sum and O are fp32.  The maximum moves only
 // when it grows by more than 2^8 (P stays below 2^8 and the sums exact), so O
-// is rescaled in tensor memory on few tiles; P V of the tile before is
-// complete then, because S of this tile was issued behind it.  P is rounded
-// to the activation type (the MMA's operand type), the row sum is not.
+// is rescaled in tensor memory on few tiles.  P is rounded to the activation
+// type (the MMA's operand type), the row sum is not.
 #include "cross_attention.cuh"
 
 #include <type_traits>
@@ -33,10 +32,9 @@ template <int DP>
 struct XtCfg {
   static constexpr int PANELS = DP / 64;            // 64-element panels of 128 rows, 128B-swizzled
   static constexpr int TILE = PANELS * 16384;
-  static constexpr int NST = DP == 128 ? 4 : 8;     // ring stages (K and V tiles in turn)
+  static constexpr int NST = DP == 128 ? 5 : 8;     // ring stages (K and V tiles in turn)
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_STG = OFF_KV + NST * TILE;   // 128 output rows in panels of 64 elements
-  static constexpr int OFF_ML = OFF_STG + TILE;         // row maxima and sums, [2 slots][128] float2
+  static constexpr int OFF_ML = OFF_KV + NST * TILE;   // row maxima and sums, [2 slots][128] float2
   static constexpr int OFF_BAR = OFF_ML + 2048;
   static constexpr int SMEM = OFF_BAR + 512;
   static constexpr int THREADS = 512;
@@ -61,6 +59,7 @@ struct XtArgs {
   int slots;          // query tiles of an item: 1 or 2
   int tiles_per_head; // ceil(Lq / 128)
   int group, tiles;   // query heads, query tiles of a key head
+  int wide;           // output rows take 32-byte stores
   int items;
   int qm[2], km[2], vm[2];   // 0 where the batch / head stride is 0 (coordinate 0), else 1
 };
@@ -155,10 +154,10 @@ __device__ __forceinline__ void mma_commit_on(uint32_t on, uint64_t* bar) {
       : "memory");
 }
 
-// Box store shared -> global, clipped at the tensor's edges.
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-               ::"l"(reinterpret_cast<uint64_t>(m)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+// 32 bytes at once (32-byte aligned)
+__device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
 
@@ -187,38 +186,13 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return v;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float v;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
-  return v;
-}
-// 2^x of two values, x <= 9 or so, on the fp32 pipe: x = n + f with n the
-// nearest integer (read out of the sum with 1.5 * 2^23), 2^f on [-1/2, 1/2] by
-// a degree-4 polynomial of least maximal relative error (2.6e-6, fitted by
-// Lawson's reweighted least squares), times 2^n built from its bits.  Below
-// -126 it stays 2^-126; NaN stays NaN.
-__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
-  float a, b;
-  untwo(x, a, b);
-  x = two(max_nan(a, -126.f), max_nan(b, -126.f));
-  const uint64_t t = add2(x, two(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, two(-12582912.f, -12582912.f)), two(-1.f, -1.f), x);
-  uint64_t p = two(0.009570102207362652f, 0.009570102207362652f);
-  p = fma2(p, f, two(0.05591785907745361f, 0.05591785907745361f));
-  p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
-  untwo(t, a, b);
-  return mul2(p, two(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u),
-                     __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
-}
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ bool all_lanes(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(XtCfg<DP>::THREADS, 1)
 xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const XtArgs a) {
+                const __grid_constant__ CUtensorMap tm_v, const XtArgs a) {
   using C = XtCfg<DP>;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NST = C::NST;
@@ -227,8 +201,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [2] TMA -> MMA
   uint64_t* q_empty = q_full + 2;       // [2] the item's last S is done -> TMA
   uint64_t* s_full = q_empty + 2;       // [2] S is done -> softmax
-  uint64_t* p_half = s_full + 2;        // [2] P's first 64 keys are written, O rescaled -> MMA (4 warps)
-  uint64_t* p_full = p_half + 2;        // [2] all of P is written -> MMA (4 warps)
+  uint64_t* p_part = s_full + 2;        // [2] P's first 96 keys are written, O rescaled -> MMA (4 warps)
+  uint64_t* p_full = p_part + 2;        // [2] all of P is written -> MMA (4 warps)
   uint64_t* o_full = p_full + 2;        // [2] the item's last P V is done -> epilogue
   uint64_t* o_empty = o_full + 2;       // [2] O is read -> MMA (4 warps)
   uint64_t* l_full = o_empty + 2;       // [2] row maxima and sums are there -> epilogue (4 warps)
@@ -248,7 +222,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
       mbar_init(s_full + i, 1);
-      mbar_init(p_half + i, 4);
+      mbar_init(p_part + i, 4);
       mbar_init(p_full + i, 4);
       mbar_init(l_full + i, 4);
       mbar_init(l_empty + i, 4);
@@ -272,7 +246,6 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
-    prefetch_tmap(&tm_o);
   }
   tc_fence_before();
   __syncthreads();
@@ -281,7 +254,18 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const bool clean = BIAS || a.x.kv_lens != nullptr;
   const uint32_t kv_base = smem_u32(smem) + C::OFF_KV;
   float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  const auto next_item = [&](int& i, XtItem& t) {
+    for (; i < a.items; i += gridDim.x) {
+      t = xt_item(a, i);
+      if (t.nt) return true;
+    }
+    return false;
+  };
 
+  // registers: 512 threads x 128 = 256 x 72 here + 256 x 184 below, where a
+  // thread holds a row of S
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -310,9 +294,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         ++qn[s];
         return true;
       };
-      for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
-        const XtItem t = xt_item(a, i);
-        if (t.nt == 0) continue;
+      XtItem t;
+      for (int i = blockIdx.x; ok && next_item(i, t); i += gridDim.x) {
         // K first: its stage frees before the Q slots of the item before
         ok = load_kv(&tm_k, t, a.km, t.key0) && load_q(t, 0) && (t.nslots < 2 || load_q(t, 1)) &&
              load_kv(&tm_v, t, a.vm, t.key0);
@@ -362,34 +345,31 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mma_commit_on(on, s_full + s);
       if (last) mma_commit_on(on, q_empty + s);
     };
-    // P V over the steps [k0, k1) of 16 keys: a half of the tile
+    // P V over the steps [k0, k1) of 16 keys
     const auto issue_pv = [&](int s, uint32_t u, int k0, int k1, uint32_t accumulate) {
       const uint64_t dv = smem_desc_mn128(kv_base + (u % NST) * C::TILE) + k0 * (2048 >> 4);
       const uint32_t pa = tmem + s * 128 + k0 * 8;
       const auto step = [&](int k) {
         mma_f16_ts_on(on, tmem + 256 + s * 128, pa + k * 8, dv + k * (2048 >> 4), i_pv, k > 0 ? 1u : accumulate);
       };
-      if (k1 - k0 == 4) {
+      if (k1 - k0 == 6) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) step(k);
+        for (int k = 0; k < 6; ++k) step(k);
       } else {
 #pragma unroll 1
         for (int k = 0; k < k1 - k0; ++k) step(k);
       }
     };
-    const auto next_item = [&](int& i, XtItem& t) {
-      for (; i < a.items; i += gridDim.x) {
-        t = xt_item(a, i);
-        t.end = uniform(t.end);
-        t.nt = uniform(t.nt);
-        t.key0 = uniform(t.key0);
-        if (t.nt) return true;
-      }
-      return false;
+    const auto next_uniform = [&](int& i, XtItem& t) {
+      const bool got = next_item(i, t);
+      t.end = uniform(t.end);
+      t.nt = uniform(t.nt);
+      t.key0 = uniform(t.key0);
+      return all_lanes(got);
     };
     int i = blockIdx.x;
     XtItem t, nx;
-    bool have = next_item(i, t), ok = true;
+    bool have = next_uniform(i, t), ok = true;
     if (have) {
       ok = tile_wait(use);
       for (int s = 0; ok && s < t.nslots; ++s) {
@@ -397,38 +377,38 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (ok) issue_s(s, use, width(t, 0), t.nt == 1);
       }
       if (ok) mma_commit_on(on, kv_empty + use % NST);
-      ++use;   // now at V of tile 0
+      ++use;
     }
     while (have && ok) {
       i += gridDim.x;
-      const bool more = next_item(i, nx);
+      const bool more = next_uniform(i, nx);
       for (int j = 0; ok && j < t.nt; ++j) {
         const bool last = j == t.nt - 1;
         const uint32_t uv = use, uk = use + 1;   // V of this tile, the K tile after it
         const int n = last ? (more ? width(nx, 0) : 0) : width(t, j + 1);
-        const int nslots = last && more ? nx.nslots : t.nslots;   // slots whose next S uses uk
-        const int pv_steps = width(t, j) / 16;
-        bool k_seen = false;
+        const int nslots = n ? (last ? nx.nslots : t.nslots) : 0;   // slots whose next S uses uk
+        const int steps = width(t, j) / 16;
         ok = tile_wait(uv);
-        for (int s = 0; ok && s < max(t.nslots, n ? nslots : 0); ++s) {
+        for (int s = 0; ok && s < max(t.nslots, nslots); ++s) {
+          // everything that the next S needs first, so that it follows P V at once
+          if (s < nslots) {
+            if (s == 0) ok = tile_wait(uk);
+            if (ok && last) ok = slot_wait(q_full, qph, s);
+            if (!ok) break;
+          }
           if (s < t.nslots) {
             if (j == 0) ok = slot_wait(o_empty, oph, s);
-            ok = ok && slot_wait(p_half, hph, s);
+            ok = ok && slot_wait(p_part, hph, s);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(s, uv, 0, min(pv_steps, 4), j > 0);
+            issue_pv(s, uv, 0, min(steps, 6), j > 0);
             ok = slot_wait(p_full, pph, s);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(s, uv, 4, pv_steps, 1u);
+            issue_pv(s, uv, 6, steps, 1u);
             if (last) mma_commit_on(on, o_full + s);
           }
-          if (n && s < nslots) {
-            if (!k_seen) ok = tile_wait(uk);
-            k_seen = true;
-            if (ok && last) ok = slot_wait(q_full, qph, s);
-            if (ok) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
-          }
+          if (s < nslots) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
         }
         if (!ok) break;
         mma_commit_on(on, kv_empty + uv % NST);
@@ -448,14 +428,22 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (clean) {
       uint32_t use = 0;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
-        const XtItem t = xt_item(a, i);
-        for (int j = 0; ok && j < 2 * t.nt; ++j, ++use) {
-          const uint32_t st = use % NST;
-          ok = all_lanes(mbar_wait(kv_full + st, (use / NST) & 1u, abort_flag));
+      const auto pass = [&](bool got) {   // the tile may be used
+        __syncwarp();
+        if (got && lane == 0) mbar_arrive(ready + use % NST);
+        ++use;
+        return got;
+      };
+      const auto landed = [&]() { return all_lanes(mbar_wait(kv_full + use % NST, (use / NST) & 1u, abort_flag)); };
+      XtItem t;
+      for (int i = blockIdx.x; ok && next_item(i, t); i += gridDim.x) {
+        for (int j = 0; ok && j < t.nt; ++j) {
+          ok = pass(landed());   // a K tile
+          ok = ok && landed();
           if (!ok) break;
-          if (j & 1) {   // a V tile
-            const int k0 = t.key0 + 64 * (j & ~1);
+          const uint32_t st = use % NST;
+          {
+            const int k0 = t.key0 + 128 * j;
             const int rows = min(128, (t.end - k0 + 15) / 16 * 16);   // rows that the MMA reads
             unsigned hide[4];
 #pragma unroll
@@ -479,8 +467,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               fence_proxy_async_smem();
             }
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(ready + st);
+          pass(true);
         }
       }
     }
@@ -489,10 +476,6 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int w = warp & 3;
     const uint32_t lane_base = (uint32_t)(w * 32) << 16;
     const bool split = a.x.splits > 1;
-    // this row's 64 elements of a panel, 128B-swizzled; a warp's panels are
-    // 32 rows, one TMA box, each
-    const uint32_t stage_w = smem_u32(smem) + C::OFF_STG + w * 4096;
-    uint8_t* stage = smem + C::OFF_STG + w * 4096 + lane * 128;
     uint32_t ph[2] = {0, 0};
     bool ok = true;
     for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
@@ -517,11 +500,6 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           ph[s] ^= 1u;
           tc_fence_after();
         }
-        if (!split) {
-          // the last slot's stores have read the staging rows
-          if (lane == 0) bulk_wait_read0();
-          __syncwarp();
-        }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const uint64_t ii = two(inv, inv);
 #pragma unroll 1
@@ -534,53 +512,54 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tmem_wait_ld();
             tie32(o);
           }
+          if (l >= a.x.Lq) {
+            // past the sample's rows
+          } else if (split) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (!split) {
-              uint32_t v[4];
+            for (int e = 0; e < 32; e += 8) {
+              if (32 * q + e < a.x.D) {
+                float v[8];
 #pragma unroll
-              for (int f = 0; f < 4; ++f) {
+                for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
+                xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
+              }
+            }
+          } else {
+            T* row = reinterpret_cast<T*>(a.x.o) + t.b * a.x.os[0] + l * a.x.os[1] + h * a.x.os[2] + 32 * q;
+#pragma unroll
+            for (int e = 0; e < 32; e += 16) {
+              uint32_t v[8];
+#pragma unroll
+              for (int f = 0; f < 8; ++f) {
                 float lo, hi;
                 untwo(mul2(two(__uint_as_float(o[e + 2 * f]), __uint_as_float(o[e + 2 * f + 1])), ii), lo, hi);
                 v[f] = pack16<T>(lo, hi);
               }
-              *reinterpret_cast<uint4*>(stage + (q >> 1) * 16384 + ((4 * (q & 1) + e / 8) ^ (lane & 7)) * 16) =
-                  make_uint4(v[0], v[1], v[2], v[3]);
-            } else if (l < a.x.Lq && 32 * q + e < a.x.D) {
-              float v[8];
-#pragma unroll
-              for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
-              xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
+              if (a.wide) {
+                if (32 * q + e < a.x.D) st_global32(row + e, v);
+              } else {
+                if (32 * q + e < a.x.D) *reinterpret_cast<uint4*>(row + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                if (32 * q + e + 8 < a.x.D) *reinterpret_cast<uint4*>(row + e + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+              }
             }
           }
+          __syncwarp();   // the next tcgen05.ld is the whole warp's
         }
         if (t.nt) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(o_empty + s);
         }
-        if (!split) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && l0 + 32 * w < a.x.Lq) {
-            for (int p = 0; 64 * p < a.x.D; ++p)
-              tma_store_4d(&tm_o, stage_w + p * 16384, 64 * p, h, l0 + 32 * w, (int)t.b);
-            bulk_commit();
-          }
-        }
       }
     }
-    if (lane == 0) bulk_wait0();   // the stores are done before the CTA leaves
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------- softmax
     const int s = warp >> 2, w = warp & 3;
     const uint32_t lane_base = (uint32_t)(w * 32) << 16;
     const uint32_t ts = tmem + s * 128 + lane_base, to = tmem + 256 + s * 128 + lane_base;
-    // scores in units of log2: S * c; a scale that is not positive is taken
-    // out of S first, so that the maximum and -inf for hidden keys stay right
-    const float c = a.x.scale == 0.f ? 1.f : fabsf(a.x.scale) * kLog2e;
-    const bool odd_scale = !(a.x.scale > 0.f);
-    const float sign = a.x.scale < 0.f ? -1.f : 0.f;
+    const float c = a.x.scale * kLog2e;   // > 0: scores in units of log2 are S c
     uint32_t sn = 0, ln = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
@@ -594,59 +573,66 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (!ok) break;
         ++sn;
         tc_fence_after();
-        // 64 scores of this row, hidden keys at -inf; with a mask they are
-        // scaled and have their bias already
-        uint32_t r[2][32];
-        const auto load_half = [&](int half) {
-          tmem_ld32(ts + 64 * half, r[0]);
-          tmem_ld32(ts + 64 * half + 32, r[1]);
-          tmem_wait_ld();
-          tie32(r[0]);
-          tie32(r[1]);
-          if (odd_scale) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) * sign);
-          }
-          if (rem < 64 * half + 64) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (32 * q + e >= rem - 64 * half) r[q][e] = 0xff800000u;   // -inf
-          }
-          if constexpr (BIAS) {
-            const float4* bias = reinterpret_cast<const float4*>(a.x.bias + t.b * a.x.Lkp + k0 + 64 * half);
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const float4 b4 = __ldg(bias + 8 * q + e / 4);
-                const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-                for (int f = 0; f < 4; ++f)
-                  r[q][e + f] = __float_as_uint(
-                      bb[f] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(r[q][e + f]), c, bb[f]));
-              }
-          }
-        };
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          if (64 * half >= rem) break;
-          load_half(half);
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t r[4][32];
+        tmem_ld32(ts, r[0]);
+        tmem_ld32(ts + 32, r[1]);
+        tmem_wait_ld();
+        tie32(r[0]);
+        tie32(r[1]);
+        tmem_ld32(ts + 64, r[2]);
+        tmem_ld32(ts + 96, r[3]);
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const auto maxima = [&](int q) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            m4[0] = fmaxf(fmaxf(m4[0], __uint_as_float(r[0][e])), __uint_as_float(r[0][e + 1]));
-            m4[1] = fmaxf(fmaxf(m4[1], __uint_as_float(r[0][e + 2])), __uint_as_float(r[0][e + 3]));
-            m4[2] = fmaxf(fmaxf(m4[2], __uint_as_float(r[1][e])), __uint_as_float(r[1][e + 1]));
-            m4[3] = fmaxf(fmaxf(m4[3], __uint_as_float(r[1][e + 2])), __uint_as_float(r[1][e + 3]));
+            m4[2 * (q & 1)] = fmaxf(fmaxf(m4[2 * (q & 1)], __uint_as_float(r[q][e])), __uint_as_float(r[q][e + 1]));
+            m4[2 * (q & 1) + 1] = fmaxf(fmaxf(m4[2 * (q & 1) + 1], __uint_as_float(r[q][e + 2])), __uint_as_float(r[q][e + 3]));
           }
-          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        };
+        if (!BIAS && rem >= 128) {
+          maxima(0);
+          maxima(1);
+        }
+        tmem_wait_ld();
+        tie32(r[2]);
+        tie32(r[3]);
+        if (rem < 128) {
+          // columns past the keys: whatever the tile held
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t keep = rem >= 32 * q + 32 ? 0xffffffffu : rem <= 32 * q ? 0u : (1u << (rem - 32 * q)) - 1u;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[q][e] = (keep >> e) & 1u ? r[q][e] : 0xff800000u;   // -inf
+          }
+          if constexpr (!BIAS) {
+            maxima(0);
+            maxima(1);
+          }
+        }
+        float mx;
+        if constexpr (BIAS) {
+          const float4* bias = reinterpret_cast<const float4*>(a.x.bias + t.b * a.x.Lkp + k0);
+          mx = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 b4 = __ldg(bias + 8 * q + e / 4);
+              const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                const float x = bb[f] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(r[q][e + f]), c, bb[f]);
+                r[q][e + f] = __float_as_uint(x);
+                mx = fmaxf(mx, x);
+              }
+            }
+        } else {
+          maxima(2);
+          maxima(3);
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         }
         if constexpr (!BIAS) mx *= c;
+        // (P V of the tile before is done: this S was issued behind it)
         if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float nm = mx > m + 8.f ? mx : m;
           const float f = nm == m ? 1.f : ex2(m - nm);
@@ -654,52 +640,54 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sum *= f;
           if (j > 0) {
 #pragma unroll 1
-            for (int q = 0; 32 * q < a.x.D; ++q) {
-              tmem_ld32(to + 32 * q, r[0]);
+            for (int q = 0; 16 * q < a.x.D; ++q) {
+              uint32_t o[16];
+              tmem_ld16(to + 16 * q, o);
               tmem_wait_ld();
-              tie32(r[0]);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[0][e] = __float_as_uint(__uint_as_float(r[0][e]) * f);
-              tmem_st32(to + 32 * q, r[0]);
+              for (int e = 0; e < 16; ++e) {
+                asm volatile("" : "+r"(o[e]));   // valid after the wait
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              }
+              tmem_st16(to + 16 * q, o);
             }
+            tmem_wait_st();
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
         const uint64_t cc = two(BIAS ? 1.f : c, BIAS ? 1.f : c), rr = two(-ref, -ref);
         uint64_t add[2] = {two(sum, 0.f), two(0.f, 0.f)};
-        // (P of half h covers columns that S's half 0 held: read by then)
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          if (64 * half < rem) {
-            load_half(half);
+        // 32 columns at a time; a block's exponentials are issued ahead of the
+        // sums and the packing of the block before, which fill their latency
+        const auto finish = [&](int q) {
+          uint32_t p[16];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t p[16];
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                uint64_t x = fma2(two(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1])), cc, rr);
-                float p0, p1;
-                // the exponentials would bound this loop (16 a clock per SM):
-                // three of eight pairs go over the fp32 pipe instead
-                if ((e / 2) % 8 == 1 || (e / 2) % 8 == 4 || (e / 2) % 8 == 6) {
-                  x = ex2_poly2(x);
-                  untwo(x, p0, p1);
-                } else {
-                  untwo(x, p0, p1);
-                  p0 = ex2(p0);
-                  p1 = ex2(p1);
-                }
-                add[(e >> 1) & 1] = add2(add[(e >> 1) & 1], two(p0, p1));
-                p[e / 2] = pack16<T>(p0, p1);
-              }
-              tmem_st16(ts + 32 * half + 16 * q, p);
-            }
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = __uint_as_float(r[q][e]), p1 = __uint_as_float(r[q][e + 1]);
+            add[(e >> 1) & 1] = add2(add[(e >> 1) & 1], two(p0, p1));
+            p[e / 2] = pack16<T>(p0, p1);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive((half ? p_full : p_half) + s);
+          tmem_st16(ts + 16 * q, p);
+          if (q >= 2) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive((q == 3 ? p_full : p_part) + s);
+          }
+        };
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t x = fma2(two(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1])), cc, rr);
+            float p0, p1;
+            untwo(x, p0, p1);
+            r[q][e] = __float_as_uint(ex2(p0));
+            r[q][e + 1] = __float_as_uint(ex2(p1));
+          }
+          if (q > 0) finish(q - 1);
         }
+        finish(3);
         float s0, s1;
         untwo(add2(add[0], add[1]), s0, s1);
         sum = s0 + s1;
@@ -725,7 +713,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // entry that every coordinate maps to; a dimension of one entry takes any
 // stride.
 static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, int64_t D, int64_t heads, int64_t tokens,
-                   int64_t batch, uint32_t rows, int* mul) {
+                   int64_t batch, int* mul) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   mul[0] = st[0] == 0 ? 0 : 1;
@@ -735,7 +723,7 @@ static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, in
   const int64_t el[3] = {st[2], st[1], st[0]};
   cuuint64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 * ((cuuint64_t)D / 8) : (cuuint64_t)el[i] * 2;
-  cuuint32_t box[4] = {64, 1, rows, 1};
+  cuuint32_t box[4] = {64, 1, 128, 1};
   cuuint32_t one[4] = {1, 1, 1, 1};
   return fn(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), dims,
             strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -743,12 +731,12 @@ static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, in
 }
 
 template <typename T, int DP, bool BIAS>
-static cudaError_t launch_xt(const CUtensorMap (&m)[4], const XtArgs& a, cudaStream_t st) {
+static cudaError_t launch_xt(const CUtensorMap (&m)[3], const XtArgs& a, cudaStream_t st) {
   auto kern = xattn_tc_kernel<T, DP, BIAS>;
   const cudaError_t e = set_smem_once(kern, XtCfg<DP>::SMEM);
   if (e != cudaSuccess) return e;
   const int grid = a.items < num_sms() ? a.items : num_sms();
-  kern<<<grid, XtCfg<DP>::THREADS, XtCfg<DP>::SMEM, st>>>(m[0], m[1], m[2], m[3], a);
+  kern<<<grid, XtCfg<DP>::THREADS, XtCfg<DP>::SMEM, st>>>(m[0], m[1], m[2], a);
   return cudaGetLastError();
 }
 
@@ -766,16 +754,16 @@ cudaError_t launch_xattn_tc(const XattnArgs& x, int slots, cudaStream_t st) {
   if (items + num_sms() >= (1 << 30) || tiles >= (1 << 30)) return cudaErrorInvalidValue;
   a.tiles = (int)tiles;
   a.items = (int)items;
+  a.wide = x.D % 16 == 0 && (reinterpret_cast<uintptr_t>(x.o) & 31) == 0 && x.os[0] % 16 == 0 && x.os[1] % 16 == 0 &&
+           x.os[2] % 16 == 0;
   a.by_split = xt_div((uint32_t)x.splits);
   a.by_head = xt_div((uint32_t)per_head);
   a.by_hk = xt_div((uint32_t)x.Hk);
   a.by_tiles = xt_div((uint32_t)a.tiles_per_head);
-  CUtensorMap m[4];
-  int om[2];
-  if (!xt_map(&m[0], BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, 128, a.qm) ||
-      !xt_map(&m[1], BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, 128, a.km) ||
-      !xt_map(&m[2], BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, 128, a.vm) ||
-      !xt_map(&m[3], BF, x.o, x.os, x.D, x.H, x.Lq, x.B, 32, om))
+  CUtensorMap m[3];
+  if (!xt_map(&m[0], BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, a.qm) ||
+      !xt_map(&m[1], BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, a.km) ||
+      !xt_map(&m[2], BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, a.vm))
     return cudaErrorInvalidValue;
   if (x.D <= 64) return x.bias ? launch_xt<T, 64, true>(m, a, st) : launch_xt<T, 64, false>(m, a, st);
   return x.bias ? launch_xt<T, 128, true>(m, a, st) : launch_xt<T, 128, false>(m, a, st);
