@@ -73,7 +73,9 @@ int ic_qk_norm_rope(const void* q, void* q_out, int64_t H, const void* k, void* 
       a.ys[i][j] = strides[6 * i + 3 + j];
     }
   }
-  if (B > (1LL << 40) / L || B * L > (1LL << 37) / (32 * ((H + Hk) / 8 + 2)))
+  // units of a launch: 16 heads of a token at least, or one head when there
+  // are few
+  if (B > (1LL << 30) / L || B * L > (1LL << 30) / ((H + 15) / 16 + (Hk + 15) / 16))
     return set_error(IC_ERR_UNSUPPORTED, "%s: too many rows for one launch", me);
   a.B = B;
   a.Lq = L;
