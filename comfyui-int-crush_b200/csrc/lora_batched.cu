@@ -43,9 +43,11 @@ struct LoraArgs {
   const void* base; int64_t ldb;       // [M, N] or NULL (zeros)
   void* out; int64_t ldo;
   float* mid; int splits;              // [splits, M, Rp]
+  int streamed;                        // lora_stream.cu has the tiles of 128 rows with one adapter
 };
 
 constexpr int kLoraWarps = 8;
+constexpr int kLoraStreamRows = 4096;   // rows from which lora_stream.cu takes over
 
 template <typename T>
 __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -60,11 +62,6 @@ __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// Barrier of one row group's warps (ids 1..15; 0 is __syncthreads').
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // Eight values of a row at k, zeros past K.
@@ -91,21 +88,33 @@ __device__ __forceinline__ int lora_id(const LoraArgs& a, int64_t m0, int rows, 
   return id < 0 ? -1 : id < a.n ? id : -2;
 }
 
-// mid partials.  A warp takes 16 * MT rows; WK warps share them and cut the
-// CTA's part of K between them, 8 / WK row groups per CTA.  blockIdx: row
-// groups, K parts, passes (pass p is taken by the CTA with z = p % gridDim.z).
-template <typename T, int NT, int MT, int WK, bool VEC>
+// The adapter that all rows of a tile of 128 share, -1 if none has one, -2 if
+// they differ (the whole warp).
+__device__ __forceinline__ int lora_tile_id(const LoraArgs& a, int64_t tile0, int lane) {
+  const int first = lora_id(a, tile0, 1, 0);
+  bool same = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = tile0 + 32 * i + lane;
+    if (m < a.M) same = same && lora_id(a, m, 1, 0) == first;
+  }
+  return __all_sync(0xffffffffu, same) ? first : -2;
+}
+
+// mid partials.  The CTA's warps share a tile of 16 * MT rows and cut its part
+// of K between them.  blockIdx: row tiles, K parts, passes (pass p is taken by
+// the CTA with z = p % gridDim.z).
+template <typename T, int NT, int MT, bool VEC>
 __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraArgs a) {
   constexpr int ROWS = 16 * MT;
-  constexpr int WR = kLoraWarps / WK;
   __shared__ float red[kLoraWarps / 2][ROWS][NT * 8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int rg = warp / WK, kw = warp % WK;
-  const int64_t m0 = ((int64_t)blockIdx.x * WR + rg) * ROWS;
+  const int64_t m0 = (int64_t)blockIdx.x * ROWS;
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* down = reinterpret_cast<const T*>(a.down);
 
+  if (a.streamed && lora_tile_id(a, m0 / 128 * 128, lane) >= -1) return;   // lora_down_stream_kernel's
   const int id = lora_id(a, m0, ROWS, lane);
   const int64_t steps = (a.K + 31) / 32;
   const int64_t per = (steps + a.splits - 1) / a.splits;
@@ -133,8 +142,8 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
-#pragma unroll 2
-    for (int64_t s = s0 + kw; s < s1; s += WK) {
+#pragma unroll (NT <= 4 ? 4 : 2)
+    for (int64_t s = s0 + warp; s < s1; s += kLoraWarps) {
       const int64_t k = s * 32 + 8 * t;
       uint4 xv[MT][2];
 #pragma unroll
@@ -155,12 +164,11 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
           lora_mma<T>(acc[i][j], xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w, dv[j].z, dv[j].w);
         }
     }
-    // the WK warps of a row group (all in this pass together) add up
-    // pairwise, in a fixed order
+    // the warps (all in this pass together) add up pairwise, in a fixed order
 #pragma unroll
-    for (int o = WK / 2; o > 0; o >>= 1) {
-      float* slot = &red[rg * (WK / 2) + (kw & (o - 1))][0][0];
-      if (kw >= o && kw < 2 * o) {
+    for (int o = kLoraWarps / 2; o > 0; o >>= 1) {
+      float* slot = &red[warp & (o - 1)][0][0];
+      if (warp >= o && warp < 2 * o) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -170,8 +178,8 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
               *reinterpret_cast<float2*>(slot + (16 * i + 8 * h + g) * (NT * 8) + j * 8 + 2 * t) =
                   make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
       }
-      group_sync(1 + rg, 32 * WK);
-      if (kw < o) {
+      __syncthreads();
+      if (warp < o) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -183,9 +191,9 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
               acc[i][j][2 * h + 1] += v.y;
             }
       }
-      group_sync(1 + rg, 32 * WK);
+      __syncthreads();
     }
-    if (kw != 0) continue;
+    if (warp != 0) continue;
     float* mid = a.mid + (int64_t)blockIdx.y * a.M * a.Rp + a.r0;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -202,18 +210,30 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
   }
 }
 
-// Four values of an up row at r, zeros past R.
-template <typename T, bool VEC>
-__device__ __forceinline__ uint2 lora_ld4(const T* row, int r, int R) {
-  if constexpr (VEC) {
-    return r < R ? __ldg(reinterpret_cast<const uint2*>(row + r)) : make_uint2(0u, 0u);
+// Ranks of a lane's MMA operand values: step k of 16 ranks, e = 0..3.  FORM 2
+// takes 16-byte loads of 8 ranks for two steps, FORM 1 8-byte loads, FORM 0
+// single values.
+template <int FORM>
+__device__ __forceinline__ int lora_rank(int k, int t) {
+  return FORM == 2 ? 32 * (k >> 1) + 8 * t + 4 * (k & 1) : 16 * k + 4 * t;
+}
+
+// An up row's operand values of steps k0 .. k0 + 1 (FORM 2) or k0, zeros past R.
+template <typename T, int FORM>
+__device__ __forceinline__ uint4 lora_ld_up(const T* row, int k0, int t, int R) {
+  const int r = lora_rank<FORM>(k0, t);
+  if constexpr (FORM == 2) {
+    return r < R ? __ldg(reinterpret_cast<const uint4*>(row + r)) : make_uint4(0u, 0u, 0u, 0u);
+  } else if constexpr (FORM == 1) {
+    const uint2 v = r < R ? __ldg(reinterpret_cast<const uint2*>(row + r)) : make_uint2(0u, 0u);
+    return make_uint4(v.x, v.y, 0u, 0u);
   } else {
     T e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = r + i < R ? row[r + i] : DT<T>::from_f(0.f);
     uint2 v;
     memcpy(&v, e, 8);
-    return v;
+    return make_uint4(v.x, v.y, 0u, 0u);
   }
 }
 
@@ -240,45 +260,13 @@ __device__ __forceinline__ uint32_t pack2(T lo, T hi) {
   return v;
 }
 
-// out = base + mid @ up^T.  A warp holds the mid fragments of 16 * MT rows
-// (KS steps of 16 ranks) and goes over blocks of 32 columns.  Column 2c + e
-// of MMA tile j stands for column 8c + 2j + e of the block, so a lane ends up
-// with 8 consecutive outputs of a row.  blockIdx: row tiles, column parts,
-// passes as above (rows without an adapter belong to z = 0).
-template <typename T, int KS, int MT, bool VECO, bool VECB>
-__global__ void __launch_bounds__(32 * kLoraWarps) lora_up_kernel(const LoraArgs a, int cols_per_cta) {
-  constexpr int ROWS = 16 * MT;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int64_t m0 = (int64_t)blockIdx.x * ROWS;
-  const T* up = reinterpret_cast<const T*>(a.up);
-  const T* base = reinterpret_cast<const T*>(a.base);
-  T* out = reinterpret_cast<T*>(a.out);
-  const int id = lora_id(a, m0, ROWS, lane);
-  const unsigned active = __ballot_sync(0xffffffffu, id >= 0);
-  const unsigned bad = __ballot_sync(0xffffffffu, id == -2);
-  if (bad && lane == 0) set_dev_error(IC_DEV_ERR_INDEX);
-
-  // rows with an adapter that this CTA writes, and without
-  unsigned mine = 0, bare = 0;
-  unsigned passes = 0;
-  for (unsigned todo = active; todo; ++passes) {
-    const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
-    const unsigned match = __ballot_sync(0xffffffffu, id == ad);
-    todo &= ~match;
-    if (passes % gridDim.z == blockIdx.z) mine |= match;
-  }
-  if (blockIdx.z == 0) {
-    const int64_t left = a.M - m0;
-    bare = left >= ROWS ? (ROWS == 32 ? 0xffffffffu : (1u << ROWS) - 1u) : (1u << left) - 1u;
-    bare &= ~active;
-    if (base == out && a.ldb == a.ldo) bare &= bad;   // already there
-  }
-  if (!(mine | bare)) return;
-
-  // mid fragments (scale included), as hi + lo 16-bit values
-  uint32_t hi[MT][KS][4], lo[MT][KS][4];
-  float grow[MT][2];   // power of two taken out of an fp16 row
+// mid fragments (scale included) of rows m0 + r with bit r of `mine`, as hi + lo
+// 16-bit values, and the power of two that was taken out of an fp16 row.  id:
+// row m0 + lane's adapter.
+template <typename T, int KS, int MT, int FORM>
+__device__ __forceinline__ void lora_mid_fragments(const LoraArgs& a, int64_t m0, unsigned mine, int id, int g, int t,
+                                                   uint32_t (&hi)[MT][KS][4], uint32_t (&lo)[MT][KS][4],
+                                                   float (&grow)[MT][2]) {
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -292,11 +280,13 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_up_kernel(const LoraArgs
         for (int sp = 0; sp < a.splits; ++sp) {
           const float* row = a.mid + ((int64_t)sp * a.M + m0 + r) * a.Rp;
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-            if (16 * k + 4 * t < a.Rp) {
-              const float4 q = *reinterpret_cast<const float4*>(row + 16 * k + 4 * t);
+          for (int k = 0; k < KS; ++k) {
+            const int rk = lora_rank<FORM>(k, t);
+            if (rk < a.Rp) {
+              const float4 q = *reinterpret_cast<const float4*>(row + rk);
               v[k][0] += q.x; v[k][1] += q.y; v[k][2] += q.z; v[k][3] += q.w;
             }
+          }
         }
         const float sc = a.scales ? __ldg(a.scales + rid) : 1.f;
 #pragma unroll
@@ -332,165 +322,300 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_up_kernel(const LoraArgs
           const float rest = v[k][e] - DT<T>::to_f(h4[e]);
           l4[e] = DT<T>::from_f(isfinite(rest) ? rest : 0.f);
         }
-        // row half h holds registers h (ranks 4t, 4t+1) and 2 + h (4t+2, 4t+3)
+        // row half h holds registers h (values 0, 1) and 2 + h (values 2, 3)
         hi[i][k][h] = pack2(h4[0], h4[1]);
         hi[i][k][2 + h] = pack2(h4[2], h4[3]);
         lo[i][k][h] = pack2(l4[0], l4[1]);
         lo[i][k][2 + h] = pack2(l4[2], l4[3]);
       }
     }
+}
 
-  const int64_t n_begin = (int64_t)blockIdx.y * cols_per_cta;
-  const int64_t n_end = min(n_begin + cols_per_cta, a.N);
-  for (int64_t nb = n_begin + 32 * warp; nb < n_end; nb += 32 * kLoraWarps) {
+// out = base + mid @ up^T.  A warp holds the mid fragments of 16 * MT rows
+// (KS steps of 16 ranks) and goes over blocks of 32 columns.  Column 2c + e
+// of MMA tile j stands for column 8c + 2j + e of the block, so a lane ends up
+// with 8 consecutive outputs of a row.  ACROSS: the CTA's warps take eight row
+// tiles and the same columns (many rows: an up row is fetched into L1 once for
+// all of them), otherwise one row tile and a share of the columns each.
+// blockIdx: row tiles, column parts, passes as above (rows without an adapter
+// belong to z = 0).
+template <typename T, int KS, int MT, bool VECO, int FORM, bool ACROSS>
+__global__ void __launch_bounds__(32 * kLoraWarps) lora_up_kernel(const LoraArgs a, int cols_per_cta) {
+  constexpr int ROWS = 16 * MT;
+  constexpr int STEP = FORM == 2 ? 2 : 1;   // steps per up load
+  static_assert(KS % STEP == 0, "two steps to a load");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t m0 = ((int64_t)blockIdx.x * (ACROSS ? kLoraWarps : 1) + (ACROSS ? warp : 0)) * ROWS;
+  if (m0 >= a.M) return;
+  const T* up = reinterpret_cast<const T*>(a.up);
+  const T* base = reinterpret_cast<const T*>(a.base);
+  T* out = reinterpret_cast<T*>(a.out);
+  const int id = lora_id(a, m0, ROWS, lane);
+  const unsigned active = __ballot_sync(0xffffffffu, id >= 0);
+  const unsigned bad = __ballot_sync(0xffffffffu, id == -2);
+  if (bad && lane == 0) set_dev_error(IC_DEV_ERR_INDEX);
+
+  // rows with an adapter that this CTA writes, and without
+  unsigned mine = 0, bare = 0;
+  unsigned passes = 0;
+  for (unsigned todo = active; todo; ++passes) {
+    const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+    const unsigned match = __ballot_sync(0xffffffffu, id == ad);
+    todo &= ~match;
+    if (passes % gridDim.z == blockIdx.z) mine |= match;
+  }
+  if (blockIdx.z == 0) {
+    const int64_t left = a.M - m0;
+    bare = left >= ROWS ? (ROWS == 32 ? 0xffffffffu : (1u << ROWS) - 1u) : (1u << left) - 1u;
+    bare &= ~active;
+    if (base == out && a.ldb == a.ldo) bare &= bad;   // already there
+  }
+  if (!(mine | bare)) return;
+
+  uint32_t hi[MT][KS][4], lo[MT][KS][4];
+  float grow[MT][2];
+  lora_mid_fragments<T, KS, MT, FORM>(a, m0, mine, id, g, t, hi, lo, grow);
+
+  const int64_t n_begin = (int64_t)blockIdx.y * cols_per_cta + (ACROSS ? 0 : 32 * warp);
+  const int64_t n_end = min((int64_t)(blockIdx.y + 1) * cols_per_cta, a.N);
+  constexpr int64_t kNext = ACROSS ? 32 : 32 * kLoraWarps;
+  const auto load_base = [&](uint4 (&bv)[MT][2], int64_t nb, unsigned match) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 16 * i + 8 * h + g;
+        bv[i][h] = make_uint4(0u, 0u, 0u, 0u);
+        if (base && ((match >> r) & 1u)) bv[i][h] = lora_row8<T, VECO>(base + (m0 + r) * a.ldb, nb + 8 * t, a.N);
+      }
+  };
+  const auto load_up = [&](uint4 (&uv)[KS / STEP][4], int64_t nb, int ad) {
+    const T* u = up + (int64_t)ad * a.N * a.R;
+#pragma unroll
+    for (int k = 0; k < KS; k += STEP)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t nrow = nb + 8 * (g >> 1) + 2 * j + (g & 1);
+        uv[k / STEP][j] = nrow < a.N ? lora_ld_up<T, FORM>(u + nrow * a.R, k, t, a.R) : make_uint4(0u, 0u, 0u, 0u);
+      }
+  };
+  const auto block = [&](const uint4 (&bv)[MT][2], const uint4 (&uv)[KS / STEP][4], int64_t nb, int ad, unsigned match) {
+    float acc[MT][4][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+    if (ad >= 0) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4& u = uv[k / STEP][j];
+            const uint32_t b0 = k % STEP ? u.z : u.x, b1 = k % STEP ? u.w : u.y;
+            lora_mma<T>(acc[i][j], hi[i][k][0], hi[i][k][1], hi[i][k][2], hi[i][k][3], b0, b1);
+            lora_mma<T>(acc[i][j], lo[i][k][0], lo[i][k][1], lo[i][k][2], lo[i][k][3], b0, b1);
+          }
+    }
     const int64_t nc = nb + 8 * t;   // this lane's 8 columns
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 16 * i + 8 * h + g;
+        if (!((match >> r) & 1u)) continue;
+        T e[8], o[8];
+        memcpy(e, &bv[i][h], 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float v = DT<T>::to_f(e[2 * j + q]);
+            if (ad >= 0) v = fmaf(acc[i][j][2 * h + q], grow[i][h], v);
+            else if (ad == -2) v = __int_as_float(0x7fc00000);
+            o[2 * j + q] = DT<T>::from_f(v);
+          }
+        T* row = out + (m0 + r) * a.ldo;
+        if constexpr (VECO) {
+          if (nc < a.N) {
+            uint4 w;
+            memcpy(&w, o, 16);
+            *reinterpret_cast<uint4*>(row + nc) = w;
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (nc + q < a.N) row[nc + q] = o[q];
+        }
+      }
+  };
+
+  const int first = __shfl_sync(0xffffffffu, id, mine ? __ffs(mine) - 1 : 0);
+  if (!bare && __ballot_sync(0xffffffffu, id == first) == mine) {
+    // one adapter for all rows: the next block's loads run under this one
+    uint4 bv[MT][2], uv[KS / STEP][4];
+    load_base(bv, n_begin, mine);
+    load_up(uv, n_begin, first);
+    for (int64_t nb = n_begin; nb < n_end; nb += kNext) {
+      uint4 bn[MT][2], un[KS / STEP][4];
+      if constexpr (KS <= 4) {   // more ranks leave no registers for it
+        load_base(bn, nb + kNext < n_end ? nb + kNext : a.N, mine);
+        load_up(un, nb + kNext < n_end ? nb + kNext : a.N, first);
+      }
+      block(bv, uv, nb, first, mine);
+      if constexpr (KS <= 4) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) { bv[i][0] = bn[i][0]; bv[i][1] = bn[i][1]; }
+#pragma unroll
+        for (int k = 0; k < KS / STEP; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) uv[k][j] = un[k][j];
+      } else if (nb + kNext < n_end) {
+        load_base(bv, nb + kNext, mine);
+        load_up(uv, nb + kNext, first);
+      }
+    }
+    return;
+  }
+  for (int64_t nb = n_begin; nb < n_end; nb += kNext)
     for (unsigned todo = mine | bare; todo;) {
       const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
       const unsigned match = __ballot_sync(0xffffffffu, id == ad) & (mine | bare);
       todo &= ~match;
-      uint4 bv[MT][2];
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = 16 * i + 8 * h + g;
-          bv[i][h] = make_uint4(0u, 0u, 0u, 0u);
-          if (base && ((match >> r) & 1u)) bv[i][h] = lora_row8<T, VECO>(base + (m0 + r) * a.ldb, nc, a.N);
-        }
-      float acc[MT][4][4];
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
-      if (ad >= 0) {
-        const T* u = up + (int64_t)ad * a.N * a.R;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint2 uv[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int64_t nrow = nb + 8 * (g >> 1) + 2 * j + (g & 1);
-            uv[j] = nrow < a.N ? lora_ld4<T, VECB>(u + nrow * a.R, 16 * k + 4 * t, a.R) : make_uint2(0u, 0u);
-          }
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              lora_mma<T>(acc[i][j], hi[i][k][0], hi[i][k][1], hi[i][k][2], hi[i][k][3], uv[j].x, uv[j].y);
-              lora_mma<T>(acc[i][j], lo[i][k][0], lo[i][k][1], lo[i][k][2], lo[i][k][3], uv[j].x, uv[j].y);
-            }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = 16 * i + 8 * h + g;
-          if (!((match >> r) & 1u)) continue;
-          T e[8], o[8];
-          memcpy(e, &bv[i][h], 16);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              float v = DT<T>::to_f(e[2 * j + q]);
-              if (ad >= 0) v = fmaf(acc[i][j][2 * h + q], grow[i][h], v);
-              else if (ad == -2) v = __int_as_float(0x7fc00000);
-              o[2 * j + q] = DT<T>::from_f(v);
-            }
-          T* row = out + (m0 + r) * a.ldo;
-          if constexpr (VECO) {
-            if (nc < a.N) {
-              uint4 w;
-              memcpy(&w, o, 16);
-              *reinterpret_cast<uint4*>(row + nc) = w;
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (nc + q < a.N) row[nc + q] = o[q];
-          }
-        }
+      uint4 bv[MT][2], uv[KS / STEP][4];
+      load_base(bv, nb, match);
+      if (ad >= 0) load_up(uv, nb, ad);
+      block(bv, uv, nb, ad, match);
     }
-  }
 }
+
+}  // namespace ic
+
+#include "lora_stream.cu"
+
+namespace ic {
 
 // ---------------------------------------------------------------- launches
 struct LoraPlan {
-  int mt_down, wk, splits, z_down;
-  int mt_up, cols, z_up;
+  int stream;
+  int mt_down, splits, z_down;
+  int mt_up, across, cols, z_up;
 };
 
-// Rules on sizes: few rows put all eight warps of a CTA on one 16-row tile's
-// K range and cut K further over CTAs until about two CTAs per SM run; many
-// rows take 32-row warp tiles.  Passes go over CTAs only while that keeps the
-// grid small (a CTA without a pass ends at once).
-static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int R, int n) {
+// Rules on sizes.  Down: a CTA takes one tile of 16 rows (32 where that still
+// gives every SM two CTAs) and its eight warps cut K; K is cut further over
+// CTAs while there are fewer than two per SM, two 32-wide steps per warp at
+// least.  Up: tiles of 32 rows (16 for up to 16, or above rank 64); eight row
+// tiles per CTA once that fills the SMs twice, else one tile and 256 columns;
+// as many columns as leave four CTAs per SM.  Passes go over CTAs only while
+// that keeps the grid small (a CTA without a pass ends at once).
+static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int R, int n, bool stream) {
   LoraPlan p;
   const int sms = num_sms();
   const int64_t steps = (K + 31) / 32;
-  const bool few = M <= 16 * (int64_t)sms;
-  p.mt_down = few || R > 64 ? 1 : 2;
-  p.wk = few ? 8 : 2;
-  const int64_t groups = (M + 16 * p.mt_down * (kLoraWarps / p.wk) - 1) / (16 * p.mt_down * (kLoraWarps / p.wk));
-  int64_t s = (2 * sms + groups - 1) / groups;
-  s = s < steps / p.wk ? s : steps / p.wk;
-  s = s < 1 ? 1 : s > 16 ? 16 : s;
-  p.splits = (int)s;
+  p.stream = stream;
+  p.mt_down = R <= 64 && (M + 31) / 32 >= 2 * sms ? 2 : 1;
+  const int64_t tiles = (M + 16 * p.mt_down - 1) / (16 * p.mt_down);
+  int64_t s = (2 * sms + tiles - 1) / tiles;
+  const int64_t most = steps / (2 * kLoraWarps);
+  s = s < most ? s : most;
+  if (stream) {   // tiles of 128 rows, eight 64-wide steps at least in a part
+    const int64_t t128 = (M + 127) / 128, k64 = (K + 511) / 512;
+    s = (3 * sms + t128 - 1) / t128;
+    s = s < k64 ? s : k64;
+  }
+  p.splits = (int)(s < 1 ? 1 : s > 16 ? 16 : s);
   const int zn = n < 16 ? n : 16;
-  p.z_down = groups * s * zn <= 8 * sms ? zn : 1;
+  p.z_down = tiles * p.splits * zn <= 8 * sms ? zn : 1;
   p.mt_up = M <= 16 || R > 64 ? 1 : 2;
-  const int64_t tiles = (M + 16 * p.mt_up - 1) / (16 * p.mt_up);
+  const int64_t rows = 16 * p.mt_up, groups = (M + rows * kLoraWarps - 1) / (rows * kLoraWarps);
+  p.across = groups * ((N + 255) / 256) >= 2 * sms;
+  const int64_t units = p.across ? groups : (M + rows - 1) / rows;
   int cols = 32 * kLoraWarps;
-  while (cols < 2048 && tiles * ((N + 2 * cols - 1) / (2 * cols)) >= 8 * sms) cols *= 2;
+  while (cols < 4096 && units * ((N + 2 * cols - 1) / (2 * cols)) >= 4 * sms) cols *= 2;
   p.cols = cols;
-  p.z_up = tiles * ((N + cols - 1) / cols) * zn <= 8 * sms ? zn : 1;
+  p.z_up = !p.across && units * ((N + cols - 1) / cols) * zn <= 8 * sms ? zn : 1;
   return p;
 }
 
+// Sizes that lora_stream.cu takes, if the rows are aligned for TMA.
+static bool lora_stream_sizes(int64_t M, int64_t K, int64_t N, int R, int n) {
+  return M >= kLoraStreamRows && R <= 64 && R % 8 == 0 && K % 8 == 0 && N % 8 == 0 && K >= 64 && N >= 64 &&
+         (int64_t)n * N < (1LL << 31) && (int64_t)n * R < (1LL << 31);
+}
+
 int64_t lora_workspace(int64_t M, int64_t K, int64_t N, int R, int n) {
-  return (int64_t)lora_plan(M, K, N, R, n).splits * M * ((R + 7) / 8 * 8);
+  int splits = lora_plan(M, K, N, R, n, false).splits;
+  if (lora_stream_sizes(M, K, N, R, n)) {   // either, by the alignment of the rows
+    const int s = lora_plan(M, K, N, R, n, true).splits;
+    splits = s > splits ? s : splits;
+  }
+  return (int64_t)splits * M * ((R + 7) / 8 * 8);
 }
 
 template <typename T, int NT, bool VEC>
 static cudaError_t lora_down_t(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
-  const int64_t rows = 16 * p.mt_down * (kLoraWarps / p.wk);
+  const int64_t rows = 16 * p.mt_down;
   const dim3 grid((unsigned)((a.M + rows - 1) / rows), (unsigned)p.splits, (unsigned)p.z_down);
-  if (p.wk == 8) lora_down_kernel<T, NT, 1, 8, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);
-  else if (p.mt_down == 1) lora_down_kernel<T, NT, 1, 2, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);
-  else if constexpr (NT <= 8) lora_down_kernel<T, NT, 2, 2, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);
+  if constexpr (NT <= 8) {
+    if (p.mt_down == 2) {
+      lora_down_kernel<T, NT, 2, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);
+      return cudaGetLastError();
+    }
+  }
+  lora_down_kernel<T, NT, 1, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, int KS, int MT>
+static cudaError_t lora_up_m(const LoraArgs& a, const LoraPlan& p, bool vec, bool wide, cudaStream_t st) {
+  const int64_t rows = 16 * MT * (p.across ? kLoraWarps : 1);
+  const dim3 grid((unsigned)((a.M + rows - 1) / rows), (unsigned)((a.N + p.cols - 1) / p.cols), (unsigned)p.z_up);
+  const int th = 32 * kLoraWarps;
+  constexpr int WIDE = KS % 2 == 0 ? 2 : 1;
+  if (!vec) lora_up_kernel<T, KS, MT, false, 0, false><<<grid, th, 0, st>>>(a, p.cols);
+  else if (p.across && wide) lora_up_kernel<T, KS, MT, true, WIDE, true><<<grid, th, 0, st>>>(a, p.cols);
+  else if (p.across) lora_up_kernel<T, KS, MT, true, 1, true><<<grid, th, 0, st>>>(a, p.cols);
+  else if (wide) lora_up_kernel<T, KS, MT, true, WIDE, false><<<grid, th, 0, st>>>(a, p.cols);
+  else lora_up_kernel<T, KS, MT, true, 1, false><<<grid, th, 0, st>>>(a, p.cols);
   return cudaGetLastError();
 }
 
 template <typename T, int KS>
-static cudaError_t lora_up_t(const LoraArgs& a, const LoraPlan& p, bool veco, bool vecb, cudaStream_t st) {
-  const int64_t rows = 16 * p.mt_up;
-  const dim3 grid((unsigned)((a.M + rows - 1) / rows), (unsigned)((a.N + p.cols - 1) / p.cols), (unsigned)p.z_up);
-  const int th = 32 * kLoraWarps;
-#define IC_UP(MT)                                                                         \
-  if (veco && vecb) lora_up_kernel<T, KS, MT, true, true><<<grid, th, 0, st>>>(a, p.cols); \
-  else lora_up_kernel<T, KS, MT, false, false><<<grid, th, 0, st>>>(a, p.cols);
-  if constexpr (KS <= 4) {
-    if (p.mt_up == 2) { IC_UP(2) return cudaGetLastError(); }
+static cudaError_t lora_up_t(const LoraArgs& a, LoraPlan p, bool vec, bool wide, cudaStream_t st) {
+  if (!vec && p.across) {   // odd rows: one tile per CTA
+    p.across = 0;
+    p.z_up = 1;
   }
-  IC_UP(1)
-#undef IC_UP
-  return cudaGetLastError();
+  if constexpr (KS <= 4) {
+    if (p.mt_up == 2) return lora_up_m<T, KS, 2>(a, p, vec, wide, st);
+  }
+  return lora_up_m<T, KS, 1>(a, p, vec, wide, st);
 }
 
 template <typename T>
-static cudaError_t lora_t(const LoraArgs& a, cudaStream_t st) {
-  const LoraPlan p = lora_plan(a.M, a.K, a.N, a.R, a.n);
+static cudaError_t lora_t(LoraArgs a, cudaStream_t st) {
   const auto al = [](const void* q, int by) { return (reinterpret_cast<uintptr_t>(q) & (by - 1)) == 0; };
   const bool vec = al(a.x, 16) && al(a.down, 16) && a.ldx % 8 == 0 && a.K % 8 == 0;
   const bool veco = (!a.base || (al(a.base, 16) && a.ldb % 8 == 0)) && al(a.out, 16) && a.ldo % 8 == 0 && a.N % 8 == 0;
-  const bool vecb = al(a.up, 8) && a.R % 4 == 0;
+  const bool vecu = veco && al(a.up, 8) && a.R % 4 == 0, wide = al(a.up, 16) && a.R % 8 == 0;
+  const bool stream = vec && vecu && wide && lora_stream_sizes(a.M, a.K, a.N, a.R, a.n);
+  const LoraPlan p = lora_plan(a.M, a.K, a.N, a.R, a.n, stream);
+  a.splits = p.splits;
+  a.streamed = stream;
+  cudaError_t e = cudaSuccess;
+  if (stream) {
+    e = a.R <= 8 ? lora_down_stream_t<T, 1>(a, st) : a.R <= 16 ? lora_down_stream_t<T, 2>(a, st)
+        : a.R <= 32 ? lora_down_stream_t<T, 4>(a, st) : lora_down_stream_t<T, 8>(a, st);
+    if (e != cudaSuccess) return e;
+  }
 #define IC_DOWN(NT) e = vec ? lora_down_t<T, NT, true>(c, p, st) : lora_down_t<T, NT, false>(c, p, st)
   for (int r0 = 0; r0 < a.R; r0 += 128) {   // accumulators hold 128 ranks
     LoraArgs c = a;
     c.r0 = r0;
     c.Rc = a.R - r0 < 128 ? a.R - r0 : 128;
-    cudaError_t e;
     if (c.Rc <= 8) IC_DOWN(1);
     else if (c.Rc <= 16) IC_DOWN(2);
     else if (c.Rc <= 32) IC_DOWN(4);
@@ -499,16 +624,17 @@ static cudaError_t lora_t(const LoraArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
   }
 #undef IC_DOWN
-  if (a.R <= 16) return lora_up_t<T, 1>(a, p, veco, vecb, st);
-  if (a.R <= 32) return lora_up_t<T, 2>(a, p, veco, vecb, st);
-  if (a.R <= 64) return lora_up_t<T, 4>(a, p, veco, vecb, st);
-  if (a.R <= 128) return lora_up_t<T, 8>(a, p, veco, vecb, st);
-  return lora_up_t<T, 16>(a, p, veco, vecb, st);
+  if (stream)
+    return a.R <= 16 ? lora_up_stream_t<T, 1>(a, st) : a.R <= 32 ? lora_up_stream_t<T, 2>(a, st) : lora_up_stream_t<T, 4>(a, st);
+  if (a.R <= 16) return lora_up_t<T, 1>(a, p, vecu, wide, st);
+  if (a.R <= 32) return lora_up_t<T, 2>(a, p, vecu, wide, st);
+  if (a.R <= 64) return lora_up_t<T, 4>(a, p, vecu, wide, st);
+  if (a.R <= 128) return lora_up_t<T, 8>(a, p, vecu, wide, st);
+  return lora_up_t<T, 16>(a, p, vecu, wide, st);
 }
 
-cudaError_t launch_lora_batched(LoraArgs a, int dtype, cudaStream_t st) {
+cudaError_t launch_lora_batched(const LoraArgs& a, int dtype, cudaStream_t st) {
   if (a.M == 0 || a.N == 0) return cudaSuccess;
-  a.splits = lora_plan(a.M, a.K, a.N, a.R, a.n).splits;
   return dtype == IC_DTYPE_BF16 ? lora_t<__nv_bfloat16>(a, st) : lora_t<__half>(a, st);
 }
 

@@ -463,6 +463,9 @@ def lora_inputs(seed, M, K, N, R, n, dtype):
     (1, 1, 8, 8, 1, 1), (1, 1, 512, 64, 16, 3), (16, 1, 1024, 520, 16, 8), (37, 1, 77, 33, 5, 4), (64, 1, 256, 264, 12, 40),
     (33, 11, 640, 96, 32, 2), (300, 100, 136, 1000, 24, 5), (2600, 650, 96, 72, 64, 3), (2500, 1, 264, 40, 20, 4),
     (700, 7, 1000, 300, 128, 6), (90, 3, 320, 136, 192, 3), (3000, 1500, 64, 344, 256, 2), (2777, 1, 61, 35, 9, 3),
+    # from 4096 rows: tiles of 128 rows through shared memory, where the rows are aligned
+    (4200, 1, 136, 200, 24, 5), (4230, 470, 1000, 136, 8, 3), (5120, 640, 72, 328, 64, 4), (4099, 4099, 520, 64, 16, 2),
+    (4864, 2432, 2056, 104, 32, 2), (4100, 100, 64, 72, 40, 30), (4096, 64, 77, 200, 16, 3),
 ])
 def test_lora_batched(M, rows, K, N, R, n, dtype):
     x, base, down, up, scales, g = lora_inputs(1, M, K, N, R, n, dtype)
@@ -479,7 +482,7 @@ def test_lora_batched(M, rows, K, N, R, n, dtype):
     assert z.data_ptr() == base.data_ptr() and torch.equal(z, y)
 
 
-@pytest.mark.parametrize("M,rows", [(48, 1), (2600, 1300), (2600, 1)])
+@pytest.mark.parametrize("M,rows", [(48, 1), (2600, 1300), (2600, 1), (4200, 1), (4500, 150), (5200, 1300)])
 def test_lora_requests_do_not_touch_each_other(M, rows):
     """NaN and infinities in one request's rows or adapter reach no other
     request, and an id that names no adapter only its own rows."""
