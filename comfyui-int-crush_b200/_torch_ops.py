@@ -11,7 +11,11 @@ graph breaks at every ctypes call:
 * ``intcrush_b200::gemm_a8(x_int8, w, s_w, s_a, bias?, out_dtype,
   group_size, repacked) -> out`` -- ``_b200_runtime.gemm_a8``;
 * ``intcrush_b200::gemm_w4a16(x, packed, scale, group_size, w_layout) ->
-  out`` -- ``_b200_runtime.gemm_w4a16``.
+  out`` -- ``_b200_runtime.gemm_w4a16``;
+* ``intcrush_b200::qk_norm_rope(q, k, q_gamma?, k_gamma?, cos?, sin?, layout,
+  positions?, eps) -> (q, k)``, ``intcrush_b200::cross_attention(q, k, v,
+  kv_lens?, key_mask?, scale) -> out`` and ``intcrush_b200::lora_batched(x,
+  down, up, ids, scales?, base?) -> out`` -- the functions of the same names.
 
 The ops mirror the reference runtime's callables (``_triton_runtime.py:
 16-41,114-130``): CUDA tensors in, freshly allocated outputs, launch on the
@@ -66,6 +70,35 @@ def register() -> None:
     @gemm_w4a16.register_fake
     def _(x, packed, scale, group_size, w_layout):
         return x.new_empty((x.shape[0], packed.shape[0]), dtype=x.dtype)
+
+    @torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=())
+    def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None,
+                     cos: torch.Tensor | None, sin: torch.Tensor | None, layout: str,
+                     positions: torch.Tensor | None, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+        return _rt.qk_norm_rope(q, k, q_gamma=q_gamma, k_gamma=k_gamma, cos=cos, sin=sin, layout=layout,
+                                positions=positions, eps=eps)
+
+    @qk_norm_rope.register_fake
+    def _(q, k, q_gamma, k_gamma, cos, sin, layout, positions, eps):
+        return q.new_empty(q.shape), k.new_empty(k.shape)
+
+    @torch.library.custom_op(f"{_NS}::cross_attention", mutates_args=())
+    def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor | None,
+                        key_mask: torch.Tensor | None, scale: float) -> torch.Tensor:
+        return _rt.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale)
+
+    @cross_attention.register_fake
+    def _(q, k, v, kv_lens, key_mask, scale):
+        return q.new_empty(q.shape)
+
+    @torch.library.custom_op(f"{_NS}::lora_batched", mutates_args=())
+    def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, ids: torch.Tensor,
+                     scales: torch.Tensor | None, base: torch.Tensor | None) -> torch.Tensor:
+        return _rt.lora_batched(x, down, up, ids, scales, base=base)
+
+    @lora_batched.register_fake
+    def _(x, down, up, ids, scales, base):
+        return x.new_empty((*x.shape[:-1], up.shape[1]))
 
     _done = True
 

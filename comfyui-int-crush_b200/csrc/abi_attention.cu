@@ -115,6 +115,7 @@ int ic_lora_batched(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
   const int bad = lora_sizes(me, M, K, N, R, n);
   if (bad != IC_OK) return bad;
   if (rows_per_id <= 0) return set_error(IC_ERR_ARG, "%s: rows_per_id must be positive", me);
+  if (rows_per_id > 0x7fffffffLL) rows_per_id = 0x7fffffffLL;   // M is below that
   if (ldx < K || ldo < N || (base && ldb < N))
     return set_error(IC_ERR_ARG, "%s: a row stride is shorter than its row", me);
   if (M == 0 || N == 0) return IC_OK;
@@ -176,6 +177,8 @@ int ic_cross_attention(const void* q, const void* k, const void* v, void* out, i
       return set_error(IC_ERR_ARG, "%s: strides must be in [0, 2^38)", me);
     if (i % 3 == 1 && strides[i] == 0 && tokens > 1)
       return set_error(IC_ERR_ARG, "%s: a token stride of 0 with more than one token", me);
+    if (strides[i] == 0 && ((i == 9 && B > 1) || (i == 11 && H > 1)))
+      return set_error(IC_ERR_ARG, "%s: out overlaps itself", me);
   }
   const XattnPlan p = xattn_plan(B, Lq, Lk, (int)H, (int)Hk, (int)D, mask_kind);
   if (p.floats && (!workspace || !at16(workspace) || workspace_elems < p.floats))

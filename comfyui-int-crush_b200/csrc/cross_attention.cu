@@ -70,11 +70,17 @@ __global__ void __launch_bounds__(1024) xattn_mask_kernel(const void* mask, int6
 // The rows of one key head (Lq tokens times the query heads that share it)
 // in tiles of 16; four warps go over the keys in blocks of 16, each warp its
 // own blocks, and the keys are split over CTAs when there are few tiles.
-// Nothing is staged: a lane's 16-byte loads of K (row = key, chunk of 8
-// elements) are MMA fragments as they are, with the order of the summed
-// elements permuted alike in Q, and V's fragments pair two keys of one
-// element by a byte permutation of two loads.  What bounds it is the stream
-// of K and V from HBM; 16 to 20 loads per lane are in flight.
+// A lane's 16-byte loads of K (row = key, chunk of 8 elements) are MMA
+// fragments as they are, with the order of the summed elements permuted alike
+// in Q, and V's fragments pair two keys of one element by a byte permutation
+// of two loads.  What bounds it is the stream of K and V from HBM and the
+// warps' own instructions beside it, so the next block is in flight (8 KB a
+// warp at D = 128) while one is computed, as asynchronous copies to a ring of
+// the warp's own in shared memory: every lane reads back what it copied, so the
+// ring needs no barrier, and its registers leave room for three CTAs per SM.
+// 8 single tokens of 32 heads over 8 key heads of 128, 1024 to 8192 keys (151
+// MB): 46 us with the join, 3.3 TB/s; loads straight to registers 49 us.  The
+// copies alone take 44 us of that, the arithmetic alone 22.
 // Softmax: scores, maxima and sums in fp32; the running maximum of a row only
 // moves when it grows by more than 2^8 (the sums stay exact, p stays below
 // 2^8), so most blocks rescale nothing.  p enters the product with V rounded
@@ -96,12 +102,31 @@ __device__ __forceinline__ void xs_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int NC>
+struct XsCfg {
+  static constexpr int NH = (NC + 1) / 2;              // 64-element halves of V
+  static constexpr int LOADS = 2 * NC + 4 * NH;        // of a lane for a block
+  static constexpr int STAGES = 2;                     // one in use, one in flight
+  static constexpr int RING = kXsWarps * STAGES * LOADS * 512;
+  static constexpr int JOIN = kXsWarps * 16 * (64 * NH + 4) * 4;
+  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+};
+
 // NC: 32-element chunks of the head (D <= 32 * NC).
 template <typename T, int NC, bool BIAS>
-__global__ void __launch_bounds__(32 * kXsWarps) xattn_rows_kernel(const XattnArgs a) {
-  constexpr int NH = (NC + 1) / 2;   // 64-element halves of V
+__global__ void __launch_bounds__(32 * kXsWarps, 3) xattn_rows_kernel(const XattnArgs a) {
+  using C = XsCfg<NC>;
+  constexpr int NH = C::NH, S = C::STAGES;
   constexpr int DP = 64 * NH;
-  __shared__ float so[kXsWarps][16][DP + 4];
+  extern __shared__ __align__(16) uint8_t ring[];
+  float (*so)[16][DP + 4] = reinterpret_cast<float (*)[16][DP + 4]>(ring);   // after the loop
   __shared__ float sm[kXsWarps][16], sl[kXsWarps][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -115,9 +140,11 @@ __global__ void __launch_bounds__(32 * kXsWarps) xattn_rows_kernel(const XattnAr
   const T* vp = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
 
   const int end = xattn_end(a, b);
+  // parts of the same length for every sample: a short one has fewer of them,
+  // and a part past its end nothing to do
   const int blocks = (end + 15) / 16;
-  const int per = (blocks + a.splits - 1) / a.splits;
-  const int blk0 = (int)blockIdx.y * per, blk1 = min(blk0 + per, blocks);
+  const int blk0 = (int)blockIdx.y * a.part_blocks, blk1 = min(blk0 + a.part_blocks, blocks);
+  if (blk0 >= blocks && blockIdx.y > 0) return;
 
   uint4 qv[2][NC];
 #pragma unroll
@@ -140,37 +167,79 @@ __global__ void __launch_bounds__(32 * kXsWarps) xattn_rows_kernel(const XattnAr
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   const float sc = a.scale * kLog2e;
 
+  const uint32_t mine = smem_u32(ring) + warp * S * C::LOADS * 512 + lane * 16;
+  // K rows 8i + g, chunk t of 32 elements; V rows 2t, + 1, + 8, + 9 (this lane's
+  // keys), chunk g of 64.  A key past the end is not read (zeros).
+  const T* kl = kp + g * a.ks[1] + 8 * t;
+  const T* vl = vp + 2 * t * a.vs[1] + 8 * g;
+  const bool full_d = a.D == 32 * NC && NC % 2 == 0;
+  const auto copy = [&](int blk, int stage) {
+    const uint32_t to = mine + stage * C::LOADS * 512;
+    const T* k0 = kl + (int64_t)(16 * blk) * a.ks[1];
+    const T* v0 = vl + (int64_t)(16 * blk) * a.vs[1];
+    if (full_d && blk < blk1 && 16 * blk + 16 <= end) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i, k0 += 8 * a.ks[1])
+#pragma unroll
+        for (int c = 0; c < NC; ++c) cp_async16(to + (i * NC + c) * 512, k0 + 32 * c, true);
+#pragma unroll
+      for (int e = 0; e < 4; ++e, v0 += e == 2 ? 7 * a.vs[1] : a.vs[1])
+#pragma unroll
+        for (int i = 0; i < NH; ++i) cp_async16(to + (2 * NC + e * NH + i) * 512, v0 + 64 * i, true);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const bool on = blk < blk1 && 16 * blk + 8 * i + g < end && 32 * c + 8 * t < a.D;
+          cp_async16(to + (i * NC + c) * 512, on ? k0 + 8 * i * a.ks[1] + 32 * c : kp, on);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < NH; ++i) {
+          const int r = (e & 1) + 8 * (e >> 1);
+          const bool on = blk < blk1 && 16 * blk + 2 * t + r < end && 64 * i + 8 * g < a.D;
+          cp_async16(to + (2 * NC + e * NH + i) * 512, on ? v0 + r * a.vs[1] + 64 * i : vp, on);
+        }
+    }
+    cp_async_commit();
+  };
+  const auto load_bias = [&](float (&bs)[4], int blk) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = blk * 16 + 2 * t + (e & 1) + 8 * (e >> 1);
+      bs[e] = 0.f;
+      if constexpr (BIAS) {
+        if (blk < blk1) bs[e] = __ldg(a.bias + b * a.Lkp + j);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) copy(blk0 + warp + kXsWarps * i, i);
+  float bs[4], bn[4];
+  load_bias(bs, blk0 + warp);
+  int stage = 0;
   for (int blk = blk0 + warp; blk < blk1; blk += kXsWarps) {
-    const int j0 = blk * 16;
-    uint4 kv[2][NC];
+    copy(blk + kXsWarps * (S - 1), stage == 0 ? S - 1 : stage - 1);   // the stage used last
+    load_bias(bn, blk + kXsWarps);
+    cp_async_wait<S - 1>();
+    uint4 kv[2][NC], vv[NH][4];
+    const uint8_t* from = ring + (mine - smem_u32(ring)) + stage * C::LOADS * 512;
+    bool seen[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      seen[e] = blk * 16 + 2 * t + (e & 1) + 8 * (e >> 1) < end && !(BIAS && bs[e] == -INFINITY);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int j = j0 + 8 * i + g;
-        kv[i][c] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < end && 32 * c + 8 * t < a.D)
-          kv[i][c] = __ldg(reinterpret_cast<const uint4*>(kp + j * a.ks[1] + 32 * c + 8 * t));
-      }
-    // this lane's keys: j0 + 2t, + 1, + 8, + 9
-    float bs[4];
-    bool seen[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
-      bs[e] = 0.f;
-      if constexpr (BIAS) bs[e] = __ldg(a.bias + b * a.Lkp + j);
-      seen[e] = j < end && !(bs[e] == -INFINITY);
-    }
-    uint4 vv[NH][4];
+      for (int c = 0; c < NC; ++c) kv[i][c] = *reinterpret_cast<const uint4*>(from + (i * NC + c) * 512);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int i = 0; i < NH; ++i) {
-        const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
-        vv[i][e] = make_uint4(0u, 0u, 0u, 0u);
-        if (seen[e] && 64 * i + 8 * g < a.D)
-          vv[i][e] = __ldg(reinterpret_cast<const uint4*>(vp + j * a.vs[1] + 64 * i + 8 * g));
+        vv[i][e] = *reinterpret_cast<const uint4*>(from + (2 * NC + e * NH + i) * 512);
+        if (BIAS && !seen[e]) vv[i][e] = make_uint4(0u, 0u, 0u, 0u);   // 0 * NaN is not 0
       }
     float s[2][4];
 #pragma unroll
@@ -239,7 +308,12 @@ __global__ void __launch_bounds__(32 * kXsWarps) xattn_rows_kernel(const XattnAr
                   __byte_perm(w[2][j >> 1], w[3][j >> 1], sel));
       }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bs[e] = bn[e];
+    stage = stage == S - 1 ? 0 : stage + 1;
   }
+  cp_async_wait<0>();
+  __syncthreads();   // the ring becomes the joined sums
   // join the warps: row sums over the quad first
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -291,11 +365,19 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XattnArgs a) {
   if (i >= rows * dq) return;
   const int64_t row = i / dq;
   const int d = (int)(i % dq) * 8;
+  // parts that the sample has (the tcgen05 kernel writes all)
+  int splits = a.splits;
+  if (a.part_blocks) {
+    const int blocks = (xattn_end(a, row / a.H / a.Lq) + 15) / 16;
+    splits = max(1, min(splits, (blocks + a.part_blocks - 1) / a.part_blocks));
+  }
   float mm = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part_ml[(s * rows + row) * 2]);
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, a.part_ml[(s * rows + row) * 2]);
   const float ref = mm == -INFINITY ? 0.f : mm;
   float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2);
     const float f = ex2(ml.x - ref);
     const float4* p = reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.D + d);
@@ -309,8 +391,9 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XattnArgs a) {
 }
 
 // ---------------------------------------------------------------- launches
-// Splits of the few-rows kernel: until about four CTAs per SM run, with at
-// least 8 blocks of 16 keys (two per warp) in a part.
+// Splits of the few-rows kernel: four CTAs per SM, with at least 8 blocks of 16
+// keys (two per warp) in a part (the case above: two CTAs 57 us, three 48 to
+// 53, four 46, six 50 to 55, ten 52).
 static int rows_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk) {
   const int64_t ctas = (Lq * (H / Hk) + 15) / 16 * B * Hk;
   const int64_t blocks = (Lk + 15) / 16;
@@ -319,6 +402,10 @@ static int rows_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk) {
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
+
+// Query tokens above which the tcgen05 kernel takes over: its tile holds 128 of
+// one head, the few-rows one 16 of all heads that share a key head.
+constexpr int64_t kTcRows = 48;
 
 // Splits and slots of the tcgen05 kernel: two query tiles per CTA share K and
 // V; with too few tiles for that to fill the SMs, one, and then the keys are
@@ -338,7 +425,7 @@ XattnPlan xattn_plan(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int D, in
   XattnPlan p;
   p.slots = 0;
   if (Lk == 0) p.splits = 1;
-  else if (Lq > 48) p.splits = tc_splits(B, Lq, Lk, H, Hk, &p.slots);
+  else if (Lq > kTcRows) p.splits = tc_splits(B, Lq, Lk, H, Hk, &p.slots);
   else p.splits = rows_splits(B, Lq, Lk, H, Hk);
   p.Lkp = mask_kind ? (Lk + 127) / 128 * 128 : 0;
   const int64_t rows = B * Lq * H;
@@ -349,12 +436,19 @@ XattnPlan xattn_plan(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int D, in
 
 template <typename T, bool BIAS>
 static cudaError_t launch_rows(const XattnArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)((a.Lq * (a.H / a.Hk) + 15) / 16 * a.B * a.Hk), (unsigned)a.splits);
-  if (a.D <= 32) xattn_rows_kernel<T, 1, BIAS><<<grid, 32 * kXsWarps, 0, st>>>(a);
-  else if (a.D <= 64) xattn_rows_kernel<T, 2, BIAS><<<grid, 32 * kXsWarps, 0, st>>>(a);
-  else if (a.D <= 96) xattn_rows_kernel<T, 3, BIAS><<<grid, 32 * kXsWarps, 0, st>>>(a);
-  else xattn_rows_kernel<T, 4, BIAS><<<grid, 32 * kXsWarps, 0, st>>>(a);
-  return cudaGetLastError();
+  const int64_t tiles = (a.Lq * (a.H / a.Hk) + 15) / 16 * a.B * a.Hk;
+  if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)tiles, (unsigned)a.splits);
+  const auto go = [&](auto* kern, int smem) {
+    const cudaError_t e = set_smem_once(kern, smem);
+    if (e != cudaSuccess) return e;
+    kern<<<grid, 32 * kXsWarps, smem, st>>>(a);
+    return cudaGetLastError();
+  };
+  if (a.D <= 32) return go(xattn_rows_kernel<T, 1, BIAS>, XsCfg<1>::SMEM);
+  if (a.D <= 64) return go(xattn_rows_kernel<T, 2, BIAS>, XsCfg<2>::SMEM);
+  if (a.D <= 96) return go(xattn_rows_kernel<T, 3, BIAS>, XsCfg<3>::SMEM);
+  return go(xattn_rows_kernel<T, 4, BIAS>, XsCfg<4>::SMEM);
 }
 
 template <typename T>
@@ -375,6 +469,7 @@ cudaError_t launch_cross_attention(XattnArgs a, int dtype, const void* mask, int
   // one.  Others are nobody's ordinary call: the few-rows kernel, unsplit.
   if (p.slots && !(a.scale > 0.f)) p.slots = 0, p.splits = 1;
   a.splits = p.splits;
+  a.part_blocks = p.slots ? 0 : (int)(((a.Lk + 15) / 16 + p.splits - 1) / p.splits);
   a.Lkp = p.Lkp;
   a.part_o = workspace;
   a.part_ml = workspace + p.part_floats / (a.D + 2) * a.D;

@@ -24,6 +24,7 @@ struct XattnArgs {
   const int32_t* ends;         // [B], with bias
   int64_t Lkp;
   int splits;                  // parts of the keys
+  int part_blocks;             // few-rows kernel: blocks of 16 keys in a part
   float* part_o;               // [splits, B, Lq, H, D] with splits > 1
   float* part_ml;              // [splits, B, Lq, H, 2]: maximum (log2), sum
 };

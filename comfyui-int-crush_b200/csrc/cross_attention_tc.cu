@@ -17,6 +17,15 @@
 // The MMAs of one slot run while the other slot's softmax does; P V starts when
 // three quarters of P are written; the next item's first S is issued behind the
 // last P V, so that nothing drains between items.
+// What bounds it: a slot's turn from S to the next S.  Of its about 3000 clocks
+// at D = 128 the softmax takes 1900 (the 128 exponentials of a row alone 1024,
+// at 16 a clock per SM), P V's rest and the next S 1100; the MMAs of both slots
+// (64 to 73 clocks for 128 x 128 x 16) fill 2200 of them.  S cannot run ahead:
+// O and S of two slots take all 512 columns, so P lies over S.  Measured and
+// not kept (8190 rows, 512 keys, 40 heads, 89 us): P through shared memory with
+// S ahead 105 us (P's traffic on top of what the MMAs read), a part of the
+// exponentials as polynomials 90 to 94, hand-interleaved 93 and more.
+// 2 x 32760 rows, 512 keys, 40 heads of 128: 630 us, 1090 TFLOP/s.
 //
 // S, the running maximum, the row sum and O are fp32.  The maximum moves only
 // when it grows by more than 2^8 (P stays below 2^8 and the sums exact), so O

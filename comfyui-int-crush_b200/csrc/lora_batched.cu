@@ -43,11 +43,13 @@ struct LoraArgs {
   const void* base; int64_t ldb;       // [M, N] or NULL (zeros)
   void* out; int64_t ldo;
   float* mid; int splits;              // [splits, M, Rp]
-  int streamed;                        // lora_stream.cu has the tiles of 128 rows with one adapter
+  int streamed;                        // lora_stream.cu takes part
 };
 
 constexpr int kLoraWarps = 8;
-constexpr int kLoraStreamRows = 4096;   // rows from which lora_stream.cu takes over
+// Rows from which lora_stream.cu takes over (2777 rows of runs of four adapters,
+// 5120 to 5120 columns, rank 24: 55 us with it, 69 us without).
+constexpr int kLoraStreamRows = 1024;
 
 template <typename T>
 __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -84,42 +86,56 @@ __device__ __forceinline__ uint4 lora_ld8(const T* row, int64_t k, int64_t K) {
 __device__ __forceinline__ int lora_id(const LoraArgs& a, int64_t m0, int rows, int lane) {
   const int64_t m = m0 + lane;
   if (lane >= rows || m >= a.M) return -1;
-  const int id = __ldg(a.ids + m / a.rows_per_id);
+  // M < 2^31
+  const int id = __ldg(a.ids + (a.rows_per_id == 1 ? (uint32_t)m : (uint32_t)m / (uint32_t)a.rows_per_id));
   return id < 0 ? -1 : id < a.n ? id : -2;
 }
 
-// The adapter that all rows of a tile of 128 share, -1 if none has one, -2 if
-// they differ (the whole warp).
-__device__ __forceinline__ int lora_tile_id(const LoraArgs& a, int64_t tile0, int lane) {
-  const int first = lora_id(a, tile0, 1, 0);
-  bool same = true;
+// The first two adapters among 16 rows (bits of `rows` in a ballot; -1: none),
+// and whether there are more.
+__device__ __forceinline__ bool lora_two(int id, unsigned rows, int& a0, int& a1) {
+  const unsigned act = __ballot_sync(0xffffffffu, id >= 0) & rows;
+  a0 = __shfl_sync(0xffffffffu, id, act ? __ffs(act) - 1 : 0);
+  const unsigned rest = act & ~__ballot_sync(0xffffffffu, id == a0);
+  a1 = __shfl_sync(0xffffffffu, id, rest ? __ffs(rest) - 1 : 0);
+  const unsigned more = rest & ~__ballot_sync(0xffffffffu, id == a1);
+  if (!act) a0 = -1;
+  if (!rest) a1 = -1;
+  return more != 0;
+}
+
+// Whether a tile of 128 rows has more than two adapters in one of its groups of
+// 16 rows, which lora_down_stream_kernel leaves to lora_down_kernel.
+__device__ __forceinline__ bool lora_tile_left(const LoraArgs& a, int64_t tile0, int lane) {
+  bool left = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = tile0 + 32 * i + lane;
-    if (m < a.M) same = same && lora_id(a, m, 1, 0) == first;
+  for (int q = 0; q < 4; ++q) {
+    const int id = lora_id(a, tile0 + 32 * q, 32, lane);
+    int a0, a1;
+    left = lora_two(id, 0xffffu, a0, a1) || left;
+    left = lora_two(id, 0xffff0000u, a0, a1) || left;
   }
-  return __all_sync(0xffffffffu, same) ? first : -2;
+  return left;
 }
 
 // mid partials.  The CTA's warps share a tile of 16 * MT rows and cut its part
-// of K between them.  blockIdx: row tiles, K parts, passes (pass p is taken by
-// the CTA with z = p % gridDim.z).
+// of K between them.  blockIdx: row tiles (in turns, beside the stream kernel),
+// K parts, passes (pass p is taken by the CTA with z = p % gridDim.z).
 template <typename T, int NT, int MT, bool VEC>
 __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraArgs a) {
   constexpr int ROWS = 16 * MT;
   __shared__ float red[kLoraWarps / 2][ROWS][NT * 8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int64_t m0 = (int64_t)blockIdx.x * ROWS;
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* down = reinterpret_cast<const T*>(a.down);
-
-  if (a.streamed && lora_tile_id(a, m0 / 128 * 128, lane) >= -1) return;   // lora_down_stream_kernel's
-  const int id = lora_id(a, m0, ROWS, lane);
   const int64_t steps = (a.K + 31) / 32;
   const int64_t per = (steps + a.splits - 1) / a.splits;
   const int64_t s0 = (int64_t)blockIdx.y * per, s1 = min(s0 + per, steps);
 
+  for (int64_t m0 = (int64_t)blockIdx.x * ROWS; m0 < a.M; m0 += (int64_t)gridDim.x * ROWS) {
+  if (a.streamed && !lora_tile_left(a, m0 / 128 * 128, lane)) continue;   // lora_down_stream_kernel's
+  const int id = lora_id(a, m0, ROWS, lane);
   unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
   for (unsigned pass = 0; todo; ++pass) {
     const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
@@ -208,6 +224,7 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
                 make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
       }
   }
+  }
 }
 
 // Ranks of a lane's MMA operand values: step k of 16 ranks, e = 0..3.  FORM 2
@@ -277,6 +294,7 @@ __device__ __forceinline__ void lora_mid_fragments(const LoraArgs& a, int64_t m0
       for (int k = 0; k < KS; ++k) v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.f;
       const int rid = __shfl_sync(0xffffffffu, id, r);
       if ((mine >> r) & 1u) {
+#pragma unroll 4
         for (int sp = 0; sp < a.splits; ++sp) {
           const float* row = a.mid + ((int64_t)sp * a.M + m0 + r) * a.Rp;
 #pragma unroll
@@ -558,7 +576,10 @@ int64_t lora_workspace(int64_t M, int64_t K, int64_t N, int R, int n) {
 template <typename T, int NT, bool VEC>
 static cudaError_t lora_down_t(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
   const int64_t rows = 16 * p.mt_down;
-  const dim3 grid((unsigned)((a.M + rows - 1) / rows), (unsigned)p.splits, (unsigned)p.z_down);
+  // beside the stream kernel most tiles are not this one's: few CTAs look them over
+  int64_t tiles = (a.M + rows - 1) / rows;
+  if (a.streamed && tiles > 2 * num_sms()) tiles = 2 * num_sms();
+  const dim3 grid((unsigned)tiles, (unsigned)p.splits, (unsigned)p.z_down);
   if constexpr (NT <= 8) {
     if (p.mt_down == 2) {
       lora_down_kernel<T, NT, 2, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);
@@ -612,7 +633,10 @@ static cudaError_t lora_t(LoraArgs a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
   }
 #define IC_DOWN(NT) e = vec ? lora_down_t<T, NT, true>(c, p, st) : lora_down_t<T, NT, false>(c, p, st)
-  for (int r0 = 0; r0 < a.R; r0 += 128) {   // accumulators hold 128 ranks
+  // (16 or more rows of a request together: 16 rows have at most two adapters,
+  // and the stream leaves nothing)
+  const int todo = stream && a.rows_per_id >= 16 ? 0 : a.R;
+  for (int r0 = 0; r0 < todo; r0 += 128) {   // accumulators hold 128 ranks
     LoraArgs c = a;
     c.r0 = r0;
     c.Rc = a.R - r0 < 128 ? a.R - r0 : 128;

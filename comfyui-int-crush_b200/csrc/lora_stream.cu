@@ -2,8 +2,9 @@
 // shared memory.  One warp feeds rings with TMA, eight warps of 16 rows each
 // compute.  HBM bounds both: loads and stores in flight take no registers here,
 // which is what limits lora_down_kernel and lora_up_kernel at this size (8 x
-// 4095 rows, 5120 to 13824 columns, rank 32: 263 us for the first product
-// register-fed, XX us here; 520 us for the second, XX us here).
+// 4095 rows, 5120 to 13824 columns, rank 32, one sample without an adapter:
+// 263 us for the first product register-fed, 77 us here; second 520 us and 360
+// us here, 5.0 TB/s).
 #include "ic_common.cuh"
 
 namespace ic {
@@ -17,19 +18,46 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
+// The ids of a tile's 128 rows and the adapters among them, in shared memory
+// (warp 0 builds the list; a __syncthreads before and after).  Returns their
+// number; `bad`: some id names no adapter.
+__device__ __forceinline__ int lora_tile_list(const int* ids, int* list, int lane, bool& bad) {
+  int n = 0;
+  bad = false;
+  for (int q = 0; q < 4; ++q) {
+    const int id = ids[32 * q + lane];
+    bad = __any_sync(0xffffffffu, id == -2) || bad;
+    for (unsigned todo = __ballot_sync(0xffffffffu, id >= 0); todo;) {
+      const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+      todo &= ~__ballot_sync(0xffffffffu, id == ad);
+      bool old = false;
+      for (int i = lane; i < n; i += 32) old = old || list[i] == ad;
+      if (!__any_sync(0xffffffffu, old)) {
+        if (lane == 0) list[n] = ad;
+        ++n;
+      }
+      __syncwarp();
+    }
+  }
+  return n;
+}
+
 // ------------------------------------------------------------------- down
-// mid[split][m] = x[m] @ down_a^T over a part of K, for tiles of 128 rows that
-// share one adapter (others: lora_down_kernel; tiles without one: nothing).
-// Stages of 64 k: 128 rows of x and R rows of down, 128B-swizzled, read as MMA
-// fragments by ldmatrix without bank conflicts.
+// mid[split][m] = x[m] @ down_a^T over a part of K, for tiles of 128 rows with
+// at most two adapters in each 16 rows (others: lora_down_kernel).  Blocks of
+// 64 k, 128B-swizzled, read as MMA fragments by ldmatrix without bank
+// conflicts, in two rings: 128 rows of x, and R rows of down for each of the
+// tile's adapters in turn.  A warp takes part in its rows' adapters only, with
+// a set of sums for each, so no row's sum sees another adapter.
 template <int NT>
 struct LdCfg {
-  static constexpr int STAGES = 4;
+  static constexpr int SX = 4, SD = 6;
   static constexpr int X = 128 * 128;
   static constexpr int DOWN = NT * 8 * 128;            // 1024 or more
-  static constexpr int STAGE = X + DOWN;
-  static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int SMEM = OFF_BAR + 128;
+  static constexpr int OFF_DOWN = SX * X;
+  static constexpr int OFF_IDS = OFF_DOWN + SD * DOWN;
+  static constexpr int OFF_BAR = OFF_IDS + 1024;       // ids of the rows, adapters among them
+  static constexpr int SMEM = OFF_BAR + 256;
   static constexpr int THREADS = 32 * (kLoraWarps + 1);
 };
 
@@ -38,94 +66,136 @@ __global__ void __launch_bounds__(LdCfg<NT>::THREADS)
 lora_down_stream_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_down,
                         const LoraArgs a) {
   using C = LdCfg<NT>;
-  constexpr int S = C::STAGES;
+  constexpr int SX = C::SX, SD = C::SD;
   extern __shared__ __align__(1024) uint8_t smem[];   // no static shared memory: the declared alignment holds
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [S] TMA -> warps
-  uint64_t* empty = full + S;                                        // [S] warps -> TMA
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S);
+  int* ids = reinterpret_cast<int*>(smem + C::OFF_IDS);
+  int* list = ids + 128;
+  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [SX] TMA -> warps
+  uint64_t* x_empty = x_full + SX;                                     // [SX] warps -> TMA
+  uint64_t* d_full = x_empty + SX;                                     // [SD]
+  uint64_t* d_empty = d_full + SD;                                     // [SD]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(d_empty + SD);
+  volatile int* count = abort_flag + 1;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int64_t m0 = (int64_t)blockIdx.x * 128;
-  const int ad = lora_tile_id(a, m0, lane);
-  if (ad < 0) return;   // all warps see the same ids
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S; ++i) {
-      mbar_init(full + i, 1);
-      mbar_init(empty + i, kLoraWarps);
+    for (int i = 0; i < SX; ++i) {
+      mbar_init(x_full + i, 1);
+      mbar_init(x_empty + i, kLoraWarps);
+    }
+    for (int i = 0; i < SD; ++i) {
+      mbar_init(d_full + i, 1);
+      mbar_init(d_empty + i, kLoraWarps);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x < 128) ids[threadIdx.x] = lora_id(a, m0 + threadIdx.x, 1, 0);
   __syncthreads();
+  bool more = false;
+  int a0 = -1, a1 = -1;   // this warp's adapters
+  if (warp < kLoraWarps) more = lora_two(lane < 16 ? ids[16 * warp + lane] : -1, 0xffffu, a0, a1);
+  if (__syncthreads_or(more)) return;
+  if (warp == 0) {
+    bool bad;
+    const int n = lora_tile_list(ids, list, lane, bad);
+    if (lane == 0) *count = n;
+  }
+  __syncthreads();
+  const int passes = *count;
+  if (passes == 0) return;
   const int all = (int)((a.K + 63) / 64), per = (all + a.splits - 1) / a.splits;
   const int k0 = min((int)blockIdx.y * per, all), steps = min(k0 + per, all) - k0;
 
   if (warp == kLoraWarps) {
     if (lane == 0) {
       bool ok = true;
-      int i = 0;
-      for (; i < steps; ++i) {
-        const int st = i % S;
-        ok = mbar_wait(empty + st, ((i / S) & 1) ^ 1, abort_flag);
+      int i = 0, u = 0;   // blocks of x and of down issued
+      while (ok && i < steps) {
+        const int st = i % SX;
+        ok = mbar_wait(x_empty + st, ((i / SX) & 1) ^ 1, abort_flag);
         if (!ok) break;
-        mbar_arrive_expect_tx(full + st, C::STAGE);
-        tma_load_2d(smem + st * C::STAGE, &tm_x, full + st, 64 * (k0 + i), (int)m0);
-        tma_load_2d(smem + st * C::STAGE + C::X, &tm_down, full + st, 64 * (k0 + i), ad * a.R);
+        mbar_arrive_expect_tx(x_full + st, C::X);
+        tma_load_2d(smem + st * C::X, &tm_x, x_full + st, 64 * (k0 + i), (int)m0);
+        ++i;
+        for (int p = 0; p < passes; ++p) {
+          const int su = u % SD;
+          ok = mbar_wait(d_empty + su, ((u / SD) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(d_full + su, C::DOWN);
+          tma_load_2d(smem + C::OFF_DOWN + su * C::DOWN, &tm_down, d_full + su, 64 * (k0 + i - 1), list[p] * a.R);
+          ++u;
+        }
       }
       if (!ok) {   // given up: every copy issued lands before the CTA may leave
         volatile int never = 0;
-        for (int u = i > S ? i - S : 0; u < i; ++u) mbar_wait(full + u % S, (u / S) & 1, &never);
+        for (int q = i > SX ? i - SX : 0; q < i; ++q) mbar_wait(x_full + q % SX, (q / SX) & 1, &never);
+        for (int q = u > SD ? u - SD : 0; q < u; ++q) mbar_wait(d_full + q % SD, (q / SD) & 1, &never);
       }
     }
     return;
   }
-  float acc[NT][4];
+  float acc[2][NT][4];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[q][j][0] = acc[q][j][1] = acc[q][j][2] = acc[q][j][3] = 0.f;
   // ldmatrix: lane i names row i % 8 of matrix i / 8.  x: rows 0-7 | 8-15 at k,
   // then at k + 8; down: ranks 0-7 at k, k + 8, then ranks 8-15
   const int row = warp * 16 + (lane & 15), xc = lane >> 4;
   const int rank = (lane & 7) + 8 * (lane >> 4), dc = (lane >> 3) & 1;
   const uint32_t base = smem_u32(smem);
-  bool ok = true;
-  for (int i = 0; ok && i < steps; ++i) {
-    const int st = i % S;
-    ok = __all_sync(0xffffffffu, mbar_wait(full + st, (i / S) & 1, abort_flag));
-    if (!ok) return;
-    const uint32_t xs = base + st * C::STAGE, ds = xs + C::X;
+  const auto product = [&](float (&c)[NT][4], uint32_t xs, uint32_t ds) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {   // 16 k: chunks 2k, 2k + 1
       uint32_t xf[4];
       ldmatrix4(xf, xs + row * 128 + (((2 * k + xc) ^ (row & 7)) << 4));
 #pragma unroll
       for (int j = 0; j < NT; j += 2) {
+        // (8 ranks: the second pair of matrices is the first again)
+        const int r = NT == 1 ? lane & 7 : 8 * j + rank;
         uint32_t df[4];
-        if constexpr (NT == 1) {   // 8 ranks: the second pair of matrices is the first again
-          ldmatrix4(df, ds + (lane & 7) * 128 + (((2 * k + dc) ^ (lane & 7)) << 4));
-        } else {
-          const int r = 8 * j + rank;
-          ldmatrix4(df, ds + r * 128 + (((2 * k + dc) ^ (r & 7)) << 4));
-        }
-        lora_mma<T>(acc[j], xf[0], xf[1], xf[2], xf[3], df[0], df[1]);
-        if constexpr (NT > 1) lora_mma<T>(acc[j + 1], xf[0], xf[1], xf[2], xf[3], df[2], df[3]);
+        ldmatrix4(df, ds + r * 128 + (((2 * k + dc) ^ (r & 7)) << 4));
+        lora_mma<T>(c[j], xf[0], xf[1], xf[2], xf[3], df[0], df[1]);
+        if constexpr (NT > 1) lora_mma<T>(c[j + 1], xf[0], xf[1], xf[2], xf[3], df[2], df[3]);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(empty + st);
+  };
+  bool ok = true;
+  int u = 0;
+  for (int i = 0; i < steps; ++i) {
+    const int st = i % SX;
+    ok = __all_sync(0xffffffffu, mbar_wait(x_full + st, (i / SX) & 1, abort_flag));
+    if (!ok) return;
+    for (int p = 0; p < passes; ++p, ++u) {
+      const int su = u % SD, ad = list[p];
+      ok = __all_sync(0xffffffffu, mbar_wait(d_full + su, (u / SD) & 1, abort_flag));
+      if (!ok) return;
+      const uint32_t xs = base + st * C::X, ds = base + C::OFF_DOWN + su * C::DOWN;
+      if (ad == a0) product(acc[0], xs, ds);
+      else if (ad == a1) product(acc[1], xs, ds);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_empty + su);
+    }
+    if (lane == 0) mbar_arrive(x_empty + st);
   }
   const int g = lane >> 2, t = lane & 3;
   float* mid = a.mid + (int64_t)blockIdx.y * a.M * a.Rp;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t m = m0 + 16 * warp + 8 * h + g;
-    if (m >= a.M) continue;
+    const int id = ids[16 * warp + 8 * h + g];
+    if (id < 0) continue;
+    const bool second = id != a0;
     // ranks past R: rows of another adapter, zeros in mid
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int r = 8 * j + 2 * t;
+      const float v0 = second ? acc[1][j][2 * h] : acc[0][j][2 * h];
+      const float v1 = second ? acc[1][j][2 * h + 1] : acc[0][j][2 * h + 1];
       if (8 * j < a.Rp)
-        *reinterpret_cast<float2*>(mid + m * a.Rp + r) =
-            make_float2(r < a.R ? acc[j][2 * h] : 0.f, r + 1 < a.R ? acc[j][2 * h + 1] : 0.f);
+        *reinterpret_cast<float2*>(mid + m * a.Rp + r) = make_float2(r < a.R ? v0 : 0.f, r + 1 < a.R ? v1 : 0.f);
     }
   }
 }
@@ -188,23 +258,9 @@ lora_up_stream_kernel(const __grid_constant__ CUtensorMap tm_base, const __grid_
     if (id == -2) set_dev_error(IC_DEV_ERR_INDEX);
   }
   __syncthreads();
-  if (warp == 0) {   // the adapters among the rows
-    int n = 0, bad = 0;
-    for (int q = 0; q < 4; ++q) {
-      const int id = ids[32 * q + lane];
-      bad |= __any_sync(0xffffffffu, id == -2);
-      for (unsigned todo = __ballot_sync(0xffffffffu, id >= 0); todo;) {
-        const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
-        todo &= ~__ballot_sync(0xffffffffu, id == ad);
-        bool old = false;
-        for (int i = lane; i < n; i += 32) old = old || list[i] == ad;
-        if (!__any_sync(0xffffffffu, old)) {
-          if (lane == 0) list[n] = ad;
-          ++n;
-        }
-        __syncwarp();
-      }
-    }
+  if (warp == 0) {
+    bool bad;
+    const int n = lora_tile_list(ids, list, lane, bad);
     if (lane == 0) *count = n == 0 && !bad && a.base == a.out && a.ldb == a.ldo ? -1 : n;   // -1: already there
   }
   __syncthreads();

@@ -583,3 +583,37 @@ def test_lora_refusals():
     with pytest.raises(RuntimeError, match="CUDA"):
         rt.lora_batched(x, down, up, ids.cpu())
     assert rt.lora_batched(h(0, 64), down, up, ids[:0]).shape == (0, 32)
+
+
+# ── together ─────────────────────────────────────────────────────────────────
+
+def test_conditioned_attention_example():
+    """INT8 projections with adapters, head norms and rotation, attention to
+    ragged texts: within a few fp16 roundings (2^-11 each, four in a row) and
+    the few INT8 steps that they flip (a step is 1/127 of a row's largest value,
+    and one value in a thousand moves)."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(__file__), "..", "examples", "conditioned_attention.py")
+    spec = importlib.util.spec_from_file_location("conditioned_attention", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main() < 4 * 2.0 ** -11
+
+
+def test_torch_library_ops():
+    load("_torch_ops")
+    ops = torch.ops.intcrush_b200
+    g = gen(20)
+    q, k = normal(g, 2, 9, 4, 64, dtype=torch.float16), normal(g, 2, 9, 2, 64, dtype=torch.float16)
+    cos, sin = tables(9, 64, g)
+    got = ops.qk_norm_rope(q, k, None, None, cos, sin, "half", None, 1e-6)
+    want = rt.qk_norm_rope(q, k, cos=cos, sin=sin, layout="half")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(ops.cross_attention(q, k, k, None, None, 0.125), rt.cross_attention(q, k, k))
+    x, base, down, up, scales, _ = lora_inputs(21, 12, 64, 40, 8, 2, torch.float16)
+    ids = torch.tensor([0, 1, -1], device="cuda")
+    assert torch.equal(ops.lora_batched(x, down, up, ids, scales, base), rt.lora_batched(x, down, up, ids, scales, base=base))
+    for op, args in ((ops.cross_attention, (q, k, k, None, None, 0.125)), (ops.lora_batched, (x, down, up, ids, None, None))):
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
