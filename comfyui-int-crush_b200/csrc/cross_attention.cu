@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(1024) xattn_mask_kernel(const void* mask, int6
 // the warp's own in shared memory: every lane reads back what it copied, so the
 // ring needs no barrier, and its registers leave room for three CTAs per SM.
 // 8 single tokens of 32 heads over 8 key heads of 128, 1024 to 8192 keys (151
-// MB): 46 us with the join, 3.3 TB/s; loads straight to registers 49 us.  The
-// copies alone take 44 us of that, the arithmetic alone 22.
+// MB): 46 us with the join, 3.3 TB/s, as the tcgen05 kernel; loads straight to
+// registers 49 us.  The copies alone take 44 us of that, the arithmetic alone 22.
 // Softmax: scores, maxima and sums in fp32; the running maximum of a row only
 // moves when it grows by more than 2^8 (the sums stay exact, p stays below
 // 2^8), so most blocks rescale nothing.  p enters the product with V rounded
@@ -391,9 +391,19 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XattnArgs a) {
 }
 
 // ---------------------------------------------------------------- launches
+// The tcgen05 kernel takes over above 8 query rows of a key head (tokens times
+// heads), and for fewer from 2^15 rows of keys in the batch.  Measured, few-rows
+// against tcgen05 kernel: 1 x 8 rows, 24 heads, 512 keys 9.9 / 10.6 us, 16 rows
+// 11.5 / 10.6; 8 x 1 token, 32 heads over 8, 1024 keys 20.5 / 15.2; 1 token of 24
+// heads over 512 keys 9.5 / 10.4, of 8 heads over 77 keys 3.9 / 5.3.
+constexpr int64_t kTcRows = 8, kTcKeys = 1 << 15;
+// Items per SM that its keys are split for: 8 x 1 token of 32 heads over 8, 1024
+// to 8192 keys: one 59 us, two 46.6, four 47.5, eight 52.
+constexpr int64_t kTcItems = 2;
+
 // Splits of the few-rows kernel: four CTAs per SM, with at least 8 blocks of 16
-// keys (two per warp) in a part (the case above: two CTAs 57 us, three 48 to
-// 53, four 46, six 50 to 55, ten 52).
+// keys (two per warp) in a part (the case above: two CTAs per SM 57 us, three
+// 48 to 53, four 46, six 50 to 55, ten 52).
 static int rows_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk) {
   const int64_t ctas = (Lq * (H / Hk) + 15) / 16 * B * Hk;
   const int64_t blocks = (Lk + 15) / 16;
@@ -403,19 +413,16 @@ static int rows_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk) {
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
-// Query tokens above which the tcgen05 kernel takes over: its tile holds 128 of
-// one head, the few-rows one 16 of all heads that share a key head.
-constexpr int64_t kTcRows = 48;
-
 // Splits and slots of the tcgen05 kernel: two query tiles per CTA share K and
 // V; with too few tiles for that to fill the SMs, one, and then the keys are
 // split with two tiles of 128 at least in a part.
 static int tc_splits(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int* slots) {
   const int64_t sms = num_sms();
-  const int64_t tiles = H / Hk * ((Lq + 127) / 128);
+  const int64_t packed = xattn_packed(H, Hk);
+  const int64_t tiles = H / Hk / packed * ((Lq * packed + 127) / 128);
   *slots = B * Hk * tiles <= sms ? 1 : 2;
   const int64_t items = B * Hk * ((tiles + *slots - 1) / *slots);
-  int64_t s = sms / items;
+  int64_t s = kTcItems * sms / items;
   const int64_t most = ((Lk + 127) / 128 + 1) / 2;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -425,7 +432,7 @@ XattnPlan xattn_plan(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int D, in
   XattnPlan p;
   p.slots = 0;
   if (Lk == 0) p.splits = 1;
-  else if (Lq > kTcRows) p.splits = tc_splits(B, Lq, Lk, H, Hk, &p.slots);
+  else if (Lq * (H / Hk) > kTcRows || B * Hk * Lk >= kTcKeys) p.splits = tc_splits(B, Lq, Lk, H, Hk, &p.slots);
   else p.splits = rows_splits(B, Lq, Lk, H, Hk);
   p.Lkp = mask_kind ? (Lk + 127) / 128 * 128 : 0;
   const int64_t rows = B * Lq * H;

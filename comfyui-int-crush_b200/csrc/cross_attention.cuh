@@ -37,6 +37,12 @@ struct XattnPlan {
   int64_t floats;              // workspace
 };
 
+// Query heads of a key head that share a tile of the tcgen05 kernel.
+inline int xattn_packed(int H, int Hk) {
+  const int group = H / Hk;
+  return 128 % group == 0 ? group : 1;
+}
+
 template <typename T>
 cudaError_t launch_xattn_tc(const XattnArgs& a, int slots, cudaStream_t st);   // cross_attention_tc.cu
 XattnPlan xattn_plan(int64_t B, int64_t Lq, int64_t Lk, int H, int Hk, int D, int mask_kind);

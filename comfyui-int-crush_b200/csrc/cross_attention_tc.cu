@@ -1,7 +1,8 @@
 // Cross attention for many query rows on tcgen05 (kind::f16).
 //
 // Persistent, one CTA per SM, 16 warps.  A work item is one key head of one
-// sample with one or two tiles of 128 query rows ("slots"; the slots share the
+// sample with one or two tiles of 128 query rows (all query heads that share the
+// key head in turn for each token, where their number divides 128) ("slots"; the slots share the
 // K and V tiles), over the item's part of the keys in tiles of 128:
 //   S_s = Q_s K^T            128 x 128 into tensor memory
 //   P_s = 2^(S_s c - m)      registers, written back over S_s as 16-bit pairs
@@ -66,8 +67,11 @@ struct XtArgs {
   XattnArgs x;
   XtDiv by_split, by_head, by_hk, by_tiles;   // splits, items of a key head, key heads, query tiles of a head
   int slots;          // query tiles of an item: 1 or 2
-  int tiles_per_head; // ceil(Lq / 128)
-  int group, tiles;   // query heads, query tiles of a key head
+  int group;          // query heads of a key head
+  int packed;         // of them in a tile: row r is token r / packed, head r % packed
+  int pack_shift;     // log2
+  int tiles_per_head; // tiles of `packed` heads
+  int tiles;          // query tiles of a key head
   int wide;           // output rows take 32-byte stores
   int items;
   int qm[2], km[2], vm[2];   // 0 where the batch / head stride is 0 (coordinate 0), else 1
@@ -97,12 +101,12 @@ __device__ __forceinline__ XtItem xt_item(const XtArgs& a, int i) {
   t.key0 = t0 * 128;
   return t;
 }
-// head and first row of slot s
+// first head and first token of slot s
 __device__ __forceinline__ void xt_slot(const XtArgs& a, const XtItem& t, int s, int& h, int& l0) {
   const int q = t.tile0 + s;
   const int sub = xt_quot(a.by_tiles, q);
-  h = t.hk * a.group + sub;
-  l0 = (q - sub * a.tiles_per_head) * 128;
+  h = t.hk * a.group + (sub << a.pack_shift);
+  l0 = (q - sub * a.tiles_per_head) * (128 >> a.pack_shift);
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
@@ -494,7 +498,9 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (s >= t.nslots || !ok) continue;
         int h, l0;
         xt_slot(a, t, s, h, l0);
-        const int64_t l = l0 + w * 32 + lane;
+        const int row_in_tile = w * 32 + lane;
+        const int64_t l = l0 + (row_in_tile >> a.pack_shift);
+        h += row_in_tile & (a.packed - 1);
         float m = -INFINITY, sum = 0.f;
         if (t.nt) {
           ok = all_lanes(mbar_wait(l_full + s, ph[s], abort_flag));
@@ -722,7 +728,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // entry that every coordinate maps to; a dimension of one entry takes any
 // stride.
 static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, int64_t D, int64_t heads, int64_t tokens,
-                   int64_t batch, int* mul) {
+                   int64_t batch, int box_heads, int* mul) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   mul[0] = st[0] == 0 ? 0 : 1;
@@ -732,7 +738,7 @@ static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, in
   const int64_t el[3] = {st[2], st[1], st[0]};
   cuuint64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 * ((cuuint64_t)D / 8) : (cuuint64_t)el[i] * 2;
-  cuuint32_t box[4] = {64, 1, 128, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)(128 / box_heads), 1};
   cuuint32_t one[4] = {1, 1, 1, 1};
   return fn(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), dims,
             strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -755,9 +761,11 @@ cudaError_t launch_xattn_tc(const XattnArgs& x, int slots, cudaStream_t st) {
   XtArgs a;
   a.x = x;
   a.slots = slots;
-  a.tiles_per_head = (int)((x.Lq + 127) / 128);
   a.group = x.H / x.Hk;
-  const int64_t tiles = (int64_t)a.group * a.tiles_per_head;
+  a.packed = x.qs[2] != 0 ? xattn_packed(x.H, x.Hk) : 1;
+  for (a.pack_shift = 0; (1 << a.pack_shift) < a.packed;) ++a.pack_shift;
+  a.tiles_per_head = (int)((x.Lq * a.packed + 127) / 128);
+  const int64_t tiles = (int64_t)(a.group / a.packed) * a.tiles_per_head;
   const int64_t per_head = (tiles + slots - 1) / slots;
   const int64_t items = x.B * x.Hk * per_head * x.splits;
   if (items + num_sms() >= (1 << 30) || tiles >= (1 << 30)) return cudaErrorInvalidValue;
@@ -770,9 +778,9 @@ cudaError_t launch_xattn_tc(const XattnArgs& x, int slots, cudaStream_t st) {
   a.by_hk = xt_div((uint32_t)x.Hk);
   a.by_tiles = xt_div((uint32_t)a.tiles_per_head);
   CUtensorMap m[3];
-  if (!xt_map(&m[0], BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, a.qm) ||
-      !xt_map(&m[1], BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, a.km) ||
-      !xt_map(&m[2], BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, a.vm))
+  if (!xt_map(&m[0], BF, x.q, x.qs, x.D, x.H, x.Lq, x.B, a.packed, a.qm) ||
+      !xt_map(&m[1], BF, x.k, x.ks, x.D, x.Hk, x.Lk, x.B, 1, a.km) ||
+      !xt_map(&m[2], BF, x.v, x.vs, x.D, x.Hk, x.Lk, x.B, 1, a.vm))
     return cudaErrorInvalidValue;
   if (x.D <= 64) return x.bias ? launch_xt<T, 64, true>(m, a, st) : launch_xt<T, 64, false>(m, a, st);
   return x.bias ? launch_xt<T, 128, true>(m, a, st) : launch_xt<T, 128, false>(m, a, st);
