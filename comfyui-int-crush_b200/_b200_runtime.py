@@ -15,7 +15,9 @@ New fused ops beyond the reference's set: ``prep_quantize`` (SmoothRot +
 Hadamard + pad + PermuQuant + smooth + per-token INT8 in one pass),
 ``gemm_a8`` (W8A8 / W4A8 with per-channel or group scales, bias and the
 zero-point term fused), ``gemm_w4a16`` (weight-streaming W4A16 with the
-low-rank residual fused), ``lowrank_down`` / ``lowrank_add``.
+low-rank residual fused), ``lowrank_down`` / ``lowrank_add``.  Beside the
+projections: ``qk_norm_rope`` (head norms and rotation in one pass),
+``cross_attention`` and ``lora_batched`` (an adapter per request).
 """
 
 from __future__ import annotations
