@@ -716,6 +716,12 @@ def _strides12(*strides):
     return (ctypes.c_int64 * 12)(*strides)
 
 
+# Workspace floats by sizes (and device: the plans go by its SM count).
+@functools.lru_cache(maxsize=4096)
+def _workspace(name: str, index: int, *sizes: int) -> int:
+    return getattr(L.lib(), name)(*sizes)
+
+
 def _same_device(what: str, index: int, *ts: torch.Tensor | None) -> None:
     """All of ``ts`` on CUDA device ``index`` (as ``_need_cuda``)."""
     if index < 0 or not B200_LIBRARY_LOADED:
@@ -898,12 +904,10 @@ def cross_attention(
             ld = Lk
     y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _out_heads("cross_attention", out, q)
     q, k, v = _heads(q), _heads(k), _heads(v)
-    lib = L.lib()
-    n = lib.ic_cross_attention_workspace(B, Lq, Lk, H, Hk, D, kind)
-    if n < 0:
-        L.check(L.IC_ERR_ARG, "ic_cross_attention")
-    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    st = lib.ic_cross_attention(
+    n = _workspace("ic_cross_attention_workspace", index, B, Lq, Lk, H, Hk, D, kind)
+    # (sizes that are refused: the call below says why)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
+    st = L.lib().ic_cross_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dtype, B, Lq, Lk, H, Hk, D,
         _strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3]),
         D ** -0.5 if scale is None else scale, None if kv_lens is None else kv_lens.data_ptr(),
@@ -984,16 +988,14 @@ def lora_batched(
             raise ValueError(f"lora_batched: out must be row-major, got strides {out.stride()}")
     if M == 0 or N == 0:
         return out
-    lib = L.lib()
-    need = lib.ic_lora_batched_workspace(M, K, N, R, n)
-    if need < 0:
-        L.check(L.IC_ERR_ARG, "ic_lora_batched")
-    ws = torch.empty(need, dtype=torch.float32, device=x.device)
+    need = _workspace("ic_lora_batched_workspace", index, M, K, N, R, n)
+    # (sizes that are refused: the call below says why)
+    ws = torch.empty(max(need, 0), dtype=torch.float32, device=x.device)
     if not down.is_contiguous():
         down = down.contiguous()
     if not up.is_contiguous():
         up = up.contiguous()
-    st = lib.ic_lora_batched(
+    st = L.lib().ic_lora_batched(
         x2.data_ptr(), dtype, M, K, x2.stride(0) if M > 1 else K, down.data_ptr(), up.data_ptr(), R, n, ids.data_ptr(),
         M // S, None if scales is None else scales.data_ptr(), None if b2 is None else b2.data_ptr(),
         N if b2 is None or M == 1 else b2.stride(0), out.data_ptr(), N, ldo, ws.data_ptr(), need, _raw_stream(index))

@@ -119,8 +119,8 @@ __device__ __forceinline__ bool lora_tile_left(const LoraArgs& a, int64_t tile0,
 }
 
 // mid partials.  The CTA's warps share a tile of 16 * MT rows and cut its part
-// of K between them.  blockIdx: row tiles (in turns, beside the stream kernel),
-// K parts, passes (pass p is taken by the CTA with z = p % gridDim.z).
+// of K between them.  blockIdx: row tiles and K parts (in turns, beside the
+// stream kernel), passes (pass p is taken by the CTA with z = p % gridDim.z).
 template <typename T, int NT, int MT, bool VEC>
 __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraArgs a) {
   constexpr int ROWS = 16 * MT;
@@ -131,11 +131,12 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
   const T* down = reinterpret_cast<const T*>(a.down);
   const int64_t steps = (a.K + 31) / 32;
   const int64_t per = (steps + a.splits - 1) / a.splits;
-  const int64_t s0 = (int64_t)blockIdx.y * per, s1 = min(s0 + per, steps);
 
   for (int64_t m0 = (int64_t)blockIdx.x * ROWS; m0 < a.M; m0 += (int64_t)gridDim.x * ROWS) {
   if (a.streamed && !lora_tile_left(a, m0 / 128 * 128, lane)) continue;   // lora_down_stream_kernel's
   const int id = lora_id(a, m0, ROWS, lane);
+  for (int part = blockIdx.y; part < a.splits; part += gridDim.y) {
+  const int64_t s0 = part * per, s1 = min(s0 + per, steps);
   unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
   for (unsigned pass = 0; todo; ++pass) {
     const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
       __syncthreads();
     }
     if (warp != 0) continue;
-    float* mid = a.mid + (int64_t)blockIdx.y * a.M * a.Rp + a.r0;
+    float* mid = a.mid + (int64_t)part * a.M * a.Rp + a.r0;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
             *reinterpret_cast<float2*>(mid + (m0 + r) * a.Rp + j * 8 + 2 * t) =
                 make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
       }
+  }
   }
   }
 }
@@ -578,8 +580,13 @@ static cudaError_t lora_down_t(const LoraArgs& a, const LoraPlan& p, cudaStream_
   const int64_t rows = 16 * p.mt_down;
   // beside the stream kernel most tiles are not this one's: few CTAs look them over
   int64_t tiles = (a.M + rows - 1) / rows;
-  if (a.streamed && tiles > 2 * num_sms()) tiles = 2 * num_sms();
-  const dim3 grid((unsigned)tiles, (unsigned)p.splits, (unsigned)p.z_down);
+  int64_t parts = p.splits;
+  if (a.streamed) {
+    const int64_t most = 2 * num_sms();
+    tiles = tiles < most ? tiles : most;
+    parts = parts < most / tiles ? parts : most / tiles;
+  }
+  const dim3 grid((unsigned)tiles, (unsigned)parts, (unsigned)p.z_down);
   if constexpr (NT <= 8) {
     if (p.mt_down == 2) {
       lora_down_kernel<T, NT, 2, VEC><<<grid, 32 * kLoraWarps, 0, st>>>(a);

@@ -423,7 +423,7 @@ def test_cross_attention_refusals():
         rt.cross_attention(q, k, k, key_mask=torch.zeros(2, 5, dtype=torch.bool, device="cuda"))
     with pytest.raises(TypeError, match="key_mask"):
         rt.cross_attention(q, k, k, key_mask=torch.zeros(2, 6, dtype=torch.int32, device="cuda"))
-    with pytest.raises(ValueError, match="multiple of 8 up to 128"):
+    with pytest.raises(RuntimeError, match="multiple of 8 up to 128"):
         rt.cross_attention(*(torch.zeros(1, 2, 2, 136, dtype=torch.float16, device="cuda"),) * 3)
     with pytest.raises(RuntimeError, match="CUDA"):
         rt.cross_attention(q.cpu(), k, k)
@@ -578,7 +578,7 @@ def test_lora_refusals():
         rt.lora_batched(x, down, up, ids, base=h(4, 31))
     with pytest.raises(ValueError, match="out must"):
         rt.lora_batched(x, down, up, ids, out=h(5, 32))
-    with pytest.raises(ValueError, match="rank"):
+    with pytest.raises(RuntimeError, match="rank"):
         rt.lora_batched(x, h(2, 257, 64), h(2, 32, 257), ids)
     with pytest.raises(RuntimeError, match="CUDA"):
         rt.lora_batched(x, down, up, ids.cpu())
