@@ -702,6 +702,7 @@ def unpack_int4_to_float16(packed: torch.Tensor, scale: torch.Tensor, K: int,
 _MASKS = {torch.bool: L.IC_MASK_BOOL, torch.float16: L.IC_MASK_F16, torch.bfloat16: L.IC_MASK_BF16,
           torch.float32: L.IC_MASK_F32}
 _ROPE = {"interleaved": L.IC_ROPE_INTERLEAVED, "half": L.IC_ROPE_HALF}
+_DENSE = torch.contiguous_format
 _HALF = {torch.float16: L.IC_DTYPE_F16, torch.bfloat16: L.IC_DTYPE_BF16}
 
 # These calls are short on the device, so their host side is kept short too:
@@ -829,7 +830,7 @@ def qk_norm_rope(
         positions = _index(positions)
     gq = _gamma16("qk_norm_rope", q_gamma, D)
     x = _heads(q)
-    y = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else _out_heads("qk_norm_rope", q_out, q)
+    y = torch.empty_like(q, memory_format=_DENSE) if q_out is None else _out_heads("qk_norm_rope", q_out, q)
     if k is None:
         if k_gamma is not None or k_out is not None:
             raise ValueError("qk_norm_rope: k_gamma / k_out without a k")
@@ -841,7 +842,7 @@ def qk_norm_rope(
         Hk = k.shape[2]
         gk = _gamma16("qk_norm_rope", k_gamma, D)
         xk = _heads(k)
-        yk = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else _out_heads("qk_norm_rope", k_out, k)
+        yk = torch.empty_like(k, memory_format=_DENSE) if k_out is None else _out_heads("qk_norm_rope", k_out, k)
         strides = _strides12(*x.stride()[:3], *y.stride()[:3], *xk.stride()[:3], *yk.stride()[:3])
     st = L.lib().ic_qk_norm_rope(
         x.data_ptr(), y.data_ptr(), H, None if xk is None else xk.data_ptr(), None if yk is None else yk.data_ptr(), Hk,
@@ -902,11 +903,11 @@ def cross_attention(
         if 0 < ld < Lk:
             key_mask = key_mask.contiguous()
             ld = Lk
-    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _out_heads("cross_attention", out, q)
+    y = torch.empty_like(q, memory_format=_DENSE) if out is None else _out_heads("cross_attention", out, q)
     q, k, v = _heads(q), _heads(k), _heads(v)
     n = _workspace("ic_cross_attention_workspace", index, B, Lq, Lk, H, Hk, D, kind)
     # (sizes that are refused: the call below says why)
-    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
+    ws = q.new_empty(2 * n) if n > 0 else None   # n floats, in 16-bit elements
     st = L.lib().ic_cross_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dtype, B, Lq, Lk, H, Hk, D,
         _strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3]),
@@ -977,7 +978,7 @@ def lora_batched(
             raise ValueError(f"lora_batched: base must be {dt} {full}, got {base.dtype} {tuple(base.shape)}")
         b2 = _rows(base, N)
     if out is None:
-        out = torch.empty(full, dtype=dt, device=x.device)
+        out = torch.empty_like(base) if base is not None and base.is_contiguous() else x.new_empty(full)
         ldo = N
     else:
         if out.dtype != dt or out.shape != full:
@@ -990,7 +991,7 @@ def lora_batched(
         return out
     need = _workspace("ic_lora_batched_workspace", index, M, K, N, R, n)
     # (sizes that are refused: the call below says why)
-    ws = torch.empty(max(need, 0), dtype=torch.float32, device=x.device)
+    ws = x.new_empty(2 * max(need, 0))   # floats, in 16-bit elements
     if not down.is_contiguous():
         down = down.contiguous()
     if not up.is_contiguous():

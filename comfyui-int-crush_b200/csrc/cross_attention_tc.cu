@@ -278,296 +278,296 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   // registers: 512 threads x 128 = 256 x 72 here + 256 x 184 below, where a
   // thread holds a row of S
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp == 8) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      uint32_t use = 0, qn[2] = {0, 0};
-      bool ok = true;
-      const auto load_kv = [&](const CUtensorMap* tm, const XtItem& t, const int* mul, int key) {
-        const uint32_t st = use % NST;
-        if (!mbar_wait(kv_empty + st, ((use / NST) & 1u) ^ 1u, abort_flag)) return false;
-        mbar_arrive_expect_tx(kv_full + st, C::TILE);
-#pragma unroll
-        for (int p = 0; p < C::PANELS; ++p)
-          tma_load_4d(kv_base + st * C::TILE + p * 16384, tm, kv_full + st, 64 * p, t.hk * mul[1], key,
-                      (int)t.b * mul[0]);
-        ++use;
-        return true;
-      };
-      const auto load_q = [&](const XtItem& t, int s) {
-        if (!mbar_wait(q_empty + s, (qn[s] & 1u) ^ 1u, abort_flag)) return false;
-        int h, l0;
-        xt_slot(a, t, s, h, l0);
-        mbar_arrive_expect_tx(q_full + s, C::TILE);
-#pragma unroll
-        for (int p = 0; p < C::PANELS; ++p)
-          tma_load_4d(smem_u32(smem) + s * C::TILE + p * 16384, &tm_q, q_full + s, 64 * p, h * a.qm[1], l0,
-                      (int)t.b * a.qm[0]);
-        ++qn[s];
-        return true;
-      };
-      XtItem t;
-      for (int i = blockIdx.x; ok && next_item(i, t); i += gridDim.x) {
-        // K first: its stage frees before the Q slots of the item before
-        ok = load_kv(&tm_k, t, a.km, t.key0) && load_q(t, 0) && (t.nslots < 2 || load_q(t, 1)) &&
-             load_kv(&tm_v, t, a.vm, t.key0);
-        for (int j = 1; ok && j < t.nt; ++j)
-          ok = load_kv(&tm_k, t, a.km, t.key0 + 128 * j) && load_kv(&tm_v, t, a.vm, t.key0 + 128 * j);
-      }
-      if (!ok) {
-        // given up: every copy issued lands before the CTA may leave
-        volatile int never = 0;
-        for (uint32_t u = use > NST ? use - NST : 0; u < use; ++u)
-          mbar_wait(kv_full + u % NST, (u / NST) & 1u, &never);
-        for (int s = 0; s < 2; ++s)
-          if (qn[s]) mbar_wait(q_full + s, (qn[s] - 1) & 1u, &never);
-      }
-    }
-  } else if (warp == 9) {
-    // ---------------------------------------------------------- MMA issuer
-    const uint32_t on = elect_one();
-    const int ksteps = (a.x.D + 15) / 16;
-    const uint32_t i_pv = idesc_f16(128, ksteps * 16, BF) | (1u << 16);   // B is MN-major
-    uint32_t use = 0, qph = 0, hph = 0, pph = 0, oph = 3;   // a phase bit per slot
-    const auto tile_wait = [&](uint32_t u) {
-      return all_lanes(mbar_wait((clean ? ready : kv_full) + u % NST, (u / NST) & 1u, abort_flag));
-    };
-    const auto slot_wait = [&](uint64_t* bar, uint32_t& ph, int s) {
-      const uint32_t parity = (ph >> s) & 1u;
-      ph ^= 1u << s;
-      return all_lanes(mbar_wait(bar + s, parity, abort_flag));
-    };
-    // keys of tile j of an item, rounded to the MMA's step
-    const auto width = [&](const XtItem& t, int j) { return min(128, (t.end - t.key0 - 128 * j + 15) / 16 * 16); };
-    const auto issue_s = [&](int s, uint32_t u, int n, bool last) {
-      const uint64_t dq = smem_desc_sw128(smem_u32(smem) + s * C::TILE);
-      const uint64_t dk = smem_desc_sw128(kv_base + (u % NST) * C::TILE);
-      const uint32_t idesc = idesc_f16(128, n, BF);
-      const auto step = [&](int k) {   // offsets in descriptor units (16 bytes)
-        const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4);
-        mma_f16_on(on, tmem + s * 128, dq + off, dk + off, idesc, k > 0);
-      };
-      if (ksteps == DP / 16) {
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) step(k);
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < ksteps; ++k) step(k);
-      }
-      mma_commit_on(on, s_full + s);
-      if (last) mma_commit_on(on, q_empty + s);
-    };
-    // P V over the steps [k0, k1) of 16 keys
-    const auto issue_pv = [&](int s, uint32_t u, int k0, int k1, uint32_t accumulate) {
-      const uint64_t dv = smem_desc_mn128(kv_base + (u % NST) * C::TILE) + k0 * (2048 >> 4);
-      const uint32_t pa = tmem + s * 128 + k0 * 8;
-      const auto step = [&](int k) {
-        mma_f16_ts_on(on, tmem + 256 + s * 128, pa + k * 8, dv + k * (2048 >> 4), i_pv, k > 0 ? 1u : accumulate);
-      };
-      if (k1 - k0 == 6) {
-#pragma unroll
-        for (int k = 0; k < 6; ++k) step(k);
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < k1 - k0; ++k) step(k);
-      }
-    };
-    const auto next_uniform = [&](int& i, XtItem& t) {
-      const bool got = next_item(i, t);
-      t.end = uniform(t.end);
-      t.nt = uniform(t.nt);
-      t.key0 = uniform(t.key0);
-      return all_lanes(got);
-    };
-    int i = blockIdx.x;
-    XtItem t, nx;
-    bool have = next_uniform(i, t), ok = true;
-    if (have) {
-      ok = tile_wait(use);
-      for (int s = 0; ok && s < t.nslots; ++s) {
-        ok = slot_wait(q_full, qph, s);
-        if (ok) issue_s(s, use, width(t, 0), t.nt == 1);
-      }
-      if (ok) mma_commit_on(on, kv_empty + use % NST);
-      ++use;
-    }
-    while (have && ok) {
-      i += gridDim.x;
-      const bool more = next_uniform(i, nx);
-      for (int j = 0; ok && j < t.nt; ++j) {
-        const bool last = j == t.nt - 1;
-        const uint32_t uv = use, uk = use + 1;   // V of this tile, the K tile after it
-        const int n = last ? (more ? width(nx, 0) : 0) : width(t, j + 1);
-        const int nslots = n ? (last ? nx.nslots : t.nslots) : 0;   // slots whose next S uses uk
-        const int steps = width(t, j) / 16;
-        ok = tile_wait(uv);
-        for (int s = 0; ok && s < max(t.nslots, nslots); ++s) {
-          // everything that the next S needs first, so that it follows P V at once
-          if (s < nslots) {
-            if (s == 0) ok = tile_wait(uk);
-            if (ok && last) ok = slot_wait(q_full, qph, s);
-            if (!ok) break;
-          }
-          if (s < t.nslots) {
-            if (j == 0) ok = slot_wait(o_empty, oph, s);
-            ok = ok && slot_wait(p_part, hph, s);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(s, uv, 0, min(steps, 6), j > 0);
-            ok = slot_wait(p_full, pph, s);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(s, uv, 6, steps, 1u);
-            if (last) mma_commit_on(on, o_full + s);
-          }
-          if (s < nslots) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
-        }
-        if (!ok) break;
-        mma_commit_on(on, kv_empty + uv % NST);
-        if (n) mma_commit_on(on, kv_empty + uk % NST);
-        use += 2;
-      }
-      t = nx;
-      have = more;
-    }
-    // MMAs in flight and their arrivals end before tensor memory is freed and
-    // the CTA leaves
-    volatile int never = 0;
-    mma_commit_on(on, drain);
-    mbar_wait(drain, 0, &never);
-  } else if (warp == 10) {
-    // ------------------------------------------------------------- cleaner
-    if (clean) {
-      uint32_t use = 0;
-      bool ok = true;
-      const auto pass = [&](bool got) {   // the tile may be used
-        __syncwarp();
-        if (got && lane == 0) mbar_arrive(ready + use % NST);
-        ++use;
-        return got;
-      };
-      const auto landed = [&]() { return all_lanes(mbar_wait(kv_full + use % NST, (use / NST) & 1u, abort_flag)); };
-      XtItem t;
-      for (int i = blockIdx.x; ok && next_item(i, t); i += gridDim.x) {
-        for (int j = 0; ok && j < t.nt; ++j) {
-          ok = pass(landed());   // a K tile
-          ok = ok && landed();
-          if (!ok) break;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      // ------------------------------------------------------------ producer
+      if (lane == 0) {
+        uint32_t use = 0, qn[2] = {0, 0};
+        bool ok = true;
+        const auto load_kv = [&](const CUtensorMap* tm, const XtItem& t, const int* mul, int key) {
           const uint32_t st = use % NST;
-          {
-            const int k0 = t.key0 + 128 * j;
-            const int rows = min(128, (t.end - k0 + 15) / 16 * 16);   // rows that the MMA reads
-            unsigned hide[4];
+          if (!mbar_wait(kv_empty + st, ((use / NST) & 1u) ^ 1u, abort_flag)) return false;
+          mbar_arrive_expect_tx(kv_full + st, C::TILE);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int key = k0 + 32 * q + lane;
-              bool no = key >= t.end;
-              if constexpr (BIAS) no = no || __ldg(a.x.bias + t.b * a.x.Lkp + key) == -INFINITY;
-              hide[q] = __ballot_sync(0xffffffffu, no && 32 * q + lane < rows);
-            }
-            if (hide[0] | hide[1] | hide[2] | hide[3]) {
-              uint8_t* tile = smem + C::OFF_KV + st * C::TILE;
-              // lane: 16-byte chunk of a row; 8 chunks per panel
-              const int sub = lane / (8 * C::PANELS), ch = lane % (8 * C::PANELS);
+          for (int p = 0; p < C::PANELS; ++p)
+            tma_load_4d(kv_base + st * C::TILE + p * 16384, tm, kv_full + st, 64 * p, t.hk * mul[1], key,
+                        (int)t.b * mul[0]);
+          ++use;
+          return true;
+        };
+        const auto load_q = [&](const XtItem& t, int s) {
+          if (!mbar_wait(q_empty + s, (qn[s] & 1u) ^ 1u, abort_flag)) return false;
+          int h, l0;
+          xt_slot(a, t, s, h, l0);
+          mbar_arrive_expect_tx(q_full + s, C::TILE);
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (hide[q])
-                  for (int r = sub; r < 32; r += 32 / (8 * C::PANELS))
-                    if ((hide[q] >> r) & 1u)
-                      *reinterpret_cast<uint4*>(tile + (ch >> 3) * 16384 + (32 * q + r) * 128 + (ch & 7) * 16) =
-                          make_uint4(0u, 0u, 0u, 0u);
-              fence_proxy_async_smem();
-            }
-          }
-          pass(true);
+          for (int p = 0; p < C::PANELS; ++p)
+            tma_load_4d(smem_u32(smem) + s * C::TILE + p * 16384, &tm_q, q_full + s, 64 * p, h * a.qm[1], l0,
+                        (int)t.b * a.qm[0]);
+          ++qn[s];
+          return true;
+        };
+        XtItem t;
+        for (int i = blockIdx.x; ok && next_item(i, t); i += gridDim.x) {
+          // K first: its stage frees before the Q slots of the item before
+          ok = load_kv(&tm_k, t, a.km, t.key0) && load_q(t, 0) && (t.nslots < 2 || load_q(t, 1)) &&
+               load_kv(&tm_v, t, a.vm, t.key0);
+          for (int j = 1; ok && j < t.nt; ++j)
+            ok = load_kv(&tm_k, t, a.km, t.key0 + 128 * j) && load_kv(&tm_v, t, a.vm, t.key0 + 128 * j);
+        }
+        if (!ok) {
+          // given up: every copy issued lands before the CTA may leave
+          volatile int never = 0;
+          for (uint32_t u = use > NST ? use - NST : 0; u < use; ++u)
+            mbar_wait(kv_full + u % NST, (u / NST) & 1u, &never);
+          for (int s = 0; s < 2; ++s)
+            if (qn[s]) mbar_wait(q_full + s, (qn[s] - 1) & 1u, &never);
         }
       }
-    }
-  } else if (warp >= 12) {
-    // ------------------------------------------------------------ epilogue
-    const int w = warp & 3;
-    const uint32_t lane_base = (uint32_t)(w * 32) << 16;
-    const bool split = a.x.splits > 1;
-    uint32_t ph[2] = {0, 0};
-    bool ok = true;
-    for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
-      const XtItem t = xt_item(a, i);
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t on = elect_one();
+      const int ksteps = (a.x.D + 15) / 16;
+      const uint32_t i_pv = idesc_f16(128, ksteps * 16, BF) | (1u << 16);   // B is MN-major
+      uint32_t use = 0, qph = 0, hph = 0, pph = 0, oph = 3;   // a phase bit per slot
+      const auto tile_wait = [&](uint32_t u) {
+        return all_lanes(mbar_wait((clean ? ready : kv_full) + u % NST, (u / NST) & 1u, abort_flag));
+      };
+      const auto slot_wait = [&](uint64_t* bar, uint32_t& ph, int s) {
+        const uint32_t parity = (ph >> s) & 1u;
+        ph ^= 1u << s;
+        return all_lanes(mbar_wait(bar + s, parity, abort_flag));
+      };
+      // keys of tile j of an item, rounded to the MMA's step
+      const auto width = [&](const XtItem& t, int j) { return min(128, (t.end - t.key0 - 128 * j + 15) / 16 * 16); };
+      const auto issue_s = [&](int s, uint32_t u, int n, bool last) {
+        const uint64_t dq = smem_desc_sw128(smem_u32(smem) + s * C::TILE);
+        const uint64_t dk = smem_desc_sw128(kv_base + (u % NST) * C::TILE);
+        const uint32_t idesc = idesc_f16(128, n, BF);
+        const auto step = [&](int k) {   // offsets in descriptor units (16 bytes)
+          const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4);
+          mma_f16_on(on, tmem + s * 128, dq + off, dk + off, idesc, k > 0);
+        };
+        if (ksteps == DP / 16) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s >= t.nslots || !ok) continue;
-        int h, l0;
-        xt_slot(a, t, s, h, l0);
-        const int row_in_tile = w * 32 + lane;
-        const int64_t l = l0 + (row_in_tile >> a.pack_shift);
-        h += row_in_tile & (a.packed - 1);
-        float m = -INFINITY, sum = 0.f;
-        if (t.nt) {
-          ok = all_lanes(mbar_wait(l_full + s, ph[s], abort_flag));
-          if (!ok) continue;
-          const float2 v = ml[s * 128 + w * 32 + lane];
-          m = v.x;
-          sum = v.y;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(l_empty + s);
-          ok = all_lanes(mbar_wait(o_full + s, ph[s], abort_flag));
-          if (!ok) continue;
-          ph[s] ^= 1u;
-          tc_fence_after();
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const uint64_t ii = two(inv, inv);
+          for (int k = 0; k < DP / 16; ++k) step(k);
+        } else {
 #pragma unroll 1
-        for (int q = 0; 32 * q < a.x.D; ++q) {
-          uint32_t o[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-          if (t.nt) {
-            tmem_ld32(tmem + 256 + s * 128 + lane_base + 32 * q, o);
-            tmem_wait_ld();
-            tie32(o);
-          }
-          if (l >= a.x.Lq) {
-            // past the sample's rows
-          } else if (split) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              if (32 * q + e < a.x.D) {
-                float v[8];
-#pragma unroll
-                for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
-                xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
-              }
-            }
-          } else {
-            T* row = reinterpret_cast<T*>(a.x.o) + t.b * a.x.os[0] + l * a.x.os[1] + h * a.x.os[2] + 32 * q;
-#pragma unroll
-            for (int e = 0; e < 32; e += 16) {
-              uint32_t v[8];
-#pragma unroll
-              for (int f = 0; f < 8; ++f) {
-                float lo, hi;
-                untwo(mul2(two(__uint_as_float(o[e + 2 * f]), __uint_as_float(o[e + 2 * f + 1])), ii), lo, hi);
-                v[f] = pack16<T>(lo, hi);
-              }
-              if (a.wide) {
-                if (32 * q + e < a.x.D) st_global32(row + e, v);
-              } else {
-                if (32 * q + e < a.x.D) *reinterpret_cast<uint4*>(row + e) = make_uint4(v[0], v[1], v[2], v[3]);
-                if (32 * q + e + 8 < a.x.D) *reinterpret_cast<uint4*>(row + e + 8) = make_uint4(v[4], v[5], v[6], v[7]);
-              }
-            }
-          }
-          __syncwarp();   // the next tcgen05.ld is the whole warp's
+          for (int k = 0; k < ksteps; ++k) step(k);
         }
-        if (t.nt) {
-          tc_fence_before();
+        mma_commit_on(on, s_full + s);
+        if (last) mma_commit_on(on, q_empty + s);
+      };
+      // P V over the steps [k0, k1) of 16 keys
+      const auto issue_pv = [&](int s, uint32_t u, int k0, int k1, uint32_t accumulate) {
+        const uint64_t dv = smem_desc_mn128(kv_base + (u % NST) * C::TILE) + k0 * (2048 >> 4);
+        const uint32_t pa = tmem + s * 128 + k0 * 8;
+        const auto step = [&](int k) {
+          mma_f16_ts_on(on, tmem + 256 + s * 128, pa + k * 8, dv + k * (2048 >> 4), i_pv, k > 0 ? 1u : accumulate);
+        };
+        if (k1 - k0 == 6) {
+#pragma unroll
+          for (int k = 0; k < 6; ++k) step(k);
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < k1 - k0; ++k) step(k);
+        }
+      };
+      const auto next_uniform = [&](int& i, XtItem& t) {
+        const bool got = next_item(i, t);
+        t.end = uniform(t.end);
+        t.nt = uniform(t.nt);
+        t.key0 = uniform(t.key0);
+        return all_lanes(got);
+      };
+      int i = blockIdx.x;
+      XtItem t, nx;
+      bool have = next_uniform(i, t), ok = true;
+      if (have) {
+        ok = tile_wait(use);
+        for (int s = 0; ok && s < t.nslots; ++s) {
+          ok = slot_wait(q_full, qph, s);
+          if (ok) issue_s(s, use, width(t, 0), t.nt == 1);
+        }
+        if (ok) mma_commit_on(on, kv_empty + use % NST);
+        ++use;
+      }
+      while (have && ok) {
+        i += gridDim.x;
+        const bool more = next_uniform(i, nx);
+        for (int j = 0; ok && j < t.nt; ++j) {
+          const bool last = j == t.nt - 1;
+          const uint32_t uv = use, uk = use + 1;   // V of this tile, the K tile after it
+          const int n = last ? (more ? width(nx, 0) : 0) : width(t, j + 1);
+          const int nslots = n ? (last ? nx.nslots : t.nslots) : 0;   // slots whose next S uses uk
+          const int steps = width(t, j) / 16;
+          ok = tile_wait(uv);
+          for (int s = 0; ok && s < max(t.nslots, nslots); ++s) {
+            // everything that the next S needs first, so that it follows P V at once
+            if (s < nslots) {
+              if (s == 0) ok = tile_wait(uk);
+              if (ok && last) ok = slot_wait(q_full, qph, s);
+              if (!ok) break;
+            }
+            if (s < t.nslots) {
+              if (j == 0) ok = slot_wait(o_empty, oph, s);
+              ok = ok && slot_wait(p_part, hph, s);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(s, uv, 0, min(steps, 6), j > 0);
+              ok = slot_wait(p_full, pph, s);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(s, uv, 6, steps, 1u);
+              if (last) mma_commit_on(on, o_full + s);
+            }
+            if (s < nslots) issue_s(s, uk, n, last ? nx.nt == 1 : j + 2 == t.nt);
+          }
+          if (!ok) break;
+          mma_commit_on(on, kv_empty + uv % NST);
+          if (n) mma_commit_on(on, kv_empty + uk % NST);
+          use += 2;
+        }
+        t = nx;
+        have = more;
+      }
+      // MMAs in flight and their arrivals end before tensor memory is freed and
+      // the CTA leaves
+      volatile int never = 0;
+      mma_commit_on(on, drain);
+      mbar_wait(drain, 0, &never);
+    } else if (warp == 10) {
+      // ------------------------------------------------------------- cleaner
+      if (clean) {
+        uint32_t use = 0;
+        bool ok = true;
+        const auto pass = [&](bool got) {   // the tile may be used
           __syncwarp();
-          if (lane == 0) mbar_arrive(o_empty + s);
+          if (got && lane == 0) mbar_arrive(ready + use % NST);
+          ++use;
+          return got;
+        };
+        const auto landed = [&]() { return all_lanes(mbar_wait(kv_full + use % NST, (use / NST) & 1u, abort_flag)); };
+        XtItem t;
+        for (int i = blockIdx.x; ok && next_item(i, t); i += gridDim.x) {
+          for (int j = 0; ok && j < t.nt; ++j) {
+            ok = pass(landed());   // a K tile
+            ok = ok && landed();
+            if (!ok) break;
+            const uint32_t st = use % NST;
+            {
+              const int k0 = t.key0 + 128 * j;
+              const int rows = min(128, (t.end - k0 + 15) / 16 * 16);   // rows that the MMA reads
+              unsigned hide[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int key = k0 + 32 * q + lane;
+                bool no = key >= t.end;
+                if constexpr (BIAS) no = no || __ldg(a.x.bias + t.b * a.x.Lkp + key) == -INFINITY;
+                hide[q] = __ballot_sync(0xffffffffu, no && 32 * q + lane < rows);
+              }
+              if (hide[0] | hide[1] | hide[2] | hide[3]) {
+                uint8_t* tile = smem + C::OFF_KV + st * C::TILE;
+                // lane: 16-byte chunk of a row; 8 chunks per panel
+                const int sub = lane / (8 * C::PANELS), ch = lane % (8 * C::PANELS);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (hide[q])
+                    for (int r = sub; r < 32; r += 32 / (8 * C::PANELS))
+                      if ((hide[q] >> r) & 1u)
+                        *reinterpret_cast<uint4*>(tile + (ch >> 3) * 16384 + (32 * q + r) * 128 + (ch & 7) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+              }
+            }
+            pass(true);
+          }
+        }
+      }
+    } else if (warp >= 12) {
+      // ------------------------------------------------------------ epilogue
+      const int w = warp & 3;
+      const uint32_t lane_base = (uint32_t)(w * 32) << 16;
+      const bool split = a.x.splits > 1;
+      uint32_t ph[2] = {0, 0};
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < a.items; i += gridDim.x) {
+        const XtItem t = xt_item(a, i);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s >= t.nslots || !ok) continue;
+          int h, l0;
+          xt_slot(a, t, s, h, l0);
+          const int row_in_tile = w * 32 + lane;
+          const int64_t l = l0 + (row_in_tile >> a.pack_shift);
+          h += row_in_tile & (a.packed - 1);
+          float m = -INFINITY, sum = 0.f;
+          if (t.nt) {
+            ok = all_lanes(mbar_wait(l_full + s, ph[s], abort_flag));
+            if (!ok) continue;
+            const float2 v = ml[s * 128 + w * 32 + lane];
+            m = v.x;
+            sum = v.y;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(l_empty + s);
+            ok = all_lanes(mbar_wait(o_full + s, ph[s], abort_flag));
+            if (!ok) continue;
+            ph[s] ^= 1u;
+            tc_fence_after();
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const uint64_t ii = two(inv, inv);
+#pragma unroll 1
+          for (int q = 0; 32 * q < a.x.D; ++q) {
+            uint32_t o[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+            if (t.nt) {
+              tmem_ld32(tmem + 256 + s * 128 + lane_base + 32 * q, o);
+              tmem_wait_ld();
+              tie32(o);
+            }
+            if (l >= a.x.Lq) {
+              // past the sample's rows
+            } else if (split) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                if (32 * q + e < a.x.D) {
+                  float v[8];
+#pragma unroll
+                  for (int f = 0; f < 8; ++f) v[f] = __uint_as_float(o[e + f]);
+                  xattn_put<T>(a.x, t.b, l, h, t.split, 32 * q + e, v, m, sum);
+                }
+              }
+            } else {
+              T* row = reinterpret_cast<T*>(a.x.o) + t.b * a.x.os[0] + l * a.x.os[1] + h * a.x.os[2] + 32 * q;
+#pragma unroll
+              for (int e = 0; e < 32; e += 16) {
+                uint32_t v[8];
+#pragma unroll
+                for (int f = 0; f < 8; ++f) {
+                  float lo, hi;
+                  untwo(mul2(two(__uint_as_float(o[e + 2 * f]), __uint_as_float(o[e + 2 * f + 1])), ii), lo, hi);
+                  v[f] = pack16<T>(lo, hi);
+                }
+                if (a.wide) {
+                  if (32 * q + e < a.x.D) st_global32(row + e, v);
+                } else {
+                  if (32 * q + e < a.x.D) *reinterpret_cast<uint4*>(row + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                  if (32 * q + e + 8 < a.x.D) *reinterpret_cast<uint4*>(row + e + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                }
+              }
+            }
+            __syncwarp();   // the next tcgen05.ld is the whole warp's
+          }
+          if (t.nt) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty + s);
+          }
         }
       }
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------- softmax

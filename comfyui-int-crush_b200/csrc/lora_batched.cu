@@ -48,7 +48,7 @@ struct LoraArgs {
 
 constexpr int kLoraWarps = 8;
 // Rows from which lora_stream.cu takes over (2777 rows of runs of four adapters,
-// 5120 to 5120 columns, rank 24: 55 us with it, 69 us without).
+// 5120 to 5120 columns, rank 24: 45 us with it, 69 us without).
 constexpr int kLoraStreamRows = 1024;
 
 template <typename T>
@@ -133,99 +133,99 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_down_kernel(const LoraAr
   const int64_t per = (steps + a.splits - 1) / a.splits;
 
   for (int64_t m0 = (int64_t)blockIdx.x * ROWS; m0 < a.M; m0 += (int64_t)gridDim.x * ROWS) {
-  if (a.streamed && !lora_tile_left(a, m0 / 128 * 128, lane)) continue;   // lora_down_stream_kernel's
-  const int id = lora_id(a, m0, ROWS, lane);
-  for (int part = blockIdx.y; part < a.splits; part += gridDim.y) {
-  const int64_t s0 = part * per, s1 = min(s0 + per, steps);
-  unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
-  for (unsigned pass = 0; todo; ++pass) {
-    const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
-    const unsigned match = __ballot_sync(0xffffffffu, id == ad);
-    todo &= ~match;
-    if (pass % gridDim.z != blockIdx.z) continue;
-    const T* dn = down + ((int64_t)ad * a.R + a.r0) * a.K;
-    bool on[MT][2];
-    const T* xr[MT][2];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 16 * i + 8 * h + g;
-        on[i][h] = (match >> r) & 1u;
-        xr[i][h] = x + (m0 + (on[i][h] ? r : 0)) * a.ldx;
-      }
-    float acc[MT][NT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
-#pragma unroll (NT <= 4 ? 4 : 2)
-    for (int64_t s = s0 + warp; s < s1; s += kLoraWarps) {
-      const int64_t k = s * 32 + 8 * t;
-      uint4 xv[MT][2];
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          xv[i][h] = on[i][h] ? lora_ld8<T, VEC>(xr[i][h], k, a.K) : make_uint4(0u, 0u, 0u, 0u);
-      uint4 dv[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        dv[j] = j * 8 + g < a.Rc ? lora_ld8<T, VEC>(dn + (int64_t)(j * 8 + g) * a.K, k, a.K)
-                                 : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          lora_mma<T>(acc[i][j], xv[i][0].x, xv[i][1].x, xv[i][0].y, xv[i][1].y, dv[j].x, dv[j].y);
-          lora_mma<T>(acc[i][j], xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w, dv[j].z, dv[j].w);
-        }
-    }
-    // the warps (all in this pass together) add up pairwise, in a fixed order
-#pragma unroll
-    for (int o = kLoraWarps / 2; o > 0; o >>= 1) {
-      float* slot = &red[warp & (o - 1)][0][0];
-      if (warp >= o && warp < 2 * o) {
+    if (a.streamed && !lora_tile_left(a, m0 / 128 * 128, lane)) continue;   // lora_down_stream_kernel's
+    const int id = lora_id(a, m0, ROWS, lane);
+    for (int part = blockIdx.y; part < a.splits; part += gridDim.y) {
+      const int64_t s0 = part * per, s1 = min(s0 + per, steps);
+      unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
+      for (unsigned pass = 0; todo; ++pass) {
+        const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+        const unsigned match = __ballot_sync(0xffffffffu, id == ad);
+        todo &= ~match;
+        if (pass % gridDim.z != blockIdx.z) continue;
+        const T* dn = down + ((int64_t)ad * a.R + a.r0) * a.K;
+        bool on[MT][2];
+        const T* xr[MT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+          for (int h = 0; h < 2; ++h) {
+            const int r = 16 * i + 8 * h + g;
+            on[i][h] = (match >> r) & 1u;
+            xr[i][h] = x + (m0 + (on[i][h] ? r : 0)) * a.ldx;
+          }
+        float acc[MT][NT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+#pragma unroll (NT <= 4 ? 4 : 2)
+        for (int64_t s = s0 + warp; s < s1; s += kLoraWarps) {
+          const int64_t k = s * 32 + 8 * t;
+          uint4 xv[MT][2];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              *reinterpret_cast<float2*>(slot + (16 * i + 8 * h + g) * (NT * 8) + j * 8 + 2 * t) =
-                  make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
-      }
-      __syncthreads();
-      if (warp < o) {
+              xv[i][h] = on[i][h] ? lora_ld8<T, VEC>(xr[i][h], k, a.K) : make_uint4(0u, 0u, 0u, 0u);
+          uint4 dv[NT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+          for (int j = 0; j < NT; ++j)
+            dv[j] = j * 8 + g < a.Rc ? lora_ld8<T, VEC>(dn + (int64_t)(j * 8 + g) * a.K, k, a.K)
+                                     : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float2 v = *reinterpret_cast<const float2*>(slot + (16 * i + 8 * h + g) * (NT * 8) + j * 8 + 2 * t);
-              acc[i][j][2 * h] += v.x;
-              acc[i][j][2 * h + 1] += v.y;
+            for (int i = 0; i < MT; ++i) {
+              lora_mma<T>(acc[i][j], xv[i][0].x, xv[i][1].x, xv[i][0].y, xv[i][1].y, dv[j].x, dv[j].y);
+              lora_mma<T>(acc[i][j], xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w, dv[j].z, dv[j].w);
             }
+        }
+        // the warps (all in this pass together) add up pairwise, in a fixed order
+#pragma unroll
+        for (int o = kLoraWarps / 2; o > 0; o >>= 1) {
+          float* slot = &red[warp & (o - 1)][0][0];
+          if (warp >= o && warp < 2 * o) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  *reinterpret_cast<float2*>(slot + (16 * i + 8 * h + g) * (NT * 8) + j * 8 + 2 * t) =
+                      make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+          }
+          __syncthreads();
+          if (warp < o) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const float2 v = *reinterpret_cast<const float2*>(slot + (16 * i + 8 * h + g) * (NT * 8) + j * 8 + 2 * t);
+                  acc[i][j][2 * h] += v.x;
+                  acc[i][j][2 * h + 1] += v.y;
+                }
+          }
+          __syncthreads();
+        }
+        if (warp != 0) continue;
+        float* mid = a.mid + (int64_t)part * a.M * a.Rp + a.r0;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = 16 * i + 8 * h + g;
+            if (!((match >> r) & 1u)) continue;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              if (a.r0 + j * 8 < a.Rp)
+                *reinterpret_cast<float2*>(mid + (m0 + r) * a.Rp + j * 8 + 2 * t) =
+                    make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+          }
       }
-      __syncthreads();
     }
-    if (warp != 0) continue;
-    float* mid = a.mid + (int64_t)part * a.M * a.Rp + a.r0;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 16 * i + 8 * h + g;
-        if (!((match >> r) & 1u)) continue;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (a.r0 + j * 8 < a.Rp)
-            *reinterpret_cast<float2*>(mid + (m0 + r) * a.Rp + j * 8 + 2 * t) =
-                make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
-      }
-  }
-  }
   }
 }
 
