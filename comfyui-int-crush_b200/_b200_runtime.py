@@ -83,6 +83,24 @@ def _need_cuda(what: str, *ts: torch.Tensor | None) -> None:
             raise RuntimeError(f"{what}: tensors on different devices ({dev}, {t.device})")
 
 
+def _on_its_device(fn):
+    """``fn``, whose first parameter is a tensor, with that tensor's CUDA device
+    current: a launch on a default stream, the SM count and a kernel's
+    attributes go by the current device, which need not be the tensors' (a
+    thread starts on device 0)."""
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        first = args[0] if args else next((t for t in kwargs.values() if isinstance(t, torch.Tensor)), None)
+        index = first.get_device() if isinstance(first, torch.Tensor) else -1
+        if index < 0 or index == torch.cuda.current_device():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(index):
+            return fn(*args, **kwargs)
+
+    return call
+
+
 def _f32c(t: torch.Tensor | None) -> torch.Tensor | None:
     if t is None:
         return None
@@ -717,7 +735,8 @@ def _strides12(*strides):
     return (ctypes.c_int64 * 12)(*strides)
 
 
-# Workspace floats by sizes (and device: the plans go by its SM count).
+# Workspace floats by sizes (and device, which is the current one: the plans go
+# by its SM count).
 @functools.lru_cache(maxsize=4096)
 def _workspace(name: str, index: int, *sizes: int) -> int:
     return getattr(L.lib(), name)(*sizes)
@@ -775,6 +794,7 @@ def _gamma16(what: str, t: torch.Tensor | None, D: int) -> torch.Tensor | None:
     return g.clone() if g.data_ptr() & 15 else g
 
 
+@_on_its_device
 def qk_norm_rope(
     q: torch.Tensor,
     k: torch.Tensor | None = None,
@@ -854,6 +874,7 @@ def qk_norm_rope(
     return y if k is None else (y, yk)
 
 
+@_on_its_device
 def cross_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -926,6 +947,7 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
 
 
+@_on_its_device
 def lora_batched(
     x: torch.Tensor,
     down: torch.Tensor,
@@ -1005,10 +1027,11 @@ def lora_batched(
     return out
 
 
-def device_error(clear: bool = True) -> int:
-    """Device error word of the library (1 = a bounded wait timed out, 2 = a
-    position or adapter id out of its range)."""
-    return L.read_device_error(clear)
+def device_error(clear: bool = True, device: torch.device | int | None = None) -> int:
+    """Error word of ``device`` (default: the current one): 1 = a bounded wait
+    timed out, 2 = a position or adapter id out of its range."""
+    with torch.cuda.device(device):
+        return L.read_device_error(clear)
 
 
 __all__ = [

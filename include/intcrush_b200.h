@@ -3,7 +3,9 @@
  *
  * Every entry point takes raw device pointers, sizes, strides (in elements
  * unless the name says bytes) and a cudaStream_t (passed as void*; NULL =
- * legacy default stream).  Nothing is allocated, nothing synchronises the
+ * legacy default stream).  The pointers' device has to be the current one
+ * (cudaSetDevice), also for the workspace sizes and the error word: a launch
+ * goes to the current device.  Nothing is allocated, nothing synchronises the
  * host: each call only enqueues kernels on `stream`, so all of them can be
  * captured into a CUDA graph.  Each returns IC_OK or an IC_ERR_* code; the
  * matching message is available from ic_last_error() on the calling thread.

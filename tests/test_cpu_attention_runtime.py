@@ -1,0 +1,89 @@
+"""Host side of the runtime's calls without a GPU: the library is a stub that
+records what it is called with, the devices are stand-ins."""
+
+import types
+
+import pytest
+import torch
+
+from _pkg import load
+
+rt = load("_b200_runtime")
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    """Two devices, 0 current and all tensors on 1; the library records (entry
+    point, current device, arguments) and answers 0."""
+    state = types.SimpleNamespace(current=0, calls=[])
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state.current = state.current, self.index
+
+        def __exit__(self, *exc):
+            state.current = self.before
+
+    class Library:
+        def __getattr__(self, name):
+            def entry(*args):
+                state.calls.append((name, state.current, args))
+                return 0
+            return entry
+
+    library = Library()
+    monkeypatch.setattr(rt, "B200_LIBRARY_LOADED", True)
+    monkeypatch.setattr(rt.L, "lib", lambda: library)
+    monkeypatch.setattr(rt, "_need_cuda", lambda what, *ts: None)
+    monkeypatch.setattr(rt, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(rt, "_stream", lambda t: 0)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state.current)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    rt._workspace.cache_clear()
+    yield state
+    rt._workspace.cache_clear()
+
+
+def half(*shape):
+    return torch.zeros(*shape, dtype=torch.float16)
+
+
+ATTENTION_SIDE = {
+    "qk_norm_rope": lambda: rt.qk_norm_rope(half(1, 2, 4, 64), half(1, 2, 4, 64)),
+    "cross_attention": lambda: rt.cross_attention(half(1, 2, 4, 64), k=half(1, 3, 4, 64), v=half(1, 3, 4, 64)),
+    "cross_attention, by name": lambda: rt.cross_attention(v=half(1, 3, 4, 64), scale=1.0, k=half(1, 3, 4, 64), q=half(1, 2, 4, 64)),
+    "lora_batched": lambda: rt.lora_batched(half(4, 64), half(2, 8, 64), half(2, 32, 8), torch.zeros(4, dtype=torch.int32)),
+}
+
+
+@pytest.mark.parametrize("call", ATTENTION_SIDE)
+def test_calls_run_on_the_tensors_device(lib, call):
+    """Every entry point, the workspace sizes among them, is called with the
+    tensors' device current; the caller's is back afterwards."""
+    ATTENTION_SIDE[call]()
+    assert lib.calls and {device for _, device, _ in lib.calls} == {1}
+    assert lib.current == 0
+
+
+@pytest.mark.parametrize("call", ATTENTION_SIDE)
+def test_the_current_device_is_not_switched(lib, monkeypatch, call):
+    lib.current = 1
+    monkeypatch.setattr(torch.cuda, "device", None)
+    ATTENTION_SIDE[call]()
+    assert {device for _, device, _ in lib.calls} == {1}
+
+
+def test_the_device_is_back_after_a_refusal(lib):
+    with pytest.raises(TypeError, match="float16/bfloat16"):
+        rt.qk_norm_rope(torch.zeros(1, 2, 4, 64))
+    assert lib.current == 0 and not lib.calls
+
+
+def test_device_error_reads_the_device_it_is_asked_for(lib):
+    rt.device_error(device=1)
+    assert [(name, device) for name, device, _ in lib.calls] == [("ic_read_device_error", 1)]
+    assert lib.current == 0
