@@ -113,6 +113,7 @@ def _round16(n: int) -> int:
 
 # ── activation prep ──────────────────────────────────────────────────────────
 
+@_on_its_device
 def prep_quantize(
     x: torch.Tensor,
     *,
@@ -257,6 +258,7 @@ def fused_rmsnorm_quantize(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e
 
 # ── GEMMs ────────────────────────────────────────────────────────────────────
 
+@_on_its_device
 def gemm_a8(
     x_int8: torch.Tensor,
     w: torch.Tensor,
@@ -417,6 +419,7 @@ def fused_int8_gemm_dequant(
                    residual=residual)
 
 
+@_on_its_device
 def int8_gemm_int8out(
     x_int8: torch.Tensor,
     w_int8: torch.Tensor,
@@ -517,6 +520,7 @@ def fused_quant_int8_gemm_dequant(
     return gemm_a8(x_int8, w_int8, s_w, s_a, bias=bias, out_dtype=out_dtype, out=out)
 
 
+@_on_its_device
 def gemm_w4a16(
     x: torch.Tensor,
     packed: torch.Tensor,
@@ -592,6 +596,7 @@ def _w4a16_splits(M: int, N: int, K: int, device) -> int:
     return s
 
 
+@_on_its_device
 def lowrank_down(x: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
     """``mid = T(x @ down^T)`` (``F.linear(x_raw, down)``, ``_ops.py:242``),
     T = x's dtype (fp16 or bf16; other dtypes compute in fp16)."""
@@ -609,6 +614,7 @@ def lowrank_down(x: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
     return mid
 
 
+@_on_its_device
 def lowrank_add(out: torch.Tensor, mid: torch.Tensor, up: torch.Tensor, scale: float) -> torch.Tensor:
     """In place ``out = T(out + scale * mid @ up^T)`` (``out.addmm_``,
     ``_ops.py:243``); out fp16 or bf16, rank up to 256."""
@@ -623,6 +629,7 @@ def lowrank_add(out: torch.Tensor, mid: torch.Tensor, up: torch.Tensor, scale: f
     return out
 
 
+@_on_its_device
 def quantize_weight(w: torch.Tensor, bits: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-row requantisation of a float weight on the device (the layout
     classes' ``quantize``, ``quant_layout.py:100-129,179-200``): returns
@@ -648,6 +655,7 @@ def quantize_weight(w: torch.Tensor, bits: int) -> tuple[torch.Tensor, torch.Ten
     return q, s
 
 
+@_on_its_device
 def lokr_add(out: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, scale: float) -> torch.Tensor:
     """``out[t] (viewed [out_l, out_k]) += scale * (w1 @ x[t].view(in_m, in_n)) @ w2^T``
     in place (``_apply_lokr``, ``_ops.py:88-138``): ``w1`` [out_l, in_m],
@@ -673,6 +681,7 @@ def lokr_add(out: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
     return out
 
 
+@_on_its_device
 def repack_int4(packed: torch.Tensor, K: int, layout: int) -> torch.Tensor:
     """Load-time nibble permutation of packed INT4 weights (``ic_repack_int4``):
     layout 0 feeds ``gemm_a8(..., repacked=True)``, layout 1 feeds
@@ -685,6 +694,7 @@ def repack_int4(packed: torch.Tensor, K: int, layout: int) -> torch.Tensor:
     return out
 
 
+@_on_its_device
 def unpack_int4_to_int8(packed: torch.Tensor, K: int) -> torch.Tensor:
     """``kernels/triton_int4_to_int8_unpack.py:55-81``."""
     _need_cuda("unpack_int4_to_int8", packed)
@@ -696,6 +706,7 @@ def unpack_int4_to_int8(packed: torch.Tensor, K: int) -> torch.Tensor:
     return out
 
 
+@_on_its_device
 def unpack_int4_to_float16(packed: torch.Tensor, scale: torch.Tensor, K: int,
                            group_size: int | None = None) -> torch.Tensor:
     """``kernels/triton_int4_unpack.py:62-88`` (scale ``[N]``), extended to

@@ -40,6 +40,7 @@ def lib(monkeypatch):
     monkeypatch.setattr(rt, "_need_cuda", lambda what, *ts: None)
     monkeypatch.setattr(rt, "_raw_stream", lambda index: 0)
     monkeypatch.setattr(rt, "_stream", lambda t: 0)
+    monkeypatch.setattr(rt, "_num_sms", lambda device: 148)
     monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: state.current)
     monkeypatch.setattr(torch.cuda, "device", Device)
@@ -60,11 +61,37 @@ ATTENTION_SIDE = {
 }
 
 
-@pytest.mark.parametrize("call", ATTENTION_SIDE)
+def int8(*shape):
+    return torch.zeros(*shape, dtype=torch.int8)
+
+
+def packed(*shape):
+    return torch.zeros(*shape, dtype=torch.uint8)
+
+
+QUANTISED = {
+    "prep_quantize": lambda: rt.prep_quantize(half(4, 64)),
+    "dynamic_quantize_activation": lambda: rt.dynamic_quantize_activation(half(4, 64)),
+    "fused_rmsnorm_quantize": lambda: rt.fused_rmsnorm_quantize(half(4, 64), torch.ones(64)),
+    "gemm_a8": lambda: rt.gemm_a8(int8(4, 64), int8(32, 64), torch.ones(32), torch.ones(4), splits=1),
+    "fused_int8_gemm_dequant": lambda: rt.fused_int8_gemm_dequant(int8(4, 64), int8(32, 64), torch.ones(32), torch.ones(4)),
+    "int8_gemm_int8out": lambda: rt.int8_gemm_int8out(int8(4, 64), int8(32, 64), torch.ones(32), torch.ones(4)),
+    "gemm_w4a16": lambda: rt.gemm_w4a16(half(4, 64), packed(32, 32), torch.ones(32, 1)),
+    "lowrank_down": lambda: rt.lowrank_down(half(4, 64), half(8, 64)),
+    "lowrank_add": lambda: rt.lowrank_add(half(4, 32), half(4, 8), half(32, 8), 1.0),
+    "quantize_weight": lambda: rt.quantize_weight(torch.zeros(32, 64), 8),
+    "lokr_add": lambda: rt.lokr_add(half(4, 32), half(4, 64), half(4, 8), half(8, 8), 1.0),
+    "repack_int4": lambda: rt.repack_int4(packed(32, 32), 64, rt.L.IC_W_INT4R),
+    "unpack_int4_to_int8": lambda: rt.unpack_int4_to_int8(packed(32, 32), 64),
+    "unpack_int4_to_float16": lambda: rt.unpack_int4_to_float16(packed(32, 32), torch.ones(32, 1), 64),
+}
+
+
+@pytest.mark.parametrize("call", [*ATTENTION_SIDE, *QUANTISED])
 def test_calls_run_on_the_tensors_device(lib, call):
     """Every entry point, the workspace sizes among them, is called with the
     tensors' device current; the caller's is back afterwards."""
-    ATTENTION_SIDE[call]()
+    {**ATTENTION_SIDE, **QUANTISED}[call]()
     assert lib.calls and {device for _, device, _ in lib.calls} == {1}
     assert lib.current == 0
 
