@@ -784,10 +784,24 @@ def _out_heads(what: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor
     return out
 
 
+_INT32_MAX = 2**31 - 1
+
+
 def _index(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype is not torch.int32:
-        if t.dtype.is_floating_point or t.dtype == torch.bool:
-            raise TypeError(f"an index tensor must hold integers, got {t.dtype}")
+    """``t`` as int32 on the way to the kernels, which check its range.  Wider
+    integers saturate: a length past the keys stays past them, and an id or a
+    position outside its range stays outside."""
+    dt = t.dtype
+    if dt is not torch.int32:
+        if dt.is_floating_point or dt.is_complex or dt is torch.bool:
+            raise TypeError(f"an index tensor must hold integers, got {dt}")
+        if dt is torch.uint64:
+            t = t.view(torch.int64)
+            t = t.masked_fill(t < 0, _INT32_MAX)   # 2^63 and more
+        elif dt is torch.uint32:
+            t = t.to(torch.int64)
+        if t.dtype is torch.int64:
+            t = t.clamp(-_INT32_MAX - 1, _INT32_MAX)
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -831,9 +845,11 @@ def qk_norm_rope(
     ``(2i, 2i + 1)`` (``layout="interleaved"``) or ``(i, i + rot / 2)``
     (``"half"``).  Without tables only the norm is applied.
 
-    A position outside the tables gives NaN for its token and sets the
-    library's device error word.  Returns ``(q, k)`` normalised, or only ``q``
-    without a ``k``; ``q_out`` / ``k_out`` may be the inputs themselves.
+    A position outside the tables, whatever the width of its integers, gives
+    NaN for its token and sets the library's device error word.  (int32
+    positions are taken as they are, others cost a conversion.)  Returns
+    ``(q, k)`` normalised, or only ``q`` without a ``k``; ``q_out`` / ``k_out``
+    may be the inputs themselves.
     """
     index = q.get_device()
     _same_device("qk_norm_rope", index, q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out)
@@ -853,8 +869,7 @@ def qk_norm_rope(
         if cos.shape != sin.shape or cos.dim() != 2:
             raise ValueError(f"qk_norm_rope: tables must be [rows, rot / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
         cos, sin = _fp32(cos), _fp32(sin)
-        rows, rot = cos.shape
-        rot *= 2
+        rows, rot = min(cos.shape[0], _INT32_MAX), 2 * cos.shape[1]   # _INT32_MAX is past every table
     if positions is not None:
         if positions.shape != (B, T):
             raise ValueError(f"qk_norm_rope: positions must be [{B}, {T}], got {tuple(positions.shape)}")

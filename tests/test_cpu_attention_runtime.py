@@ -114,3 +114,24 @@ def test_device_error_reads_the_device_it_is_asked_for(lib):
     rt.device_error(device=1)
     assert [(name, device) for name, device, _ in lib.calls] == [("ic_read_device_error", 1)]
     assert lib.current == 0
+
+
+# ── index tensors ────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("dtype,values,want", [
+    (torch.int64, [2**63 - 1, 2**32 + 1, 2**31, 2**31 - 1, 5, 0, -1, -2**32 + 3, -2**63],
+     [2**31 - 1, 2**31 - 1, 2**31 - 1, 2**31 - 1, 5, 0, -1, -2**31, -2**31]),
+    (torch.uint64, [2**63 + 1, 2**64 - 1, 2**32 + 1, 9], [2**31 - 1, 2**31 - 1, 2**31 - 1, 9]),
+    (torch.uint32, [2**32 - 1, 2**31 + 1, 9], [2**31 - 1, 2**31 - 1, 9]),
+    (torch.int16, [-3, 7], [-3, 7]), (torch.uint8, [255, 0], [255, 0]),
+])
+def test_index_tensors_saturate(dtype, values, want):
+    """Narrowing keeps what is out of range out of range (2^32 + 1 is not 1)."""
+    got = rt._index(torch.tensor(values, dtype=dtype))
+    assert got.dtype == torch.int32 and got.tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bool, torch.complex64])
+def test_index_tensors_hold_integers(dtype):
+    with pytest.raises(TypeError, match="integers"):
+        rt._index(torch.zeros(2, dtype=dtype))

@@ -1,0 +1,53 @@
+"""Calls of the attention-side operators at the ends of their ranges: wide
+index types, lengths without a limit, odd strides, long keys, mixed errors.
+
+References and bounds are those of the operators' other tests (64-bit forms; u
+the unit roundoff of the tensors' type)."""
+
+import math
+
+import pytest
+import torch
+
+from _pkg import load
+from test_gpu_attention_ops import (U, attention_inputs, attention_reference, check, gen, lora_inputs, lora_reference, normal,
+                                    qk_reference, qk_tolerance, tables)
+
+pytestmark = pytest.mark.gpu
+rt = load("_b200_runtime") if torch.cuda.is_available() else None
+
+
+# ── wide integers ────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("Lq", [1, 200])
+def test_lengths_without_a_limit(Lq):
+    """Lengths past the keys are the keys', also where 32 bits do not hold
+    them; negative ones see nothing."""
+    q, k, v, _ = attention_inputs(30, 4, Lq, 90, 2, 2, 64, torch.float16)
+    lens = torch.tensor([2**63 - 1, 2**32 + 5, -2**32 + 5, 7], device="cuda")
+    want, tol = attention_reference(q, k, v, torch.tensor([90, 90, 0, 7]))
+    got = rt.cross_attention(q, k, v, kv_lens=lens)
+    check(got, want, tol)
+    assert (got[2] == 0).all()
+
+
+def test_wide_ids_and_positions_outside_their_range():
+    g = gen(31)
+    q = normal(g, 1, 4, 3, 64, dtype=torch.float16)
+    cos, sin = tables(10, 64, g)
+    pos = torch.tensor([[2**32 + 1, 3, -2**32 + 2, 2**63 - 1]], device="cuda")
+    assert rt.device_error() == 0
+    y = rt.qk_norm_rope(q, cos=cos, sin=sin, positions=pos)
+    assert rt.device_error() == 2
+    want = qk_reference(q, None, cos, sin, "interleaved", torch.full_like(pos, 3), 1e-6)
+    check(y[:, 1], want[:, 1], qk_tolerance(want[:, 1], torch.float16))
+    assert y[:, [0, 2, 3]].isnan().all()
+
+    x, base, down, up, scales, _ = lora_inputs(32, 4, 64, 40, 8, 2, torch.float16)
+    ids = torch.tensor([2**32 + 1, 1, -2**32 + 1, -1], device="cuda")   # none, 1, negative, negative
+    got = rt.lora_batched(x, down, up, ids, scales, base=base)
+    assert rt.device_error() == 2 and rt.device_error() == 0
+    assert got[0].isnan().all()
+    want, tol = lora_reference(x[1:], down, up, torch.tensor([1, -1, -1], device="cuda"), scales, base[1:], 1)
+    check(got[1:], want, tol)
+    assert torch.equal(got[2:], base[2:])
