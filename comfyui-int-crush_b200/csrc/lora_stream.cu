@@ -6,6 +6,7 @@
 // 263 us for the first product register-fed, 77 us here; second 520 us and 360
 // us here, 5.0 TB/s).
 #include "ic_common.cuh"
+#include "lora_feed.h"
 
 namespace ic {
 
@@ -110,29 +111,20 @@ lora_down_stream_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
 
   if (warp == kLoraWarps) {
     if (lane == 0) {
-      bool ok = true;
-      int i = 0, u = 0;   // blocks of x and of down issued
-      while (ok && i < steps) {
-        const int st = i % SX;
-        ok = mbar_wait(x_empty + st, ((i / SX) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        mbar_arrive_expect_tx(x_full + st, C::X);
-        tma_load_2d(smem + st * C::X, &tm_x, x_full + st, 64 * (k0 + i), (int)m0);
-        ++i;
-        for (int p = 0; p < passes; ++p) {
-          const int su = u % SD;
-          ok = mbar_wait(d_empty + su, ((u / SD) & 1) ^ 1, abort_flag);
-          if (!ok) break;
-          mbar_arrive_expect_tx(d_full + su, C::DOWN);
-          tma_load_2d(smem + C::OFF_DOWN + su * C::DOWN, &tm_down, d_full + su, 64 * (k0 + i - 1), list[p] * a.R);
-          ++u;
-        }
-      }
-      if (!ok) {   // given up: every copy issued lands before the CTA may leave
-        volatile int never = 0;
-        for (int q = i > SX ? i - SX : 0; q < i; ++q) mbar_wait(x_full + q % SX, (q / SX) & 1, &never);
-        for (int q = u > SD ? u - SD : 0; q < u; ++q) mbar_wait(d_full + q % SD, (q / SD) & 1, &never);
-      }
+      volatile int never = 0;
+      lora_feed<SX, SD>(
+          steps, passes, [&](int i) { return mbar_wait(x_empty + i % SX, ((i / SX) & 1) ^ 1, abort_flag); },
+          [&](int i) {
+            mbar_arrive_expect_tx(x_full + i % SX, C::X);
+            tma_load_2d(smem + i % SX * C::X, &tm_x, x_full + i % SX, 64 * (k0 + i), (int)m0);
+          },
+          [&](int i) { mbar_wait(x_full + i % SX, (i / SX) & 1, &never); },
+          [&](int u) { return mbar_wait(d_empty + u % SD, ((u / SD) & 1) ^ 1, abort_flag); },
+          [&](int u, int i, int p) {
+            mbar_arrive_expect_tx(d_full + u % SD, C::DOWN);
+            tma_load_2d(smem + C::OFF_DOWN + u % SD * C::DOWN, &tm_down, d_full + u % SD, 64 * (k0 + i), list[p] * a.R);
+          },
+          [&](int u) { mbar_wait(d_full + u % SD, (u / SD) & 1, &never); });
     }
     return;
   }
@@ -271,32 +263,25 @@ lora_up_stream_kernel(const __grid_constant__ CUtensorMap tm_base, const __grid_
 
   if (warp == kLoraWarps) {
     if (lane == 0) {
-      bool ok = true;
-      int i = 0, u = 0;
-      for (; ok && i < blocks; ++i) {
-        const int n = (int)n0 + 64 * i, st = i % SB;
-        ok = mbar_wait(b_empty + st, ((i / SB) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        if (has_base) {
-          mbar_arrive_expect_tx(b_full + st, C::BASE);
-          tma_load_2d(smem + st * C::BASE, &tm_base, b_full + st, n, (int)m0);
-        } else {
-          mbar_arrive(b_full + st);
-        }
-        for (int p = 0; p < passes; ++p, ++u) {
-          const int su = u % SU;
-          ok = mbar_wait(u_empty + su, ((u / SU) & 1) ^ 1, abort_flag);
-          if (!ok) break;
-          mbar_arrive_expect_tx(u_full + su, 128 * a.R);
-          tma_load_2d(smem + C::OFF_UP + su * C::UP, &tm_up, u_full + su, 0, list[p] * (int)a.N + n);
-        }
-      }
-      if (!ok) {   // given up: every copy issued lands before the CTA may leave
-        volatile int never = 0;
-        for (int q = i >= SB ? i - SB + 1 : 0; q < i; ++q) mbar_wait(b_full + q % SB, (q / SB) & 1, &never);
-        if (i < blocks && (u % (passes > 0 ? passes : 1)) != 0) mbar_wait(b_full + i % SB, (i / SB) & 1, &never);
-        for (int q = u > SU ? u - SU : 0; q < u; ++q) mbar_wait(u_full + q % SU, (q / SU) & 1, &never);
-      }
+      volatile int never = 0;
+      lora_feed<SB, SU>(
+          blocks, passes, [&](int i) { return mbar_wait(b_empty + i % SB, ((i / SB) & 1) ^ 1, abort_flag); },
+          [&](int i) {
+            if (has_base) {
+              mbar_arrive_expect_tx(b_full + i % SB, C::BASE);
+              tma_load_2d(smem + i % SB * C::BASE, &tm_base, b_full + i % SB, (int)n0 + 64 * i, (int)m0);
+            } else {
+              mbar_arrive(b_full + i % SB);
+            }
+          },
+          [&](int i) { mbar_wait(b_full + i % SB, (i / SB) & 1, &never); },
+          [&](int u) { return mbar_wait(u_empty + u % SU, ((u / SU) & 1) ^ 1, abort_flag); },
+          [&](int u, int i, int p) {
+            mbar_arrive_expect_tx(u_full + u % SU, 128 * a.R);
+            tma_load_2d(smem + C::OFF_UP + u % SU * C::UP, &tm_up, u_full + u % SU, 0,
+                        list[p] * (int)a.N + (int)n0 + 64 * i);
+          },
+          [&](int u) { mbar_wait(u_full + u % SU, (u / SU) & 1, &never); });
     }
     return;
   }
