@@ -315,14 +315,11 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int j = 1; ok && j < t.nt; ++j)
             ok = load_kv(&tm_k, t, a.km, t.key0 + 128 * j) && load_kv(&tm_v, t, a.vm, t.key0 + 128 * j);
         }
-        if (!ok) {
-          // given up: every copy issued lands before the CTA may leave
-          volatile int never = 0;
-          for (uint32_t u = use > NST ? use - NST : 0; u < use; ++u)
-            mbar_wait(kv_full + u % NST, (u / NST) & 1u, &never);
-          for (int s = 0; s < 2; ++s)
-            if (qn[s]) mbar_wait(q_full + s, (qn[s] - 1) & 1u, &never);
-        }
+        // every copy issued lands before the CTA may leave, whoever gave up
+        volatile int never = 0;
+        for (uint32_t u = use > NST ? use - NST : 0; u < use; ++u) mbar_wait(kv_full + u % NST, (u / NST) & 1u, &never);
+        for (int s = 0; s < 2; ++s)
+          if (qn[s]) mbar_wait(q_full + s, (qn[s] - 1) & 1u, &never);
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------- MMA issuer
