@@ -1054,8 +1054,9 @@ def lora_batched(
 
 
 def device_error(clear: bool = True, device: torch.device | int | None = None) -> int:
-    """Error word of ``device`` (default: the current one): 1 = a bounded wait
-    timed out, 2 = a position or adapter id out of its range."""
+    """Error code of ``device`` (default: the current one): 1 = a bounded wait
+    timed out, 2 = a position or adapter id out of its range.  Where both
+    happened 1 is reported first; ``clear`` takes out what is reported."""
     with torch.cuda.device(device):
         return L.read_device_error(clear)
 

@@ -99,18 +99,24 @@ int ic_selftest_wait_timeout(int64_t limit_ns, void* stream) {
 }
 
 int ic_read_device_error(int clear, int* code_out) {
-  int v = 0;
+  // the words of both translation units; the gravest code first, and only the
+  // code that is reported is cleared
+  int v = 0, w = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_ic_dev_error, sizeof(int));
+  if (e == cudaSuccess) e = ic::attention_device_error(&w, false);
   if (e != cudaSuccess) return cuda_status(e, "reading the device error word");
-  if (clear && v) {
-    const int z = 0;
-    e = cudaMemcpyToSymbol(g_ic_dev_error, &z, sizeof(int));
-    if (e != cudaSuccess) return cuda_status(e, "clearing the device error word");
+  const int both = v | w;
+  const int code = both & IC_DEV_ERR_TIMEOUT ? IC_DEV_ERR_TIMEOUT : both & IC_DEV_ERR_INDEX ? IC_DEV_ERR_INDEX : IC_DEV_ERR_NONE;
+  if (clear && (v & code)) {
+    v &= ~code;
+    e = cudaMemcpyToSymbol(g_ic_dev_error, &v, sizeof(int));
   }
-  int w = 0;
-  e = ic::attention_device_error(clear, &w);
-  if (e != cudaSuccess) return cuda_status(e, "reading the device error word");
-  if (code_out) *code_out = v ? v : w;
+  if (clear && e == cudaSuccess && (w & code)) {
+    w &= ~code;
+    e = ic::attention_device_error(&w, true);
+  }
+  if (e != cudaSuccess) return cuda_status(e, "clearing the device error word");
+  if (code_out) *code_out = code;
   return IC_OK;
 }
 

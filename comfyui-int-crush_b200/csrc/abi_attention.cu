@@ -5,13 +5,8 @@
 
 namespace ic {
 
-cudaError_t attention_device_error(int clear, int* code) {
-  cudaError_t e = cudaMemcpyFromSymbol(code, g_ic_dev_error, sizeof(int));
-  if (e == cudaSuccess && clear && *code) {
-    const int z = 0;
-    e = cudaMemcpyToSymbol(g_ic_dev_error, &z, sizeof(int));
-  }
-  return e;
+cudaError_t attention_device_error(int* word, bool store) {
+  return store ? cudaMemcpyToSymbol(g_ic_dev_error, word, sizeof(int)) : cudaMemcpyFromSymbol(word, g_ic_dev_error, sizeof(int));
 }
 
 static int launched(cudaError_t e, const char* what) {

@@ -33,7 +33,7 @@ namespace ic {
 // Shared by the translation units (defined in abi.cu and gemm_tc.cu).
 int set_error(int code, const char* fmt, ...);      // records ic_last_error's text, returns code
 void clear_error();
-cudaError_t attention_device_error(int clear, int* code);   // abi_attention.cu
+cudaError_t attention_device_error(int* word, bool store);   // that unit's word: load or store (abi_attention.cu)
 int num_sms();
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -80,8 +80,10 @@ __device__ __forceinline__ uint64_t globaltimer() {
   return t;
 }
 
+// The word holds every code seen since it was cleared (the codes are bits): an
+// earlier bad index must not hide a wait that ran out.
 __device__ __forceinline__ void set_dev_error(int code) {
-  atomicCAS(&g_ic_dev_error, 0, code);
+  atomicOr(&g_ic_dev_error, code);
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

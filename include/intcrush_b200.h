@@ -28,7 +28,7 @@ extern "C" {
 #define IC_ERR_UNSUPPORTED 2  /* valid request outside what is built      */
 #define IC_ERR_CUDA 3         /* a CUDA runtime or driver call failed     */
 
-/* device-side error word (ic_read_device_error) */
+/* device-side error word (ic_read_device_error): bits */
 #define IC_DEV_ERR_NONE 0
 #define IC_DEV_ERR_TIMEOUT 1  /* a bounded mbarrier wait expired          */
 #define IC_DEV_ERR_INDEX 2    /* a position or adapter id out of its range */
@@ -50,8 +50,11 @@ int ic_version(void);
 /* Message for the last error returned on this host thread ("" if none). */
 const char* ic_last_error(void);
 
-/* Read (and optionally clear) the device error word of the current device.
- * Synchronises the device: test/diagnostic use only. */
+/* Read the device error word of the current device: the gravest code that was
+ * recorded (a wait that ran out, whose outputs are incomplete, before a bad
+ * index), IC_DEV_ERR_NONE for none.  With clear that code is taken out; a
+ * further read reports what else there is.  Synchronises the device:
+ * test/diagnostic use only. */
 int ic_read_device_error(int clear, int* code_out);
 
 /*

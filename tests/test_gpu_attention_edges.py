@@ -51,3 +51,30 @@ def test_wide_ids_and_positions_outside_their_range():
     want, tol = lora_reference(x[1:], down, up, torch.tensor([1, -1, -1], device="cuda"), scales, base[1:], 1)
     check(got[1:], want, tol)
     assert torch.equal(got[2:], base[2:])
+
+
+# ── the error word ───────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("index_first", [True, False])
+def test_error_word_keeps_both_codes(index_first):
+    """A bad index and a wait that runs out: both are reported, the wait
+    first, one a read."""
+    import ctypes
+
+    L = load("_lib")
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.float16, device="cuda")
+    cos, sin = tables(4, 64, gen(33))
+
+    def index():
+        rt.qk_norm_rope(q, cos=cos, sin=sin, positions=torch.tensor([[4]], device="cuda"))
+
+    def timeout():
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        assert L.lib().ic_selftest_wait_timeout(1_000_000, stream) == L.IC_OK
+
+    assert rt.device_error() == 0
+    for call in (index, timeout) if index_first else (timeout, index):
+        call()
+    torch.cuda.synchronize()
+    assert rt.device_error(clear=False) == L.IC_DEV_ERR_TIMEOUT
+    assert [rt.device_error() for _ in range(3)] == [L.IC_DEV_ERR_TIMEOUT, L.IC_DEV_ERR_INDEX, 0]
