@@ -764,24 +764,35 @@ def _same_device(what: str, index: int, *ts: torch.Tensor | None) -> None:
             raise RuntimeError(f"{what}: tensors on different devices")
 
 
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """``t`` ([batch, tokens, heads, D]) as the kernels read it: elements
-    contiguous, 16-byte aligned rows; a copy where it is not."""
+def _heads_ok(t: torch.Tensor) -> bool:
+    """``t`` ([batch, tokens, heads, D]) can be read as it is: elements
+    contiguous, 16-byte aligned rows, tokens apart."""
     b, l, h, d = t.stride()
-    if d == 1 and not ((b | l | h) & 7 or t.data_ptr() & 15) and (l or t.shape[1] <= 1):
+    return d == 1 and not ((b | l | h) & 7 or t.data_ptr() & 15) and (l != 0 or t.shape[1] <= 1)
+
+
+def _plain_ones(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with the strides of its dimensions of one entry, which say nothing
+    and may be anything, as 0."""
+    return t.as_strided(t.shape, tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())) + t.stride()[3:])
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the kernels read it; a copy where it is not."""
+    if _heads_ok(t):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    t = _plain_ones(t)
+    return t if _heads_ok(t) else t.clone(memory_format=_DENSE)
 
 
 def _out_heads(what: str, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
-    b, l, h, d = out.stride() if out.dim() == 4 else (0, 0, 0, 0)
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"{what}: out must be {like.dtype} {tuple(like.shape)}, got {out.dtype} {tuple(out.shape)}")
-    if d != 1 or (b | l | h) & 7 or out.data_ptr() & 15 or any(
-            s == 0 and n > 1 for s, n in zip((b, l, h), out.shape)):
+    y = out if _heads_ok(out) else _plain_ones(out)
+    if not _heads_ok(y) or any(s == 0 and n > 1 for s, n in zip(y.stride(), y.shape)):
         raise ValueError(f"{what}: out must have contiguous elements, strides that are multiples of 8 and a 16-byte "
                          f"aligned start, got strides {out.stride()}")
-    return out
+    return y
 
 
 _INT32_MAX = 2**31 - 1
@@ -897,7 +908,8 @@ def qk_norm_rope(
         None if positions is None else positions.data_ptr(), _raw_stream(index))
     if st:
         L.check(st, "ic_qk_norm_rope")
-    return y if k is None else (y, yk)
+    y = y if q_out is None else q_out
+    return y if k is None else (y, yk if k_out is None else k_out)
 
 
 @_on_its_device
@@ -963,7 +975,7 @@ def cross_attention(
         _raw_stream(index))
     if st:
         L.check(st, "ic_cross_attention")
-    return y
+    return y if out is None else out
 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:

@@ -135,3 +135,49 @@ def test_index_tensors_saturate(dtype, values, want):
 def test_index_tensors_hold_integers(dtype):
     with pytest.raises(TypeError, match="integers"):
         rt._index(torch.zeros(2, dtype=dtype))
+
+
+# ── strides that say nothing ─────────────────────────────────────────────────
+
+def one_sample(batch_stride, L=5, H=3, D=16):
+    """[1, L, H, D] cut from a buffer whose samples are batch_stride apart."""
+    return torch.zeros(2 * batch_stride, dtype=torch.float16).as_strided((2, L, H, D), (batch_stride, H * D, D, 1))[:1]
+
+
+@pytest.mark.parametrize("call", ["qk_norm_rope", "cross_attention"])
+def test_strides_of_dimensions_of_one_entry(lib, call):
+    """A batch of one may have any batch stride: nothing is copied, and the
+    library gets strides that it takes (multiples of 8)."""
+    t, out = one_sample(5 * 3 * 16 + 1), one_sample(5 * 3 * 16 + 3)
+    assert t.stride(0) % 8 and out.stride(0) % 8
+    if call == "qk_norm_rope":
+        y = rt.qk_norm_rope(t, q_out=out)
+        (_, _, args), = [c for c in lib.calls if c[0] == "ic_qk_norm_rope"]
+        tensors, strides = (args[0], args[1]), list(args[10])
+    else:
+        y = rt.cross_attention(t, t, t, out=out)
+        (_, _, args), = [c for c in lib.calls if c[0] == "ic_cross_attention"]
+        tensors, strides = (args[0], args[3]), list(args[11])
+    assert y is out
+    assert tensors == (t.data_ptr(), out.data_ptr())
+    assert all(s % 8 == 0 for s in strides)
+    assert strides[:3] == [0, 48, 16] and [0, 48, 16] in (strides[3:6], strides[9:])
+
+
+def test_strides_that_need_a_copy(lib):
+    """Rows at odd addresses are copied to a layout of their own, also where
+    torch calls them contiguous; out is refused."""
+    buf = torch.arange(2 + 5 * 3 * 16, dtype=torch.float16)
+    buf = buf[1:] if buf.data_ptr() % 16 == 0 else buf
+    odd = buf[:5 * 3 * 16].as_strided((1, 5, 3, 16), (7, 48, 16, 1))
+    assert odd.is_contiguous() and odd.data_ptr() % 16
+    got = rt._heads(odd)
+    assert torch.equal(got, odd) and got.stride() == (240, 48, 16, 1) and got.data_ptr() % 16 == 0
+    with pytest.raises(ValueError, match="out must have contiguous"):
+        rt.qk_norm_rope(odd, q_out=odd)
+    rows = torch.zeros(2, 5, 3, 17, dtype=torch.float16)[..., :16]
+    assert rt._heads(rows).stride() == (240, 48, 16, 1)
+    with pytest.raises(ValueError, match="out must have contiguous"):
+        rt.qk_norm_rope(rows, q_out=rows)
+    with pytest.raises(ValueError, match="out must have contiguous"):
+        rt.qk_norm_rope(rows, q_out=torch.zeros(1, 5, 3, 16, dtype=torch.float16).expand(2, 5, 3, 16))

@@ -78,3 +78,25 @@ def test_error_word_keeps_both_codes(index_first):
     torch.cuda.synchronize()
     assert rt.device_error(clear=False) == L.IC_DEV_ERR_TIMEOUT
     assert [rt.device_error() for _ in range(3)] == [L.IC_DEV_ERR_TIMEOUT, L.IC_DEV_ERR_INDEX, 0]
+
+
+# ── a batch of one with an odd batch stride ──────────────────────────────────
+
+@pytest.mark.parametrize("Lq", [1, 5, 200])
+def test_one_sample_of_an_odd_buffer(Lq):
+    """One sample cut from a buffer whose samples are an odd number of elements
+    apart."""
+    g = gen(34)
+    H, D = 3, 64
+
+    def cut(L):
+        stride = L * H * D + 5
+        return normal(g, 2 * stride, dtype=torch.float16).as_strided((1, L, H, D), (stride, H * D, D, 1))
+
+    q, k, v, out = cut(Lq), cut(70), cut(70), cut(Lq)
+    want, tol = attention_reference(q, k, v)
+    assert rt.cross_attention(q, k, v, out=out) is out
+    check(out, want, tol)
+    cos, sin = tables(Lq, D, g)
+    want = qk_reference(q, None, cos, sin, "half", None, 1e-6)
+    check(rt.qk_norm_rope(q, cos=cos, sin=sin, layout="half"), want, qk_tolerance(want, torch.float16))
