@@ -981,7 +981,7 @@ def cross_attention(
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """``t`` as a [rows, width] matrix with contiguous rows."""
     if t.dim() != 2:
-        t = t.reshape(-1, width)
+        t = t.flatten(0, -2) if t.dim() > 2 else t.view(1, width)
     return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
 
 

@@ -181,3 +181,26 @@ def test_strides_that_need_a_copy(lib):
         rt.qk_norm_rope(rows, q_out=rows)
     with pytest.raises(ValueError, match="out must have contiguous"):
         rt.qk_norm_rope(rows, q_out=torch.zeros(1, 5, 3, 16, dtype=torch.float16).expand(2, 5, 3, 16))
+
+
+# ── empty sizes ──────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("lead,N", [((2, 3), 0), ((), 0), ((0, 3), 0), ((0, 3), 32), ((2, 0), 32)])
+@pytest.mark.parametrize("with_base,with_out", [(False, False), (True, False), (True, True)])
+def test_adapters_of_empty_sizes(lib, lead, N, with_base, with_out):
+    """No rows or no columns: an empty result, nothing launched."""
+    x, base, out = half(*lead, 64), half(*lead, N), half(*lead, N)
+    rows = x.numel() // 64
+    y = rt.lora_batched(x, half(2, 8, 64), half(2, N, 8), torch.zeros(rows, dtype=torch.int32),
+                        base=base if with_base else None, out=out if with_out else None)
+    assert y.shape == (*lead, N) and not lib.calls
+
+
+@pytest.mark.parametrize("lead", [(), (6,), (2, 3), (1, 2, 3)])
+def test_adapter_rows(lib, lead):
+    """Leading dimensions fold into rows."""
+    x = half(*lead, 64)
+    rows = x.numel() // 64
+    y = rt.lora_batched(x, half(2, 8, 64), half(2, 32, 8), torch.zeros(rows, dtype=torch.int32), base=half(*lead, 32))
+    (_, _, args), = [c for c in lib.calls if c[0] == "ic_lora_batched"]
+    assert y.shape == (*lead, 32) and args[2:5] == (rows, 64, 64) and args[0] == x.data_ptr()
