@@ -1043,9 +1043,11 @@ def lora_batched(
     else:
         if out.dtype != dt or out.shape != full:
             raise ValueError(f"lora_batched: out must be {dt} {full}, got {out.dtype} {tuple(out.shape)}")
-        o2 = out.view(-1, N) if M and N else out   # raises where the leading dimensions do not fold
+        if M == 0 or N == 0:
+            return out
+        o2 = out.view(-1, N)   # raises where the leading dimensions do not fold
         ldo = o2.stride(0) if M > 1 else N
-        if N and (o2.stride(1) != 1 or ldo < N):
+        if o2.stride(1) != 1 or ldo < N:
             raise ValueError(f"lora_batched: out must be row-major, got strides {out.stride()}")
     if M == 0 or N == 0:
         return out
