@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(32 * kXsWarps, 3) xattn_rows_kernel(const Xatt
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+    if (__any_sync(0xffffffffu, xattn_moves(mx[0], m[0]) || xattn_moves(mx[1], m[1]))) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float nm = fmaxf(m[h], mx[h]);

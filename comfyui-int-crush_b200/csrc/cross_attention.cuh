@@ -54,6 +54,11 @@ __device__ __forceinline__ int xattn_end(const XattnArgs& a, int64_t b) {
   return (int)a.Lk;
 }
 
+// Whether a row's running maximum moves: when it grows by more than 2^8.  (As a
+// difference: m + 8 would round where scores are large, and let fp16 weights
+// pass 65504.)
+__device__ __forceinline__ bool xattn_moves(float mx, float m) { return mx - m > 8.f; }
+
 // 2^x (the hardware's approximation, 2 ulp; 2^-inf = 0)
 __device__ __forceinline__ float ex2(float x) {
   float y;

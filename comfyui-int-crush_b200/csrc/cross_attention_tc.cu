@@ -645,8 +645,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         if constexpr (!BIAS) mx *= c;
         // (P V of the tile before is done: this S was issued behind it)
-        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-          const float nm = mx > m + 8.f ? mx : m;
+        if (__any_sync(0xffffffffu, xattn_moves(mx, m))) {
+          const float nm = xattn_moves(mx, m) ? mx : m;
           const float f = nm == m ? 1.f : ex2(m - nm);
           m = nm;
           sum *= f;

@@ -100,3 +100,27 @@ def test_one_sample_of_an_odd_buffer(Lq):
     cos, sin = tables(Lq, D, g)
     want = qk_reference(q, None, cos, sin, "half", None, 1e-6)
     check(rt.qk_norm_rope(q, cos=cos, sin=sin, layout="half"), want, qk_tolerance(want, torch.float16))
+
+
+# ── fp16 weights ─────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Lq,later", [(1, 64), (200, 130)])
+def test_scores_whose_steps_pass_the_room(Lq, later, dtype):
+    """Scores of 2^27, where fp32 counts in steps of 16: the later key has 2^16
+    times the weight of the first one and takes (nearly) all of the output."""
+    Lk, D = 300, 64
+    q = torch.zeros(1, Lq, 1, D, dtype=dtype, device="cuda")
+    k = torch.zeros(1, Lk, 1, D, dtype=dtype, device="cuda")
+    q[..., 0], q[..., 1] = 2.0**14, 4.0
+    k[0, 0, 0, 0], k[0, 0, 0, 1] = 2.0**13, 4.0
+    k[0, later, 0, 0], k[0, later, 0, 1] = 2.0**13, 8.0
+    v = normal(gen(36), 1, Lk, 1, D, dtype=dtype)
+    # the scale whose product with log2(e), in fp32, is 1: scores in log2 are q k
+    e = torch.tensor(math.log2(math.e))
+    scale = next(s.item() for s in (1 / e + torch.arange(-4, 5) * 2.0**-24) if (s * e).item() == 1.0)
+    got = rt.cross_attention(q, k, v, scale=scale)
+    a, b = v[0, 0, 0].double(), v[0, later, 0].double()
+    want = (b + a * 2.0**-16) / (1 + 2.0**-16)
+    tol = (U[dtype] + 3e-5) * (b.abs() + a.abs() * 2.0**-16) + U[dtype] * want.abs() + 2.0**-25 + 2.0**-32
+    check(got[0, :, 0], want.expand(Lq, D), tol)
