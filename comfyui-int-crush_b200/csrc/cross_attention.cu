@@ -81,10 +81,9 @@ __global__ void __launch_bounds__(1024) xattn_mask_kernel(const void* mask, int6
 // 8 single tokens of 32 heads over 8 key heads of 128, 1024 to 8192 keys (151
 // MB): 46 us with the join, 3.3 TB/s, as the tcgen05 kernel; loads straight to
 // registers 49 us.  The copies alone take 44 us of that, the arithmetic alone 22.
-// Softmax: scores, maxima and sums in fp32; the running maximum of a row only
-// moves when it grows by more than 2^8 (the sums stay exact, p stays below
-// 2^8), so most blocks rescale nothing.  p enters the product with V rounded
-// to the activation type (the MMA's operand), its sum unrounded.
+// Softmax: scores, references (kXattnUp) and sums in fp32.  p enters the product
+// with V rounded to the activation type, which is the MMA's operand type, its
+// sum unrounded: at most u sum_j p_j |v_j| beside the output's own rounding.
 constexpr int kXsWarps = 4;
 
 template <typename T>
@@ -164,7 +163,7 @@ __global__ void __launch_bounds__(32 * kXsWarps, 3) xattn_rows_kernel(const Xatt
   for (int i = 0; i < NH; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // references, sums
   const float sc = a.scale * kLog2e;
 
   const uint32_t mine = smem_u32(ring) + warp * S * C::LOADS * 512 + lane * 16;
@@ -265,10 +264,10 @@ __global__ void __launch_bounds__(32 * kXsWarps, 3) xattn_rows_kernel(const Xatt
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
     }
-    if (__any_sync(0xffffffffu, xattn_moves(mx[0], m[0]) || xattn_moves(mx[1], m[1]))) {
+    if (__any_sync(0xffffffffu, xattn_moves<T>(mx[0], m[0]) || xattn_moves<T>(mx[1], m[1]))) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float nm = fmaxf(m[h], mx[h]);
+        const float nm = fmaxf(m[h], mx[h] - kXattnUp<T>);
         const float f = nm == m[h] ? 1.f : ex2(m[h] - nm);
         m[h] = nm;
         l[h] *= f;
@@ -356,7 +355,7 @@ __global__ void __launch_bounds__(32 * kXsWarps, 3) xattn_rows_kernel(const Xatt
 
 // ------------------------------------------------------------------- join
 // One thread per 8 elements of an output row: the splits' sums weighted to
-// their common maximum, in split order.
+// their largest reference, in split order.
 template <typename T>
 __global__ void __launch_bounds__(128) xattn_join_kernel(const XattnArgs a) {
   const int dq = a.D / 8;

@@ -3,6 +3,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "ic_common.cuh"
 
 namespace ic {
@@ -26,7 +28,7 @@ struct XattnArgs {
   int splits;                  // parts of the keys
   int part_blocks;             // few-rows kernel: blocks of 16 keys in a part
   float* part_o;               // [splits, B, Lq, H, D] with splits > 1
-  float* part_ml;              // [splits, B, Lq, H, 2]: maximum (log2), sum
+  float* part_ml;              // [splits, B, Lq, H, 2]: reference (log2), sum
 };
 
 struct XattnPlan {
@@ -54,10 +56,22 @@ __device__ __forceinline__ int xattn_end(const XattnArgs& a, int64_t b) {
   return (int)a.Lk;
 }
 
-// Whether a row's running maximum moves: when it grows by more than 2^8.  (As a
-// difference: m + 8 would round where scores are large, and let fp16 weights
-// pass 65504.)
-__device__ __forceinline__ bool xattn_moves(float mx, float m) { return mx - m > 8.f; }
+// A row's weights are p = 2^(x - ref) of its scores x in units of log2.  The
+// reference follows the running maximum: it is set kXattnUp<T> below it and stays
+// until the maximum is more than kXattnRoom<T> above it, so that most tiles
+// rescale nothing.  In fp16 the largest weight so lies between 2^7 and 2^15, and
+// the others are held to 2^-32 of it; with the maximum itself as reference it is
+// 2^-25, and 2^15 keys of little weight could lose as much as the output's own
+// rounding.  bf16 has fp32's range and needs neither.
+template <typename T>
+constexpr float kXattnUp = std::is_same<T, __half>::value ? 7.f : 0.f;
+template <typename T>
+constexpr float kXattnRoom = 8.f + kXattnUp<T>;
+// (as a difference: ref + room would round where scores are large)
+template <typename T>
+__device__ __forceinline__ bool xattn_moves(float mx, float ref) {
+  return mx - ref > kXattnRoom<T>;
+}
 
 // 2^x (the hardware's approximation, 2 ulp; 2^-inf = 0)
 __device__ __forceinline__ float ex2(float x) {

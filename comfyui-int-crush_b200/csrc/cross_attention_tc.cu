@@ -28,10 +28,10 @@
 // exponentials as polynomials 90 to 94, hand-interleaved 93 and more.
 // 2 x 32760 rows, 512 keys, 40 heads of 128: 630 us, 1090 TFLOP/s.
 //
-// S, the running maximum, the row sum and O are fp32.  The maximum moves only
-// when it grows by more than 2^8 (P stays below 2^8 and the sums exact), so O
-// is rescaled in tensor memory on few tiles.  P is rounded to the activation
-// type (the MMA's operand type), the row sum is not.
+// S, the reference of a row's weights (kXattnUp), the row sum and O are fp32; the
+// reference moves on few tiles, where O is rescaled in tensor memory.  P is
+// rounded to the activation type, the MMA's operand type (at most u sum_j p_j
+// |v_j| beside the output's own rounding), the row sum is not.
 #include "cross_attention.cuh"
 
 #include <type_traits>
@@ -44,7 +44,7 @@ struct XtCfg {
   static constexpr int TILE = PANELS * 16384;
   static constexpr int NST = DP == 128 ? 5 : 8;     // ring stages (K and V tiles in turn)
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_ML = OFF_KV + NST * TILE;   // row maxima and sums, [2 slots][128] float2
+  static constexpr int OFF_ML = OFF_KV + NST * TILE;   // row references and sums, [2 slots][128] float2
   static constexpr int OFF_BAR = OFF_ML + 2048;
   static constexpr int SMEM = OFF_BAR + 512;
   static constexpr int THREADS = 512;
@@ -218,7 +218,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* p_full = p_part + 2;        // [2] all of P is written -> MMA (4 warps)
   uint64_t* o_full = p_full + 2;        // [2] the item's last P V is done -> epilogue
   uint64_t* o_empty = o_full + 2;       // [2] O is read -> MMA (4 warps)
-  uint64_t* l_full = o_empty + 2;       // [2] row maxima and sums are there -> epilogue (4 warps)
+  uint64_t* l_full = o_empty + 2;       // [2] row references and sums are there -> epilogue (4 warps)
   uint64_t* l_empty = l_full + 2;       // [2] and read -> softmax (4 warps)
   uint64_t* kv_full = l_empty + 2;      // [NST] TMA -> MMA, cleaner
   uint64_t* kv_empty = kv_full + NST;   // [NST] MMA -> TMA
@@ -645,8 +645,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         if constexpr (!BIAS) mx *= c;
         // (P V of the tile before is done: this S was issued behind it)
-        if (__any_sync(0xffffffffu, xattn_moves(mx, m))) {
-          const float nm = xattn_moves(mx, m) ? mx : m;
+        if (__any_sync(0xffffffffu, xattn_moves<T>(mx, m))) {
+          const float nm = xattn_moves<T>(mx, m) ? mx - kXattnUp<T> : m;
           const float f = nm == m ? 1.f : ex2(m - nm);
           m = nm;
           sum *= f;

@@ -343,7 +343,8 @@ int ic_qk_norm_rope(const void* q, void* q_out, int64_t H, const void* k, void* 
  * sees no key gets zeros.  A constant in an additive mask changes nothing,
  * whatever its size (a sample whose seen keys all hold a type's lowest value
  * gets the softmax of its scores).  Scores, softmax and sums in fp32; the weights are
- * rounded to dtype for the product with v.
+ * rounded to dtype for the product with v (f16: to 2^-32 of a row's largest one
+ * where that is coarser).
  *   q, out  [B, Lq, H, D], k, v [B, Lk, Hk, D] in dtype (f16 / bf16), D a
  *           multiple of 8 up to 128, H a multiple of Hk
  *   strides 12 element strides, batch / token / head of q, k, v, out;

@@ -105,6 +105,32 @@ def test_one_sample_of_an_odd_buffer(Lq):
 # ── fp16 weights ─────────────────────────────────────────────────────────────
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Lq,scale", [(1, 1.0), (1, -1.0), (20, -1.0), (38400, 1.0)])
+def test_many_keys_of_little_weight(Lq, scale, dtype):
+    """One key that outweighs each of 2^19 others by 2^25.5 but not all of them
+    together (their sum is 1.1 percent of it).  A weight is held to 2^-8 (bf16)
+    or 2^-11 and 2^-32 of the largest one (fp16)."""
+    Lk, D = 2**19, 64
+    g = gen(35)
+    q = torch.zeros(1, 1, 1, D, dtype=dtype, device="cuda")
+    k = torch.zeros(1, Lk, 1, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    k[0, 0, 0, 0] = 17.675 / scale
+    v = torch.rand(1, Lk, 1, D, device="cuda", generator=g).to(dtype)
+    v[0, 0] = 0
+    s = k[0, :, 0, 0].double() * scale
+    p = torch.softmax(s, 0)[:, None]
+    vd = v[0, :, 0].double()
+    want = (p * vd).sum(0)
+    tol = (U[dtype] + 3e-5) * want + U[dtype] * want
+    if dtype == torch.float16:
+        tol = tol + 2.0**-25 + 2.0**-32 * p.max() * vd.sum(0)
+    got = rt.cross_attention(q.expand(1, Lq, 1, D), k, v, scale=scale)
+    assert rt.device_error() == 0
+    check(got[0, :, 0], want.expand(Lq, D), tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("Lq,later", [(1, 64), (200, 130)])
 def test_scores_whose_steps_pass_the_room(Lq, later, dtype):
     """Scores of 2^27, where fp32 counts in steps of 16: the later key has 2^16
