@@ -83,6 +83,9 @@ def _need_cuda(what: str, *ts: torch.Tensor | None) -> None:
             raise RuntimeError(f"{what}: tensors on different devices ({dev}, {t.device})")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _on_its_device(fn):
     """``fn``, whose first parameter is a tensor, with that tensor's CUDA device
     current: a launch on a default stream, the SM count and a kernel's
@@ -93,12 +96,14 @@ def _on_its_device(fn):
     def call(*args, **kwargs):
         first = args[0] if args else next((t for t in kwargs.values() if isinstance(t, torch.Tensor)), None)
         index = first.get_device() if isinstance(first, torch.Tensor) else -1
-        if index < 0 or index == torch.cuda.current_device():
-            return fn(*args, **kwargs)
-        with torch.cuda.device(index):
-            return fn(*args, **kwargs)
+        return fn(*args, **kwargs) if index < 0 or index == _current_device() else _on_device(index, fn, *args, **kwargs)
 
     return call
+
+
+def _on_device(index: int, fn, *args, **kwargs):
+    with torch.cuda.device(index):
+        return fn(*args, **kwargs)
 
 
 def _f32c(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -736,7 +741,8 @@ _HALF = {torch.float16: L.IC_DTYPE_F16, torch.bfloat16: L.IC_DTYPE_BF16}
 
 # These calls are short on the device, so their host side is kept short too:
 # plain integers for pointers, the raw stream handle, one ctypes array per set
-# of strides.
+# of strides, the tensors' device compared with the current one in place
+# (_on_its_device takes half a microsecond to hand the arguments on).
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -779,7 +785,8 @@ def _plain_ones(t: torch.Tensor) -> torch.Tensor:
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """``t`` as the kernels read it; a copy where it is not."""
-    if _heads_ok(t):
+    b, l, h, d = t.stride()
+    if d == 1 and l and not ((b | l | h) & 7 or t.data_ptr() & 15):   # (_heads_ok, in place)
         return t
     t = _plain_ones(t)
     return t if _heads_ok(t) else t.clone(memory_format=_DENSE)
@@ -830,7 +837,6 @@ def _gamma16(what: str, t: torch.Tensor | None, D: int) -> torch.Tensor | None:
     return g.clone() if g.data_ptr() & 15 else g
 
 
-@_on_its_device
 def qk_norm_rope(
     q: torch.Tensor,
     k: torch.Tensor | None = None,
@@ -863,6 +869,9 @@ def qk_norm_rope(
     may be the inputs themselves.
     """
     index = q.get_device()
+    if index >= 0 and index != _current_device():
+        return _on_device(index, qk_norm_rope, q, k, q_gamma=q_gamma, k_gamma=k_gamma, cos=cos, sin=sin, layout=layout,
+                          positions=positions, eps=eps, q_out=q_out, k_out=k_out)
     _same_device("qk_norm_rope", index, q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out)
     dtype = _HALF.get(q.dtype)
     if dtype is None:
@@ -880,7 +889,10 @@ def qk_norm_rope(
         if cos.shape != sin.shape or cos.dim() != 2:
             raise ValueError(f"qk_norm_rope: tables must be [rows, rot / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
         cos, sin = _fp32(cos), _fp32(sin)
-        rows, rot = min(cos.shape[0], _INT32_MAX), 2 * cos.shape[1]   # _INT32_MAX is past every table
+        rows, rot = cos.shape
+        rot *= 2
+        if rows > _INT32_MAX:
+            rows = _INT32_MAX   # as a position it is past every table (_index)
     if positions is not None:
         if positions.shape != (B, T):
             raise ValueError(f"qk_norm_rope: positions must be [{B}, {T}], got {tuple(positions.shape)}")
@@ -912,7 +924,6 @@ def qk_norm_rope(
     return y if k is None else (y, yk if k_out is None else k_out)
 
 
-@_on_its_device
 def cross_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -935,6 +946,8 @@ def cross_attention(
     zeros.  All may be strided views.  Returns [B, Lq, H, D].
     """
     index = q.get_device()
+    if index >= 0 and index != _current_device():
+        return _on_device(index, cross_attention, q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale, out=out)
     _same_device("cross_attention", index, q, k, v, kv_lens, key_mask, out)
     dtype = _HALF.get(q.dtype)
     if dtype is None or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -985,7 +998,6 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
 
 
-@_on_its_device
 def lora_batched(
     x: torch.Tensor,
     down: torch.Tensor,
@@ -1009,6 +1021,8 @@ def lora_batched(
     :func:`lowrank_add`, ``_ops.py:236-244``.)
     """
     index = x.get_device()
+    if index >= 0 and index != _current_device():
+        return _on_device(index, lora_batched, x, down, up, ids, scales, base=base, out=out)
     _same_device("lora_batched", index, x, down, up, ids, scales, base, out)
     dt = x.dtype
     dtype = _HALF.get(dt)

@@ -42,7 +42,7 @@ def lib(monkeypatch):
     monkeypatch.setattr(rt, "_stream", lambda t: 0)
     monkeypatch.setattr(rt, "_num_sms", lambda device: 148)
     monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: state.current)
+    monkeypatch.setattr(rt, "_current_device", lambda: state.current)
     monkeypatch.setattr(torch.cuda, "device", Device)
     rt._workspace.cache_clear()
     yield state
