@@ -1017,7 +1017,9 @@ def lora_batched(
     (one per sample of a batch).  ``base`` [..., N] is the shared projection's
     output (None: zeros); ``out`` [..., N] may be ``base``.  An id that names
     no adapter gives NaN for its rows and sets the library's device error
-    word.  (One adapter for all rows: :func:`lowrank_down` /
+    word.  Same inputs give the same bits; a request's last bits may change
+    with which adapters (not with what) its neighbours use, as the order of the
+    fp32 sums goes by them.  (One adapter for all rows: :func:`lowrank_down` /
     :func:`lowrank_add`, ``_ops.py:236-244``.)
     """
     index = x.get_device()

@@ -105,7 +105,8 @@ __device__ __forceinline__ bool lora_two(int id, unsigned rows, int& a0, int& a1
 }
 
 // Whether a tile of 128 rows has more than two adapters in one of its groups of
-// 16 rows, which lora_down_stream_kernel leaves to lora_down_kernel.
+// 16 rows, which lora_down_stream_kernel leaves to lora_down_kernel.  The two add
+// up K in different orders, so a row's last bits depend on its neighbours' ids.
 __device__ __forceinline__ bool lora_tile_left(const LoraArgs& a, int64_t tile0, int lane) {
   bool left = false;
 #pragma unroll

@@ -380,7 +380,11 @@ int64_t ic_cross_attention_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t 
  *   workspace  ic_lora_batched_workspace(...) floats, 16-byte aligned,
  *         contents arbitrary, in use until the call's work has run
  * Any alignment works; 16-byte aligned rows (K, N and strides multiples of 8,
- * R a multiple of 4) are faster.  The sums' order depends on the sizes only. */
+ * R a multiple of 4) are faster.  Same inputs, same bits; what other rows and
+ * adapters hold never matters.  The order of a row's sums over K goes by the
+ * sizes, by whether the rows are 16-byte aligned, and from 1024 rows also by the
+ * ids around it: a tile of 128 rows with more than two adapters among any 16 of
+ * them sums in another order than the others (both in fp32). */
 int ic_lora_batched(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* down, const void* up,
                     int64_t R, int64_t n, const int32_t* ids, int64_t rows_per_id, const float* scales,
                     const void* base, int64_t ldb, void* out, int64_t N, int64_t ldo, float* workspace,

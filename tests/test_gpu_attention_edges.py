@@ -150,3 +150,25 @@ def test_scores_whose_steps_pass_the_room(Lq, later, dtype):
     want = (b + a * 2.0**-16) / (1 + 2.0**-16)
     tol = (U[dtype] + 3e-5) * (b.abs() + a.abs() * 2.0**-16) + U[dtype] * want.abs() + 2.0**-25 + 2.0**-32
     check(got[0, :, 0], want.expand(Lq, D), tol)
+
+
+# ── adapters of the neighbours ───────────────────────────────────────────────
+
+@pytest.mark.parametrize("M", [1024, 1500, 4200])
+def test_neighbours_other_adapters(M):
+    """Neighbours that change to other valid adapters: a request stays within
+    the operator's bound (the order of its sums may change with their ids), and
+    rows of other tiles of 128 keep their bits."""
+    x, base, down, up, scales, g = lora_inputs(37, M, 1000, 72, 16, 6, torch.float16)
+    few = torch.arange(M, device="cuda") // 300 % 2
+    many = few.clone()
+    many[128:256:2] = torch.randint(-1, 6, (64,), device="cuda", generator=g)
+    one = rt.lora_batched(x, down, up, few, scales, base=base)
+    two = rt.lora_batched(x, down, up, many, scales, base=base)
+    for got, ids in ((one, few), (two, many)):
+        want, tol = lora_reference(x, down, up, ids, scales, base, 1)
+        check(got, want, tol)
+    other = torch.ones(M, dtype=torch.bool, device="cuda")
+    other[128:256] = False
+    assert torch.equal(one[other], two[other])
+    assert torch.equal(rt.lora_batched(x, down, up, many, scales, base=base), two)
