@@ -26,7 +26,10 @@
 // not kept (8190 rows, 512 keys, 40 heads, 89 us): P through shared memory with
 // S ahead 105 us (P's traffic on top of what the MMAs read), a part of the
 // exponentials as polynomials 90 to 94, hand-interleaved 93 and more.
-// 2 x 32760 rows, 512 keys, 40 heads of 128: 630 us, 1090 TFLOP/s.
+// 2 x 32760 rows, 512 keys, 40 heads of 128: 620 to 630 us, 1100 TFLOP/s, at
+// 1965 MHz (three launches with pauses); 731 us, 940 TFLOP/s, back to back for
+// seconds, where the power cap holds the clock at 1510 MHz (graph replays and
+// single calls alike).
 //
 // S, the reference of a row's weights (kXattnUp), the row sum and O are fp32; the
 // reference moves on few tiles, where O is rescaled in tensor memory.  P is

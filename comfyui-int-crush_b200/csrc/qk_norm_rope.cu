@@ -15,7 +15,8 @@
 // layout's partner chunk comes by shuffle of the raw 16-bit pairs when rot/2
 // is a multiple of 8, otherwise element by element from the row (an L1 hit);
 // every lane reads before any lane of the warp writes, so the output may be
-// the input.
+// the input.  80 registers for three CTAs per SM; the half layout (LAYOUT 2)
+// keeps 32 to 44 bytes a thread in local memory for it.
 #include "cross_attention.cuh"   // pack16
 
 namespace ic {
@@ -182,6 +183,9 @@ __global__ void __launch_bounds__(kQkThreads, LAYOUT == 3 ? 2 : 3) qk_norm_rope_
   const bool whole = d0 + 8 <= a.rot || d0 >= a.D;
   const float inv_d = 1.f / (float)a.D;
 
+  // The groups of a warp may belong to queries and to keys and so leave this loop
+  // at different turns; the shuffles name the whole warp all the same, which holds
+  // because a lane that leaves the loop leaves the kernel: nothing may come after it.
   for (int hb = 0; hb < a.per_unit[which]; hb += kQkHeads) {
     load(next, hb + kQkHeads);   // of other heads: nothing that is written before it is read
     // partners from memory (LAYOUT 3): all of them before any store
