@@ -86,24 +86,27 @@ def _need_cuda(what: str, *ts: torch.Tensor | None) -> None:
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _on_its_device(fn):
-    """``fn``, whose first parameter is a tensor, with that tensor's CUDA device
-    current: a launch on a default stream, the SM count and a kernel's
-    attributes go by the current device, which need not be the tensors' (a
-    thread starts on device 0)."""
+class _LibraryOn:
+    """The library's entry points, called with CUDA device ``index`` current."""
 
-    @functools.wraps(fn)
-    def call(*args, **kwargs):
-        first = args[0] if args else next((t for t in kwargs.values() if isinstance(t, torch.Tensor)), None)
-        index = first.get_device() if isinstance(first, torch.Tensor) else -1
-        return fn(*args, **kwargs) if index < 0 or index == _current_device() else _on_device(index, fn, *args, **kwargs)
+    def __init__(self, index: int):
+        self._index = index
 
-    return call
+    def __getattr__(self, name: str):
+        entry = getattr(L.lib(), name)
+
+        def call(*args):
+            with torch.cuda.device(self._index):
+                return entry(*args)
+
+        return call
 
 
-def _on_device(index: int, fn, *args, **kwargs):
-    with torch.cuda.device(index):
-        return fn(*args, **kwargs)
+def _lib(index: int):
+    """The library for tensors of CUDA device ``index``: a launch on a default
+    stream, the SM count and a kernel's attributes go by the current device,
+    which need not be the tensors' (a thread starts on device 0)."""
+    return L.lib() if index == _current_device() else _LibraryOn(index)
 
 
 def _f32c(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -118,7 +121,6 @@ def _round16(n: int) -> int:
 
 # ── activation prep ──────────────────────────────────────────────────────────
 
-@_on_its_device
 def prep_quantize(
     x: torch.Tensor,
     *,
@@ -193,13 +195,13 @@ def prep_quantize(
         if g.numel() != K or (b is not None and b.numel() != K):
             raise ValueError("prep_quantize: gamma / beta must have K entries")
         _need_cuda("prep_quantize", g, b)
-        st = L.lib().ic_prep_quant_norm(
+        st = _lib(x2.get_device()).ic_prep_quant_norm(
             _p(x2), _DT[x2.dtype], M, K, x2.stride(0), code, _p(g), _p(b), float(eps), _p(sr), int(rot_size), w_in,
             _p(perm), _p(xq_full), xq_full.stride(0) if xq_full is not None else 0, _p(s_a), _p(x_prep),
             _p(rowsum), _stream(x2))
         L.check(st, "ic_prep_quant_norm")
         return x_int8, s_a, x_prep, rowsum
-    st = L.lib().ic_prep_quant(
+    st = _lib(x2.get_device()).ic_prep_quant(
         _p(x2), _DT[x2.dtype], M, K, x2.stride(0), _p(sr), int(rot_size), w_in, _p(perm), _p(sm),
         _p(xq_full), xq_full.stride(0) if xq_full is not None else 0, _p(s_a), _p(x_prep), _p(rowsum),
         _stream(x2))
@@ -263,7 +265,6 @@ def fused_rmsnorm_quantize(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e
 
 # ── GEMMs ────────────────────────────────────────────────────────────────────
 
-@_on_its_device
 def gemm_a8(
     x_int8: torch.Tensor,
     w: torch.Tensor,
@@ -342,7 +343,7 @@ def gemm_a8(
             if r.stride(1) != 1:
                 r = r.contiguous()
         ws = torch.empty(splits * M * N if splits > 1 else 0, dtype=torch.float32, device=x_int8.device)
-        st = L.lib().ic_gemm_a8_ex(
+        st = _lib(x_int8.get_device()).ic_gemm_a8_ex(
             _p(x_int8), M, K, x_int8.stride(0), _p(w), kind, N, w.stride(0), _p(sw), G, gs, _p(sa),
             _p(b), _DT[b.dtype] if b is not None else 0, _p(rs), _p(zc), int(activation),
             _p(r), _DT[r.dtype] if r is not None else 0, r.stride(0) if r is not None else 0,
@@ -352,13 +353,13 @@ def gemm_a8(
         return out
     if splits > 1:
         ws = torch.empty(splits * M * N, dtype=torch.float32, device=x_int8.device)
-        st = L.lib().ic_gemm_a8_splitk(
+        st = _lib(x_int8.get_device()).ic_gemm_a8_splitk(
             _p(x_int8), M, K, x_int8.stride(0), _p(w), kind, N, w.stride(0), _p(sw), G, gs, _p(sa),
             _p(b), _DT[b.dtype] if b is not None else 0, _p(rs), _p(zc), _p(out), _DT[out.dtype], out.stride(0),
             int(splits), _p(ws), ws.numel(), _stream(x_int8))
         L.check(st, "ic_gemm_a8_splitk")
         return out
-    st = L.lib().ic_gemm_a8(
+    st = _lib(x_int8.get_device()).ic_gemm_a8(
         _p(x_int8), M, K, x_int8.stride(0), _p(w), kind, N, w.stride(0), _p(sw), G, gs, _p(sa),
         _p(b), _DT[b.dtype] if b is not None else 0, _p(rs), _p(zc), _p(out), _DT[out.dtype], out.stride(0),
         _stream(x_int8))
@@ -424,7 +425,6 @@ def fused_int8_gemm_dequant(
                    residual=residual)
 
 
-@_on_its_device
 def int8_gemm_int8out(
     x_int8: torch.Tensor,
     w_int8: torch.Tensor,
@@ -486,7 +486,7 @@ def int8_gemm_int8out(
         s_c = torch.empty(M, dtype=torch.float32, device=x_int8.device)
     b = None if bias is None else bias.contiguous()
     ws = torch.empty(M * N + M, dtype=torch.float32, device=x_int8.device)
-    st = L.lib().ic_gemm_a8_int8out(
+    st = _lib(x_int8.get_device()).ic_gemm_a8_int8out(
         _p(x_int8), M, K, x_int8.stride(0), _p(w), kind, N, w.stride(0), _p(sw), G, gs, _p(sa),
         _p(b), _DT[b.dtype] if b is not None else 0, int(activation), _p(c), c.stride(0), _p(s_c),
         _p(ws), ws.numel(), _stream(x_int8))
@@ -525,7 +525,6 @@ def fused_quant_int8_gemm_dequant(
     return gemm_a8(x_int8, w_int8, s_w, s_a, bias=bias, out_dtype=out_dtype, out=out)
 
 
-@_on_its_device
 def gemm_w4a16(
     x: torch.Tensor,
     packed: torch.Tensor,
@@ -578,7 +577,7 @@ def gemm_w4a16(
     if splits is None:
         splits = _w4a16_splits(M, N, K, x.device)
     ws = torch.empty(splits * M * N if (splits > 1 and M > 128) else 0, dtype=torch.float32, device=x.device)
-    st = L.lib().ic_gemm_w4a16_splitk(
+    st = _lib(x2.get_device()).ic_gemm_w4a16_splitk(
         _p(x2), _DT[x.dtype], M, K, x2.stride(0), _p(packed), N, packed.stride(0), int(w_layout),
         _p(sc), _DT[sc.dtype],
         G, gs, _p(b), _DT[b.dtype] if b is not None else 0, _p(mid), _p(up), R, float(lr_scale),
@@ -601,7 +600,6 @@ def _w4a16_splits(M: int, N: int, K: int, device) -> int:
     return s
 
 
-@_on_its_device
 def lowrank_down(x: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
     """``mid = T(x @ down^T)`` (``F.linear(x_raw, down)``, ``_ops.py:242``),
     T = x's dtype (fp16 or bf16; other dtypes compute in fp16)."""
@@ -614,12 +612,12 @@ def lowrank_down(x: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
     M, K = x2.shape
     R = d.shape[0]
     mid = torch.empty((M, R), dtype=dt, device=x.device)
-    L.check(L.lib().ic_lowrank_down_ex(_p(x2), _DT[dt], M, K, x2.stride(0), _p(d), R, _p(mid), _stream(x2)),
-            "ic_lowrank_down_ex")
+    st = _lib(x2.get_device()).ic_lowrank_down_ex(
+        _p(x2), _DT[dt], M, K, x2.stride(0), _p(d), R, _p(mid), _stream(x2))
+    L.check(st, "ic_lowrank_down_ex")
     return mid
 
 
-@_on_its_device
 def lowrank_add(out: torch.Tensor, mid: torch.Tensor, up: torch.Tensor, scale: float) -> torch.Tensor:
     """In place ``out = T(out + scale * mid @ up^T)`` (``out.addmm_``,
     ``_ops.py:243``); out fp16 or bf16, rank up to 256."""
@@ -629,12 +627,12 @@ def lowrank_add(out: torch.Tensor, mid: torch.Tensor, up: torch.Tensor, scale: f
     m = mid.to(out.dtype).contiguous()
     u = up.to(out.dtype).contiguous()
     M, N = out.shape
-    L.check(L.lib().ic_lowrank_add_ex(_p(out), _DT[out.dtype], M, N, out.stride(0), _p(m), _p(u), m.shape[1],
-                                      float(scale), _stream(out)), "ic_lowrank_add_ex")
+    st = _lib(out.get_device()).ic_lowrank_add_ex(
+        _p(out), _DT[out.dtype], M, N, out.stride(0), _p(m), _p(u), m.shape[1], float(scale), _stream(out))
+    L.check(st, "ic_lowrank_add_ex")
     return out
 
 
-@_on_its_device
 def quantize_weight(w: torch.Tensor, bits: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-row requantisation of a float weight on the device (the layout
     classes' ``quantize``, ``quant_layout.py:100-129,179-200``): returns
@@ -655,12 +653,12 @@ def quantize_weight(w: torch.Tensor, bits: int) -> tuple[torch.Tensor, torch.Ten
         s = torch.empty(N, dtype=torch.float32, device=w.device)
     else:
         raise ValueError(f"bits must be 4 or 8, got {bits}")
-    st = L.lib().ic_quantize_weight(_p(wf), N, K, wf.stride(0), int(bits), _p(q), q.stride(0), _p(s), _stream(wf))
+    st = _lib(wf.get_device()).ic_quantize_weight(
+        _p(wf), N, K, wf.stride(0), int(bits), _p(q), q.stride(0), _p(s), _stream(wf))
     L.check(st, "ic_quantize_weight")
     return q, s
 
 
-@_on_its_device
 def lokr_add(out: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, scale: float) -> torch.Tensor:
     """``out[t] (viewed [out_l, out_k]) += scale * (w1 @ x[t].view(in_m, in_n)) @ w2^T``
     in place (``_apply_lokr``, ``_ops.py:88-138``): ``w1`` [out_l, in_m],
@@ -680,13 +678,13 @@ def lokr_add(out: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
     out_l, in_m = w1c.shape
     out_k, in_n = w2c.shape
     temp = torch.empty(M * out_l * in_n, dtype=out.dtype, device=out.device)
-    st = L.lib().ic_lokr_add(_p(out), _DT[out.dtype], M, N, _p(x), x.stride(0), x.shape[1], _p(w1c), out_l, in_m,
-                             _p(w2c), out_k, in_n, float(scale), _p(temp), temp.numel(), _stream(out))
+    st = _lib(out.get_device()).ic_lokr_add(
+        _p(out), _DT[out.dtype], M, N, _p(x), x.stride(0), x.shape[1], _p(w1c), out_l, in_m, _p(w2c), out_k, in_n,
+        float(scale), _p(temp), temp.numel(), _stream(out))
     L.check(st, "ic_lokr_add")
     return out
 
 
-@_on_its_device
 def repack_int4(packed: torch.Tensor, K: int, layout: int) -> torch.Tensor:
     """Load-time nibble permutation of packed INT4 weights (``ic_repack_int4``):
     layout 0 feeds ``gemm_a8(..., repacked=True)``, layout 1 feeds
@@ -694,24 +692,24 @@ def repack_int4(packed: torch.Tensor, K: int, layout: int) -> torch.Tensor:
     _need_cuda("repack_int4", packed)
     p = packed.contiguous()
     out = torch.empty_like(p)
-    L.check(L.lib().ic_repack_int4(_p(p), p.shape[0], K, p.stride(0), _p(out), out.stride(0), int(layout),
-                                   _stream(p)), "ic_repack_int4")
+    st = _lib(p.get_device()).ic_repack_int4(
+        _p(p), p.shape[0], K, p.stride(0), _p(out), out.stride(0), int(layout), _stream(p))
+    L.check(st, "ic_repack_int4")
     return out
 
 
-@_on_its_device
 def unpack_int4_to_int8(packed: torch.Tensor, K: int) -> torch.Tensor:
     """``kernels/triton_int4_to_int8_unpack.py:55-81``."""
     _need_cuda("unpack_int4_to_int8", packed)
     p = packed.contiguous()
     N = p.shape[0]
     out = torch.empty((N, K), dtype=torch.int8, device=p.device)
-    L.check(L.lib().ic_unpack_int4_to_int8(_p(p), N, K, p.stride(0), _p(out), _stream(p)),
-            "ic_unpack_int4_to_int8")
+    st = _lib(p.get_device()).ic_unpack_int4_to_int8(
+        _p(p), N, K, p.stride(0), _p(out), _stream(p))
+    L.check(st, "ic_unpack_int4_to_int8")
     return out
 
 
-@_on_its_device
 def unpack_int4_to_float16(packed: torch.Tensor, scale: torch.Tensor, K: int,
                            group_size: int | None = None) -> torch.Tensor:
     """``kernels/triton_int4_unpack.py:62-88`` (scale ``[N]``), extended to
@@ -726,8 +724,9 @@ def unpack_int4_to_float16(packed: torch.Tensor, scale: torch.Tensor, K: int,
     G = sc.shape[1]
     gs = int(group_size) if group_size else -(-K // G)
     out = torch.empty((N, K), dtype=torch.float16, device=p.device)
-    L.check(L.lib().ic_unpack_int4_to_f16(_p(p), N, K, p.stride(0), _p(sc), _DT[sc.dtype], G, gs,
-                                          _p(out), _stream(p)), "ic_unpack_int4_to_f16")
+    st = _lib(p.get_device()).ic_unpack_int4_to_f16(
+        _p(p), N, K, p.stride(0), _p(sc), _DT[sc.dtype], G, gs, _p(out), _stream(p))
+    L.check(st, "ic_unpack_int4_to_f16")
     return out
 
 
@@ -741,8 +740,7 @@ _HALF = {torch.float16: L.IC_DTYPE_F16, torch.bfloat16: L.IC_DTYPE_BF16}
 
 # These calls are short on the device, so their host side is kept short too:
 # plain integers for pointers, the raw stream handle, one ctypes array per set
-# of strides, the tensors' device compared with the current one in place
-# (_on_its_device takes half a microsecond to hand the arguments on).
+# of strides.
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -752,11 +750,10 @@ def _strides12(*strides):
     return (ctypes.c_int64 * 12)(*strides)
 
 
-# Workspace floats by sizes (and device, which is the current one: the plans go
-# by its SM count).
+# Workspace floats by sizes (and device: the plans go by its SM count).
 @functools.lru_cache(maxsize=4096)
 def _workspace(name: str, index: int, *sizes: int) -> int:
-    return getattr(L.lib(), name)(*sizes)
+    return getattr(_lib(index), name)(*sizes)
 
 
 def _same_device(what: str, index: int, *ts: torch.Tensor | None) -> None:
@@ -869,9 +866,6 @@ def qk_norm_rope(
     may be the inputs themselves.
     """
     index = q.get_device()
-    if index >= 0 and index != _current_device():
-        return _on_device(index, qk_norm_rope, q, k, q_gamma=q_gamma, k_gamma=k_gamma, cos=cos, sin=sin, layout=layout,
-                          positions=positions, eps=eps, q_out=q_out, k_out=k_out)
     _same_device("qk_norm_rope", index, q, k, q_gamma, k_gamma, cos, sin, positions, q_out, k_out)
     dtype = _HALF.get(q.dtype)
     if dtype is None:
@@ -913,7 +907,7 @@ def qk_norm_rope(
         xk = _heads(k)
         yk = torch.empty_like(k, memory_format=_DENSE) if k_out is None else _out_heads("qk_norm_rope", k_out, k)
         strides = _strides12(*x.stride()[:3], *y.stride()[:3], *xk.stride()[:3], *yk.stride()[:3])
-    st = L.lib().ic_qk_norm_rope(
+    st = _lib(index).ic_qk_norm_rope(
         x.data_ptr(), y.data_ptr(), H, None if xk is None else xk.data_ptr(), None if yk is None else yk.data_ptr(), Hk,
         dtype, B, T, D, strides, None if gq is None else gq.data_ptr(), None if gk is None else gk.data_ptr(), eps, form,
         rot, cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, rows,
@@ -946,8 +940,6 @@ def cross_attention(
     zeros.  All may be strided views.  Returns [B, Lq, H, D].
     """
     index = q.get_device()
-    if index >= 0 and index != _current_device():
-        return _on_device(index, cross_attention, q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale, out=out)
     _same_device("cross_attention", index, q, k, v, kv_lens, key_mask, out)
     dtype = _HALF.get(q.dtype)
     if dtype is None or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -980,7 +972,7 @@ def cross_attention(
     n = _workspace("ic_cross_attention_workspace", index, B, Lq, Lk, H, Hk, D, kind)
     # (sizes that are refused: the call below says why)
     ws = q.new_empty(2 * n) if n > 0 else None   # n floats, in 16-bit elements
-    st = L.lib().ic_cross_attention(
+    st = _lib(index).ic_cross_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dtype, B, Lq, Lk, H, Hk, D,
         _strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3]),
         D ** -0.5 if scale is None else scale, None if kv_lens is None else kv_lens.data_ptr(),
@@ -1023,8 +1015,6 @@ def lora_batched(
     :func:`lowrank_add`, ``_ops.py:236-244``.)
     """
     index = x.get_device()
-    if index >= 0 and index != _current_device():
-        return _on_device(index, lora_batched, x, down, up, ids, scales, base=base, out=out)
     _same_device("lora_batched", index, x, down, up, ids, scales, base, out)
     dt = x.dtype
     dtype = _HALF.get(dt)
@@ -1074,7 +1064,7 @@ def lora_batched(
         down = down.contiguous()
     if not up.is_contiguous():
         up = up.contiguous()
-    st = L.lib().ic_lora_batched(
+    st = _lib(index).ic_lora_batched(
         x2.data_ptr(), dtype, M, K, x2.stride(0) if M > 1 else K, down.data_ptr(), up.data_ptr(), R, n, ids.data_ptr(),
         M // S, None if scales is None else scales.data_ptr(), None if b2 is None else b2.data_ptr(),
         N if b2 is None or M == 1 else b2.stride(0), out.data_ptr(), N, ldo, ws.data_ptr(), need, _raw_stream(index))
