@@ -17,7 +17,9 @@ Hadamard + pad + PermuQuant + smooth + per-token INT8 in one pass),
 zero-point term fused), ``gemm_w4a16`` (weight-streaming W4A16 with the
 low-rank residual fused), ``lowrank_down`` / ``lowrank_add``.  Beside the
 projections: ``qk_norm_rope`` (head norms and rotation in one pass),
-``cross_attention`` and ``lora_batched`` (an adapter per request).
+``cross_attention`` and ``lora_batched`` (an adapter per request).  The 8-bit
+floating point linear: ``quantize_fp8_block``, ``gemm_fp8_block``, and
+``group_norm`` / ``fused_groupnorm_quantize`` in front of it.
 """
 
 from __future__ import annotations
@@ -1073,6 +1075,273 @@ def lora_batched(
     return out
 
 
+# ── 8-bit floating point linear ──────────────────────────────────────────────
+
+_ACTIVATION_CODES = (0, 1, 2, 3)
+_E4M3 = torch.float8_e4m3fn
+
+
+def _folded(t: torch.Tensor, width: int) -> torch.Tensor:
+    """``t`` [..., width] as a matrix with contiguous rows, a copy only where its
+    strides need one."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    ld = t.stride(0)
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or ld >= width) else t.contiguous()
+
+
+def _fp8_buffers(M: int, K: int, scale_rows: int, device: torch.device, by_block: bool):
+    """Uninitialised e4m3 rows [M, K] whose stride is K rounded up to 16, and
+    scales [scale_rows, K / 128], stored block by block where ``by_block``."""
+    q = torch.empty((M, _round16(K)), dtype=_E4M3, device=device)
+    kb = -(-K // 128)
+    if by_block:
+        return q[:, :K] if K & 15 else q, torch.empty((kb, scale_rows), dtype=torch.float32, device=device).t()
+    return q[:, :K] if K & 15 else q, torch.empty((scale_rows, kb), dtype=torch.float32, device=device)
+
+
+def quantize_fp8_block(x: torch.Tensor, *, rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 values with an fp32 scale for each block of 128 along the last
+    dimension: ``s = max(max |x|, 1e-8) / 448``, ``q = e4m3(x / s)`` with IEEE
+    division, ties to even.
+
+    ``rows=1`` (activations): ``x`` [..., K] (fp16 / bf16 / fp32) gives ``q``
+    [..., K] and ``s`` [..., ceil(K / 128)].  ``rows=128`` (weights): ``x``
+    [N, K] gives ``q`` [N, K] and ``s`` [ceil(N / 128), ceil(K / 128)], a scale
+    for each 128 x 128 block.  Both are what :func:`gemm_fp8_block` takes: ``q``'s
+    rows start at multiples of 16 bytes (it is a view where K is no multiple of
+    16), activations' scales are stored block by block.
+
+    A NaN makes its block's scale NaN, an infinity infinite; neither is lost
+    in a product.  (INT8 per token: :func:`dynamic_quantize_activation`,
+    ``kernels/triton_quantize.py:151-198``.)
+    """
+    index = x.get_device()
+    _same_device("quantize_fp8_block", index, x)
+    dtype = _DT.get(x.dtype)
+    if dtype is None:
+        raise TypeError(f"quantize_fp8_block: x must be float16, bfloat16 or float32, got {x.dtype}")
+    if rows not in (1, 128):
+        raise ValueError(f"quantize_fp8_block: rows must be 1 or 128, got {rows}")
+    if x.dim() < 1 or x.shape[-1] == 0 or (rows == 128 and x.dim() != 2):
+        raise ValueError(f"quantize_fp8_block: x must be {'[..., K]' if rows == 1 else '[N, K]'}, got {tuple(x.shape)}")
+    K = x.shape[-1]
+    x2 = _folded(x, K)
+    M = x2.shape[0]
+    q, s = _fp8_buffers(M, K, M if rows == 1 else -(-M // 128), x.device, rows == 1)
+    if M:
+        st = _lib(index).ic_quantize_fp8_block(
+            x2.data_ptr(), dtype, M, K, x2.stride(0) if M > 1 else K, rows, q.data_ptr(), q.stride(0) if M > 1 else _round16(K),
+            s.data_ptr(), s.stride(0), s.stride(1), _raw_stream(index))
+        if st:
+            L.check(st, "ic_quantize_fp8_block")
+    if x.dim() == 2:
+        return q, s
+    return q.view(x.shape), s.view(*x.shape[:-1], s.shape[1])
+
+
+def _fp8_rows(t: torch.Tensor, K: int) -> torch.Tensor:
+    """An e4m3 operand as the kernel reads it: 16-byte aligned rows; a copy
+    where it is not."""
+    if t.dim() != 2:
+        t = t.reshape(-1, K)
+    M = t.shape[0]
+    ld = t.stride(0)
+    if t.stride(1) == 1 and not t.data_ptr() & 15 and (M <= 1 or (not ld & 15 and ld >= K)):
+        return t
+    rows = torch.empty((M, _round16(K)), dtype=t.dtype, device=t.device)[:, :K]
+    rows.view(torch.uint8).copy_(t.view(torch.uint8) if t.stride(1) == 1 else t.contiguous().view(torch.uint8))
+    return rows
+
+
+def gemm_fp8_block(
+    x: torch.Tensor,
+    w: torch.Tensor,
+    s_w: torch.Tensor,
+    s_a: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``out[m, n] = sum_b s_a[m, b] s_w[n // 128, b] (x @ w^T)_b + bias`` of e4m3
+    operands with a scale for each block of 128, fp32 sums, one rounding.
+
+    ``x`` [..., K] and ``w`` [N, K] are ``float8_e4m3fn``, ``s_a`` [..., KB] and
+    ``s_w`` [ceil(N / 128), KB] fp32 with KB = ceil(K / 128), as
+    :func:`quantize_fp8_block` returns them or as a checkpoint holds them (any
+    strides; rows of ``x`` or ``w`` that do not start at multiples of 16 bytes
+    are copied first).  ``bias`` [N] and ``out_dtype`` are fp16, bf16 or fp32;
+    ``out`` [..., N] sets the latter.  Same inputs give the same bits.
+    (INT8 and INT4 operands: :func:`gemm_a8`, ``kernels/triton_int8_gemm.py:135-205``.)
+    """
+    index = x.get_device()
+    _same_device("gemm_fp8_block", index, x, w, s_w, s_a, bias, out)
+    if x.dtype is not _E4M3 or w.dtype is not _E4M3:
+        raise TypeError(f"gemm_fp8_block: x and w must be float8_e4m3fn, got {x.dtype}, {w.dtype}")
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or w.shape[1] == 0:
+        raise ValueError(f"gemm_fp8_block: x must be [..., K] and w [N, K], got {tuple(x.shape)}, {tuple(w.shape)}")
+    N, K = w.shape
+    kb = -(-K // 128)
+    lead = x.shape[:-1]
+    if s_a.shape != (*lead, kb) or s_w.shape != (-(-N // 128), kb):
+        raise ValueError(f"gemm_fp8_block: scales must be {(*lead, kb)} and {(-(-N // 128), kb)}, got {tuple(s_a.shape)}, "
+                         f"{tuple(s_w.shape)}")
+    if s_a.dtype is not torch.float32 or s_w.dtype is not torch.float32:
+        raise TypeError(f"gemm_fp8_block: scales must be float32, got {s_a.dtype}, {s_w.dtype}")
+    if out is not None:
+        out_dtype = out.dtype
+    code = _DT.get(out_dtype)
+    if code is None:
+        raise TypeError(f"gemm_fp8_block: the output must be float16, bfloat16 or float32, got {out_dtype}")
+    bias_code = 0
+    if bias is not None:
+        bias_code = _DT.get(bias.dtype)
+        if bias_code is None:
+            raise TypeError(f"gemm_fp8_block: bias must be float16, bfloat16 or float32, got {bias.dtype}")
+        if bias.shape != (N,):
+            raise ValueError(f"gemm_fp8_block: bias must be [{N}], got {tuple(bias.shape)}")
+        if bias.stride(0) != 1:
+            bias = bias.contiguous()
+    if out is None:
+        out = torch.empty((*lead, N), dtype=out_dtype, device=x.device)
+        M = out.numel() // N if N else 0
+        ldo = N
+    else:
+        if out.shape != (*lead, N):
+            raise ValueError(f"gemm_fp8_block: out must be {(*lead, N)}, got {tuple(out.shape)}")
+        if out.numel() == 0:
+            return out
+        o2 = out if out.dim() == 2 else out.view(-1, N)   # raises where the leading dimensions do not fold
+        M = o2.shape[0]
+        ldo = o2.stride(0) if M > 1 else N
+        if (N > 1 and o2.stride(1) != 1) or ldo < N:
+            raise ValueError(f"gemm_fp8_block: out must be row-major, got strides {out.stride()}")
+    if M == 0 or N == 0:
+        return out
+    x2 = _fp8_rows(x, K)
+    w = _fp8_rows(w, K)
+    sa = s_a if s_a.dim() == 2 else s_a.reshape(-1, kb)
+    ld = _round16(K)
+    st = _lib(index).ic_gemm_fp8_block(
+        x2.data_ptr(), M, K, x2.stride(0) if M > 1 else ld, w.data_ptr(), N, w.stride(0) if N > 1 else ld,
+        sa.data_ptr(), sa.stride(0), sa.stride(1), s_w.data_ptr(), s_w.stride(0), s_w.stride(1),
+        None if bias is None else bias.data_ptr(), bias_code, out.data_ptr(), code, ldo, _raw_stream(index))
+    if st:
+        L.check(st, "ic_gemm_fp8_block")
+    return out
+
+
+def _channels_last(t: torch.Tensor):
+    """``t`` [B, ..., C] as [B, L, C], its elements contiguous along C, and
+    whether that is a view."""
+    C = t.shape[-1]
+    try:
+        v = t.view(t.shape[0], -1, C) if t.dim() != 3 else t
+    except RuntimeError:
+        return None
+    return v if v.stride(2) == 1 or C == 1 else None
+
+
+def _group_norm(what, x, groups, weight, bias, eps, activation, out, quantize):
+    index = x.get_device()
+    _same_device(what, index, x, weight, bias, out)
+    dtype = _HALF.get(x.dtype)
+    if dtype is None:
+        raise TypeError(f"{what}: x must be float16/bfloat16, got {x.dtype}")
+    if x.dim() < 2:
+        raise ValueError(f"{what}: x must be [batch, ..., channels], got {tuple(x.shape)}")
+    if activation not in _ACTIVATION_CODES:
+        raise ValueError(f"{what}: activation must be 0 (none), 1 (SiLU), 2 (GELU erf) or 3 (GELU tanh), got {activation}")
+    B, C = x.shape[0], x.shape[-1]
+    if groups < 1 or C == 0 or C % groups:
+        raise ValueError(f"{what}: {C} channels do not divide into {groups} groups")
+    codes = []
+    for t in (weight, bias):
+        code = 0
+        if t is not None:
+            code = _DT.get(t.dtype)
+            if code is None:
+                raise TypeError(f"{what}: weight and bias must be float16, bfloat16 or float32, got {t.dtype}")
+            if t.shape != (C,):
+                raise ValueError(f"{what}: weight and bias must be [{C}], got {tuple(t.shape)}")
+        codes.append(code)
+    if weight is not None and weight.stride(0) != 1:
+        weight = weight.contiguous()
+    if bias is not None and bias.stride(0) != 1:
+        bias = bias.contiguous()
+    y = yv = q = s = None
+    if quantize:
+        rows = x.numel() // C
+        q, s = _fp8_buffers(rows, C, rows, x.device, True)
+    else:
+        if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+            raise ValueError(f"{what}: out must be {x.dtype} {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    if x.numel():
+        xv = None if x.dim() == 2 else _channels_last(x)
+        if x.dim() == 2:
+            xv = x[:, None] if x.stride(1) == 1 else x.contiguous()[:, None]
+        if xv is None or (xv.shape[1] > 1 and xv.stride(1) < C):
+            xv = x.contiguous().view(B, -1, C)
+        T = xv.shape[1]
+        ys = (0, C)
+        if y is not None:
+            yv = y[:, None] if y.dim() == 2 else _channels_last(y)
+            if yv is None or yv.stride(2) != 1 and C > 1 or (T > 1 and yv.stride(1) < C) or (B > 1 and yv.stride(0) < C):
+                raise ValueError(f"{what}: out must be channels last with rows that do not overlap, got strides {out.stride()}")
+            ys = (yv.stride(0), yv.stride(1) if T > 1 else C)
+        n = _workspace("ic_group_norm_workspace", index, B, T, C, groups, int(quantize))
+        # (sizes that are refused: the call below says why)
+        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
+        st = _lib(index).ic_group_norm(
+            xv.data_ptr(), dtype, B, T, C, xv.stride(0), xv.stride(1) if T > 1 else C, groups,
+            None if weight is None else weight.data_ptr(), codes[0], None if bias is None else bias.data_ptr(), codes[1],
+            eps, activation, None if y is None else y.data_ptr(), *ys, None if q is None else q.data_ptr(), _round16(C),
+            None if s is None else s.data_ptr(), 1, 0 if s is None else s.stride(1), None if ws is None else ws.data_ptr(), n,
+            _raw_stream(index))
+        if st:
+            L.check(st, "ic_group_norm")
+    return y if not quantize else (q.view(x.shape), s.view(*x.shape[:-1], s.shape[1]))
+
+
+def group_norm(
+    x: torch.Tensor,
+    groups: int,
+    weight: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    eps: float = 1e-5,
+    activation: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)`` over all positions and
+    the ``C // groups`` channels of each group of each sample, in fp32, one
+    rounding.
+
+    ``x`` [B, ..., C] (fp16 / bf16) has its channels last, e.g. [B, H, W, C] or
+    [B, L, C]; a [B, C, H, W] tensor in ``torch.channels_last`` format comes as
+    ``x.permute(0, 2, 3, 1)``, without a copy.  ``weight`` and ``bias`` [C] are
+    fp16, bf16 or fp32 (None: ones, zeros), ``activation`` 0 none, 1 SiLU, 2 GELU
+    (erf), 3 GELU (tanh) as in :func:`gemm_a8`.  Returns a contiguous tensor;
+    ``out`` may be ``x`` itself.  Up to 8192 channels.
+    """
+    return _group_norm("group_norm", x, groups, weight, bias, eps, activation, out, False)
+
+
+def fused_groupnorm_quantize(
+    x: torch.Tensor,
+    groups: int,
+    weight: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    eps: float = 1e-5,
+    activation: int = 0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`group_norm` whose result goes to e4m3 blocks of 128 channels in the
+    same pass: ``(q, s)`` as :func:`quantize_fp8_block` returns them, for
+    :func:`gemm_fp8_block`.  Quantised from the fp32 values, without a rounding to
+    ``x``'s type in between."""
+    return _group_norm("fused_groupnorm_quantize", x, groups, weight, bias, eps, activation, None, True)
+
+
 def device_error(clear: bool = True, device: torch.device | int | None = None) -> int:
     """Error code of ``device`` (default: the current one): 1 = a bounded wait
     timed out, 2 = a position or adapter id out of its range.  Where both
@@ -1091,4 +1360,5 @@ __all__ = [
     "prep_quantize", "gemm_a8", "gemm_w4a16", "repack_int4", "lowrank_down", "lowrank_add", "device_error",
     "fused_layernorm_quantize", "fused_rmsnorm_quantize",
     "qk_norm_rope", "cross_attention", "lora_batched",
+    "quantize_fp8_block", "gemm_fp8_block", "group_norm", "fused_groupnorm_quantize",
 ]

@@ -20,7 +20,7 @@ __all__ = [
     "make_hadamard_regular", "is_power_of_two", "rotate_activations", "pack_int4", "unpack_int4",
     "pack_int8", "unpack_int8", "validate_int4_range", "calculate_scales", "calculate_scales_int8",
     "quantize_weights", "quantize_weights_int8", "INT4_MIN", "INT4_MAX", "INT4_SCALE_DIVISOR",
-    "INT4_TWOS_COMPLEMENT_BIAS", "INT8_MIN", "INT8_MAX", "INT8_SCALE_DIVISOR", "DEFAULT_GROUP_SIZE",
+    "quantize_weights_fp8", "INT4_TWOS_COMPLEMENT_BIAS", "INT8_MIN", "INT8_MAX", "INT8_SCALE_DIVISOR", "DEFAULT_GROUP_SIZE",
 ]
 
 INT4_MIN = -8
@@ -181,3 +181,18 @@ def quantize_weights(W: torch.Tensor, scales: torch.Tensor, group_size: int = DE
 
 def quantize_weights_int8(W: torch.Tensor, scales: torch.Tensor, group_size: int = DEFAULT_GROUP_SIZE) -> torch.Tensor:
     return _quantize_weights(W, scales, INT8_MIN, INT8_MAX, group_size)
+
+
+def quantize_weights_fp8(W: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 values [N, K] and fp32 scales [ceil(N / 128), ceil(K / 128)], one for
+    each 128 x 128 block: ``max(max |w|, 1e-8) / 448``, ties to even.  (On a CUDA
+    tensor ``_b200_runtime.quantize_fp8_block`` gives the same in one pass.)"""
+    if W.dim() != 2:
+        raise ValueError(f"Expected 2D tensor, got {W.dim()}D")
+    N, K = W.shape
+    g = F.pad(W.float(), (0, -K % 128, 0, -N % 128))
+    g = g.reshape(g.shape[0] // 128, 128, g.shape[1] // 128, 128)
+    top = g.abs().amax(dim=(1, 3)).clamp(min=1e-8)
+    scale = top / torch.full_like(top, 448.0)
+    q = (g / scale[:, None, :, None]).to(torch.float8_e4m3fn)
+    return q.reshape(-1, g.shape[2] * 128)[:N, :K].contiguous(), scale

@@ -15,7 +15,12 @@ graph breaks at every ctypes call:
 * ``intcrush_b200::qk_norm_rope(q, k, q_gamma?, k_gamma?, cos?, sin?, layout,
   positions?, eps) -> (q, k)``, ``intcrush_b200::cross_attention(q, k, v,
   kv_lens?, key_mask?, scale) -> out`` and ``intcrush_b200::lora_batched(x,
-  down, up, ids, scales?, base?) -> out`` -- the functions of the same names.
+  down, up, ids, scales?, base?) -> out`` -- the functions of the same names;
+* ``intcrush_b200::quantize_fp8_block(x, rows) -> (q, s)``,
+  ``intcrush_b200::gemm_fp8_block(x, w, s_w, s_a, bias?, out_dtype) -> out``,
+  ``intcrush_b200::group_norm(x, groups, weight?, bias?, eps, activation) -> y``
+  and ``intcrush_b200::fused_groupnorm_quantize(...) -> (q, s)`` -- likewise (rows
+  and scales in the layout that the product takes without a copy).
 
 The ops mirror the reference runtime's callables (``_triton_runtime.py:
 16-41,114-130``): CUDA tensors in, freshly allocated outputs, launch on the
@@ -99,6 +104,52 @@ def register() -> None:
     @lora_batched.register_fake
     def _(x, down, up, ids, scales, base):
         return x.new_empty((*x.shape[:-1], up.shape[1]))
+
+    def e4m3(x, rows):
+        # the layout of _b200_runtime._fp8_buffers
+        K = x.shape[-1]
+        kb = (K + 127) // 128
+        lead = x.shape[:-1]
+        n = x.numel() // K
+        q = x.new_empty((n, (K + 15) // 16 * 16), dtype=torch.float8_e4m3fn)[:, :K].view(x.shape)
+        if rows == 128:
+            return q, x.new_empty(((n + 127) // 128, kb), dtype=torch.float32)
+        return q, x.new_empty((kb, n), dtype=torch.float32).t().view(*lead, kb)
+
+    @torch.library.custom_op(f"{_NS}::quantize_fp8_block", mutates_args=())
+    def quantize_fp8_block(x: torch.Tensor, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return _rt.quantize_fp8_block(x, rows=rows)
+
+    @quantize_fp8_block.register_fake
+    def _(x, rows):
+        return e4m3(x, rows)
+
+    @torch.library.custom_op(f"{_NS}::gemm_fp8_block", mutates_args=())
+    def gemm_fp8_block(x: torch.Tensor, w: torch.Tensor, s_w: torch.Tensor, s_a: torch.Tensor,
+                       bias: torch.Tensor | None, out_dtype: int) -> torch.Tensor:
+        return _rt.gemm_fp8_block(x, w, s_w, s_a, bias=bias, out_dtype=_DTYPES[out_dtype])
+
+    @gemm_fp8_block.register_fake
+    def _(x, w, s_w, s_a, bias, out_dtype):
+        return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=_DTYPES[out_dtype])
+
+    @torch.library.custom_op(f"{_NS}::group_norm", mutates_args=())
+    def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                   activation: int) -> torch.Tensor:
+        return _rt.group_norm(x, groups, weight, bias, eps, activation)
+
+    @group_norm.register_fake
+    def _(x, groups, weight, bias, eps, activation):
+        return x.new_empty(x.shape)
+
+    @torch.library.custom_op(f"{_NS}::fused_groupnorm_quantize", mutates_args=())
+    def fused_groupnorm_quantize(x: torch.Tensor, groups: int, weight: torch.Tensor | None, bias: torch.Tensor | None,
+                                 eps: float, activation: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return _rt.fused_groupnorm_quantize(x, groups, weight, bias, eps, activation)
+
+    @fused_groupnorm_quantize.register_fake
+    def _(x, groups, weight, bias, eps, activation):
+        return e4m3(x, 1)
 
     _done = True
 

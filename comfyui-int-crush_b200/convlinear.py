@@ -15,6 +15,10 @@ rotation + permutation, then the W4A16 GEMM with the bias fused; fp16 or
 bf16 CUDA activations).  The INT8 module is a W8A16 layer: its activation
 prep runs on the B200 prep kernel on CUDA, and the dequantised linear is
 torch's, which is the reference's own arithmetic for this module.
+
+``ConvLinearFP8`` is the third format: e4m3 weights with a scale for each
+128 x 128 block; ``forward`` quantises the activations (1 x 128 blocks) and
+multiplies on the B200 kernels, bias fused.
 """
 
 from __future__ import annotations
@@ -25,7 +29,7 @@ import torch.nn.functional as F
 
 from . import _quant_utils as _qu
 
-__all__ = ["ConvLinear4bit", "ConvLinear8bit"]
+__all__ = ["ConvLinear4bit", "ConvLinear8bit", "ConvLinearFP8"]
 
 
 def _rotated_weight(linear: nn.Linear, rot_need: bool, rot_size: int, perm: torch.Tensor | None) -> torch.Tensor:
@@ -127,3 +131,46 @@ class ConvLinear4bit(_QuantLinearBase):
         b = None if module.bias is None else module.bias.detach().clone()
         return ConvLinear4bit(weight=packed, scale=s, rot_need=rot_need, bias=b, rot_size=rot_size, perm=perm,
                               in_features=w.shape[1])
+
+
+class ConvLinearFP8(_QuantLinearBase):
+    """W8A8 linear in e4m3: weights with a scale for each 128 x 128 block,
+    activations quantised 1 x 128 in ``forward``; optional rotation.  B200
+    kernels only (CUDA fp16 / bf16 activations).  ``weight`` [N, K] is kept with
+    its rows filled up to a multiple of 16 bytes, as the kernel reads them."""
+
+    def __init__(self, weight, scale, rot_need=False, bias=None, rot_size=256, in_features=None):
+        K = weight.shape[-1] if in_features is None else in_features
+        if weight.shape[-1] % 16:
+            rows = torch.zeros(weight.shape[0], -(-K // 16) * 16, dtype=torch.uint8, device=weight.device)
+            rows[:, :K] = weight[:, :K].contiguous().view(torch.uint8)
+            weight = rows.view(weight.dtype)
+        super().__init__(weight, scale, rot_need, bias, rot_size, in_features=K)
+
+    def _apply(self, fn, recurse=True):
+        # a cast of the model's floating point tensors is not one of e4m3 values
+        # or of their scales
+        weight, scale = self.weight, self.scale
+        super()._apply(fn, recurse)
+        self.weight, self.scale = weight.to(self.weight.device), scale.to(self.scale.device)
+        return self
+
+    def forward(self, x):
+        if not (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16)):
+            raise RuntimeError("ConvLinearFP8 runs on the B200 kernels: float16 / bfloat16 CUDA activations "
+                               f"required (got {x.dtype} on {x.device})")
+        from . import _b200_runtime as rt
+        q, s = rt.quantize_fp8_block(self._prepared(x.reshape(-1, x.shape[-1])))
+        y = rt.gemm_fp8_block(q, self.weight[:, :self.in_features], self.scale, s, bias=self.bias, out_dtype=x.dtype)
+        return y.reshape(*x.shape[:-1], -1)
+
+    @staticmethod
+    def from_float(module: nn.Linear, rot_need: bool = False, rot_size: int = 256) -> "ConvLinearFP8":
+        w = _rotated_weight(module, rot_need, rot_size, None)
+        if w.is_cuda:
+            from . import _b200_runtime as rt
+            q, s = rt.quantize_fp8_block(w, rows=128)
+        else:
+            q, s = _qu.quantize_weights_fp8(w)
+        b = None if module.bias is None else module.bias.detach().clone()
+        return ConvLinearFP8(weight=q, scale=s, rot_need=rot_need, bias=b, rot_size=rot_size, in_features=w.shape[1])

@@ -99,14 +99,15 @@ int ic_selftest_wait_timeout(int64_t limit_ns, void* stream) {
 }
 
 int ic_read_device_error(int clear, int* code_out) {
-  // the words of both translation units; the gravest code first, and only the
-  // code that is reported is cleared
-  int v = 0, w = 0;
+  // the words of the three translation units; the gravest code first, and only
+  // the code that is reported is cleared
+  int v = 0, w = 0, u = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_ic_dev_error, sizeof(int));
   if (e == cudaSuccess) e = ic::attention_device_error(&w, false);
+  if (e == cudaSuccess) e = ic::fp8_device_error(&u, false);
   if (e != cudaSuccess) return cuda_status(e, "reading the device error word");
-  const int both = v | w;
-  const int code = both & IC_DEV_ERR_TIMEOUT ? IC_DEV_ERR_TIMEOUT : both & IC_DEV_ERR_INDEX ? IC_DEV_ERR_INDEX : IC_DEV_ERR_NONE;
+  const int all = v | w | u;
+  const int code = all & IC_DEV_ERR_TIMEOUT ? IC_DEV_ERR_TIMEOUT : all & IC_DEV_ERR_INDEX ? IC_DEV_ERR_INDEX : IC_DEV_ERR_NONE;
   if (clear && (v & code)) {
     v &= ~code;
     e = cudaMemcpyToSymbol(g_ic_dev_error, &v, sizeof(int));
@@ -114,6 +115,10 @@ int ic_read_device_error(int clear, int* code_out) {
   if (clear && e == cudaSuccess && (w & code)) {
     w &= ~code;
     e = ic::attention_device_error(&w, true);
+  }
+  if (clear && e == cudaSuccess && (u & code)) {
+    u &= ~code;
+    e = ic::fp8_device_error(&u, true);
   }
   if (e != cudaSuccess) return cuda_status(e, "clearing the device error word");
   if (code_out) *code_out = code;

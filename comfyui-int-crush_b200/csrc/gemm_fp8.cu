@@ -1,0 +1,532 @@
+// Product of two e4m3 matrices with a scale for each block of 128:
+//   out[m, n] = sum_b s_a[m, b] s_w[n / 128, b] sum_{k in block b} x[m, k] w[n, k] + bias[n]
+// on tcgen05 (kind::f8f6f4).
+//
+// Persistent, one CTA per SM, 12 warps: warp 0 TMA producer, warp 1 MMA issuer,
+// warps 4-11 the sums.  Tokens are the MMA's rows (TMEM lanes), features its
+// columns, so that a thread owns one token row and a block's factor
+// s_a * s_w is one number a thread: a weight block is 128 features wide and a
+// warp's columns lie in one.  The 128 products of a block are summed on the
+// tensor core (fp32 in tensor memory, accumulation off at the block's first
+// MMA); the warps read the block's sums, hand the buffer back, and add them, times the
+// factor, onto fp32 registers, two a time.  Two buffers: a block's MMAs run
+// while the block before is read.
+//
+// Large problems: pairs of CTAs (cta_group::2), 256 x 256 a pair, every CTA
+// staging half of each operand.  Others: 128 x 128 a CTA; where those are fewer
+// than the SMs, clusters of CTAs share a tile's blocks and add their sums through
+// distributed shared memory in a fixed order.
+#include <string.h>
+
+#include <type_traits>
+
+namespace ic {
+
+template <int BN_, bool PAIR_>
+struct F8Cfg {
+  static constexpr int BN = BN_;
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int BM = 128;                       // rows of a CTA
+  static constexpr int A_BYTES = BM * 128;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;    // features that a CTA stages
+  static constexpr int STAGE = A_BYTES + B_ROWS * 128;
+  static constexpr int NST = 6;
+  static constexpr int CPT = BN / 2;                   // columns of a thread (8 warps: 4 x 32 rows, 2 halves)
+  static constexpr int OFF_STG = NST * STAGE;          // output staging, 4 KB a warp
+  static constexpr int OFF_BAR = OFF_STG + 8 * 4096;
+  static constexpr int SMEM = OFF_BAR + 256;
+  static constexpr int THREADS = 384;
+  static_assert(BM * BN * 4 <= NST * STAGE || PAIR, "a cluster's partial sums lie over the ring");
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct F8Args {
+  int M, N, kb;                 // kb: blocks along K
+  int m_tiles, n_tiles;
+  int splits;                   // CTAs of a cluster that share a tile's blocks
+  const float* s_a;
+  long long sa_row, sa_block;
+  const float* s_w;
+  long long sw_row, sw_block;
+  const void* bias;
+  int bias_dtype;
+  void* out;
+  int out_dtype;
+  long long ldo;
+  int tma_store;
+};
+
+__device__ __forceinline__ void mma_f8_on(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f8_2_on(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t f8_elect() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on;
+}
+__device__ __forceinline__ void f8_commit_on(uint32_t on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(on)
+      : "memory");
+}
+// on this barrier of both CTAs of the pair
+__device__ __forceinline__ void f8_commit2_on(uint32_t on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
+      ::"r"(smem_u32(bar)), "r"(on)
+      : "memory");
+}
+// D = F32, A and B = e4m3 (format 0), both K-major
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ uint64_t f8_two(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 f8_untwo(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t f8_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ void f8_tie(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Tiles in groups of 8 row tiles, features slowest inside a group, so that the
+// CTAs of a wave share rows and features in L2.
+template <typename A>
+__device__ __forceinline__ void f8_tile(const A& a, int tile, int& mt, int& nt) {
+  constexpr int G = 8;
+  const int per = G * a.n_tiles;
+  const int g = tile / per, r = tile - g * per;
+  const int rows = min(G, a.m_tiles - g * G);
+  nt = r / rows;
+  mt = g * G + r - nt * rows;
+}
+
+template <typename C>
+__global__ void __launch_bounds__(C::THREADS, 1)
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                const __grid_constant__ CUtensorMap tm_o, const F8Args a) {
+  constexpr int NST = C::NST, BN = C::BN, CPT = C::CPT;
+  constexpr bool PAIR = C::PAIR;
+  extern __shared__ __align__(1024) uint8_t smem[];   // no static shared memory: the declared alignment holds
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [NST] TMA -> MMA
+  uint64_t* empty = full + NST;                                       // [NST] MMA -> TMA
+  uint64_t* acc_full = empty + NST;                                   // [2] MMA -> sums
+  uint64_t* acc_empty = acc_full + 2;                                 // [2] sums -> MMA (8 warps of each CTA)
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 2);
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();       // of the pair, or of the split
+  const bool leader = !PAIR || rank == 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, PAIR ? 16 : 8);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc2(tmem_slot, 2 * BN);
+      tmem_relinquish2();
+    } else {
+      tmem_alloc(tmem_slot, 2 * BN);
+      tmem_relinquish();
+    }
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_o);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();   // the peer's barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  const int tiles = a.m_tiles * a.n_tiles;
+  const int first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x / a.splits;
+  const int step = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x / a.splits;
+  // this CTA's blocks of a tile
+  int kb0 = 0, kb1 = a.kb;
+  if (!PAIR && a.splits > 1) {
+    kb0 = (int)((long long)a.kb * rank / a.splits);
+    kb1 = (int)((long long)a.kb * (rank + 1) / a.splits);
+  }
+  constexpr int TILE_M = PAIR ? 256 : 128;
+  const int m_off = PAIR ? (int)rank * 128 : 0;
+  const uint32_t ring = smem_u32(smem);
+
+  // registers: 384 threads x 168 = 128 x 72 + 256 x 216
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step) {
+          int mt, nt;
+          f8_tile(a, t, mt, nt);
+          const int row = mt * TILE_M + m_off, col = nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const uint32_t s = it % NST, ph = (it / NST) & 1u;
+            if (!mbar_wait_cl(empty + s, ph ^ 1u, abort_flag)) { ok = false; break; }
+            uint8_t* st = smem + s * C::STAGE;
+            if constexpr (PAIR) {
+              // both halves count on the leader's barrier
+              if (leader) mbar_arrive_expect_tx(full + s, 2 * C::STAGE);
+              const uint32_t bar = mapa_u32(smem_u32(full + s), 0u);
+              tma_load_2d_pair(st, &tm_x, bar, kb * 128, row);
+              tma_load_2d_pair(st + C::A_BYTES, &tm_w, bar, kb * 128, col);
+            } else {
+              mbar_arrive_expect_tx(full + s, C::STAGE);
+              tma_load_2d(st, &tm_x, full + s, kb * 128, row);
+              tma_load_2d(st + C::A_BYTES, &tm_w, full + s, kb * 128, col);
+            }
+          }
+        }
+        // every copy issued lands before the CTA may leave, whoever gave up
+        // (a pair's count on the leader's barriers: the leader waits for both)
+        if (leader) {
+          volatile int never = 0;
+          for (uint32_t u = it > NST ? it - NST : 0; u < it; ++u) mbar_wait_cl(full + u % NST, (u / NST) & 1u, &never);
+        }
+      }
+    } else if (warp == 1 && leader) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t on = f8_elect();
+      constexpr uint32_t idesc = idesc_f8(PAIR ? 256 : 128, BN);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t s = it % NST, b = it & 1u;
+          ok = mbar_wait_cl(acc_empty + b, ((it >> 1) & 1u) ^ 1u, abort_flag) &&
+               mbar_wait_cl(full + s, (it / NST) & 1u, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = smem_desc_sw128(ring + s * C::STAGE);
+          const uint64_t bd = smem_desc_sw128(ring + s * C::STAGE + C::A_BYTES);
+          const uint32_t d = tmem + b * BN;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (PAIR) mma_f8_2_on(on, d, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+            else mma_f8_on(on, d, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+          }
+          if constexpr (PAIR) {
+            f8_commit2_on(on, empty + s);
+            f8_commit2_on(on, acc_full + b);
+          } else {
+            f8_commit_on(on, empty + s);
+            f8_commit_on(on, acc_full + b);
+          }
+        }
+      }
+      // all MMAs are done before tensor memory is freed
+      volatile int never = 0;
+      if (lane == 0) {
+        if constexpr (PAIR) mma_commit2_local(drain);
+        else mma_commit(drain);
+      }
+      mbar_wait(drain, 0, &never);
+    }
+  } else {
+    // ------------------------------------------------------------------ sums
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int e = warp - 4, q = e & 3, half = e >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * CPT);
+    uint8_t* stg = smem + C::OFF_STG + e * 4096;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += step) {
+      int mt, nt;
+      f8_tile(a, t, mt, nt);
+      const int m0 = mt * TILE_M + m_off + 32 * q, n0 = nt * BN + half * CPT;
+      const int m = m0 + lane;
+      const float* sa = a.s_a + (long long)min(m, a.M - 1) * a.sa_row;
+      const float* sw = a.s_w + (long long)(min(n0, a.N - 1) / 128) * a.sw_row;
+      uint64_t acc[CPT / 2];
+#pragma unroll
+      for (int j = 0; j < CPT / 2; ++j) acc[j] = 0ull;
+      float fa = __ldg(sa + kb0 * a.sa_block), fw = __ldg(sw + kb0 * a.sw_block);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t b = it & 1u;
+        const float f = fa * fw;
+        if (kb + 1 < kb1) {   // the next block's factors, while this one is waited for
+          fa = __ldg(sa + (kb + 1) * a.sa_block);
+          fw = __ldg(sw + (kb + 1) * a.sw_block);
+        }
+        ok = mbar_wait_cl(acc_full + b, (it >> 1) & 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t f2 = f8_two(f, f);
+        uint32_t r[2][32];
+        tmem_ld32(lanes + b * BN, r[0]);
+#pragma unroll
+        for (int c = 0; c < CPT / 32; ++c) {
+          tmem_wait_ld();
+          f8_tie(r[c & 1]);
+          if (c + 1 < CPT / 32) {
+            tmem_ld32(lanes + b * BN + 32 * (c + 1), r[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty + b), 0u));
+              else mbar_arrive(acc_empty + b);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[16 * c + j] = f8_fma2(f8_two(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), f2,
+                                      acc[16 * c + j]);
+        }
+      }
+      if (!ok) break;
+      if (!PAIR && a.splits > 1) {
+        // partial sums of this CTA's blocks, over the ring: every copy has
+        // landed and every MMA is done.  16-byte chunks of a row are XORed with
+        // the row's number, or all lanes would use the same banks.
+        const int r = 32 * q + lane;
+#pragma unroll
+        for (int c = 0; c < CPT / 4; ++c) {
+          const float2 u = f8_untwo(acc[2 * c]), v = f8_untwo(acc[2 * c + 1]);
+          const int chunk = (half * (CPT / 4) + c) ^ lane;
+          *reinterpret_cast<float4*>(smem + r * (BN * 4) + chunk * 16) = make_float4(u.x, u.y, v.x, v.y);
+        }
+        break;   // one tile a cluster
+      }
+      if (a.bias) {
+#pragma unroll
+        for (int j = 0; j < CPT / 2; ++j) {
+          const int n = n0 + 2 * j;
+          const float2 v = f8_untwo(acc[j]);
+          acc[j] = f8_two(v.x + (n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f),
+                          v.y + (n + 1 < a.N ? load_any(a.bias, a.bias_dtype, n + 1) : 0.f));
+        }
+      }
+      // 4 KB of output at a time: 32 rows of 128 bytes, 128-byte-swizzled
+      const int per = a.out_dtype == IC_DTYPE_F32 ? 32 : 64;   // columns
+#pragma unroll
+      for (int c = 0; c < CPT / 32; ++c) {
+        const int n = n0 + 32 * c;   // 32 columns: a whole row of the box in fp32, half of one else
+        const bool begin = per == 32 || (c & 1) == 0, end = per == 32 || (c & 1) == 1;
+        if (begin) {
+          if (lane == 0) bulk_wait_read0();   // the box before has left
+          __syncwarp();
+        }
+        if (per == 32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2 u = f8_untwo(acc[16 * c + 2 * j]), v = f8_untwo(acc[16 * c + 2 * j + 1]);
+            *reinterpret_cast<float4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(u.x, u.y, v.x, v.y);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 u = f8_untwo(acc[16 * c + 4 * j + i]);
+              if (a.out_dtype == IC_DTYPE_F16) {
+                const __half2 h = __floats2half2_rn(u.x, u.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+              } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(u.x, u.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+            }
+            const int chunk = 4 * (c & 1) + j;
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (end) {
+          const int nb = per == 32 ? n : n - 32;
+          if (a.tma_store) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && nb < a.N && m0 < a.M) {
+              tma_store_2d(&tm_o, stg, nb, m0);
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            const int rows = min(32, a.M - m0);
+            for (int r = 0; r < rows; ++r) {
+              if (per == 32) {
+                if (nb + lane < a.N)
+                  reinterpret_cast<float*>(a.out)[(long long)(m0 + r) * a.ldo + nb + lane] =
+                      *reinterpret_cast<const float*>(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const int x = lane + 32 * i;
+                  if (nb + x < a.N)
+                    reinterpret_cast<uint16_t*>(a.out)[(long long)(m0 + r) * a.ldo + nb + x] =
+                        *reinterpret_cast<const uint16_t*>(stg + r * 128 + (((x >> 3) ^ (r & 7)) << 4) + (x & 7) * 2);
+                }
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait0();   // the output has left before the CTA does
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (!PAIR && a.splits > 1) {
+    // the sums of all CTAs of the cluster, in rank order; each takes a share
+    cluster_sync_all();
+    int mt, nt;
+    f8_tile(a, first, mt, nt);
+    const int rows = min(128, a.M - mt * 128);
+    const int all = rows * (BN / 4), per = (all + a.splits - 1) / a.splits;
+    const int lo = (int)rank * per, hi = min(all, lo + per);
+    for (int i = lo + (int)threadIdx.x; i < hi; i += C::THREADS) {
+      const int r = i / (BN / 4), c = i % (BN / 4);
+      const uint32_t at = ring + r * (BN * 4) + (c ^ (r & 31)) * 16;
+      float4 s = ld_cluster4(mapa_u32(at, 0));
+      for (int p = 1; p < a.splits; ++p) {
+        const float4 v = ld_cluster4(mapa_u32(at, p));
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+      const float got[4] = {s.x, s.y, s.z, s.w};
+      const long long m = mt * 128 + r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = nt * BN + 4 * c + j;
+        if (n < a.N)
+          store_out(a.out, a.out_dtype, m * a.ldo + n, got[j] + (a.bias ? load_any(a.bias, a.bias_dtype, n) : 0.f));
+      }
+    }
+  }
+  // nobody leaves while another CTA of the cluster may reach its shared memory
+  if (PAIR || a.splits > 1) cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc2(tmem, 2 * BN);
+    else tmem_dealloc(tmem, 2 * BN);
+  }
+}
+
+// ============================================================== host side
+
+static bool f8_tmap(CUtensorMap* m, CUtensorMapDataType dt, const void* p, uint64_t inner, uint64_t outer, uint64_t ld_bytes,
+                    uint32_t box_inner, uint32_t box_outer) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {inner, outer}, strides[1] = {ld_bytes};
+  const cuuint32_t box[2] = {box_inner, box_outer}, es[2] = {1, 1};
+  return fn(m, dt, 2, const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct F8Operands {
+  const void *x, *w;
+  long long M, K, N, ldx, ldw;
+};
+
+template <typename C>
+static cudaError_t f8_launch(const F8Operands& o, F8Args a, int splits, cudaStream_t st) {
+  constexpr int TILE_M = C::PAIR ? 256 : 128;
+  a.m_tiles = (a.M + TILE_M - 1) / TILE_M;
+  a.n_tiles = (a.N + C::BN - 1) / C::BN;
+  a.splits = splits;
+  CUtensorMap tx, tw, to;
+  memset(&to, 0, sizeof(to));
+  if (!f8_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.x, o.K, o.M, o.ldx, 128, 128) ||
+      !f8_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.w, o.K, o.N, o.ldw, 128, C::B_ROWS))
+    return cudaErrorInvalidValue;
+  const int es = a.out_dtype == IC_DTYPE_F32 ? 4 : 2;
+  a.tma_store = a.ldo * es % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  if (a.tma_store &&
+      !f8_tmap(&to, a.out_dtype == IC_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, a.out,
+               a.N, a.M, a.ldo * es, 128 / es, 32))
+    return cudaErrorInvalidValue;
+  auto kern = gemm_fp8_kernel<C>;
+  cudaError_t e = set_smem_once(kern, C::SMEM);
+  if (e != cudaSuccess) return e;
+  const long long tiles = (long long)a.m_tiles * a.n_tiles;
+  const int cluster = C::PAIR ? 2 : splits;
+  long long grid = tiles * cluster;
+  if (splits == 1) {
+    const long long most = num_sms() / cluster * cluster;
+    if (grid > most) grid = most;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+cudaError_t launch_gemm_fp8(const F8Operands& o, const F8Args& a, cudaStream_t st) {
+  const long long sms = num_sms();
+  const long long pairs = ((o.M + 255) / 256) * ((o.N + 255) / 256);
+  if (pairs >= sms / 2) return f8_launch<F8Cfg<256, true>>(o, a, 1, st);
+  const long long tiles = ((o.M + 127) / 128) * ((o.N + 127) / 128);
+  int splits = 1;
+  while (splits < 8 && tiles * (splits + 1) <= sms && a.kb >= 2 * (splits + 1)) ++splits;
+  return f8_launch<F8Cfg<128, false>>(o, a, splits, st);
+}
+
+}  // namespace ic

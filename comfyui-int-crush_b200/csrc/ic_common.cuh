@@ -24,8 +24,8 @@
 #endif
 
 // Device-side error word (IC_DEV_ERR_* codes of include/intcrush_b200.h), one
-// per translation unit (intcrush_b200.cu, attention_b200.cu);
-// ic_read_device_error reads both.
+// per translation unit (intcrush_b200.cu, attention_b200.cu, fp8_b200.cu);
+// ic_read_device_error reads all.
 static __device__ int g_ic_dev_error = 0;
 
 namespace ic {
@@ -34,6 +34,7 @@ namespace ic {
 int set_error(int code, const char* fmt, ...);      // records ic_last_error's text, returns code
 void clear_error();
 cudaError_t attention_device_error(int* word, bool store);   // that unit's word: load or store (abi_attention.cu)
+cudaError_t fp8_device_error(int* word, bool store);         // and that unit's (abi_fp8.cu)
 int num_sms();
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

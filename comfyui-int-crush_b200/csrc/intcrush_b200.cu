@@ -1,5 +1,5 @@
-// Translation unit of the quantised-linear kernels (the other one is
-// attention_b200.cu): its kernels share one device error word and are linked
+// Translation unit of the quantised-linear kernels (the others are
+// attention_b200.cu and fp8_b200.cu): its kernels share one device error word and are linked
 // without relocatable device code.
 #include "ic_common.cuh"
 #include "prep.cu"
