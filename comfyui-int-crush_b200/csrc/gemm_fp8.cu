@@ -97,21 +97,6 @@ __host__ __device__ constexpr uint32_t idesc_f8(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-__device__ __forceinline__ uint64_t f8_two(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ float2 f8_untwo(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t f8_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t v;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-  return v;
-}
 __device__ __forceinline__ void f8_tie(uint32_t (&r)[32]) {
   asm volatile(""
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -203,9 +188,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const int m_off = PAIR ? (int)rank * 128 : 0;
   const uint32_t ring = smem_u32(smem);
 
-  // registers: 384 threads x 168 = 128 x 72 + 256 x 216
+  // registers: 384 threads x 168 = 128 x 40 + 256 x 232
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ------------------------------------------------------------ producer
       if (lane == 0) {
@@ -217,7 +202,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           const int row = mt * TILE_M + m_off, col = nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const uint32_t s = it % NST, ph = (it / NST) & 1u;
-            if (!mbar_wait_cl(empty + s, ph ^ 1u, abort_flag)) { ok = false; break; }
+            if (!mbar_wait(empty + s, ph ^ 1u, abort_flag)) { ok = false; break; }
             uint8_t* st = smem + s * C::STAGE;
             if constexpr (PAIR) {
               // both halves count on the leader's barrier
@@ -236,7 +221,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         // (a pair's count on the leader's barriers: the leader waits for both)
         if (leader) {
           volatile int never = 0;
-          for (uint32_t u = it > NST ? it - NST : 0; u < it; ++u) mbar_wait_cl(full + u % NST, (u / NST) & 1u, &never);
+          for (uint32_t u = it > NST ? it - NST : 0; u < it; ++u) mbar_wait(full + u % NST, (u / NST) & 1u, &never);
         }
       }
     } else if (warp == 1 && leader) {
@@ -248,8 +233,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t s = it % NST, b = it & 1u;
-          ok = mbar_wait_cl(acc_empty + b, ((it >> 1) & 1u) ^ 1u, abort_flag) &&
-               mbar_wait_cl(full + s, (it / NST) & 1u, abort_flag);
+          // operands first: the buffer is what comes last
+          ok = mbar_wait(full + s, (it / NST) & 1u, abort_flag) &&
+               mbar_wait(acc_empty + b, ((it >> 1) & 1u) ^ 1u, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -280,7 +266,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
   } else {
     // ------------------------------------------------------------------ sums
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int e = warp - 4, q = e & 3, half = e >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * CPT);
     uint8_t* stg = smem + C::OFF_STG + e * 4096;
@@ -290,45 +276,57 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       int mt, nt;
       f8_tile(a, t, mt, nt);
       const int m0 = mt * TILE_M + m_off + 32 * q, n0 = nt * BN + half * CPT;
-      const int m = m0 + lane;
-      const float* sa = a.s_a + (long long)min(m, a.M - 1) * a.sa_row;
+      const float* sa = a.s_a + (long long)min(m0 + lane, a.M - 1) * a.sa_row;
       const float* sw = a.s_w + (long long)(min(n0, a.N - 1) / 128) * a.sw_row;
-      uint64_t acc[CPT / 2];
+      float acc[CPT];
 #pragma unroll
-      for (int j = 0; j < CPT / 2; ++j) acc[j] = 0ull;
-      float fa = __ldg(sa + kb0 * a.sa_block), fw = __ldg(sw + kb0 * a.sw_block);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t b = it & 1u;
-        const float f = fa * fw;
-        if (kb + 1 < kb1) {   // the next block's factors, while this one is waited for
-          fa = __ldg(sa + (kb + 1) * a.sa_block);
-          fw = __ldg(sw + (kb + 1) * a.sw_block);
-        }
-        ok = mbar_wait_cl(acc_full + b, (it >> 1) & 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t f2 = f8_two(f, f);
-        uint32_t r[2][32];
-        tmem_ld32(lanes + b * BN, r[0]);
+      for (int j = 0; j < CPT; ++j) acc[j] = 0.f;
+      // factors of two blocks ahead
+      float fa[2], fw[2];
 #pragma unroll
-        for (int c = 0; c < CPT / 32; ++c) {
-          tmem_wait_ld();
-          f8_tie(r[c & 1]);
-          if (c + 1 < CPT / 32) {
-            tmem_ld32(lanes + b * BN + 32 * (c + 1), r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty + b), 0u));
-              else mbar_arrive(acc_empty + b);
+      for (int i = 0; i < 2; ++i) {
+        const int kb = min(kb0 + i, kb1 - 1);
+        fa[i] = __ldg(sa + kb * a.sa_block);
+        fw[i] = __ldg(sw + kb * a.sw_block);
+      }
+      for (int kb2 = kb0; ok && kb2 < kb1; kb2 += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (kb2 + i < kb1) {
+            const uint32_t b = it & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full + b, (it >> 1) & 1u, abort_flag));
+            if (!ok) break;
+            ++it;
+            tc_fence_after();
+            const float f = fa[i] * fw[i];
+            const int ahead = min(kb2 + i + 2, kb1 - 1);
+            fa[i] = __ldg(sa + ahead * a.sa_block);
+            fw[i] = __ldg(sw + ahead * a.sw_block);
+            const uint32_t src = lanes + b * BN;
+            uint32_t r[2][32];
+            tmem_ld32(src, r[0]);
+            tmem_ld32(src + 32, r[1]);
+#pragma unroll
+            for (int c = 0; c < CPT / 32; c += 2) {
+              tmem_wait_ld();
+              f8_tie(r[0]);
+              f8_tie(r[1]);
+              if (c + 2 >= CPT / 32) {   // all is read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                  if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty + b), 0u));
+                  else mbar_arrive(acc_empty + b);
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(r[0][j]), f, acc[32 * c + j]);
+              if (c + 2 < CPT / 32) tmem_ld32(src + 32 * (c + 2), r[0]);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) acc[32 * c + 32 + j] = fmaf(__uint_as_float(r[1][j]), f, acc[32 * c + 32 + j]);
+              if (c + 2 < CPT / 32) tmem_ld32(src + 32 * (c + 3), r[1]);
             }
           }
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[16 * c + j] = f8_fma2(f8_two(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), f2,
-                                      acc[16 * c + j]);
         }
       }
       if (!ok) break;
@@ -339,20 +337,16 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         const int r = 32 * q + lane;
 #pragma unroll
         for (int c = 0; c < CPT / 4; ++c) {
-          const float2 u = f8_untwo(acc[2 * c]), v = f8_untwo(acc[2 * c + 1]);
           const int chunk = (half * (CPT / 4) + c) ^ lane;
-          *reinterpret_cast<float4*>(smem + r * (BN * 4) + chunk * 16) = make_float4(u.x, u.y, v.x, v.y);
+          *reinterpret_cast<float4*>(smem + r * (BN * 4) + chunk * 16) =
+              make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
         }
         break;   // one tile a cluster
       }
       if (a.bias) {
 #pragma unroll
-        for (int j = 0; j < CPT / 2; ++j) {
-          const int n = n0 + 2 * j;
-          const float2 v = f8_untwo(acc[j]);
-          acc[j] = f8_two(v.x + (n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f),
-                          v.y + (n + 1 < a.N ? load_any(a.bias, a.bias_dtype, n + 1) : 0.f));
-        }
+        for (int j = 0; j < CPT; ++j)
+          if (n0 + j < a.N) acc[j] += load_any(a.bias, a.bias_dtype, n0 + j);
       }
       // 4 KB of output at a time: 32 rows of 128 bytes, 128-byte-swizzled
       const int per = a.out_dtype == IC_DTYPE_F32 ? 32 : 64;   // columns
@@ -367,8 +361,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (per == 32) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float2 u = f8_untwo(acc[16 * c + 2 * j]), v = f8_untwo(acc[16 * c + 2 * j + 1]);
-            *reinterpret_cast<float4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(u.x, u.y, v.x, v.y);
+            const float* v = acc + 32 * c + 4 * j;
+            *reinterpret_cast<float4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
           }
         } else {
 #pragma unroll
@@ -376,7 +370,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float2 u = f8_untwo(acc[16 * c + 4 * j + i]);
+              const float2 u = make_float2(acc[32 * c + 8 * j + 2 * i], acc[32 * c + 8 * j + 2 * i + 1]);
               if (a.out_dtype == IC_DTYPE_F16) {
                 const __half2 h = __floats2half2_rn(u.x, u.y);
                 w[i] = *reinterpret_cast<const uint32_t*>(&h);
