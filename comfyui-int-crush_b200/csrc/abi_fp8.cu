@@ -133,11 +133,11 @@ int ic_group_norm(const void* x, int dtype, int64_t B, int64_t L, int64_t C, int
   a.vec = C % 8 == 0 && f8_at16(x) && x_row % 8 == 0 && (x_batch % 8 == 0 || B == 1) &&
           (!y || (f8_at16(y) && y_row % 8 == 0 && (y_batch % 8 == 0 || B == 1)));
   a.gamma = gamma; a.gamma_dtype = gamma_dtype; a.beta = beta; a.beta_dtype = beta_dtype;
-  a.eps = eps; a.act = activation;
+  a.eps = eps;
   a.y = y; a.y_batch = y_batch; a.y_row = y_row;
   a.q = static_cast<uint8_t*>(q); a.ldq = ldq; a.s = s; a.s_row = s_row; a.s_block = s_block; a.width = (int)width;
   a.part = reinterpret_cast<float2*>(workspace);
-  return f8_launched(launch_group_norm(a, p, dtype, (cudaStream_t)stream), "ic_group_norm launch");
+  return f8_launched(launch_group_norm(a, p, dtype, activation, (cudaStream_t)stream), "ic_group_norm launch");
 }
 
 }  // extern "C"

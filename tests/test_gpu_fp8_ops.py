@@ -570,3 +570,11 @@ def test_torch_library_ops():
     torch.library.opcheck(ops.quantize_fp8_block.default, (x[0], 128), **fake)
     torch.library.opcheck(ops.fused_groupnorm_quantize.default, (x, 4, None, None, 1e-5, 0), **fake)
     torch.library.opcheck(ops.group_norm.default, (x, 4, None, None, 1e-5, 0), test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("C,groups,L", [(8192, 8192, 700), (8192, 1, 300), (4096, 4096, 37), (8190, 2730, 64)])
+def test_group_norm_widest(C, groups, L):
+    g = gen(35)
+    x = normal(g, 1, L, C, dtype=torch.bfloat16)
+    check_norm(rt.group_norm(x, groups), x, groups, None, None, 1e-5, 0)
+    check_norm_quantized(*rt.fused_groupnorm_quantize(x, groups), x, groups, None, None, 1e-5, 0)
