@@ -128,7 +128,7 @@ int ic_group_norm(const void* x, int dtype, int64_t B, int64_t L, int64_t C, int
                      (long long)workspace_elems);
   GnArgs a;
   memset(&a, 0, sizeof(a));
-  a.x = x; a.B = (int)B; a.L = L; a.C = (int)C; a.G = (int)groups; a.Cg = (int)(C / groups);
+  a.x = x; a.L = L; a.C = (int)C; a.G = (int)groups; a.Cg = (int)(C / groups);
   a.x_batch = x_batch; a.x_row = x_row;
   a.vec = C % 8 == 0 && f8_at16(x) && x_row % 8 == 0 && (x_batch % 8 == 0 || B == 1) &&
           (!y || (f8_at16(y) && y_row % 8 == 0 && (y_batch % 8 == 0 || B == 1)));
@@ -137,7 +137,7 @@ int ic_group_norm(const void* x, int dtype, int64_t B, int64_t L, int64_t C, int
   a.y = y; a.y_batch = y_batch; a.y_row = y_row;
   a.q = static_cast<uint8_t*>(q); a.ldq = ldq; a.s = s; a.s_row = s_row; a.s_block = s_block; a.width = (int)width;
   a.part = reinterpret_cast<float2*>(workspace);
-  return f8_launched(launch_group_norm(a, p, dtype, activation, (cudaStream_t)stream), "ic_group_norm launch");
+  return f8_launched(launch_group_norm(a, p, B, dtype, activation, (cudaStream_t)stream), "ic_group_norm launch");
 }
 
 }  // extern "C"

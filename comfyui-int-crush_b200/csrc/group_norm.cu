@@ -12,11 +12,14 @@
 //   mean = sum n_i mean_i / N,  M2 = sum M2_i + n_i (mean_i - mean)^2
 // in a fixed order.
 //
-// Two forms.  A sample that fits the shared memory of a cluster of up to 8 CTAs
-// is read once: each CTA keeps its rows in shared memory while the statistics
-// cross the cluster.  Others take two launches: statistics of runs of rows, a
-// cluster's worth each, into a workspace, then the norm; the second walks
-// the rows from the end, where L2 still holds them.
+// Two forms.  What fits the shared memory of clusters of up to 16 CTAs is read
+// once: each CTA keeps its rows in shared memory while the statistics cross the
+// cluster; a sample's groups are dealt to several clusters (`parts`), as they have
+// nothing to do with one another, until the SMs are busy.  Others take two
+// launches: statistics of runs of rows, a cluster's worth each, into a
+// workspace, then the norm; the second walks the rows from the end, where L2 still
+// holds them.
+#include <atomic>
 #include <type_traits>
 
 namespace ic {
@@ -26,7 +29,8 @@ constexpr int kGnThreads = 512;
 struct GnArgs {
   const void* x;
   long long L, x_batch, x_row;
-  int B, C, G, Cg;
+  int C, G, Cg;             // channels and groups of a part
+  int parts;                // of a sample
   int vec;                  // rows of x and y can be taken 16 bytes at a time
   int cols;                 // threads of a row: C / 8, rounded up to 16 for e4m3 blocks
   int slots;                // rows that a CTA holds side by side
@@ -43,10 +47,29 @@ struct GnArgs {
   int width;                // C rounded up to 16
   long long chunk;          // rows of a CTA
   int cluster, cluster_shift;   // CTAs of a cluster, a power of two
-  int runs;                 // clusters of a sample
+  int runs;                 // clusters of a part
   long long span;           // rows of a cluster
-  float2* part;             // [B, runs, G] mean, M2
+  float2* part;             // [B, parts, G, runs] mean, M2
 };
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t gn_two(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void gn_untwo(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t gn_add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t gn_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t gn_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
 constexpr int kGnRing = 8;   // rows of a thread on their way to shared memory
 
@@ -68,51 +91,68 @@ __device__ __forceinline__ void gn_commit() { asm volatile("cp.async.commit_grou
 template <int LEFT>
 __device__ __forceinline__ void gn_arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-template <typename T> struct Gn8 {
-  uint4 w;
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// 8 values of 16 bits as four pairs in fp32, and back
+template <typename T>
+__device__ __forceinline__ void gn_unpack(const uint4& w, uint64_t (&v)[4]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (std::is_same<T, __half>::value) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      }
-    }
-  }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[8], int n, bool vec) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    if (vec) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  for (int i = 0; i < 4; ++i) {
+    if (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      v[i] = gn_two(f.x, f.y);
     } else {
-      unsigned short* o = reinterpret_cast<unsigned short*>(p);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) o[i] = (unsigned short)(u[i / 2] >> (16 * (i & 1)));
+      v[i] = gn_two(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
     }
   }
-};
+}
+template <typename T>
+__device__ __forceinline__ void gn_store(T* p, const float (&v)[8], int n, bool vec) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  if (vec) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+    unsigned short* o = reinterpret_cast<unsigned short*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) o[i] = (unsigned short)(u[i / 2] >> (16 * (i & 1)));
+  }
+}
 
+// y1 / (1 + 2^-z1) and y2 / (1 + 2^-z2) with one reciprocal for both (these
+// functions run at a quarter of the other instructions' rate and bound the norm of a
+// tensor in L2).  -z is cut off at 62, so that the product of both denominators
+// stays in range: the quotients there are below 2^-62 |y| either way.
+__device__ __forceinline__ void gn_sigmoid2(float& y1, float& y2, float z1, float z2) {
+  float e1, e2, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(-z1, 62.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e2) : "f"(fminf(-z2, 62.f)));
+  const float a = 1.f + e1, b = 1.f + e2;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  y1 *= r * b;
+  y2 *= r * a;
+}
 template <int ACT>
-__device__ __forceinline__ float gn_act(float y) {
-  if (ACT == 1) return __fdividef(y, 1.f + __expf(-y));
-  if (ACT == 2) return 0.5f * y * (1.f + erff(y * 0.70710678f));
-  if (ACT == 3) return 0.5f * y * (1.f + tanhf(0.79788456f * (y + 0.044715f * y * y * y)));
-  return y;
+__device__ __forceinline__ void gn_act2(float& y1, float& y2) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  if (ACT == 1) gn_sigmoid2(y1, y2, y1 * kLog2e, y2 * kLog2e);
+  if (ACT == 2) {
+    y1 = 0.5f * y1 * (1.f + erff(y1 * 0.7071067811865476f));
+    y2 = 0.5f * y2 * (1.f + erff(y2 * 0.7071067811865476f));
+  }
+  if (ACT == 3) {   // 1 + tanh(u) = 2 / (1 + exp(-2 u))
+    constexpr float k = 2.f * 0.7978845608028654f * kLog2e;
+    gn_sigmoid2(y1, y2, k * fmaf(0.044715f * y1, y1 * y1, y1), k * fmaf(0.044715f * y2, y2 * y2, y2));
+  }
 }
 
 // Two equal counts n of a channel each, joined.
@@ -129,89 +169,72 @@ __device__ __forceinline__ float gn_warp_sum(float v) {
   return v;
 }
 
-// A thread's factors: mean, rstd gamma and beta of its 8 channels.
+// A thread's factors: -mean, rstd gamma and beta of its 8 channels, in pairs.
+// (a x + b with b = beta - mean a would save an addition, but a constant group,
+// whose rstd is large, would show b's rounding.)
 struct GnFactors {
-  float mean[8], a[8], b[8];
-  // channels [c0, c0 + 8) of a vector of C
-  static __device__ __forceinline__ void vector(float (&v)[8], const void* p, int dtype, int c0, int C, float none) {
+  uint64_t m[4], a[4], b[4];
+  // channels [c0, c0 + 8) of a vector, n of them there
+  static __device__ __forceinline__ void vector(float (&v)[8], const void* p, int dtype, int c0, int n, float none) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = none;
     if (!p) return;
-    if (dtype != IC_DTYPE_F32 && c0 + 8 <= C && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-      const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p) + c0);
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p) + c0;
+    if (dtype != IC_DTYPE_F32 && n >= 8 && (reinterpret_cast<uintptr_t>(h) & 15) == 0) {
+      const uint4 w = *reinterpret_cast<const uint4*>(h);
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t h = i & 1 ? u[i / 2] >> 16 : u[i / 2] & 0xffffu;
-        v[i] = dtype == IC_DTYPE_F16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16);
+        const uint32_t e = i & 1 ? u[i / 2] >> 16 : u[i / 2] & 0xffffu;
+        v[i] = dtype == IC_DTYPE_F16 ? __half2float(__ushort_as_half((unsigned short)e)) : __uint_as_float(e << 16);
       }
       return;
     }
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 8; ++i)
-      if (c0 + i < C) v[i] = load_any(p, dtype, c0 + i);
+      if (i < n) {
+        const float e = load_any(p, dtype, c0 + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = i == j ? e : v[j];
+      }
   }
-  __device__ __forceinline__ void load(const GnArgs& g, const float2* fin, int c0) {
-    vector(a, g.gamma, g.gamma_dtype, c0, g.C, 1.f);
-    vector(b, g.beta, g.beta_dtype, c0, g.C, 0.f);
-    int group = c0 / g.Cg, left = (group + 1) * g.Cg - c0;   // channels up to the next group
+  // column v of the part that begins at channel c
+  __device__ __forceinline__ void load(const GnArgs& g, const float2* fin, int c, int v) {
+    float m_[8], a_[8], b_[8];
+    vector(a_, g.gamma, g.gamma_dtype, c + 8 * v, g.C - 8 * v, 1.f);
+    vector(b_, g.beta, g.beta_dtype, c + 8 * v, g.C - 8 * v, 0.f);
+    int group = 8 * v / g.Cg, left = (group + 1) * g.Cg - 8 * v;   // channels up to the next group
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 f = fin[min(group, g.G - 1)];
-      mean[i] = f.x;
-      a[i] *= f.y;
+      m_[i] = -f.x;
+      a_[i] *= f.y;
       if (--left == 0) {
         ++group;
         left = g.Cg;
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = gn_two(m_[2 * i], m_[2 * i + 1]);
+      a[i] = gn_two(a_[2 * i], a_[2 * i + 1]);
+      b[i] = gn_two(b_[2 * i], b_[2 * i + 1]);
+    }
   }
 };
 
-// Norm, activation and output of 8 channels of row l of sample b.  For e4m3 the
-// 16 threads of a block of 128 channels (half a warp) come here together.
-template <typename T, bool F8, int ACT>
-__device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, const Gn8<T>& in, long long b, long long l,
-                                          int v) {
-  float y[8];
-  in.get(y);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = gn_act<ACT>(fmaf(y[i] - f.mean[i], f.a[i], f.b[i]));
-  if constexpr (!F8) {
-    Gn8<T>::store(reinterpret_cast<T*>(g.y) + b * g.y_batch + l * g.y_row + 8 * v, y, g.C - 8 * v, g.vec != 0);
-  } else {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (8 * v + i >= g.C) y[i] = 0.f;
-      top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-    }
-    const uint32_t half = 0xffffu << (threadIdx.x & 16);
-#pragma unroll
-    for (int d = 8; d; d >>= 1) top = max(top, __shfl_xor_sync(half, top, d));
-    const F8Scale sc = f8_scale(__uint_as_float(top));
-    const long long row = b * g.L + l;
-    uint2 o;
-    if (sc.s <= 3.4e38f) {
-      o = make_uint2(f8_four(y[0], y[1], y[2], y[3], sc), f8_four(y[4], y[5], y[6], y[7], sc));
-    } else {
-      o = make_uint2(f8_four_div(y[0], y[1], y[2], y[3], sc.s), f8_four_div(y[4], y[5], y[6], y[7], sc.s));
-    }
-    if (8 * v < g.width) *reinterpret_cast<uint2*>(g.q + row * g.ldq + 8 * v) = o;
-    if ((v & 15) == 0 && 8 * v < g.C) g.s[row * g.s_row + (v >> 4) * g.s_block] = sc.s;
-  }
-}
-
-// Where a CTA works: its sample, rows and threads.
+// Where a CTA works: its sample, part, rows and threads.
 struct GnPlace {
-  int b, run, rank, s0, v0, wide;
+  int b, part, run, rank, s0, v0, wide;
   long long lo, hi;
   bool busy;
   __device__ __forceinline__ GnPlace(const GnArgs& g) {
     const int t = threadIdx.x, unit = (int)blockIdx.x >> g.cluster_shift;
     rank = (int)blockIdx.x - (unit << g.cluster_shift);
-    b = unit / g.runs;
-    run = unit - b * g.runs;
+    const int bp = unit / g.runs;
+    run = unit - bp * g.runs;
+    b = bp / g.parts;
+    part = bp - b * g.parts;
     lo = min(g.L, run * g.span + rank * g.chunk);
     hi = min(g.L, lo + g.chunk);
     wide = g.slots == 1 ? kGnThreads : g.cols;   // columns a pass
@@ -221,7 +244,72 @@ struct GnPlace {
   }
 };
 
-// Statistics of a cluster's rows (`KEEP`: the whole sample, kept in shared memory
+// Where a thread's column v of row l goes, and rows further on.
+template <typename T, bool F8> struct GnOut {
+  T* y;
+  uint8_t* q;
+  float* s;
+  long long step, s_step;
+  __device__ __forceinline__ GnOut(const GnArgs& g, const GnPlace& at, long long l, int v, int rows) {
+    const int c = at.part * g.C + 8 * v;
+    if (F8) {
+      const long long row = at.b * g.L + l;
+      q = g.q + row * g.ldq + c;
+      s = g.s + row * g.s_row + (c >> 7) * g.s_block;
+      step = rows * g.ldq;
+      s_step = rows * g.s_row;
+    } else {
+      y = reinterpret_cast<T*>(g.y) + at.b * g.y_batch + l * g.y_row + c;
+      step = rows * g.y_row;
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (F8) {
+      q += step;
+      s += s_step;
+    } else {
+      y += step;
+    }
+  }
+};
+
+// Norm, activation and output of 8 channels of a row.  For e4m3 the 16 threads of
+// a block of 128 channels (half a warp) come here together.
+template <typename T, bool F8, int ACT>
+__device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, const uint4& in, const GnOut<T, F8>& o, int v) {
+  uint64_t x[4];
+  gn_unpack<T>(in, x);
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    gn_untwo(gn_fma2(gn_add2(x[i], f.m[i]), f.a[i], f.b[i]), y[2 * i], y[2 * i + 1]);
+    gn_act2<ACT>(y[2 * i], y[2 * i + 1]);
+  }
+  const int n = g.C - 8 * v;
+  if constexpr (!F8) {
+    gn_store(o.y, y, n, g.vec != 0);
+  } else {
+    // The scale to a unit or two and the quotients as products: y is no nearer to
+    // its exact value.  (An infinity's reciprocal is 0, a NaN's NaN.)
+    if (n < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = i < n ? y[i] : 0.f;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+    const float amax = __uint_as_float(__reduce_max_sync(0xffffu << (threadIdx.x & 16), top));
+    const float s = (amax < kF8AmaxMin ? kF8AmaxMin : amax) * (1.f / kF8Max);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const uint2 w = make_uint2(f8_pair(y[0] * inv, y[1] * inv) | f8_pair(y[2] * inv, y[3] * inv) << 16,
+                               f8_pair(y[4] * inv, y[5] * inv) | f8_pair(y[6] * inv, y[7] * inv) << 16);
+    if (8 * v < g.width) *reinterpret_cast<uint2*>(o.q) = w;
+    if ((v & 15) == 0 && n > 0) *o.s = s;
+  }
+}
+
+// Statistics of a cluster's rows (`KEEP`: all rows of a part, kept in shared memory
 // and normalised; else into the workspace).
 template <typename T, bool KEEP, bool F8, int ACT>
 __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(const GnArgs g) {
@@ -229,7 +317,7 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
   // the norm's launch may begin, its CTAs wait for the statistics themselves
   if (!KEEP) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int shift = 31 - __clz(g.sub), per = 8 >> shift;          // entries of a thread
-  const int width = g.cols * per;                                 // of a slot
+  const int width = (g.cols * per) | 1;                           // of a slot, odd: slots lie in other banks
   float2* sums = reinterpret_cast<float2*>(smem);                 // [slots, width]
   float2* own = sums + g.slots * width;                           // [G] this CTA's
   float2* fin = own + g.G;                                        // [G] mean, rstd (KEEP)
@@ -242,7 +330,7 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
   const int least = rows / g.slots, rest = rows - least * g.slots;
   const int mine = at.busy ? least + (at.s0 < rest) : 0;          // this thread's rows
   const long long step = g.slots * g.x_row;
-  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + (at.lo + at.s0) * g.x_row;
+  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + at.part * g.C + (at.lo + at.s0) * g.x_row;
   const int keep_step = KEEP ? g.slots * g.cols : kGnThreads;
   if (at.busy) {
     for (int v = at.v0; v < g.cols; v += at.wide) {
@@ -251,7 +339,8 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
       const T* p = x + 8 * v;
       uint4* keep = KEEP ? kept + at.s0 * g.cols + v : kept + t;
       if (KEEP) {   // all of them at once
-        for (int r = 0; r < mine; ++r, p += step) gn_fetch(keep + r * keep_step, p, n, g.vec != 0);
+        uint4* to = keep;
+        for (int r = 0; r < mine; ++r, p += step, to += keep_step) gn_fetch(to, p, n, g.vec != 0);
         gn_commit();
         gn_arrived<0>();
       } else {
@@ -262,43 +351,55 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
           gn_commit();
         }
       }
-      float x0[8], s[8], q[8];
+      uint64_t x0[4], s2[4], q2[4];   // -x0
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x0[i] = s[i] = q[i] = 0.f;
-      for (int r0 = 0; r0 < mine; r0 += kGnRing) {
+      for (int i = 0; i < 4; ++i) x0[i] = s2[i] = q2[i] = 0;
+      const auto add = [&](const uint4& in, bool first) {
+        uint64_t f[4];
+        gn_unpack<T>(in, f);
+        if (first) {
 #pragma unroll
-        for (int k = 0; k < kGnRing; ++k) {
-          const int r = r0 + k;
-          if (r < mine) {
-            if (!KEEP) gn_arrived<kGnRing - 1>();
-            Gn8<T> in;
-            in.w = keep[(KEEP ? r : k) * keep_step];
-            float f[8];
-            in.get(f);
-            if (r == 0) {
+          for (int j = 0; j < 4; ++j) x0[j] = gn_neg2(f[j]);
+        }
 #pragma unroll
-              for (int j = 0; j < 8; ++j) x0[j] = f[j];
-            }
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t d = gn_add2(f[j], x0[j]);
+          s2[j] = gn_add2(s2[j], d);
+          q2[j] = gn_fma2(d, d, q2[j]);
+        }
+      };
+      if (KEEP) {
+        const uint4* from = keep;
+#pragma unroll 2
+        for (int r = 0; r < mine; ++r, from += keep_step) add(*from, r == 0);
+      } else {
+        for (int r0 = 0; r0 < mine; r0 += kGnRing) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float d = f[j] - x0[j];
-              s[j] += d;
-              q[j] = fmaf(d, d, q[j]);
-            }
-            if (!KEEP) {
-              if (r + kGnRing < mine) gn_fetch(keep + k * keep_step, p, n, g.vec != 0);
+          for (int k = 0; k < kGnRing; ++k) {
+            if (r0 + k < mine) {
+              gn_arrived<kGnRing - 1>();
+              add(keep[k * keep_step], r0 + k == 0);
+              if (r0 + k + kGnRing < mine) gn_fetch(keep + k * keep_step, p, n, g.vec != 0);
               p += step;
               gn_commit();
             }
           }
         }
+        gn_arrived<0>();
       }
-      if (!KEEP) gn_arrived<0>();
-      const float count = (float)mine, inv = mine ? 1.f / count : 0.f;
+      const float count = (float)mine, inv = mine ? __frcp_rn(count) : 0.f;
+      float s[8], q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        q[i] = fmaxf(0.f, q[i] - s[i] * s[i] * inv);
-        s[i] = fmaf(s[i], inv, x0[i]);
+      for (int i = 0; i < 4; ++i) {
+        float z[2];
+        gn_untwo(s2[i], s[2 * i], s[2 * i + 1]);
+        gn_untwo(q2[i], q[2 * i], q[2 * i + 1]);
+        gn_untwo(x0[i], z[0], z[1]);
+#pragma unroll
+        for (int j = 2 * i; j < 2 * i + 2; ++j) {
+          q[j] = fmaxf(0.f, q[j] - s[j] * s[j] * inv);
+          s[j] = fmaf(s[j], inv, -z[j & 1]);
+        }
       }
       // channels of one group, two by two
 #pragma unroll
@@ -318,36 +419,37 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
   // from 0 only its own rounding is lost.
   const int entries = g.Cg >> shift;   // of a group and slot
   const int dq = 32 / entries, dr = 32 - dq * entries, sl0 = lane / entries, e0 = lane - sl0 * entries;
+  const float inv_total = __frcp_rn((float)max(rows, 1) * (float)g.Cg);
   for (int i = warp; i < g.G; i += kGnThreads / 32) {
     const float2* from = sums + i * entries;
-    const float ref = from[0].x, total = (float)max(rows, 1) * (float)g.Cg;
-    float sum = 0.f, dev = 0.f;
-    for (int sl = sl0, e = e0; sl < g.slots;) {
-      sum = fmaf((float)((least + (sl < rest)) << shift), from[sl * width + e].x - ref, sum);
-      sl += dq;
-      e += dr;
-      if (e >= entries) { e -= entries; ++sl; }
+    const float ref = from[0].x;
+    float mean = ref, dev = 0.f;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      float sum = 0.f;
+      for (int sl = sl0, e = e0; sl < g.slots;) {
+        const float2 v = from[sl * width + e];
+        const float count = (float)((least + (sl < rest)) << shift), d = v.x - mean;
+        sum += pass ? fmaf(count * d, d, v.y) : count * d;
+        sl += dq;
+        e += dr;
+        if (e >= entries) { e -= entries; ++sl; }
+      }
+      sum = gn_warp_sum(sum);
+      if (pass) dev = sum;
+      else mean = fmaf(sum, inv_total, ref);
     }
-    const float mean = ref + gn_warp_sum(sum) / total;
-    for (int sl = sl0, e = e0; sl < g.slots;) {
-      const float2 v = from[sl * width + e];
-      const float d = v.x - mean;
-      dev += fmaf((float)((least + (sl < rest)) << shift) * d, d, v.y);
-      sl += dq;
-      e += dr;
-      if (e >= entries) { e -= entries; ++sl; }
-    }
-    dev = gn_warp_sum(dev);
     if (lane == 0) own[i] = make_float2(mean, dev);
   }
-  cluster_sync_all();
+  if (g.cluster > 1) cluster_sync_all();
+  else __syncthreads();
   // the cluster's CTAs, a lane each
   if (KEEP || at.rank == 0) {
     const long long run_lo = at.run * g.span;
     const int p = lane & (g.cluster - 1);
     const long long first = min(g.L, run_lo + p * g.chunk);
     const float count = (float)(min(g.L, first + g.chunk) - first) * (float)g.Cg;
-    const float total = (float)(min(g.L, run_lo + g.span) - run_lo) * (float)g.Cg;
+    const float inv = __frcp_rn((float)(min(g.L, run_lo + g.span) - run_lo) * (float)g.Cg);
     for (int i0 = 0; i0 < g.G; i0 += kGnThreads >> g.cluster_shift) {
       const int i = i0 + (t >> g.cluster_shift);
       float2 v;
@@ -356,12 +458,12 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
       const float ref = __shfl_sync(0xffffffffu, v.x, lane & ~(g.cluster - 1));
       float sum = count * (v.x - ref);
       for (int d = 1; d < g.cluster; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const float mean = ref + sum / total, dev = v.x - mean;
+      const float mean = fmaf(sum, inv, ref), dev = v.x - mean;
       float m2 = fmaf(count * dev, dev, v.y);
       for (int d = 1; d < g.cluster; d *= 2) m2 += __shfl_xor_sync(0xffffffffu, m2, d);
       if (p == 0 && i < g.G) {
-        if (KEEP) fin[i] = make_float2(mean, 1.f / sqrtf(m2 / total + g.eps));
-        else g.part[((long long)at.b * g.runs + at.run) * g.G + i] = make_float2(mean, m2);
+        if (KEEP) fin[i] = make_float2(mean, rsqrtf(fmaf(m2, inv, g.eps)));
+        else g.part[((long long)(at.b * g.parts + at.part) * g.G + i) * g.runs + at.run] = make_float2(mean, m2);
       }
     }
   }
@@ -369,20 +471,19 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
     __syncthreads();
     if (at.busy) {
       for (int v = at.v0; v < g.cols; v += at.wide) {
-        GnFactors f;
-        f.load(g, fin, 8 * v);
         const bool in_row = 8 * v < g.C;
         if (!F8 && !in_row) continue;
-        const uint4* keep = kept + at.s0 * g.cols + v;
-        for (int r = 0; r < mine; ++r) {
-          Gn8<T> in;
-          in.w = in_row ? keep[r * keep_step] : make_uint4(0, 0, 0, 0);
-          gn_finish<T, F8, ACT>(g, f, in, at.b, at.lo + at.s0 + r * g.slots, v);
-        }
+        GnFactors f;
+        f.load(g, fin, at.part * g.C, v);
+        const uint4* from = kept + at.s0 * g.cols + v;
+        GnOut<T, F8> o(g, at, at.lo + at.s0, v, g.slots);
+#pragma unroll 2
+        for (int r = 0; r < mine; ++r, from += keep_step, o.next())
+          gn_finish<T, F8, ACT>(g, f, in_row ? *from : make_uint4(0, 0, 0, 0), o, v);
       }
     }
   }
-  cluster_sync_all();   // nobody leaves while another CTA may read its shared memory
+  if (g.cluster > 1) cluster_sync_all();   // nobody leaves while another CTA may read its shared memory
 }
 
 // The norm from the workspace's statistics, with the first launch's shares of the
@@ -397,7 +498,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_apply_kernel(const GnArgs g)
   const int rows = (int)(at.hi - at.lo) - at.s0;
   const int mine = at.busy && rows > 0 ? (rows + g.slots - 1) / g.slots : 0;   // this thread's rows
   const long long step = g.slots * g.x_row;
-  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + (at.hi - 1 - at.s0) * g.x_row;
+  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + at.part * g.C + (at.hi - 1 - at.s0) * g.x_row;
   const auto begin = [&](int v) {
     const T* p = x + 8 * v;
 #pragma unroll
@@ -408,51 +509,46 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_apply_kernel(const GnArgs g)
     }
   };
   if (at.v0 < g.cols) begin(at.v0);   // x is no output of the first launch
+  // two runs a lane at most (kGnRuns)
+  float count[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int j = lane + 32 * k;
+    const long long a = min(g.L, j * g.span);
+    count[k] = j < g.runs ? (float)(min(g.L, a + g.span) - a) * (float)g.Cg : 0.f;
+  }
+  const int j0 = min(lane, g.runs - 1), j1 = min(lane + 32, g.runs - 1);
+  const float inv = __frcp_rn((float)g.L * (float)g.Cg);
+  const float2* part = g.part + (long long)(at.b * g.parts + at.part) * g.runs * g.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float total = (float)g.L * (float)g.Cg;
-  const float2* part = g.part + (long long)at.b * g.runs * g.G;
+#pragma unroll 2
   for (int i = warp; i < g.G; i += kGnThreads / 32) {
-    // two runs a lane at most (kGnRuns)
-    float2 v[2];
-    float count[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int j = lane + 32 * k;
-      const long long a = min(g.L, j * g.span);
-      v[k] = __ldcg(part + min(j, g.runs - 1) * g.G + i);
-      count[k] = j < g.runs ? (float)(min(g.L, a + g.span) - a) * (float)g.Cg : 0.f;
-    }
-    const float ref = __shfl_sync(0xffffffffu, v[0].x, 0);
-    const float mean = ref + gn_warp_sum(fmaf(count[0], v[0].x - ref, count[1] * (v[1].x - ref))) / total;
-    float dev = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float d = v[k].x - mean;
-      dev += count[k] > 0.f ? fmaf(count[k] * d, d, v[k].y) : 0.f;
-    }
+    const float2 v0 = __ldcg(part + (long long)i * g.runs + j0), v1 = __ldcg(part + (long long)i * g.runs + j1);
+    const float ref = __shfl_sync(0xffffffffu, v0.x, 0);
+    const float mean = fmaf(gn_warp_sum(fmaf(count[0], v0.x - ref, count[1] * (v1.x - ref))), inv, ref);
+    const float d0 = v0.x - mean, d1 = v1.x - mean;
+    float dev = count[0] > 0.f ? fmaf(count[0] * d0, d0, v0.y) : 0.f;
+    if (count[1] > 0.f) dev += fmaf(count[1] * d1, d1, v1.y);
     dev = gn_warp_sum(dev);
-    if (lane == 0) fin[i] = make_float2(mean, 1.f / sqrtf(dev / total + g.eps));
+    if (lane == 0) fin[i] = make_float2(mean, rsqrtf(fmaf(dev, inv, g.eps)));
   }
   __syncthreads();
   for (int v = at.v0; v < g.cols; v += at.wide) {
     if (v != at.v0) begin(v);
     GnFactors f;
-    f.load(g, fin, 8 * v);
+    f.load(g, fin, at.part * g.C, v);
     const int n = g.C - 8 * v;
     const T* p = x + 8 * v - kGnRing * step;
-    long long l = at.hi - 1 - at.s0;
+    GnOut<T, F8> o(g, at, at.hi - 1 - at.s0, v, -g.slots);
     for (int r0 = 0; r0 < mine; r0 += kGnRing) {
-#pragma unroll 2
+#pragma unroll 4
       for (int k = 0; k < kGnRing; ++k) {
-        const int r = r0 + k;
-        if (r < mine) {
+        if (r0 + k < mine) {
           gn_arrived<kGnRing - 1>();
-          Gn8<T> in;
-          in.w = n > 0 ? ring[k * kGnThreads] : make_uint4(0, 0, 0, 0);
-          if (F8 || n > 0) gn_finish<T, F8, ACT>(g, f, in, at.b, l, v);
-          if (r + kGnRing < mine && n > 0) gn_fetch(ring + k * kGnThreads, p, n, g.vec != 0);
+          if (F8 || n > 0) gn_finish<T, F8, ACT>(g, f, n > 0 ? ring[k * kGnThreads] : make_uint4(0, 0, 0, 0), o, v);
+          if (r0 + k + kGnRing < mine && n > 0) gn_fetch(ring + k * kGnThreads, p, n, g.vec != 0);
           p -= step;
-          l -= g.slots;
+          o.next();
           gn_commit();
         }
       }
@@ -463,54 +559,82 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_apply_kernel(const GnArgs g)
 
 // ============================================================== host side
 
-constexpr int kGnCluster = 8;
-constexpr int kGnRuns = 64;        // of a sample, what the norm's warps join
 constexpr int kGnShared = 200 * 1024;
+constexpr int kGnRuns = 64;        // of a part, what the norm's warps join
 
 struct GnPlan {
-  int cols, slots, sub, cluster, runs;
-  long long chunk;           // rows of a CTA of the first launch
+  int parts, cols, slots, sub, cluster, runs;
+  long long chunk;           // rows of a CTA
   bool keep;                 // one launch
   int shared;
   long long floats;          // workspace
 };
 
-static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f8) {
-  GnPlan p;
+// parts: C and G are one part's
+static void gn_threads(GnPlan& p, long long C, long long G, bool f8) {
   p.cols = (int)((C + 7) / 8);
   if (f8) p.cols = (p.cols + 15) / 16 * 16;
   p.slots = p.cols <= kGnThreads ? kGnThreads / p.cols : 1;
   p.sub = 1;
   while (p.sub < 8 && C / G % (2 * p.sub) == 0) p.sub *= 2;
-  const long long sums = (long long)p.slots * p.cols * (8 / p.sub);
-  const long long head = ((sums + 2 * G) * 8 + 15) / 16 * 16;
-  const long long row = (long long)p.cols * 16;
-  // one launch: as few CTAs as keep a sample, but several where it has rows for them
-  const long long most = (kGnShared - head) / row;   // rows of a CTA
-  p.keep = most > 0 && L <= most * kGnCluster;
-  if (p.keep) {
-    p.cluster = 1;
-    while (p.cluster < kGnCluster && (p.cluster * most < L || L >= 2 * p.cluster * (long long)p.slots)) p.cluster *= 2;
-    p.chunk = (L + p.cluster - 1) / p.cluster;
-    p.runs = 1;
-    p.shared = (int)(head + p.chunk * row);
-    p.floats = 0;
-    return p;
+}
+
+static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f8) {
+  GnPlan p;
+  const long long sms = num_sms();
+  // One launch where what a cluster keeps fits.  A part is whole groups and whole
+  // 16-byte columns (128 channels for e4m3).  The cheapest of the ways to deal it
+  // out, in clocks as they were measured: a wave costs 6000, a cluster's exchange
+  // 3500, a value 0.3 (an SM), rows in pieces below 64 bytes half as much again.
+  double best = 0;
+  for (long long parts = 1; parts <= G; ++parts) {
+    if (G % parts || (parts > 1 && C / parts % (f8 ? 128 : 8))) continue;
+    GnPlan t;
+    t.parts = (int)parts;
+    gn_threads(t, C / parts, G / parts, f8);
+    const long long sums = (long long)t.slots * ((t.cols * (8 / t.sub)) | 1);
+    const long long head = ((sums + 2 * (G / parts)) * 8 + 15) / 16 * 16;
+    const long long most = (kGnShared - head) / ((long long)t.cols * 16);   // rows of a CTA
+    if (most <= 0) continue;
+    for (t.cluster = 1; t.cluster <= 16; t.cluster *= 2) {
+      t.chunk = (L + t.cluster - 1) / t.cluster;
+      if (t.chunk > most) continue;
+      const long long held = sms / t.cluster * t.cluster;   // CTAs at a time: clusters do not fill every SM
+      const double waves = (double)((B * parts * t.cluster + held - 1) / held);
+      double cost = waves * (6000 + 0.3 * t.chunk * t.cols * 8 * (C / parts < 32 ? 1.5 : 1.0)) + (t.cluster > 1 ? 3500 : 0) +
+                    (t.cluster == 16 ? 1000 : 0);
+      if (best && cost >= best) continue;
+      best = cost;
+      t.runs = 1;
+      t.keep = true;
+      t.shared = (int)(head + t.chunk * t.cols * 16);
+      t.floats = 0;
+      p = t;
+    }
   }
-  const long long ctas = 2LL * num_sms();
-  p.cluster = kGnCluster;
-  long long runs = ctas / kGnCluster / B;
-  const long long useful = (L + 4LL * p.slots * kGnCluster - 1) / (4LL * p.slots * kGnCluster);   // 4 rows a thread at least
+  // Two launches: 20000, and 0.5 a value at all SMs' rate.
+  if (best && best <= 20000 + 0.5 * (double)B * (double)L * (double)C / sms) return p;
+  p.parts = 1;
+  p.keep = false;
+  gn_threads(p, C, G, f8);
+  p.cluster = 8;
+  long long runs = 2 * sms / p.cluster / B;
+  const long long useful = (L + 4LL * p.slots * p.cluster - 1) / (4LL * p.slots * p.cluster);   // 4 rows a thread at least
   runs = runs < useful ? runs : useful;
   p.runs = (int)(runs < 1 ? 1 : runs > kGnRuns ? kGnRuns : runs);
   p.chunk = ((L + p.runs - 1) / p.runs + p.cluster - 1) / p.cluster;
+  const long long sums = (long long)p.slots * ((p.cols * (8 / p.sub)) | 1);
   p.shared = (int)(((sums + G) * 8 + 15) / 16 * 16) + kGnRing * kGnThreads * 16;
   p.floats = 2 * B * p.runs * G;
   return p;
 }
 
 template <typename T, bool F8, int ACT>
-static cudaError_t gn_launch(GnArgs a, const GnPlan& p, cudaStream_t st) {
+static cudaError_t gn_launch(GnArgs a, const GnPlan& p, long long B, cudaStream_t st) {
+  a.parts = p.parts;
+  a.C /= p.parts;
+  a.G /= p.parts;
+  if (p.parts > 1) a.width = a.C;
   a.cols = p.cols;
   a.slots = p.slots;
   a.sub = p.sub;
@@ -524,7 +648,7 @@ static cudaError_t gn_launch(GnArgs a, const GnPlan& p, cudaStream_t st) {
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = p.cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)((long long)a.B * p.runs * p.cluster));
+  cfg.gridDim = dim3((unsigned)(B * p.parts * p.runs * p.cluster));
   cfg.blockDim = dim3(kGnThreads);
   cfg.dynamicSmemBytes = p.shared;
   cfg.stream = st;
@@ -533,6 +657,15 @@ static cudaError_t gn_launch(GnArgs a, const GnPlan& p, cudaStream_t st) {
   if (p.keep) {
     auto kern = gn_stats_kernel<T, true, F8, ACT>;
     cudaError_t e = set_smem_once(kern, 227 * 1024);
+    if (e == cudaSuccess && p.cluster > 8) {
+      static std::atomic<unsigned long long> devices{0};   // that the attribute is set on
+      int dev = 0;
+      cudaGetDevice(&dev);
+      if (!(devices.load() >> (dev & 63) & 1)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) devices.fetch_or(1ull << (dev & 63));
+      }
+    }
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kern, a);
   }
   auto stats = gn_stats_kernel<T, false, false, 0>;
@@ -548,16 +681,16 @@ static cudaError_t gn_launch(GnArgs a, const GnPlan& p, cudaStream_t st) {
 }
 
 template <typename T, bool F8>
-static cudaError_t gn_launch_act(const GnArgs& a, const GnPlan& p, int act, cudaStream_t st) {
-  if (act == 0) return gn_launch<T, F8, 0>(a, p, st);
-  if (act == 1) return gn_launch<T, F8, 1>(a, p, st);
-  if (act == 2) return gn_launch<T, F8, 2>(a, p, st);
-  return gn_launch<T, F8, 3>(a, p, st);
+static cudaError_t gn_launch_act(const GnArgs& a, const GnPlan& p, long long B, int act, cudaStream_t st) {
+  if (act == 0) return gn_launch<T, F8, 0>(a, p, B, st);
+  if (act == 1) return gn_launch<T, F8, 1>(a, p, B, st);
+  if (act == 2) return gn_launch<T, F8, 2>(a, p, B, st);
+  return gn_launch<T, F8, 3>(a, p, B, st);
 }
 
-cudaError_t launch_group_norm(const GnArgs& a, const GnPlan& p, int dtype, int act, cudaStream_t st) {
-  if (dtype == IC_DTYPE_F16) return a.q ? gn_launch_act<__half, true>(a, p, act, st) : gn_launch_act<__half, false>(a, p, act, st);
-  return a.q ? gn_launch_act<__nv_bfloat16, true>(a, p, act, st) : gn_launch_act<__nv_bfloat16, false>(a, p, act, st);
+cudaError_t launch_group_norm(const GnArgs& a, const GnPlan& p, int64_t B, int dtype, int act, cudaStream_t st) {
+  if (dtype == IC_DTYPE_F16) return a.q ? gn_launch_act<__half, true>(a, p, B, act, st) : gn_launch_act<__half, false>(a, p, B, act, st);
+  return a.q ? gn_launch_act<__nv_bfloat16, true>(a, p, B, act, st) : gn_launch_act<__nv_bfloat16, false>(a, p, B, act, st);
 }
 
 }  // namespace ic
