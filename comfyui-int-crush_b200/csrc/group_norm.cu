@@ -17,8 +17,8 @@
 // cluster; a sample's groups are dealt to several clusters (`parts`), as they have
 // nothing to do with one another, until the SMs are busy.  Others take two
 // launches: statistics of runs of rows, a cluster's worth each, into a
-// workspace, then the norm; the second walks the rows from the end, where L2 still
-// holds them.
+// workspace, then the norm; the second takes the rows from the end, which the first
+// read last, so that L2 still holds some of them.
 #include <atomic>
 #include <type_traits>
 
@@ -45,11 +45,14 @@ struct GnArgs {
   float* s;
   long long s_row, s_block;
   int width;                // C rounded up to 16
-  long long chunk;          // rows of a CTA
   int cluster, cluster_shift;   // CTAs of a cluster, a power of two
   int runs;                 // clusters of a part
-  long long span;           // rows of a cluster
+  // tiles of `tile` rows (all of a CTA's, or kGnRing a thread), dealt to a part's
+  // CTAs in turn: `deal` each, the first `more` CTAs one more; the last tile lacks
+  // `lack` rows
+  int tile, deal, more, lack;
   float2* part;             // [B, parts, G, runs] mean, M2
+  int* tiles;               // [B, parts] tiles that CTAs of the second launch have taken
 };
 
 // two fp32 operations in one instruction
@@ -72,6 +75,7 @@ __device__ __forceinline__ uint64_t gn_fma2(uint64_t a, uint64_t b, uint64_t c) 
 __device__ __forceinline__ uint64_t gn_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
 constexpr int kGnRing = 8;   // rows of a thread on their way to shared memory
+constexpr int kGnLaneRuns = 5;   // runs of a part that a lane of the second launch joins, at most
 
 // 8 channels of a row to shared memory: one asynchronous 16-byte copy, or n
 // values one by one.  Committed by gn_commit; only the thread that fetched reads them.
@@ -223,10 +227,21 @@ struct GnFactors {
   }
 };
 
-// Where a CTA works: its sample, part, rows and threads.
+// rows of CTA c of a part
+__device__ __forceinline__ int gn_rows(const GnArgs& g, int c) {
+  const int last = g.more ? g.more - 1 : (g.runs << g.cluster_shift) - 1;
+  return (g.deal + (c < g.more)) * g.tile - (c == last ? g.lack : 0);
+}
+// of a cluster
+__device__ __forceinline__ int gn_run_rows(const GnArgs& g, int run) {
+  int n = 0;
+  for (int i = 0; i < g.cluster; ++i) n += gn_rows(g, (run << g.cluster_shift) + i);
+  return n;
+}
+
+// Where a CTA works: its sample, part and threads; c: its number in the part.
 struct GnPlace {
-  int b, part, run, rank, s0, v0, wide;
-  long long lo, hi;
+  int b, part, run, rank, c, s0, v0, wide;
   bool busy;
   __device__ __forceinline__ GnPlace(const GnArgs& g) {
     const int t = threadIdx.x, unit = (int)blockIdx.x >> g.cluster_shift;
@@ -235,8 +250,7 @@ struct GnPlace {
     run = unit - bp * g.runs;
     b = bp / g.parts;
     part = bp - b * g.parts;
-    lo = min(g.L, run * g.span + rank * g.chunk);
-    hi = min(g.L, lo + g.chunk);
+    c = (run << g.cluster_shift) + rank;
     wide = g.slots == 1 ? kGnThreads : g.cols;   // columns a pass
     s0 = g.slots == 1 ? 0 : t / g.cols;
     v0 = t - s0 * g.cols;
@@ -244,7 +258,7 @@ struct GnPlace {
   }
 };
 
-// Where a thread's column v of row l goes, and rows further on.
+// Where a thread's column v of row l goes, and `rows` rows further on.
 template <typename T, bool F8> struct GnOut {
   T* y;
   uint8_t* q;
@@ -325,13 +339,16 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
   uint4* kept = reinterpret_cast<uint4*>(smem + (((g.slots * width + (KEEP ? 2 : 1) * g.G) * 8 + 15) & ~15));
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const GnPlace at(g);
-  const int rows = (int)(at.hi - at.lo);
+  const int rows = gn_rows(g, at.c);
   // slot i takes rows i, i + slots, ...: more of them the first `rest` slots
   const int least = rows / g.slots, rest = rows - least * g.slots;
   const int mine = at.busy ? least + (at.s0 < rest) : 0;          // this thread's rows
   const long long step = g.slots * g.x_row;
-  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + at.part * g.C + (at.lo + at.s0) * g.x_row;
+  const long long jump = (long long)((g.runs << g.cluster_shift) - 1) * g.tile * g.x_row;   // to the next tile
+  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + at.part * g.C + ((long long)at.c * g.tile + at.s0) * g.x_row;
   const int keep_step = KEEP ? g.slots * g.cols : kGnThreads;
+  // the second launch's CTAs begin with a tile each
+  if (!KEEP && at.run == 0 && at.rank == 0 && t == 0) g.tiles[at.b * g.parts + at.part] = g.runs << g.cluster_shift;
   if (at.busy) {
     for (int v = at.v0; v < g.cols; v += at.wide) {
       const int n = g.C - 8 * v;   // <= 0: a column that only fills up a block
@@ -350,6 +367,7 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
           p += step;
           gn_commit();
         }
+        p += jump;
       }
       uint64_t x0[4], s2[4], q2[4];   // -x0
 #pragma unroll
@@ -384,6 +402,7 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
               gn_commit();
             }
           }
+          p += jump;
         }
         gn_arrived<0>();
       }
@@ -445,11 +464,9 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
   else __syncthreads();
   // the cluster's CTAs, a lane each
   if (KEEP || at.rank == 0) {
-    const long long run_lo = at.run * g.span;
     const int p = lane & (g.cluster - 1);
-    const long long first = min(g.L, run_lo + p * g.chunk);
-    const float count = (float)(min(g.L, first + g.chunk) - first) * (float)g.Cg;
-    const float inv = __frcp_rn((float)(min(g.L, run_lo + g.span) - run_lo) * (float)g.Cg);
+    const float count = (float)gn_rows(g, (at.run << g.cluster_shift) + p) * (float)g.Cg;
+    const float inv = __frcp_rn((float)gn_run_rows(g, at.run) * (float)g.Cg);
     for (int i0 = 0; i0 < g.G; i0 += kGnThreads >> g.cluster_shift) {
       const int i = i0 + (t >> g.cluster_shift);
       float2 v;
@@ -476,7 +493,7 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
         GnFactors f;
         f.load(g, fin, at.part * g.C, v);
         const uint4* from = kept + at.s0 * g.cols + v;
-        GnOut<T, F8> o(g, at, at.lo + at.s0, v, g.slots);
+        GnOut<T, F8> o(g, at, (long long)at.c * g.tile + at.s0, v, g.slots);
 #pragma unroll 2
         for (int r = 0; r < mine; ++r, from += keep_step, o.next())
           gn_finish<T, F8, ACT>(g, f, in_row ? *from : make_uint4(0, 0, 0, 0), o, v);
@@ -486,85 +503,110 @@ __global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(cons
   if (g.cluster > 1) cluster_sync_all();   // nobody leaves while another CTA may read its shared memory
 }
 
-// The norm from the workspace's statistics, with the first launch's shares of the
-// rows, each from its end.
+// The norm from the workspace's statistics, tile by tile from the last row on.  A
+// CTA takes the next tile when it has time: those far from the memory that they
+// read need a third longer for the same rows.  (Every value goes by its own row
+// and the statistics, whoever computes it.)
 template <typename T, bool F8, int ACT>
 __global__ void __launch_bounds__(kGnThreads, 2) gn_apply_kernel(const GnArgs g) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;          // [kGnRing, threads]
   float2* fin = reinterpret_cast<float2*>(smem + kGnRing * kGnThreads * 16);   // [G] mean, rstd
+  int* box = reinterpret_cast<int*>(fin + g.G);                        // [2] a tile taken
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const GnPlace at(g);
-  const int rows = (int)(at.hi - at.lo) - at.s0;
-  const int mine = at.busy && rows > 0 ? (rows + g.slots - 1) / g.slots : 0;   // this thread's rows
+  const int tiles = (int)((g.L + g.tile - 1) / g.tile);
   const long long step = g.slots * g.x_row;
-  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + at.part * g.C + (at.hi - 1 - at.s0) * g.x_row;
-  const auto begin = [&](int v) {
-    const T* p = x + 8 * v;
+  const T* x = reinterpret_cast<const T*>(g.x) + at.b * g.x_batch + at.part * g.C;
+  // this thread's rows of the i-th tile from the end, and how many
+  const auto first = [&](int i) { return (long long)(tiles - 1 - i) * g.tile + at.s0; };
+  const auto number = [&](int i) {
+    const long long left = g.L - first(i);
+    return !at.busy || i >= tiles || left <= 0 ? 0 : left >= g.tile ? kGnRing : (int)min((long long)kGnRing, (left + g.slots - 1) / g.slots);
+  };
+  int cur = at.c, have = number(cur);
+  {   // x is no output of the first launch
+    const T* p = x + (have ? first(cur) * g.x_row : 0) + 8 * at.v0;
 #pragma unroll
     for (int r = 0; r < kGnRing; ++r) {
-      if (r < mine && 8 * v < g.C) gn_fetch(ring + r * kGnThreads, p, g.C - 8 * v, g.vec != 0);
-      p -= step;
+      if (r < have && 8 * at.v0 < g.C) gn_fetch(ring + r * kGnThreads, p + r * step, g.C - 8 * at.v0, g.vec != 0);
       gn_commit();
     }
-  };
-  if (at.v0 < g.cols) begin(at.v0);   // x is no output of the first launch
-  // two runs a lane at most (kGnRuns)
-  float count[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int j = lane + 32 * k;
-    const long long a = min(g.L, j * g.span);
-    count[k] = j < g.runs ? (float)(min(g.L, a + g.span) - a) * (float)g.Cg : 0.f;
   }
-  const int j0 = min(lane, g.runs - 1), j1 = min(lane + 32, g.runs - 1);
+  float count[kGnLaneRuns];
+#pragma unroll
+  for (int k = 0; k < kGnLaneRuns; ++k) {
+    const int j = lane + 32 * k;
+    count[k] = j < g.runs ? (float)gn_run_rows(g, j) * (float)g.Cg : 0.f;
+  }
   const float inv = __frcp_rn((float)g.L * (float)g.Cg);
   const float2* part = g.part + (long long)(at.b * g.parts + at.part) * g.runs * g.G;
+  int* taken = g.tiles + at.b * g.parts + at.part;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (threadIdx.x == 0) box[0] = atomicAdd(taken, 1);
 #pragma unroll 2
   for (int i = warp; i < g.G; i += kGnThreads / 32) {
-    const float2 v0 = __ldcg(part + (long long)i * g.runs + j0), v1 = __ldcg(part + (long long)i * g.runs + j1);
-    const float ref = __shfl_sync(0xffffffffu, v0.x, 0);
-    const float mean = fmaf(gn_warp_sum(fmaf(count[0], v0.x - ref, count[1] * (v1.x - ref))), inv, ref);
-    const float d0 = v0.x - mean, d1 = v1.x - mean;
-    float dev = count[0] > 0.f ? fmaf(count[0] * d0, d0, v0.y) : 0.f;
-    if (count[1] > 0.f) dev += fmaf(count[1] * d1, d1, v1.y);
+    float2 w[kGnLaneRuns];
+#pragma unroll
+    for (int k = 0; k < kGnLaneRuns; ++k) w[k] = __ldcg(part + (long long)i * g.runs + min(lane + 32 * k, g.runs - 1));
+    const float ref = __shfl_sync(0xffffffffu, w[0].x, 0);
+    float sum = 0.f, dev = 0.f;
+#pragma unroll
+    for (int k = 0; k < kGnLaneRuns; ++k) sum = fmaf(count[k], w[k].x - ref, sum);
+    const float mean = fmaf(gn_warp_sum(sum), inv, ref);
+#pragma unroll
+    for (int k = 0; k < kGnLaneRuns; ++k) {
+      const float d = w[k].x - mean;
+      if (count[k] > 0.f) dev += fmaf(count[k] * d, d, w[k].y);
+    }
     dev = gn_warp_sum(dev);
     if (lane == 0) fin[i] = make_float2(mean, rsqrtf(fmaf(dev, inv, g.eps)));
   }
   __syncthreads();
-  for (int v = at.v0; v < g.cols; v += at.wide) {
-    if (v != at.v0) begin(v);
-    GnFactors f;
-    f.load(g, fin, at.part * g.C, v);
-    const int n = g.C - 8 * v;
-    const T* p = x + 8 * v - kGnRing * step;
-    GnOut<T, F8> o(g, at, at.hi - 1 - at.s0, v, -g.slots);
-    for (int r0 = 0; r0 < mine; r0 += kGnRing) {
+  GnFactors f;
+  f.load(g, fin, at.part * g.C, min(at.v0, g.cols - 1));
+  int next = box[0];
+  for (int it = 1; cur < tiles; ++it) {
+    int got = 0;
+    if (threadIdx.x == 0) got = atomicAdd(taken, 1);
+    const int then = number(next);
+    for (int v = at.v0; v < g.cols; v += at.wide) {
+      if (at.wide < g.cols) f.load(g, fin, at.part * g.C, v);
+      // what the ring is filled up with: this tile's next columns, or the next tile
+      const bool more = v + at.wide < g.cols;
+      const int vn = more ? v + at.wide : at.v0, hn = 8 * vn < g.C ? (more ? have : then) : 0;
+      const T* p = x + (hn ? first(more ? cur : next) * g.x_row : 0) + 8 * vn;
+      const int n = g.C - 8 * v;
+      GnOut<T, F8> o(g, at, first(cur), v, g.slots);
 #pragma unroll 4
-      for (int k = 0; k < kGnRing; ++k) {
-        if (r0 + k < mine) {
+      for (int r = 0; r < kGnRing; ++r) {
+        if (r < have) {
           gn_arrived<kGnRing - 1>();
-          if (F8 || n > 0) gn_finish<T, F8, ACT>(g, f, n > 0 ? ring[k * kGnThreads] : make_uint4(0, 0, 0, 0), o, v);
-          if (r0 + k + kGnRing < mine && n > 0) gn_fetch(ring + k * kGnThreads, p, n, g.vec != 0);
-          p -= step;
+          if (F8 || n > 0) gn_finish<T, F8, ACT>(g, f, n > 0 ? ring[r * kGnThreads] : make_uint4(0, 0, 0, 0), o, v);
           o.next();
-          gn_commit();
         }
+        if (r < hn) gn_fetch(ring + r * kGnThreads, p, g.C - 8 * vn, g.vec != 0);
+        p += step;
+        gn_commit();
       }
     }
-    gn_arrived<0>();
+    if (threadIdx.x == 0) box[it & 1] = got;
+    __syncthreads();
+    cur = next;
+    have = then;
+    next = box[it & 1];
   }
+  gn_arrived<0>();
 }
 
 // ============================================================== host side
 
 constexpr int kGnShared = 200 * 1024;
-constexpr int kGnRuns = 64;        // of a part, what the norm's warps join
+constexpr int kGnRuns = 32 * kGnLaneRuns;
 
 struct GnPlan {
   int parts, cols, slots, sub, cluster, runs;
-  long long chunk;           // rows of a CTA
+  long long tile;            // rows: all of a CTA's (one launch), or kGnRing a thread
   bool keep;                 // one launch
   int shared;
   long long floats;          // workspace
@@ -597,17 +639,18 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
     const long long most = (kGnShared - head) / ((long long)t.cols * 16);   // rows of a CTA
     if (most <= 0) continue;
     for (t.cluster = 1; t.cluster <= 16; t.cluster *= 2) {
-      t.chunk = (L + t.cluster - 1) / t.cluster;
-      if (t.chunk > most) continue;
-      const long long held = sms / t.cluster * t.cluster;   // CTAs at a time: clusters do not fill every SM
+      t.tile = (L + t.cluster - 1) / t.cluster;
+      if (t.tile > most) continue;
+      // CTAs at a time: clusters of four or more leave SMs of a processor group empty
+      const long long held = t.cluster < 4 ? sms : sms * 7 / 8 / t.cluster * t.cluster;
       const double waves = (double)((B * parts * t.cluster + held - 1) / held);
-      double cost = waves * (6000 + 0.3 * t.chunk * t.cols * 8 * (C / parts < 32 ? 1.5 : 1.0)) + (t.cluster > 1 ? 3500 : 0) +
+      double cost = waves * (6000 + 0.3 * t.tile * t.cols * 8 * (C / parts < 32 ? 1.5 : 1.0)) + (t.cluster > 1 ? 3500 : 0) +
                     (t.cluster == 16 ? 1000 : 0);
       if (best && cost >= best) continue;
       best = cost;
       t.runs = 1;
       t.keep = true;
-      t.shared = (int)(head + t.chunk * t.cols * 16);
+      t.shared = (int)(head + t.tile * t.cols * 16);
       t.floats = 0;
       p = t;
     }
@@ -617,15 +660,15 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
   p.parts = 1;
   p.keep = false;
   gn_threads(p, C, G, f8);
-  p.cluster = 8;
+  p.cluster = 2;   // (of four or eight, not as many as the SMs have room for fit at once: a few were left for a second wave)
   long long runs = 2 * sms / p.cluster / B;
-  const long long useful = (L + 4LL * p.slots * p.cluster - 1) / (4LL * p.slots * p.cluster);   // 4 rows a thread at least
+  p.tile = (long long)p.slots * kGnRing;
+  const long long useful = (L + p.tile * p.cluster - 1) / (p.tile * p.cluster);   // each has a tile
   runs = runs < useful ? runs : useful;
   p.runs = (int)(runs < 1 ? 1 : runs > kGnRuns ? kGnRuns : runs);
-  p.chunk = ((L + p.runs - 1) / p.runs + p.cluster - 1) / p.cluster;
   const long long sums = (long long)p.slots * ((p.cols * (8 / p.sub)) | 1);
   p.shared = (int)(((sums + G) * 8 + 15) / 16 * 16) + kGnRing * kGnThreads * 16;
-  p.floats = 2 * B * p.runs * G;
+  p.floats = 2 * B * p.runs * G + B;
   return p;
 }
 
@@ -641,8 +684,12 @@ static cudaError_t gn_launch(GnArgs a, const GnPlan& p, long long B, cudaStream_
   a.cluster = p.cluster;
   a.cluster_shift = 31 - __builtin_clz(p.cluster);
   a.runs = p.runs;
-  a.chunk = p.chunk;
-  a.span = p.chunk * p.cluster;
+  const long long tiles = (a.L + p.tile - 1) / p.tile, ctas = (long long)p.runs * p.cluster;
+  a.tile = (int)p.tile;
+  a.deal = (int)(tiles / ctas);
+  a.more = (int)(tiles % ctas);
+  a.lack = (int)(tiles * p.tile - a.L);
+  a.tiles = reinterpret_cast<int*>(a.part + B * p.runs * a.G);   // (two launches have one part)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -676,7 +723,7 @@ static cudaError_t gn_launch(GnArgs a, const GnPlan& p, long long B, cudaStream_
   if (e != cudaSuccess) return e;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.dynamicSmemBytes = kGnRing * kGnThreads * 16 + a.G * 8;
+  cfg.dynamicSmemBytes = kGnRing * kGnThreads * 16 + a.G * 8 + 8;
   return cudaLaunchKernelEx(&cfg, apply, a);
 }
 

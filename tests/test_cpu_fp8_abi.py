@@ -94,4 +94,4 @@ def test_workspaces():
     assert lib.ic_group_norm_workspace(2, 256, 1280, 32, 0) == 0      # kept in shared memory
     assert lib.ic_group_norm_workspace(2, 256, 1280, 32, 1) == 0
     n = lib.ic_group_norm_workspace(3, 1 << 20, 128, 32, 0)
-    assert n > 0 and n % (2 * 3 * 32) == 0
+    assert n > 3 and (n - 3) % (2 * 3 * 32) == 0     # statistics of runs of rows, tiles taken
