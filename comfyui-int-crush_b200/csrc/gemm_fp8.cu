@@ -2,8 +2,8 @@
 //   out[m, n] = sum_b s_a[m, b] s_w[n / 128, b] sum_{k in block b} x[m, k] w[n, k] + bias[n]
 // on tcgen05 (kind::f8f6f4).
 //
-// Persistent, one CTA per SM, 12 warps: warp 0 TMA producer, warp 1 MMA issuer,
-// warps 4-11 the sums.  Tokens are the MMA's rows (TMEM lanes), features its
+// Persistent, one CTA per SM, 12 warps: warps 0 and 2 TMA producers, warp 1 MMA
+// issuer, warps 4-11 the sums.  Tokens are the MMA's rows (TMEM lanes), features its
 // columns, so that a thread owns one token row and a block's factor
 // s_a * s_w is one number a thread: a weight block is 128 features wide and a
 // warp's columns lie in one.  The 128 products of a block are summed on the
@@ -30,13 +30,16 @@ struct F8Cfg {
   static constexpr int A_BYTES = BM * 128;
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;    // features that a CTA stages
   static constexpr int STAGE = A_BYTES + B_ROWS * 128;
-  static constexpr int NST = 6;
+  static constexpr int NST = BN == 256 ? 6 : PAIR ? 8 : 4;
+  static constexpr int NB = 512 / BN;                  // buffers of tensor memory
   static constexpr int CPT = BN / 2;                   // columns of a thread (8 warps: 4 x 32 rows, 2 halves)
   static constexpr int OFF_STG = NST * STAGE;          // output staging, 4 KB a warp
-  static constexpr int OFF_BAR = OFF_STG + 8 * 4096;
+  // a cluster's partial sums: of every CTA, the rows that this one adds up (they
+  // lie over the staging, which a cluster does not use)
+  static constexpr int PARTS = PAIR ? 0 : (128 + 8) * 128 * 4;
+  static constexpr int OFF_BAR = OFF_STG + (PARTS > 8 * 4096 ? PARTS : 8 * 4096);
   static constexpr int SMEM = OFF_BAR + 256;
   static constexpr int THREADS = 384;
-  static_assert(BM * BN * 4 <= NST * STAGE || PAIR, "a cluster's partial sums lie over the ring");
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -54,6 +57,7 @@ struct F8Args {
   int out_dtype;
   long long ldo;
   int tma_store;
+  int a_rows;                   // rows of x that a CTA stages: 128, or fewer where there are
 };
 
 __device__ __forceinline__ void mma_f8_on(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -105,11 +109,28 @@ __device__ __forceinline__ void f8_tie(uint32_t (&r)[32]) {
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31]));
 }
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// Whether a phase is complete, without waiting for it.
+__device__ __forceinline__ bool f8_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// A wait that was asked about beforehand: `early` is f8_test's answer, taken
+// while there was other work.  Asking takes 100 to 150 clocks beside the MMAs'
+// operand reads, also where the phase is long complete.
+__device__ __forceinline__ bool f8_wait(bool early, uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (__all_sync(0xffffffffu, early)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
 }
 
 // Tiles in groups of 8 row tiles, features slowest inside a group, so that the
@@ -128,14 +149,14 @@ template <typename C>
 __global__ void __launch_bounds__(C::THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                 const __grid_constant__ CUtensorMap tm_o, const F8Args a) {
-  constexpr int NST = C::NST, BN = C::BN, CPT = C::CPT;
+  constexpr int NST = C::NST, BN = C::BN, CPT = C::CPT, NB = C::NB;
   constexpr bool PAIR = C::PAIR;
   extern __shared__ __align__(1024) uint8_t smem[];   // no static shared memory: the declared alignment holds
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);   // [NST] TMA -> MMA
   uint64_t* empty = full + NST;                                       // [NST] MMA -> TMA
-  uint64_t* acc_full = empty + NST;                                   // [2] MMA -> sums
-  uint64_t* acc_empty = acc_full + 2;                                 // [2] sums -> MMA (8 warps of each CTA)
-  uint64_t* drain = acc_empty + 2;
+  uint64_t* acc_full = empty + NST;                                   // [NB] MMA -> sums
+  uint64_t* acc_empty = acc_full + NB;                                // [NB] sums -> MMA (8 warps of each CTA)
+  uint64_t* drain = acc_empty + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 2);
 
@@ -144,10 +165,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const bool leader = !PAIR || rank == 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NST; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, 1);   // (warp 0's; the bytes of both operands)
       mbar_init(empty + i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NB; ++i) {
       mbar_init(acc_full + i, 1);
       mbar_init(acc_empty + i, PAIR ? 16 : 8);
     }
@@ -157,10 +178,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   }
   if (warp == 1) {
     if constexpr (PAIR) {
-      tmem_alloc2(tmem_slot, 2 * BN);
+      tmem_alloc2(tmem_slot, NB * BN);
       tmem_relinquish2();
     } else {
-      tmem_alloc(tmem_slot, 2 * BN);
+      tmem_alloc(tmem_slot, NB * BN);
       tmem_relinquish();
     }
   }
@@ -171,7 +192,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();   // the peer's barriers are initialised
+  if (PAIR || a.splits > 1) cluster_sync_all();   // the others are there, their barriers initialised
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
@@ -184,42 +205,58 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     kb0 = (int)((long long)a.kb * rank / a.splits);
     kb1 = (int)((long long)a.kb * (rank + 1) / a.splits);
   }
+  // what a cluster's CTA adds up: rows [rank * share, ...) of the tile, a lane four
+  // columns from nc on, whose biases are here early
+  int mt0 = 0, share = 1, nc = 0;
+  float bias4[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t parts = smem_u32(smem) + C::OFF_STG;
+  if (!PAIR && a.splits > 1) {
+    int nt0;
+    f8_tile(a, first, mt0, nt0);
+    share = (min(128, a.M - mt0 * 128) + a.splits - 1) / a.splits;
+    nc = nt0 * BN + 4 * lane;
+    if (a.bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (nc + j < a.N) bias4[j] = load_any(a.bias, a.bias_dtype, nc + j);
+    }
+  }
   constexpr int TILE_M = PAIR ? 256 : 128;
   const int m_off = PAIR ? (int)rank * 128 : 0;
   const uint32_t ring = smem_u32(smem);
 
-  // registers: 384 threads x 168 = 128 x 40 + 256 x 232
+  // registers with 128 columns a thread: 384 threads x 168 = 128 x 40 + 256 x 232
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0) {
-      // ------------------------------------------------------------ producer
+    if constexpr (CPT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 || warp == 2) {
+      // ----------------------------------------- producers: 0 for x, 2 for w
       if (lane == 0) {
+        const bool of_x = warp == 0;
+        const CUtensorMap* tm = of_x ? &tm_x : &tm_w;
         uint32_t it = 0;
-        bool ok = true;
+        bool ok = true, early = false;
         for (int t = first; ok && t < tiles; t += step) {
           int mt, nt;
           f8_tile(a, t, mt, nt);
-          const int row = mt * TILE_M + m_off, col = nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
+          const int row = of_x ? mt * TILE_M + m_off : nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const uint32_t s = it % NST, ph = (it / NST) & 1u;
-            if (!mbar_wait(empty + s, ph ^ 1u, abort_flag)) { ok = false; break; }
-            uint8_t* st = smem + s * C::STAGE;
+            if (!early && !mbar_wait(empty + s, ph ^ 1u, abort_flag)) { ok = false; break; }
+            uint8_t* st = smem + s * C::STAGE + (of_x ? 0 : C::A_BYTES);
             if constexpr (PAIR) {
               // both halves count on the leader's barrier
-              if (leader) mbar_arrive_expect_tx(full + s, 2 * C::STAGE);
-              const uint32_t bar = mapa_u32(smem_u32(full + s), 0u);
-              tma_load_2d_pair(st, &tm_x, bar, kb * 128, row);
-              tma_load_2d_pair(st + C::A_BYTES, &tm_w, bar, kb * 128, col);
+              if (of_x && leader) mbar_arrive_expect_tx(full + s, 2 * (a.a_rows * 128 + C::B_ROWS * 128));
+              tma_load_2d_pair(st, tm, mapa_u32(smem_u32(full + s), 0u), kb * 128, row);
             } else {
-              mbar_arrive_expect_tx(full + s, C::STAGE);
-              tma_load_2d(st, &tm_x, full + s, kb * 128, row);
-              tma_load_2d(st + C::A_BYTES, &tm_w, full + s, kb * 128, col);
+              if (of_x) mbar_arrive_expect_tx(full + s, a.a_rows * 128 + C::B_ROWS * 128);
+              tma_load_2d(st, tm, full + s, kb * 128, row);
             }
+            early = f8_test(empty + (it + 1) % NST, (((it + 1) / NST) & 1u) ^ 1u);
           }
         }
         // every copy issued lands before the CTA may leave, whoever gave up
         // (a pair's count on the leader's barriers: the leader waits for both)
-        if (leader) {
+        if (leader && of_x) {
           volatile int never = 0;
           for (uint32_t u = it > NST ? it - NST : 0; u < it; ++u) mbar_wait(full + u % NST, (u / NST) & 1u, &never);
         }
@@ -229,14 +266,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       const uint32_t on = f8_elect();
       constexpr uint32_t idesc = idesc_f8(PAIR ? 256 : 128, BN);
       uint32_t it = 0;
-      bool ok = true;
+      bool ok = true, staged = false, freed = false;
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t s = it % NST, b = it & 1u;
+          const uint32_t s = it % NST, b = it % NB;
           // operands first: the buffer is what comes last
-          ok = mbar_wait(full + s, (it / NST) & 1u, abort_flag) &&
-               mbar_wait(acc_empty + b, ((it >> 1) & 1u) ^ 1u, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = f8_wait(staged, full + s, (it / NST) & 1u, abort_flag) &&
+               f8_wait(freed, acc_empty + b, ((it / NB) & 1u) ^ 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const uint64_t ad = smem_desc_sw128(ring + s * C::STAGE);
@@ -248,12 +284,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
             else mma_f8_on(on, d, ad + 2 * k, bd + 2 * k, idesc, k > 0);
           }
           if constexpr (PAIR) {
-            f8_commit2_on(on, empty + s);
             f8_commit2_on(on, acc_full + b);
+            f8_commit2_on(on, empty + s);
           } else {
-            f8_commit_on(on, empty + s);
             f8_commit_on(on, acc_full + b);
+            f8_commit_on(on, empty + s);
           }
+          staged = f8_test(full + (it + 1) % NST, ((it + 1) / NST) & 1u);
+          freed = f8_test(acc_empty + (it + 1) % NB, (((it + 1) / NB) & 1u) ^ 1u);
         }
       }
       // all MMAs are done before tensor memory is freed
@@ -266,87 +304,119 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
   } else {
     // ------------------------------------------------------------------ sums
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if constexpr (CPT == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int e = warp - 4, q = e & 3, half = e >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * CPT);
     uint8_t* stg = smem + C::OFF_STG + e * 4096;
     uint32_t it = 0;
-    bool ok = true;
+    bool ok = true, early = false;
     for (int t = first; ok && t < tiles; t += step) {
       int mt, nt;
       f8_tile(a, t, mt, nt);
       const int m0 = mt * TILE_M + m_off + 32 * q, n0 = nt * BN + half * CPT;
-      const float* sa = a.s_a + (long long)min(m0 + lane, a.M - 1) * a.sa_row;
-      const float* sw = a.s_w + (long long)(min(n0, a.N - 1) / 128) * a.sw_row;
+      const bool rows = m0 < a.M;   // or 32 rows that are not there
+      const float* sa = a.s_a + (long long)min(m0 + lane, a.M - 1) * a.sa_row + kb0 * a.sa_block;
+      const float* sw = a.s_w + (long long)(min(n0, a.N - 1) / 128) * a.sw_row + kb0 * a.sw_block;
       float acc[CPT];
 #pragma unroll
       for (int j = 0; j < CPT; ++j) acc[j] = 0.f;
+      // biases of columns n0 + lane + 32 i, here early
+      float bias[CPT / 32];
+      if (!(!PAIR && a.splits > 1)) {
+#pragma unroll
+        for (int i = 0; i < CPT / 32; ++i) {
+          const int n = n0 + 32 * i + lane;
+          bias[i] = a.bias && n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f;
+        }
+      }
       // factors of two blocks ahead
       float fa[2], fw[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int kb = min(kb0 + i, kb1 - 1);
-        fa[i] = __ldg(sa + kb * a.sa_block);
-        fw[i] = __ldg(sw + kb * a.sw_block);
-      }
+      fa[0] = __ldg(sa);
+      fw[0] = __ldg(sw);
+      sa += kb1 - kb0 > 1 ? a.sa_block : 0;
+      sw += kb1 - kb0 > 1 ? a.sw_block : 0;
+      fa[1] = __ldg(sa);
+      fw[1] = __ldg(sw);
+      // 32 columns at a time, the next ones on their way from tensor memory while
+      // these are added; a block's last 32 are added under the next block's first
+      uint32_t r[2][32];
+      constexpr int NC = CPT / 32;
       for (int kb2 = kb0; ok && kb2 < kb1; kb2 += 2) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (kb2 + i < kb1) {
-            const uint32_t b = it & 1u;
-            ok = __all_sync(0xffffffffu, mbar_wait(acc_full + b, (it >> 1) & 1u, abort_flag));
+            const uint32_t b = it % NB;
+            ok = f8_wait(early, acc_full + b, (it / NB) & 1u, abort_flag);
             if (!ok) break;
             ++it;
             tc_fence_after();
-            const float f = fa[i] * fw[i];
-            const int ahead = min(kb2 + i + 2, kb1 - 1);
-            fa[i] = __ldg(sa + ahead * a.sa_block);
-            fw[i] = __ldg(sw + ahead * a.sw_block);
-            const uint32_t src = lanes + b * BN;
-            uint32_t r[2][32];
-            tmem_ld32(src, r[0]);
-            tmem_ld32(src + 32, r[1]);
-#pragma unroll
-            for (int c = 0; c < CPT / 32; c += 2) {
-              tmem_wait_ld();
-              f8_tie(r[0]);
-              f8_tie(r[1]);
-              if (c + 2 >= CPT / 32) {   // all is read
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                  if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty + b), 0u));
-                  else mbar_arrive(acc_empty + b);
-                }
+            if (!rows) {
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty + b), 0u));
+                else mbar_arrive(acc_empty + b);
               }
-#pragma unroll
-              for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(r[0][j]), f, acc[32 * c + j]);
-              if (c + 2 < CPT / 32) tmem_ld32(src + 32 * (c + 2), r[0]);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) acc[32 * c + 32 + j] = fmaf(__uint_as_float(r[1][j]), f, acc[32 * c + 32 + j]);
-              if (c + 2 < CPT / 32) tmem_ld32(src + 32 * (c + 3), r[1]);
+              early = f8_test(acc_full + it % NB, (it / NB) & 1u);
+              continue;
             }
+            const float f = fa[i] * fw[i];
+            const uint32_t src = lanes + b * BN;
+            tmem_ld32(src, r[0]);
+            if (kb2 + i + 2 < kb1) {
+              sa += a.sa_block;
+              sw += a.sw_block;
+              fa[i] = __ldg(sa);
+              fw[i] = __ldg(sw);
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              tmem_wait_ld();
+              f8_tie(r[c & 1]);
+              if (c + 1 < NC) {
+                tmem_ld32(src + 32 * (c + 1), r[(c + 1) & 1]);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(r[c & 1][j]), f, acc[32 * c + j]);
+              }
+            }
+            // all is read: the buffer is the next MMAs'
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty + b), 0u));
+              else mbar_arrive(acc_empty + b);
+            }
+            early = f8_test(acc_full + it % NB, (it / NB) & 1u);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[CPT - 32 + j] = fmaf(__uint_as_float(r[1][j]), f, acc[CPT - 32 + j]);
           }
         }
       }
       if (!ok) break;
       if (!PAIR && a.splits > 1) {
-        // partial sums of this CTA's blocks, over the ring: every copy has
-        // landed and every MMA is done.  16-byte chunks of a row are XORed with
-        // the row's number, or all lanes would use the same banks.
-        const int r = 32 * q + lane;
+        // this CTA's partial sums to the CTAs that add them up.  16-byte chunks of a
+        // row are XORed with the row's number, or all lanes would use the same banks.
+        if (m0 + lane < a.M) {
+          const int r = 32 * q + lane, owner = r / share;
+          const uint32_t to = mapa_u32(parts + (rank * share + r - owner * share) * 512, owner);
 #pragma unroll
-        for (int c = 0; c < CPT / 4; ++c) {
-          const int chunk = (half * (CPT / 4) + c) ^ lane;
-          *reinterpret_cast<float4*>(smem + r * (BN * 4) + chunk * 16) =
-              make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+          for (int c = 0; c < CPT / 4; ++c)
+            st_cluster4(to + (((half * (CPT / 4) + c) ^ lane) << 4), acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
         }
         break;   // one tile a cluster
       }
       if (a.bias) {
+        // to all lanes through the staging, once the box before has left it
+        if (lane == 0) bulk_wait_read0();
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < CPT; ++j)
-          if (n0 + j < a.N) acc[j] += load_any(a.bias, a.bias_dtype, n0 + j);
+        for (int i = 0; i < CPT / 32; ++i) reinterpret_cast<float*>(stg)[32 * i + lane] = bias[i];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < CPT / 4; ++j) {
+          const float4 v = reinterpret_cast<const float4*>(stg)[j];
+          acc[4 * j] += v.x; acc[4 * j + 1] += v.y; acc[4 * j + 2] += v.z; acc[4 * j + 3] += v.w;
+        }
+        __syncwarp();
       }
       // 4 KB of output at a time: 32 rows of 128 bytes, 128-byte-swizzled
       const int per = a.out_dtype == IC_DTYPE_F32 ? 32 : 64;   // columns
@@ -420,37 +490,46 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   if (!PAIR && a.splits > 1) {
-    // the sums of all CTAs of the cluster, in rank order; each takes a share
+    // the sums of all CTAs of the cluster, in rank order
     cluster_sync_all();
-    int mt, nt;
-    f8_tile(a, first, mt, nt);
-    const int rows = min(128, a.M - mt * 128);
-    const int all = rows * (BN / 4), per = (all + a.splits - 1) / a.splits;
-    const int lo = (int)rank * per, hi = min(all, lo + per);
-    for (int i = lo + (int)threadIdx.x; i < hi; i += C::THREADS) {
-      const int r = i / (BN / 4), c = i % (BN / 4);
-      const uint32_t at = ring + r * (BN * 4) + (c ^ (r & 31)) * 16;
-      float4 s = ld_cluster4(mapa_u32(at, 0));
-      for (int p = 1; p < a.splits; ++p) {
-        const float4 v = ld_cluster4(mapa_u32(at, p));
-        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+#pragma unroll 1
+    for (int lr = warp; lr < share; lr += C::THREADS / 32) {
+      const int r = (int)rank * share + lr;
+      const long long m = mt0 * 128 + r;
+      if (r >= 128 || m >= a.M) break;
+      const float4* from = reinterpret_cast<const float4*>(smem + C::OFF_STG + lr * 512 + ((lane ^ (r & 31)) << 4));
+      float4 sum = make_float4(bias4[0], bias4[1], bias4[2], bias4[3]);
+#pragma unroll 1
+      for (int p = 0; p < a.splits; ++p) {
+        const float4 v = from[p * share * 32];
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
       }
-      const float got[4] = {s.x, s.y, s.z, s.w};
-      const long long m = mt * 128 + r;
+      const long long at = m * a.ldo + nc;
+      if (a.tma_store && nc + 4 <= a.N) {   // 8 or 16 aligned bytes
+        if (a.out_dtype == IC_DTYPE_F32) {
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) = sum;
+        } else {
+          const bool f16 = a.out_dtype == IC_DTYPE_F16;
+          const __half2 h0 = __floats2half2_rn(sum.x, sum.y), h1 = __floats2half2_rn(sum.z, sum.w);
+          const __nv_bfloat162 g0 = __floats2bfloat162_rn(sum.x, sum.y), g1 = __floats2bfloat162_rn(sum.z, sum.w);
+          *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at) =
+              make_uint2(f16 ? *reinterpret_cast<const uint32_t*>(&h0) : *reinterpret_cast<const uint32_t*>(&g0),
+                         f16 ? *reinterpret_cast<const uint32_t*>(&h1) : *reinterpret_cast<const uint32_t*>(&g1));
+        }
+      } else {
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = nt * BN + 4 * c + j;
-        if (n < a.N)
-          store_out(a.out, a.out_dtype, m * a.ldo + n, got[j] + (a.bias ? load_any(a.bias, a.bias_dtype, n) : 0.f));
+        for (int j = 0; j < 4; ++j)
+          if (nc + j < a.N) store_out(a.out, a.out_dtype, at + j, v[j]);
       }
     }
   }
-  // nobody leaves while another CTA of the cluster may reach its shared memory
-  if (PAIR || a.splits > 1) cluster_sync_all();
+  // neither CTA of a pair leaves while the other may reach its shared memory
+  if constexpr (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (PAIR) tmem_dealloc2(tmem, 2 * BN);
-    else tmem_dealloc(tmem, 2 * BN);
+    if constexpr (PAIR) tmem_dealloc2(tmem, NB * BN);
+    else tmem_dealloc(tmem, NB * BN);
   }
 }
 
@@ -477,9 +556,11 @@ static cudaError_t f8_launch(const F8Operands& o, F8Args a, int splits, cudaStre
   a.m_tiles = (a.M + TILE_M - 1) / TILE_M;
   a.n_tiles = (a.N + C::BN - 1) / C::BN;
   a.splits = splits;
+  // (rows that are not staged keep what shared memory held; they end in rows of D that nobody reads)
+  a.a_rows = a.M < 128 ? (a.M + 7) / 8 * 8 : 128;
   CUtensorMap tx, tw, to;
   memset(&to, 0, sizeof(to));
-  if (!f8_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.x, o.K, o.M, o.ldx, 128, 128) ||
+  if (!f8_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.x, o.K, o.M, o.ldx, 128, a.a_rows) ||
       !f8_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.w, o.K, o.N, o.ldw, 128, C::B_ROWS))
     return cudaErrorInvalidValue;
   const int es = a.out_dtype == IC_DTYPE_F32 ? 4 : 2;
@@ -513,14 +594,21 @@ static cudaError_t f8_launch(const F8Operands& o, F8Args a, int splits, cudaStre
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// The cheapest way to deal the tiles out, by what a block of 128 along K was
+// measured to take where every SM works (in ns): it goes by the bytes that a CTA fetches
+// from L2, 70 a ns.  Tiles beyond whole rounds wait for a round of their own.
 cudaError_t launch_gemm_fp8(const F8Operands& o, const F8Args& a, cudaStream_t st) {
   const long long sms = num_sms();
-  const long long pairs = ((o.M + 255) / 256) * ((o.N + 255) / 256);
-  if (pairs >= sms / 2) return f8_launch<F8Cfg<256, true>>(o, a, 1, st);
-  const long long tiles = ((o.M + 127) / 128) * ((o.N + 127) / 128);
+  const auto rounds = [](long long tiles, long long places) { return (double)((tiles + places - 1) / places); };
+  const long long m128 = (o.M + 127) / 128, m256 = (o.M + 255) / 256, n128 = (o.N + 127) / 128, n256 = (o.N + 255) / 256;
+  const double wide = rounds(m256 * n256, sms / 2) * (470. * a.kb + 2500), pair = rounds(m256 * n128, sms / 2) * (350. * a.kb + 1500);
+  const double one = rounds(m128 * n128, sms) * (460. * a.kb + 1500);
   int splits = 1;
-  while (splits < 8 && tiles * (splits + 1) <= sms && a.kb >= 2 * (splits + 1)) ++splits;
-  return f8_launch<F8Cfg<128, false>>(o, a, splits, st);
+  while (splits < 8 && m128 * n128 * (splits + 1) <= sms && a.kb >= 2 * (splits + 1)) ++splits;
+  if (splits > 1) return f8_launch<F8Cfg<128, false>>(o, a, splits, st);
+  if (wide <= pair && wide <= one) return f8_launch<F8Cfg<256, true>>(o, a, 1, st);
+  if (pair <= one) return f8_launch<F8Cfg<128, true>>(o, a, 1, st);
+  return f8_launch<F8Cfg<128, false>>(o, a, 1, st);
 }
 
 }  // namespace ic
