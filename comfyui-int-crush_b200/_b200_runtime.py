@@ -1093,11 +1093,13 @@ def _folded(t: torch.Tensor, width: int) -> torch.Tensor:
 def _fp8_buffers(M: int, K: int, scale_rows: int, device: torch.device, by_block: bool):
     """Uninitialised e4m3 rows [M, K] whose stride is K rounded up to 16, and
     scales [scale_rows, K / 128], stored block by block where ``by_block``."""
+    # (whole rows are there, the last one's filling too)
     q = torch.empty((M, _round16(K)), dtype=_E4M3, device=device)
+    if K & 15:
+        q = q[:, :K]
     kb = -(-K // 128)
-    if by_block:
-        return q[:, :K] if K & 15 else q, torch.empty((kb, scale_rows), dtype=torch.float32, device=device).t()
-    return q[:, :K] if K & 15 else q, torch.empty((scale_rows, kb), dtype=torch.float32, device=device)
+    s = torch.empty_strided((scale_rows, kb), (1, scale_rows) if by_block else (kb, 1), dtype=torch.float32, device=device)
+    return q, s
 
 
 def quantize_fp8_block(x: torch.Tensor, *, rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1132,7 +1134,7 @@ def quantize_fp8_block(x: torch.Tensor, *, rows: int = 1) -> tuple[torch.Tensor,
     if M:
         st = _lib(index).ic_quantize_fp8_block(
             x2.data_ptr(), dtype, M, K, x2.stride(0) if M > 1 else K, rows, q.data_ptr(), q.stride(0) if M > 1 else _round16(K),
-            s.data_ptr(), s.stride(0), s.stride(1), _raw_stream(index))
+            s.data_ptr(), *s.stride(), _raw_stream(index))
         if st:
             L.check(st, "ic_quantize_fp8_block")
     if x.dim() == 2:
@@ -1146,8 +1148,8 @@ def _fp8_rows(t: torch.Tensor, K: int) -> torch.Tensor:
     if t.dim() != 2:
         t = t.reshape(-1, K)
     M = t.shape[0]
-    ld = t.stride(0)
-    if t.stride(1) == 1 and not t.data_ptr() & 15 and (M <= 1 or (not ld & 15 and ld >= K)):
+    ld, one = t.stride()
+    if one == 1 and not t.data_ptr() & 15 and (M <= 1 or (not ld & 15 and ld >= K)):
         return t
     rows = torch.empty((M, _round16(K)), dtype=t.dtype, device=t.device)[:, :K]
     rows.view(torch.uint8).copy_(t.view(torch.uint8) if t.stride(1) == 1 else t.contiguous().view(torch.uint8))
@@ -1224,7 +1226,7 @@ def gemm_fp8_block(
     ld = _round16(K)
     st = _lib(index).ic_gemm_fp8_block(
         x2.data_ptr(), M, K, x2.stride(0) if M > 1 else ld, w.data_ptr(), N, w.stride(0) if N > 1 else ld,
-        sa.data_ptr(), sa.stride(0), sa.stride(1), s_w.data_ptr(), s_w.stride(0), s_w.stride(1),
+        sa.data_ptr(), *sa.stride(), s_w.data_ptr(), *s_w.stride(),
         None if bias is None else bias.data_ptr(), bias_code, out.data_ptr(), code, ldo, _raw_stream(index))
     if st:
         L.check(st, "ic_gemm_fp8_block")

@@ -162,7 +162,7 @@ class ConvLinearFP8(_QuantLinearBase):
         from . import _b200_runtime as rt
         q, s = rt.quantize_fp8_block(self._prepared(x.reshape(-1, x.shape[-1])))
         y = rt.gemm_fp8_block(q, self.weight[:, :self.in_features], self.scale, s, bias=self.bias, out_dtype=x.dtype)
-        return y.reshape(*x.shape[:-1], -1)
+        return y.reshape(*x.shape[:-1], self.out_features)
 
     @staticmethod
     def from_float(module: nn.Linear, rot_need: bool = False, rot_size: int = 256) -> "ConvLinearFP8":

@@ -295,11 +295,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         }
       }
       // all MMAs are done before tensor memory is freed
+      // (committed by the lane that issued them)
       volatile int never = 0;
-      if (lane == 0) {
+      if (on) {
         if constexpr (PAIR) mma_commit2_local(drain);
         else mma_commit(drain);
       }
+      __syncwarp();
       mbar_wait(drain, 0, &never);
     }
   } else {
@@ -594,21 +596,24 @@ static cudaError_t f8_launch(const F8Operands& o, F8Args a, int splits, cudaStre
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// The cheapest way to deal the tiles out, by what a block of 128 along K was
-// measured to take where every SM works (in ns): it goes by the bytes that a CTA fetches
-// from L2, 70 a ns.  Tiles beyond whole rounds wait for a round of their own.
+// The cheapest way to deal the tiles out, in ns as measured (every SM at work, 1500
+// to 1900 MHz): a block of 128 along K takes 560 in a pair's 256 x 256, 375 in its
+// 256 x 128, 400 in one CTA's 128 x 128; a tile's output 1000 to 1500; a cluster's
+// exchange 2500.  Tiles beyond whole rounds wait for a round of their own.
+// (4608 x 12288 -> 4096: 240, 298 and 316 us; 768 x 2048 -> 8192: 23.3, 21.7 and 22.0;
+// 256 x 8192 -> 4096: 32.7, 29.9 and 28.6, in clusters of two 20.9.)
 cudaError_t launch_gemm_fp8(const F8Operands& o, const F8Args& a, cudaStream_t st) {
   const long long sms = num_sms();
   const auto rounds = [](long long tiles, long long places) { return (double)((tiles + places - 1) / places); };
   const long long m128 = (o.M + 127) / 128, m256 = (o.M + 255) / 256, n128 = (o.N + 127) / 128, n256 = (o.N + 255) / 256;
-  const double wide = rounds(m256 * n256, sms / 2) * (470. * a.kb + 2500), pair = rounds(m256 * n128, sms / 2) * (350. * a.kb + 1500);
-  const double one = rounds(m128 * n128, sms) * (460. * a.kb + 1500);
+  const double wide = rounds(m256 * n256, sms / 2) * (560. * a.kb + 1500), pair = rounds(m256 * n128, sms / 2) * (375. * a.kb + 1000);
+  const double one = rounds(m128 * n128, sms) * (400. * a.kb + 1000);
   int splits = 1;
   while (splits < 8 && m128 * n128 * (splits + 1) <= sms && a.kb >= 2 * (splits + 1)) ++splits;
-  if (splits > 1) return f8_launch<F8Cfg<128, false>>(o, a, splits, st);
-  if (wide <= pair && wide <= one) return f8_launch<F8Cfg<256, true>>(o, a, 1, st);
-  if (pair <= one) return f8_launch<F8Cfg<128, true>>(o, a, 1, st);
-  return f8_launch<F8Cfg<128, false>>(o, a, 1, st);
+  const double shared = splits > 1 ? 400. * ((a.kb + splits - 1) / splits) + 3500 : wide;
+  if (wide <= pair && wide <= one && wide <= shared) return f8_launch<F8Cfg<256, true>>(o, a, 1, st);
+  if (pair <= one && pair <= shared) return f8_launch<F8Cfg<128, true>>(o, a, 1, st);
+  return f8_launch<F8Cfg<128, false>>(o, a, shared < one ? splits : 1, st);
 }
 
 }  // namespace ic

@@ -303,8 +303,9 @@ __device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, c
   if constexpr (!F8) {
     gn_store(o.y, y, n, g.vec != 0);
   } else {
-    // The scale to a unit or two and the quotients as products: y is no nearer to
-    // its exact value.  (An infinity's reciprocal is 0, a NaN's NaN.)
+    // The scale as it is defined (quant_fp8.cu, with the quotient's correction in
+    // place of a division), the quotients as products with its reciprocal to a unit:
+    // y is no nearer to its exact value.  (An infinity's reciprocal is 0, a NaN's NaN.)
     if (n < 8) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = i < n ? y[i] : 0.f;
@@ -313,9 +314,11 @@ __device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, c
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
     const float amax = __uint_as_float(__reduce_max_sync(0xffffu << (threadIdx.x & 16), top));
-    const float s = (amax < kF8AmaxMin ? kF8AmaxMin : amax) * (1.f / kF8Max);
+    const F8Scale of448 = {kF8Max, 1.f / kF8Max};
+    const float s = amax <= 3e38f ? f8_quotient(fmaxf(amax, kF8AmaxMin), of448) : amax;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    if (inv > 0.f) inv = fmaf(inv, fmaf(-s, inv, 1.f), inv);   // (a NaN stays, a 0 too)
     const uint2 w = make_uint2(f8_pair(y[0] * inv, y[1] * inv) | f8_pair(y[2] * inv, y[3] * inv) << 16,
                                f8_pair(y[4] * inv, y[5] * inv) | f8_pair(y[6] * inv, y[7] * inv) << 16);
     if (8 * v < g.width) *reinterpret_cast<uint2*>(o.q) = w;
@@ -629,7 +632,7 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
   // out, in clocks as they were measured: a wave costs 6000, a cluster's exchange
   // 3500, a value 0.3 (an SM), rows in pieces below 64 bytes half as much again.
   double best = 0;
-  for (long long parts = 1; parts <= G; ++parts) {
+  for (long long parts = 1; parts <= G && parts <= 4 * sms; ++parts) {
     if (G % parts || (parts > 1 && C / parts % (f8 ? 128 : 8))) continue;
     GnPlan t;
     t.parts = (int)parts;
@@ -640,7 +643,7 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
     if (most <= 0) continue;
     for (t.cluster = 1; t.cluster <= 16; t.cluster *= 2) {
       t.tile = (L + t.cluster - 1) / t.cluster;
-      if (t.tile > most) continue;
+      if (t.tile > most || B * parts * t.cluster > (1LL << 30)) continue;
       // CTAs at a time: clusters of four or more leave SMs of a processor group empty
       const long long held = t.cluster < 4 ? sms : sms * 7 / 8 / t.cluster * t.cluster;
       const double waves = (double)((B * parts * t.cluster + held - 1) / held);
