@@ -18,6 +18,8 @@
 // distributed shared memory in a fixed order.
 #include <string.h>
 
+#include <atomic>
+
 #include <type_traits>
 
 namespace ic {
@@ -596,6 +598,35 @@ static cudaError_t f8_launch(const F8Operands& o, F8Args a, int splits, cudaStre
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// Clusters of `splits` CTAs that the device holds at once (45 of 3, 33 of 4, 15 of 7
+// or 8 on 148 SMs: they do not fill its processor groups).  Asked once a device.
+static long long f8_clusters(int splits) {
+  static std::atomic<int> known[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  std::atomic<int>& at = known[dev & 63][splits];
+  if (at.load()) return at.load();
+  using C = F8Cfg<128, false>;
+  auto kern = gemm_fp8_kernel<C>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = splits;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(840 * 8);   // a multiple of every size
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (set_smem_once(kern, C::SMEM) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    n = 0;
+  }
+  if (n > 0) at.store(n);
+  return n;
+}
+
 // The cheapest way to deal the tiles out, in ns as measured (every SM at work, 1500
 // to 1900 MHz): a block of 128 along K takes 560 in a pair's 256 x 256, 375 in its
 // 256 x 128, 400 in one CTA's 128 x 128; a tile's output 1000 to 1500; a cluster's
@@ -609,7 +640,8 @@ cudaError_t launch_gemm_fp8(const F8Operands& o, const F8Args& a, cudaStream_t s
   const double wide = rounds(m256 * n256, sms / 2) * (560. * a.kb + 1500), pair = rounds(m256 * n128, sms / 2) * (375. * a.kb + 1000);
   const double one = rounds(m128 * n128, sms) * (400. * a.kb + 1000);
   int splits = 1;
-  while (splits < 8 && m128 * n128 * (splits + 1) <= sms && a.kb >= 2 * (splits + 1)) ++splits;
+  for (int n = 2; n <= 8 && m128 * n128 * n <= sms && a.kb >= 2 * n; ++n)
+    if (m128 * n128 <= f8_clusters(n)) splits = n;
   const double shared = splits > 1 ? 400. * ((a.kb + splits - 1) / splits) + 3500 : wide;
   if (wide <= pair && wide <= one && wide <= shared) return f8_launch<F8Cfg<256, true>>(o, a, 1, st);
   if (pair <= one && pair <= shared) return f8_launch<F8Cfg<128, true>>(o, a, 1, st);

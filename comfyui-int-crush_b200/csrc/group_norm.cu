@@ -329,7 +329,7 @@ __device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, c
 // Statistics of a cluster's rows (`KEEP`: all rows of a part, kept in shared memory
 // and normalised; else into the workspace).
 template <typename T, bool KEEP, bool F8, int ACT>
-__global__ void __launch_bounds__(kGnThreads, KEEP ? 1 : 2) gn_stats_kernel(const GnArgs g) {
+__global__ void __launch_bounds__(kGnThreads, 2) gn_stats_kernel(const GnArgs g) {
   extern __shared__ __align__(1024) uint8_t smem[];
   // the norm's launch may begin, its CTAs wait for the statistics themselves
   if (!KEEP) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_apply_kernel(const GnArgs g)
 
 // ============================================================== host side
 
-constexpr int kGnShared = 200 * 1024;
+constexpr int kGnShared = 200 * 1024, kGnHalf = 110 * 1024;   // one and two CTAs an SM
 constexpr int kGnRuns = 32 * kGnLaneRuns;
 
 struct GnPlan {
@@ -624,13 +624,46 @@ static void gn_threads(GnPlan& p, long long C, long long G, bool f8) {
   while (p.sub < 8 && C / G % (2 * p.sub) == 0) p.sub *= 2;
 }
 
+// CTAs in clusters of 1 << shift that the device holds at once, `two` on an SM (of 4
+// and more they do not fill its processor groups: 132 of 148 in clusters of 4,
+// 120 of 8, 112 of 16).  Asked once a device; without one, seven eighths.
+static long long gn_places(int shift, bool two) {
+  static std::atomic<int> known[64][5][2];
+  const long long sms = num_sms();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  std::atomic<int>& at = known[dev & 63][shift][two];
+  if (at.load()) return at.load();
+  int clusters = 0;
+  auto kern = gn_stats_kernel<__half, true, false, 1>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = 1u << shift;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(16384);
+  cfg.blockDim = dim3(kGnThreads);
+  cfg.dynamicSmemBytes = two ? kGnHalf : kGnShared;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  const bool asked = set_smem_once(kern, 227 * 1024) == cudaSuccess &&
+                     cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                     cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess;
+  if (!asked) (void)cudaGetLastError();
+  const long long guess = shift < 2 ? sms : sms * 7 / 8 >> shift << shift;
+  const long long n = asked && clusters > 0 ? (long long)clusters << shift : asked ? 0 : two ? 2 * guess : guess;
+  if (n > 0) at.store((int)n);
+  return n;
+}
+
 static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f8) {
   GnPlan p;
   const long long sms = num_sms();
   // One launch where what a cluster keeps fits.  A part is whole groups and whole
   // 16-byte columns (128 channels for e4m3).  The cheapest of the ways to deal it
-  // out, in clocks as they were measured: a wave costs 6000, a cluster's exchange
-  // 3500, a value 0.3 (an SM), rows in pieces below 64 bytes half as much again.
+  // out, in clocks as they were measured: a CTA takes 6000 and 0.3 a value, two that
+  // share an SM 7500 and 0.6, a cluster's exchange 3500; rows in pieces below 64
+  // bytes half as much again.
   double best = 0;
   for (long long parts = 1; parts <= G && parts <= 4 * sms; ++parts) {
     if (G % parts || (parts > 1 && C / parts % (f8 ? 128 : 8))) continue;
@@ -641,25 +674,31 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
     const long long head = ((sums + 2 * (G / parts)) * 8 + 15) / 16 * 16;
     const long long most = (kGnShared - head) / ((long long)t.cols * 16);   // rows of a CTA
     if (most <= 0) continue;
-    for (t.cluster = 1; t.cluster <= 16; t.cluster *= 2) {
+    int shift = 0;
+    for (t.cluster = 1; t.cluster <= 16; t.cluster *= 2, ++shift) {
       t.tile = (L + t.cluster - 1) / t.cluster;
-      if (t.tile > most || B * parts * t.cluster > (1LL << 30)) continue;
-      // CTAs at a time: clusters of four or more leave SMs of a processor group empty
-      const long long held = t.cluster < 4 ? sms : sms * 7 / 8 / t.cluster * t.cluster;
-      const double waves = (double)((B * parts * t.cluster + held - 1) / held);
-      double cost = waves * (6000 + 0.3 * t.tile * t.cols * 8 * (C / parts < 32 ? 1.5 : 1.0)) + (t.cluster > 1 ? 3500 : 0) +
-                    (t.cluster == 16 ? 1000 : 0);
+      const long long ctas = B * parts * t.cluster;
+      if (t.tile > most || ctas > (1LL << 30)) continue;
+      t.shared = (int)(head + t.tile * t.cols * 16);
+      const long long one = gn_places(shift, false), two = t.shared <= kGnHalf ? gn_places(shift, true) : 0;
+      if (one <= 0) continue;   // clusters of this size do not fit at all
+      const double values = (double)t.tile * t.cols * 8 * (C / parts < 32 ? 1.5 : 1.0);
+      double cost = (double)((ctas + one - 1) / one) * (6000 + 0.3 * values);
+      if (two > 0) {
+        const double shared = (double)((ctas + two - 1) / two) * (7500 + 0.6 * values);
+        if (ctas > one && shared < cost) cost = shared;
+      }
+      if (t.cluster > 1) cost += 3500;
       if (best && cost >= best) continue;
       best = cost;
       t.runs = 1;
       t.keep = true;
-      t.shared = (int)(head + t.tile * t.cols * 16);
       t.floats = 0;
       p = t;
     }
   }
-  // Two launches: 20000, and 0.5 a value at all SMs' rate.
-  if (best && best <= 20000 + 0.5 * (double)B * (double)L * (double)C / sms) return p;
+  // Two launches: 22000, and 0.27 a value at all SMs' rate.
+  if (best && best <= 22000 + 0.27 * (double)B * (double)L * (double)C / sms) return p;
   p.parts = 1;
   p.keep = false;
   gn_threads(p, C, G, f8);
