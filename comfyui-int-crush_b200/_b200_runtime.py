@@ -1077,29 +1077,52 @@ def lora_batched(
 
 # ── 8-bit floating point linear ──────────────────────────────────────────────
 
-_ACTIVATION_CODES = (0, 1, 2, 3)
 _E4M3 = torch.float8_e4m3fn
 
 
-def _folded(t: torch.Tensor, width: int) -> torch.Tensor:
+# What a call's checks and sizes come to goes by shapes, strides and types alone:
+# kept for calls of the same form, so that those of a few microseconds on the
+# device are not waited for.
+def _sizes(*values: int):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _row_major(t: torch.Tensor, width: int) -> torch.Tensor:
     """``t`` [..., width] as a matrix with contiguous rows, a copy only where its
     strides need one."""
-    if t.dim() != 2:
-        t = t.reshape(-1, width)
-    ld = t.stride(0)
-    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or ld >= width) else t.contiguous()
+    t = t.reshape(-1, width)
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
 
 
-def _fp8_buffers(M: int, K: int, scale_rows: int, device: torch.device, by_block: bool):
-    """Uninitialised e4m3 rows [M, K] whose stride is K rounded up to 16, and
-    scales [scale_rows, K / 128], stored block by block where ``by_block``."""
-    # (whole rows are there, the last one's filling too)
-    q = torch.empty((M, _round16(K)), dtype=_E4M3, device=device)
-    if K & 15:
-        q = q[:, :K]
+def _fp8_buffers(x: torch.Tensor, M: int, K: int, scale_rows: int, by_block: bool):
+    """Uninitialised e4m3 rows [M, K] whose stride is K rounded up to 16 (the last
+    one whole too), and scales [scale_rows, K / 128], stored block by block where
+    ``by_block``, on the device of ``x``."""
+    q = x.new_empty((M, _round16(K)), dtype=_E4M3)
     kb = -(-K // 128)
-    s = torch.empty_strided((scale_rows, kb), (1, scale_rows) if by_block else (kb, 1), dtype=torch.float32, device=device)
-    return q, s
+    s = x.new_empty_strided((scale_rows, kb), (1, scale_rows) if by_block else (kb, 1), dtype=torch.float32)
+    return q[:, :K] if K & 15 else q, s
+
+
+@functools.lru_cache(maxsize=4096)
+def _quantize_form(dtype, shape, stride, rows):
+    """Sizes for the library (None: a matrix has to be made of x first), and of the
+    results."""
+    what = "quantize_fp8_block"
+    code = _DT.get(dtype)
+    if code is None:
+        raise TypeError(f"{what}: x must be float16, bfloat16 or float32, got {dtype}")
+    if rows not in (1, 128):
+        raise ValueError(f"{what}: rows must be 1 or 128, got {rows}")
+    if not shape or shape[-1] == 0 or (rows == 128 and len(shape) != 2):
+        raise ValueError(f"{what}: x must be {'[..., K]' if rows == 1 else '[N, K]'}, got {tuple(shape)}")
+    if len(shape) != 2:
+        return None, 0, 0, 0
+    M, K = shape
+    scale_rows = M if rows == 1 else -(-M // 128)
+    if stride[1] != 1 and K > 1 or (M > 1 and stride[0] < K):
+        return None, 0, 0, 0
+    return _sizes(code, M, K, stride[0] if M > 1 else K, rows, _round16(K), *((1, M) if rows == 1 else (-(-K // 128), 1))), M, K, scale_rows
 
 
 def quantize_fp8_block(x: torch.Tensor, *, rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1120,40 +1143,68 @@ def quantize_fp8_block(x: torch.Tensor, *, rows: int = 1) -> tuple[torch.Tensor,
     """
     index = x.get_device()
     _same_device("quantize_fp8_block", index, x)
-    dtype = _DT.get(x.dtype)
-    if dtype is None:
-        raise TypeError(f"quantize_fp8_block: x must be float16, bfloat16 or float32, got {x.dtype}")
-    if rows not in (1, 128):
-        raise ValueError(f"quantize_fp8_block: rows must be 1 or 128, got {rows}")
-    if x.dim() < 1 or x.shape[-1] == 0 or (rows == 128 and x.dim() != 2):
-        raise ValueError(f"quantize_fp8_block: x must be {'[..., K]' if rows == 1 else '[N, K]'}, got {tuple(x.shape)}")
-    K = x.shape[-1]
-    x2 = _folded(x, K)
-    M = x2.shape[0]
-    q, s = _fp8_buffers(M, K, M if rows == 1 else -(-M // 128), x.device, rows == 1)
+    sizes, M, K, scale_rows = _quantize_form(x.dtype, x.shape, x.stride(), rows)
+    if sizes is None:
+        q, s = quantize_fp8_block(_row_major(x, x.shape[-1]), rows=rows)
+        return (q, s) if x.dim() == 2 else (q.view(x.shape), s.view(*x.shape[:-1], s.shape[1]))
+    q, s = _fp8_buffers(x, M, K, scale_rows, rows == 1)
     if M:
-        st = _lib(index).ic_quantize_fp8_block(
-            x2.data_ptr(), dtype, M, K, x2.stride(0) if M > 1 else K, rows, q.data_ptr(), q.stride(0) if M > 1 else _round16(K),
-            s.data_ptr(), *s.stride(), _raw_stream(index))
+        st = _lib(index).ic_quantize_fp8_block(x.data_ptr(), q.data_ptr(), s.data_ptr(), sizes, _raw_stream(index))
         if st:
             L.check(st, "ic_quantize_fp8_block")
-    if x.dim() == 2:
-        return q, s
-    return q.view(x.shape), s.view(*x.shape[:-1], s.shape[1])
+    return q, s
 
 
 def _fp8_rows(t: torch.Tensor, K: int) -> torch.Tensor:
-    """An e4m3 operand as the kernel reads it: 16-byte aligned rows; a copy
-    where it is not."""
-    if t.dim() != 2:
-        t = t.reshape(-1, K)
-    M = t.shape[0]
-    ld, one = t.stride()
-    if one == 1 and not t.data_ptr() & 15 and (M <= 1 or (not ld & 15 and ld >= K)):
-        return t
-    rows = torch.empty((M, _round16(K)), dtype=t.dtype, device=t.device)[:, :K]
-    rows.view(torch.uint8).copy_(t.view(torch.uint8) if t.stride(1) == 1 else t.contiguous().view(torch.uint8))
+    """A copy of an e4m3 matrix whose rows start at multiples of 16 bytes."""
+    rows = t.new_empty((t.shape[0], _round16(K)))[:, :K]
+    rows.view(torch.uint8).copy_((t if t.stride(1) == 1 else t.contiguous()).view(torch.uint8))
     return rows
+
+
+@functools.lru_cache(maxsize=4096)
+def _product_form(x, w, s_w, s_a, bias, out_dtype, out):
+    """Each a tensor's (dtype, shape, stride), or None: what to copy first (1: x, 2:
+    w, 4: bias), sizes for the library, M and N."""
+    what = "gemm_fp8_block"
+    if x[0] is not _E4M3 or w[0] is not _E4M3:
+        raise TypeError(f"{what}: x and w must be float8_e4m3fn, got {x[0]}, {w[0]}")
+    if not x[1] or len(w[1]) != 2 or x[1][-1] != w[1][1] or w[1][1] == 0:
+        raise ValueError(f"{what}: x must be [..., K] and w [N, K], got {tuple(x[1])}, {tuple(w[1])}")
+    N, K = w[1]
+    kb = -(-K // 128)
+    lead = tuple(x[1][:-1])
+    if s_a[1] != (*lead, kb) or s_w[1] != (-(-N // 128), kb):
+        raise ValueError(f"{what}: scales must be {(*lead, kb)} and {(-(-N // 128), kb)}, got {tuple(s_a[1])}, {tuple(s_w[1])}")
+    if s_a[0] is not torch.float32 or s_w[0] is not torch.float32:
+        raise TypeError(f"{what}: scales must be float32, got {s_a[0]}, {s_w[0]}")
+    code = _DT.get(out_dtype if out is None else out[0])
+    if code is None:
+        raise TypeError(f"{what}: the output must be float16, bfloat16 or float32, got {out_dtype if out is None else out[0]}")
+    copies = bias_code = 0
+    if bias is not None:
+        bias_code = _DT.get(bias[0])
+        if bias_code is None:
+            raise TypeError(f"{what}: bias must be float16, bfloat16 or float32, got {bias[0]}")
+        if bias[1] != (N,):
+            raise ValueError(f"{what}: bias must be [{N}], got {tuple(bias[1])}")
+        copies = 0 if bias[2][0] == 1 or N <= 1 else 4
+    if out is not None and out[1] != (*lead, N):
+        raise ValueError(f"{what}: out must be {(*lead, N)}, got {tuple(out[1])}")
+    if len(lead) != 1:
+        return copies, None, 0, N
+    M = lead[0]
+    ldo = N
+    if out is not None and M and N:
+        ldo = out[2][0] if M > 1 else N
+        if (N > 1 and out[2][1] != 1) or ldo < N:
+            raise ValueError(f"{what}: out must be row-major, got strides {out[2]}")
+    ld = []
+    for i, (t, rows) in enumerate(((x, M), (w, N))):
+        if (t[2][1] != 1 and K > 1) or (rows > 1 and (t[2][0] & 15 or t[2][0] < K)):
+            copies |= 1 << i
+        ld.append(t[2][0] if rows > 1 else _round16(K))
+    return copies, _sizes(M, K, N, *ld, ldo, *s_a[2], *s_w[2], bias_code, code), M, N
 
 
 def gemm_fp8_block(
@@ -1178,129 +1229,121 @@ def gemm_fp8_block(
     """
     index = x.get_device()
     _same_device("gemm_fp8_block", index, x, w, s_w, s_a, bias, out)
-    if x.dtype is not _E4M3 or w.dtype is not _E4M3:
-        raise TypeError(f"gemm_fp8_block: x and w must be float8_e4m3fn, got {x.dtype}, {w.dtype}")
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or w.shape[1] == 0:
-        raise ValueError(f"gemm_fp8_block: x must be [..., K] and w [N, K], got {tuple(x.shape)}, {tuple(w.shape)}")
-    N, K = w.shape
-    kb = -(-K // 128)
-    lead = x.shape[:-1]
-    if s_a.shape != (*lead, kb) or s_w.shape != (-(-N // 128), kb):
-        raise ValueError(f"gemm_fp8_block: scales must be {(*lead, kb)} and {(-(-N // 128), kb)}, got {tuple(s_a.shape)}, "
-                         f"{tuple(s_w.shape)}")
-    if s_a.dtype is not torch.float32 or s_w.dtype is not torch.float32:
-        raise TypeError(f"gemm_fp8_block: scales must be float32, got {s_a.dtype}, {s_w.dtype}")
-    if out is not None:
-        out_dtype = out.dtype
-    code = _DT.get(out_dtype)
-    if code is None:
-        raise TypeError(f"gemm_fp8_block: the output must be float16, bfloat16 or float32, got {out_dtype}")
-    bias_code = 0
-    if bias is not None:
-        bias_code = _DT.get(bias.dtype)
-        if bias_code is None:
-            raise TypeError(f"gemm_fp8_block: bias must be float16, bfloat16 or float32, got {bias.dtype}")
-        if bias.shape != (N,):
-            raise ValueError(f"gemm_fp8_block: bias must be [{N}], got {tuple(bias.shape)}")
-        if bias.stride(0) != 1:
-            bias = bias.contiguous()
-    if out is None:
-        out = torch.empty((*lead, N), dtype=out_dtype, device=x.device)
-        M = out.numel() // N if N else 0
-        ldo = N
-    else:
-        if out.shape != (*lead, N):
-            raise ValueError(f"gemm_fp8_block: out must be {(*lead, N)}, got {tuple(out.shape)}")
-        if out.numel() == 0:
+    copies, sizes, M, N = _product_form(
+        (x.dtype, x.shape, x.stride()), (w.dtype, w.shape, w.stride()), (s_w.dtype, s_w.shape, s_w.stride()),
+        (s_a.dtype, s_a.shape, s_a.stride()), None if bias is None else (bias.dtype, bias.shape, bias.stride()),
+        out_dtype, None if out is None else (out.dtype, out.shape, out.stride()))
+    if sizes is None:   # rows first
+        K, lead = w.shape[1], x.shape[:-1]
+        if out is not None and out.numel() == 0:
             return out
-        o2 = out if out.dim() == 2 else out.view(-1, N)   # raises where the leading dimensions do not fold
-        M = o2.shape[0]
-        ldo = o2.stride(0) if M > 1 else N
-        if (N > 1 and o2.stride(1) != 1) or ldo < N:
-            raise ValueError(f"gemm_fp8_block: out must be row-major, got strides {out.stride()}")
+        flat = None if out is None else out.view(-1, N)   # raises where the leading dimensions do not fold
+        rows = x.reshape(-1, K) if lead.numel() else x.new_empty((0, K))
+        y = gemm_fp8_block(rows, w, s_w, s_a.reshape(rows.shape[0], -(-K // 128)), bias, out_dtype, flat)
+        return y.view(*lead, N) if out is None else out
+    y = x.new_empty((M, N), dtype=out_dtype) if out is None else out
     if M == 0 or N == 0:
-        return out
-    x2 = _fp8_rows(x, K)
-    w = _fp8_rows(w, K)
-    sa = s_a if s_a.dim() == 2 else s_a.reshape(-1, kb)
-    ld = _round16(K)
-    st = _lib(index).ic_gemm_fp8_block(
-        x2.data_ptr(), M, K, x2.stride(0) if M > 1 else ld, w.data_ptr(), N, w.stride(0) if N > 1 else ld,
-        sa.data_ptr(), *sa.stride(), s_w.data_ptr(), *s_w.stride(),
-        None if bias is None else bias.data_ptr(), bias_code, out.data_ptr(), code, ldo, _raw_stream(index))
+        return y
+    xp, wp = x.data_ptr(), w.data_ptr()
+    if copies or (xp | wp) & 15:
+        if copies & 1 or xp & 15:
+            x = _fp8_rows(x, w.shape[1])
+        if copies & 2 or wp & 15:
+            w = _fp8_rows(w, w.shape[1])
+        if copies & 4:
+            bias = bias.contiguous()
+        return gemm_fp8_block(x, w, s_w, s_a, bias, out_dtype, y)
+    st = _lib(index).ic_gemm_fp8_block(xp, wp, s_a.data_ptr(), s_w.data_ptr(), None if bias is None else bias.data_ptr(),
+                                       y.data_ptr(), sizes, _raw_stream(index))
     if st:
         L.check(st, "ic_gemm_fp8_block")
-    return out
+    return y
 
 
-def _channels_last(t: torch.Tensor):
-    """``t`` [B, ..., C] as [B, L, C], its elements contiguous along C, and
-    whether that is a view."""
-    C = t.shape[-1]
-    try:
-        v = t.view(t.shape[0], -1, C) if t.dim() != 3 else t
-    except RuntimeError:
+def _rows_of(shape, stride):
+    """(L, batch stride, row stride) of a [B, ..., C] tensor whose positions are
+    evenly spaced rows with contiguous channels that do not overlap, else None."""
+    C = shape[-1]
+    if stride[-1] != 1 and C > 1:
         return None
-    return v if v.stride(2) == 1 or C == 1 else None
+    L, row = 1, C
+    for n, s in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
+        if n == 1:
+            continue
+        if L == 1:
+            row = s
+        elif s != L * row:
+            return None
+        L *= n
+    return None if L > 1 and row < C else (L, stride[0], row)
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_form(what, index, x, groups, weight, bias, activation, out, quantize):
+    """x, weight, bias and out as (dtype, shape, stride) or None: what to copy first
+    (1: x, 2: weight, 4: bias), sizes for the library, workspace floats."""
+    dtype, shape, stride = x
+    code = _HALF.get(dtype)
+    if code is None:
+        raise TypeError(f"{what}: x must be float16/bfloat16, got {dtype}")
+    if len(shape) < 2:
+        raise ValueError(f"{what}: x must be [batch, ..., channels], got {tuple(shape)}")
+    if activation not in (0, 1, 2, 3):
+        raise ValueError(f"{what}: activation must be 0 (none), 1 (SiLU), 2 (GELU erf) or 3 (GELU tanh), got {activation}")
+    B, C = shape[0], shape[-1]
+    if groups < 1 or C == 0 or C % groups:
+        raise ValueError(f"{what}: {C} channels do not divide into {groups} groups")
+    codes, copies = [], 0
+    for i, t in enumerate((weight, bias)):
+        codes.append(0 if t is None else _DT.get(t[0]))
+        if codes[-1] is None:
+            raise TypeError(f"{what}: weight and bias must be float16, bfloat16 or float32, got {t[0]}")
+        if t is not None and t[1] != (C,):
+            raise ValueError(f"{what}: weight and bias must be [{C}], got {tuple(t[1])}")
+        if t is not None and t[2][0] != 1 and C > 1:
+            copies |= 2 << i
+    if out is not None and (out[1] != shape or out[0] != dtype):
+        raise ValueError(f"{what}: out must be {dtype} {tuple(shape)}, got {out[0]} {tuple(out[1])}")
+    if 0 in shape:
+        return copies, None, 0
+    rows = _rows_of(shape, stride)
+    if rows is None:
+        return copies | 1, None, 0
+    T, x_batch, x_row = rows
+    y_batch, y_row = T * C, C
+    if out is not None:
+        rows = _rows_of(shape, out[2])
+        if rows is None or (B > 1 and rows[1] < C):
+            raise ValueError(f"{what}: out must be channels last with rows that do not overlap, got strides {out[2]}")
+        _, y_batch, y_row = rows
+    n = _workspace("ic_group_norm_workspace", index, B, T, C, groups, int(quantize))
+    # (sizes that are refused: the call says why)
+    return copies, _sizes(code, B, T, C, x_batch, x_row, groups, *codes, activation, y_batch, y_row, _round16(C), 1, B * T, n), n
 
 
 def _group_norm(what, x, groups, weight, bias, eps, activation, out, quantize):
     index = x.get_device()
     _same_device(what, index, x, weight, bias, out)
-    dtype = _HALF.get(x.dtype)
-    if dtype is None:
-        raise TypeError(f"{what}: x must be float16/bfloat16, got {x.dtype}")
-    if x.dim() < 2:
-        raise ValueError(f"{what}: x must be [batch, ..., channels], got {tuple(x.shape)}")
-    if activation not in _ACTIVATION_CODES:
-        raise ValueError(f"{what}: activation must be 0 (none), 1 (SiLU), 2 (GELU erf) or 3 (GELU tanh), got {activation}")
-    B, C = x.shape[0], x.shape[-1]
-    if groups < 1 or C == 0 or C % groups:
-        raise ValueError(f"{what}: {C} channels do not divide into {groups} groups")
-    codes = []
-    for t in (weight, bias):
-        code = 0
-        if t is not None:
-            code = _DT.get(t.dtype)
-            if code is None:
-                raise TypeError(f"{what}: weight and bias must be float16, bfloat16 or float32, got {t.dtype}")
-            if t.shape != (C,):
-                raise ValueError(f"{what}: weight and bias must be [{C}], got {tuple(t.shape)}")
-        codes.append(code)
-    if weight is not None and weight.stride(0) != 1:
-        weight = weight.contiguous()
-    if bias is not None and bias.stride(0) != 1:
-        bias = bias.contiguous()
-    y = yv = q = s = None
+    copies, sizes, n = _norm_form(
+        what, index, (x.dtype, x.shape, x.stride()), groups, None if weight is None else (weight.dtype, weight.shape, weight.stride()),
+        None if bias is None else (bias.dtype, bias.shape, bias.stride()), activation,
+        None if out is None else (out.dtype, out.shape, out.stride()), quantize)
+    if copies:
+        return _group_norm(what, x.contiguous() if copies & 1 else x, groups, weight.contiguous() if copies & 2 else weight,
+                           bias.contiguous() if copies & 4 else bias, eps, activation, out, quantize)
+    y = q = s = qp = sp = yp = None
     if quantize:
-        rows = x.numel() // C
-        q, s = _fp8_buffers(rows, C, rows, x.device, True)
+        rows, C = x.numel() // x.shape[-1], x.shape[-1]
+        q, s = _fp8_buffers(x, rows, C, rows, True)
+        qp, sp = q.data_ptr(), s.data_ptr()
     else:
-        if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
-            raise ValueError(f"{what}: out must be {x.dtype} {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    if x.numel():
-        xv = None if x.dim() == 2 else _channels_last(x)
-        if x.dim() == 2:
-            xv = x[:, None] if x.stride(1) == 1 else x.contiguous()[:, None]
-        if xv is None or (xv.shape[1] > 1 and xv.stride(1) < C):
-            xv = x.contiguous().view(B, -1, C)
-        T = xv.shape[1]
-        ys = (0, C)
-        if y is not None:
-            yv = y[:, None] if y.dim() == 2 else _channels_last(y)
-            if yv is None or yv.stride(2) != 1 and C > 1 or (T > 1 and yv.stride(1) < C) or (B > 1 and yv.stride(0) < C):
-                raise ValueError(f"{what}: out must be channels last with rows that do not overlap, got strides {out.stride()}")
-            ys = (yv.stride(0), yv.stride(1) if T > 1 else C)
-        n = _workspace("ic_group_norm_workspace", index, B, T, C, groups, int(quantize))
-        # (sizes that are refused: the call below says why)
-        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
+        y = x.new_empty(x.shape) if out is None else out
+        yp = y.data_ptr()
+    if sizes is not None:
+        ws = x.new_empty(n, dtype=torch.float32) if n > 0 else None
         st = _lib(index).ic_group_norm(
-            xv.data_ptr(), dtype, B, T, C, xv.stride(0), xv.stride(1) if T > 1 else C, groups,
-            None if weight is None else weight.data_ptr(), codes[0], None if bias is None else bias.data_ptr(), codes[1],
-            eps, activation, None if y is None else y.data_ptr(), *ys, None if q is None else q.data_ptr(), _round16(C),
-            None if s is None else s.data_ptr(), 1, 0 if s is None else s.stride(1), None if ws is None else ws.data_ptr(), n,
-            _raw_stream(index))
+            x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), eps, yp, qp, sp,
+            None if ws is None else ws.data_ptr(), sizes, _raw_stream(index))
         if st:
             L.check(st, "ic_group_norm")
     return y if not quantize else (q.view(x.shape), s.view(*x.shape[:-1], s.shape[1]))

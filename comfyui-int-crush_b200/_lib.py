@@ -76,9 +76,10 @@ SIGNATURES: dict[str, list] = {
     "ic_cross_attention_workspace": [_L, _L, _L, _L, _L, _L, _I],
     "ic_lora_batched": [_P, _I, _L, _L, _L, _P, _P, _L, _L, _P, _L, _P, _P, _L, _P, _L, _L, _P, _L, _P],
     "ic_lora_batched_workspace": [_L, _L, _L, _L, _L],
-    "ic_quantize_fp8_block": [_P, _I, _L, _L, _L, _I, _P, _L, _P, _L, _L, _P],
-    "ic_gemm_fp8_block": [_P, _L, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _I, _P, _I, _L, _P],
-    "ic_group_norm": [_P, _I, _L, _L, _L, _L, _L, _L, _P, _I, _P, _I, _F, _I, _P, _L, _L, _P, _L, _P, _L, _L, _P, _L, _P],
+    # (the last but one: the sizes structure, all int64)
+    "ic_quantize_fp8_block": [_P, _P, _P, _P, _P],
+    "ic_gemm_fp8_block": [_P, _P, _P, _P, _P, _P, _P, _P],
+    "ic_group_norm": [_P, _P, _P, _F, _P, _P, _P, _P, _P, _P],
     "ic_group_norm_workspace": [_L, _L, _L, _L, _I],
 }
 _RESTYPES = {"ic_last_error": ctypes.c_char_p, "ic_cross_attention_workspace": _L, "ic_lora_batched_workspace": _L,

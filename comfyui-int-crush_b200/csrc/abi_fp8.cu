@@ -15,6 +15,8 @@ static int f8_launched(cudaError_t e, const char* what) {
 }
 static bool f8_at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static bool f8_float(int dtype) { return dtype == IC_DTYPE_F16 || dtype == IC_DTYPE_BF16 || dtype == IC_DTYPE_F32; }
+// a code of a sizes structure; what no int holds is no code
+static int f8_code(int64_t v) { return v == (int)v ? (int)v : -1; }
 static int64_t f8_up(int64_t n, int64_t m) { return (n + m - 1) / m; }
 
 constexpr int64_t kF8Rows = 0x7fffffffLL - 1024;   // row and column numbers are 32-bit in the kernels
@@ -24,11 +26,13 @@ constexpr int64_t kF8Stride = 1LL << 38;           // of a tensor map
 
 extern "C" {
 
-int ic_quantize_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int rows, void* q, int64_t ldq,
-                          float* s, int64_t s_row, int64_t s_block, void* stream) {
+int ic_quantize_fp8_block(const void* x, void* q, float* s, const ic_quantize_fp8_sizes* sizes, void* stream) {
   using namespace ic;
   const char* me = "ic_quantize_fp8_block";
   clear_error();
+  if (!sizes) return set_error(IC_ERR_ARG, "%s: sizes is NULL", me);
+  const int64_t M = sizes->M, K = sizes->K, ldx = sizes->ldx, ldq = sizes->ldq, s_row = sizes->s_row, s_block = sizes->s_block;
+  const int dtype = f8_code(sizes->dtype), rows = f8_code(sizes->rows);
   if (!f8_float(dtype)) return set_error(IC_ERR_ARG, "%s: dtype must be f16, bf16 or f32", me);
   if (M < 0 || K <= 0 || ldx < K) return set_error(IC_ERR_ARG, "%s: bad M/K/ldx (%lld, %lld, %lld)", me, (long long)M, (long long)K, (long long)ldx);
   if (rows != 1 && rows != 128) return set_error(IC_ERR_ARG, "%s: rows of a block must be 1 or 128, got %d", me, rows);
@@ -50,12 +54,14 @@ int ic_quantize_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_
   return f8_launched(launch_quant_fp8(a, dtype, rows, (cudaStream_t)stream), "ic_quantize_fp8_block launch");
 }
 
-int ic_gemm_fp8_block(const void* x, int64_t M, int64_t K, int64_t ldx, const void* w, int64_t N, int64_t ldw,
-                      const float* s_a, int64_t sa_row, int64_t sa_block, const float* s_w, int64_t sw_row, int64_t sw_block,
-                      const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, void* stream) {
+int ic_gemm_fp8_block(const void* x, const void* w, const float* s_a, const float* s_w, const void* bias, void* out,
+                      const ic_gemm_fp8_sizes* sizes, void* stream) {
   using namespace ic;
   const char* me = "ic_gemm_fp8_block";
   clear_error();
+  if (!sizes) return set_error(IC_ERR_ARG, "%s: sizes is NULL", me);
+  const int64_t M = sizes->M, K = sizes->K, N = sizes->N, ldx = sizes->ldx, ldw = sizes->ldw, ldo = sizes->ldo;
+  const int bias_dtype = f8_code(sizes->bias_dtype), out_dtype = f8_code(sizes->out_dtype);
   if (M < 0 || N < 0 || K <= 0) return set_error(IC_ERR_ARG, "%s: bad M/N/K (%lld, %lld, %lld)", me, (long long)M, (long long)N, (long long)K);
   if (!f8_float(out_dtype) || (bias && !f8_float(bias_dtype)))
     return set_error(IC_ERR_ARG, "%s: out and bias must be f16, bf16 or f32", me);
@@ -74,8 +80,8 @@ int ic_gemm_fp8_block(const void* x, int64_t M, int64_t K, int64_t ldx, const vo
   F8Args a;
   memset(&a, 0, sizeof(a));
   a.M = (int)M; a.N = (int)N; a.kb = (int)f8_up(K, 128);
-  a.s_a = s_a; a.sa_row = sa_row; a.sa_block = sa_block;
-  a.s_w = s_w; a.sw_row = sw_row; a.sw_block = sw_block;
+  a.s_a = s_a; a.sa_row = sizes->sa_row; a.sa_block = sizes->sa_block;
+  a.s_w = s_w; a.sw_row = sizes->sw_row; a.sw_block = sizes->sw_block;
   a.bias = bias; a.bias_dtype = bias_dtype; a.out = out; a.out_dtype = out_dtype; a.ldo = ldo;
   return f8_launched(launch_gemm_fp8(o, a, (cudaStream_t)stream), "ic_gemm_fp8_block launch");
 }
@@ -95,13 +101,16 @@ int64_t ic_group_norm_workspace(int64_t B, int64_t L, int64_t C, int64_t groups,
   return B && L ? ic::gn_plan(B, L, C, groups, quantize != 0).floats : 0;
 }
 
-int ic_group_norm(const void* x, int dtype, int64_t B, int64_t L, int64_t C, int64_t x_batch, int64_t x_row, int64_t groups,
-                  const void* gamma, int gamma_dtype, const void* beta, int beta_dtype, float eps, int activation, void* y,
-                  int64_t y_batch, int64_t y_row, void* q, int64_t ldq, float* s, int64_t s_row, int64_t s_block,
-                  float* workspace, int64_t workspace_elems, void* stream) {
+int ic_group_norm(const void* x, const void* gamma, const void* beta, float eps, void* y, void* q, float* s, float* workspace,
+                  const ic_group_norm_sizes* sizes, void* stream) {
   using namespace ic;
   const char* me = "ic_group_norm";
   clear_error();
+  if (!sizes) return set_error(IC_ERR_ARG, "%s: sizes is NULL", me);
+  const int64_t B = sizes->B, L = sizes->L, C = sizes->C, groups = sizes->groups, x_batch = sizes->x_batch, x_row = sizes->x_row;
+  const int64_t y_batch = sizes->y_batch, y_row = sizes->y_row, ldq = sizes->ldq, workspace_elems = sizes->floats;
+  const int dtype = f8_code(sizes->dtype), activation = f8_code(sizes->activation);
+  const int gamma_dtype = f8_code(sizes->gamma_dtype), beta_dtype = f8_code(sizes->beta_dtype);
   if (dtype != IC_DTYPE_F16 && dtype != IC_DTYPE_BF16) return set_error(IC_ERR_ARG, "%s: dtype must be f16 or bf16", me);
   const int bad = gn_sizes(me, B, L, C, groups);
   if (bad != IC_OK) return bad;
@@ -135,7 +144,7 @@ int ic_group_norm(const void* x, int dtype, int64_t B, int64_t L, int64_t C, int
   a.gamma = gamma; a.gamma_dtype = gamma_dtype; a.beta = beta; a.beta_dtype = beta_dtype;
   a.eps = eps;
   a.y = y; a.y_batch = y_batch; a.y_row = y_row;
-  a.q = static_cast<uint8_t*>(q); a.ldq = ldq; a.s = s; a.s_row = s_row; a.s_block = s_block; a.width = (int)width;
+  a.q = static_cast<uint8_t*>(q); a.ldq = ldq; a.s = s; a.s_row = sizes->s_row; a.s_block = sizes->s_block; a.width = (int)width;
   a.part = reinterpret_cast<float2*>(workspace);
   return f8_launched(launch_group_norm(a, p, B, dtype, activation, (cudaStream_t)stream), "ic_group_norm launch");
 }

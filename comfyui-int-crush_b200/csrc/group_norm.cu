@@ -627,11 +627,8 @@ static void gn_threads(GnPlan& p, long long C, long long G, bool f8) {
 // CTAs in clusters of 1 << shift that the device holds at once, `two` on an SM (of 4
 // and more they do not fill its processor groups: 132 of 148 in clusters of 4,
 // 120 of 8, 112 of 16).  Asked once a device; without one, seven eighths.
-static long long gn_places(int shift, bool two) {
+static long long gn_places(int dev, long long sms, int shift, bool two) {
   static std::atomic<int> known[64][5][2];
-  const long long sms = num_sms();
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
   std::atomic<int>& at = known[dev & 63][shift][two];
   if (at.load()) return at.load();
   int clusters = 0;
@@ -664,6 +661,13 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
   // out, in clocks as they were measured: a CTA takes 6000 and 0.3 a value, two that
   // share an SM 7500 and 0.6, a cluster's exchange 3500; rows in pieces below 64
   // bytes half as much again.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  long long ones[5], twos[5];
+  for (int i = 0; i < 5; ++i) {
+    ones[i] = gn_places(dev, sms, i, false);
+    twos[i] = gn_places(dev, sms, i, true);
+  }
   double best = 0;
   for (long long parts = 1; parts <= G && parts <= 4 * sms; ++parts) {
     if (G % parts || (parts > 1 && C / parts % (f8 ? 128 : 8))) continue;
@@ -680,7 +684,7 @@ static GnPlan gn_plan(long long B, long long L, long long C, long long G, bool f
       const long long ctas = B * parts * t.cluster;
       if (t.tile > most || ctas > (1LL << 30)) continue;
       t.shared = (int)(head + t.tile * t.cols * 16);
-      const long long one = gn_places(shift, false), two = t.shared <= kGnHalf ? gn_places(shift, true) : 0;
+      const long long one = ones[shift], two = t.shared <= kGnHalf ? twos[shift] : 0;
       if (one <= 0) continue;   // clusters of this size do not fit at all
       const double values = (double)t.tile * t.cols * 8 * (C / parts < 32 ? 1.5 : 1.0);
       double cost = (double)((ctas + one - 1) / one) * (6000 + 0.3 * values);

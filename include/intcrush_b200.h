@@ -393,18 +393,23 @@ int ic_lora_batched(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
  * that ic_lora_batched refuses. */
 int64_t ic_lora_batched_workspace(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n);
 
+/* The sizes and strides of the 8-bit floating point linear come as structures of
+ * int64_t, which a caller fills once for calls of the same shape. */
+
 /* Values to e4m3 with an fp32 scale for each block of 128 along K:
  *   s = max(max |x|, 1e-8) / 448,  q = e4m3(x / s), ties to even
  * both in fp32 with IEEE division.  A NaN makes its block's scale NaN, an
  * infinity infinite.
- *   x     [M, K] f16 / bf16 / f32, row stride ldx, any alignment
+ *   x     [M, K] of `dtype` (f16 / bf16 / f32), row stride ldx, any alignment
  *   rows  1 (activations: a block is a part of one row) or 128 (weights: 128 x
  *         128, as ic_gemm_fp8_block takes them)
  *   q     [M, ldq] e4m3, 16-byte aligned, ldq % 16 == 0; columns from K up to
  *         the next multiple of 16 are written with zeros, others are left
  *   s     scale of block b of row (or of 128 rows) i at s[i * s_row + b * s_block] */
-int ic_quantize_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int rows, void* q, int64_t ldq,
-                          float* s, int64_t s_row, int64_t s_block, void* stream);
+typedef struct {
+  int64_t dtype, M, K, ldx, rows, ldq, s_row, s_block;
+} ic_quantize_fp8_sizes;
+int ic_quantize_fp8_block(const void* x, void* q, float* s, const ic_quantize_fp8_sizes* sizes, void* stream);
 
 /* Product of two e4m3 matrices with scales for blocks of 128, on tcgen05
  * (kind::f8f6f4):
@@ -414,31 +419,36 @@ int ic_quantize_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_
  *         what lies behind a row's K values does not matter
  *   s_a   fp32, of row m and block b at s_a[m * sa_row + b * sa_block]; s_w
  *         likewise for rows 128 i .. 128 i + 127 of w
- *   bias  [N] f16 / bf16 / f32 or NULL
- *   out   [M, N] f16 / bf16 / f32, row stride ldo; fastest 16-byte aligned
+ *   bias  [N] of `bias_dtype` (f16 / bf16 / f32) or NULL
+ *   out   [M, N] of `out_dtype` (f16 / bf16 / f32), row stride ldo; fastest 16-byte
+ *         aligned
  * The sums' order depends on the sizes only: same inputs, same bits. */
-int ic_gemm_fp8_block(const void* x, int64_t M, int64_t K, int64_t ldx, const void* w, int64_t N, int64_t ldw,
-                      const float* s_a, int64_t sa_row, int64_t sa_block, const float* s_w, int64_t sw_row, int64_t sw_block,
-                      const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, void* stream);
+typedef struct {
+  int64_t M, K, N, ldx, ldw, ldo, sa_row, sa_block, sw_row, sw_block, bias_dtype, out_dtype;
+} ic_gemm_fp8_sizes;
+int ic_gemm_fp8_block(const void* x, const void* w, const float* s_a, const float* s_w, const void* bias, void* out,
+                      const ic_gemm_fp8_sizes* sizes, void* stream);
 
 /* Group norm with an activation, channels last:
  *   y = act((x - mean) / sqrt(var + eps) * gamma + beta)
  * over the L rows and C / groups channels of each group of each sample (var
  * biased), in fp32.
- *   x     [B, L, C] f16 / bf16, sample stride x_batch, row stride x_row
+ *   x     [B, L, C] of `dtype` (f16 / bf16), sample stride x_batch, row stride x_row
  *   gamma, beta  [C] f16 / bf16 / f32 or NULL (ones, zeros)
  *   activation   0 none, 1 SiLU, 2 GELU (erf), 3 GELU (tanh)
  *   y     [B, L, C] in dtype (may be x itself), or NULL for
  *   q, s  the result as e4m3 rows [B * L, ldq] with scales for blocks of 128
  *         channels, from the fp32 values (layout: ic_quantize_fp8_block)
- *   workspace  ic_group_norm_workspace(...) floats, 16-byte aligned, contents
- *         arbitrary, in use until the call's work has run
+ *   workspace  ic_group_norm_workspace(...) floats (`floats` is what there is),
+ *         16-byte aligned, contents arbitrary, in use until the call's work has run
  * C up to 8192.  Any alignment works; 16-byte aligned rows (C and strides
  * multiples of 8) are faster.  Same inputs, same bits. */
-int ic_group_norm(const void* x, int dtype, int64_t B, int64_t L, int64_t C, int64_t x_batch, int64_t x_row, int64_t groups,
-                  const void* gamma, int gamma_dtype, const void* beta, int beta_dtype, float eps, int activation, void* y,
-                  int64_t y_batch, int64_t y_row, void* q, int64_t ldq, float* s, int64_t s_row, int64_t s_block,
-                  float* workspace, int64_t workspace_elems, void* stream);
+typedef struct {
+  int64_t dtype, B, L, C, x_batch, x_row, groups, gamma_dtype, beta_dtype, activation, y_batch, y_row, ldq, s_row, s_block,
+      floats;
+} ic_group_norm_sizes;
+int ic_group_norm(const void* x, const void* gamma, const void* beta, float eps, void* y, void* q, float* s, float* workspace,
+                  const ic_group_norm_sizes* sizes, void* stream);
 /* Floats of workspace for these sizes (0: none needed); -1 and an error message
  * for sizes that ic_group_norm refuses.  quantize: q instead of y. */
 int64_t ic_group_norm_workspace(int64_t B, int64_t L, int64_t C, int64_t groups, int quantize);

@@ -13,25 +13,39 @@ ODD = ctypes.c_void_p(264)
 ODDER = ctypes.c_void_p(257)
 
 
+def sizes(**kw):
+    return (ctypes.c_int64 * len(kw))(*kw.values())
+
+
+def call(entry, pointers, numbers, eps, kw):
+    """The entry with what ``kw`` changes among pointers and sizes."""
+    p, n = dict(pointers), dict(numbers)
+    for k, v in kw.items():
+        (p if k in p else n)[k] = v
+    packed = None if n.pop("none", False) else sizes(**n)
+    args = list(p.values())
+    if eps is not None:
+        args.insert(3, kw.get("eps", eps))
+    n.pop("eps", None)
+    return getattr(L.lib(), entry)(*args, packed, None)
+
+
 def quant(**kw):
-    a = dict(x=P, dtype=0, M=8, K=300, ldx=300, rows=1, q=P, ldq=304, s=P, s_row=1, s_block=8, stream=None)
-    a.update(kw)
-    return L.lib().ic_quantize_fp8_block(*a.values())
+    return call("ic_quantize_fp8_block", dict(x=P, q=P, s=P),
+                dict(dtype=0, M=8, K=300, ldx=300, rows=1, ldq=304, s_row=1, s_block=8), None, kw)
 
 
 def gemm(**kw):
-    a = dict(x=P, M=8, K=300, ldx=304, w=P, N=40, ldw=304, s_a=P, sa_row=1, sa_block=8, s_w=P, sw_row=3, sw_block=1,
-             bias=P, bias_dtype=0, out=P, out_dtype=1, ldo=40, stream=None)
-    a.update(kw)
-    return L.lib().ic_gemm_fp8_block(*a.values())
+    return call("ic_gemm_fp8_block", dict(x=P, w=P, s_a=P, s_w=P, bias=P, out=P),
+                dict(M=8, K=300, N=40, ldx=304, ldw=304, ldo=40, sa_row=1, sa_block=8, sw_row=3, sw_block=1, bias_dtype=0,
+                     out_dtype=1), None, kw)
 
 
 def norm(**kw):
-    a = dict(x=P, dtype=0, B=2, L=16, C=64, x_batch=1024, x_row=64, groups=4, gamma=P, gamma_dtype=0, beta=P, beta_dtype=2,
-             eps=1e-5, activation=1, y=P, y_batch=1024, y_row=64, q=None, ldq=0, s=None, s_row=0, s_block=0, ws=P,
-             elems=1 << 40, stream=None)
-    a.update(kw)
-    return L.lib().ic_group_norm(*a.values())
+    eps = kw.pop("eps", 1e-5)
+    return call("ic_group_norm", dict(x=P, gamma=P, beta=P, y=P, q=None, s=None, ws=P),
+                dict(dtype=0, B=2, L=16, C=64, x_batch=1024, x_row=64, groups=4, gamma_dtype=0, beta_dtype=2, activation=1,
+                     y_batch=1024, y_row=64, ldq=0, s_row=0, s_block=0, elems=1 << 40), eps, kw)
 
 
 def refused(status, code, text):
@@ -40,6 +54,7 @@ def refused(status, code, text):
 
 
 @pytest.mark.parametrize("change,code,text", [
+    (dict(none=True), 1, "sizes"), (dict(dtype=1 << 32), 1, "dtype"),
     (dict(dtype=3), 1, "dtype"), (dict(dtype=-1), 1, "dtype"), (dict(M=-1), 1, "bad M"), (dict(K=0), 1, "bad M"),
     (dict(ldx=299), 1, "bad M"), (dict(rows=2), 1, "rows of a block"), (dict(x=None), 1, "NULL"), (dict(q=None), 1, "NULL"),
     (dict(s=None), 1, "NULL"), (dict(ldq=300), 1, "row stride"), (dict(ldq=312), 1, "row stride"), (dict(q=ODD), 1, "aligned"),
@@ -51,6 +66,7 @@ def test_quantize_refusals(change, code, text):
 
 
 @pytest.mark.parametrize("change,code,text", [
+    (dict(none=True), 1, "sizes"), (dict(out_dtype=1 << 32), 1, "f16"),
     (dict(M=-1), 1, "bad M"), (dict(N=-1), 1, "bad M"), (dict(K=0), 1, "bad M"), (dict(out_dtype=3), 1, "f16, bf16 or f32"),
     (dict(bias_dtype=-1), 1, "f16, bf16 or f32"), (dict(ldx=299), 1, "row stride"), (dict(ldw=288), 1, "row stride"),
     (dict(ldo=39), 1, "row stride"), (dict(x=None), 1, "NULL"), (dict(w=None), 1, "NULL"), (dict(s_a=None), 1, "NULL"),
@@ -64,6 +80,7 @@ def test_product_refusals(change, code, text):
 
 
 @pytest.mark.parametrize("change,code,text", [
+    (dict(none=True), 1, "sizes"), (dict(activation=1 << 32), 1, "activation"),
     (dict(dtype=2), 1, "dtype"), (dict(B=-1), 1, "bad sizes"), (dict(L=-1), 1, "bad sizes"), (dict(C=0), 1, "bad sizes"),
     (dict(groups=0), 1, "bad sizes"), (dict(groups=5), 1, "bad sizes"), (dict(C=8256, x_row=8256, y_row=8256), 2, "8192"),
     (dict(B=1 << 30), 2, "too many"), (dict(L=1 << 40), 2, "too many"), (dict(B=1 << 20, L=1 << 20), 2, "too many"),
