@@ -2,24 +2,33 @@
 //   out[m, n] = sum_b s_a[m, b] s_w[n / 128, b] sum_{k in block b} x[m, k] w[n, k] + bias[n]
 // on tcgen05 (kind::f8f6f4).
 //
-// Persistent, one CTA per SM, 12 warps: warps 0 and 2 TMA producers, warp 1 MMA
-// issuer, warps 4-11 the sums.  Tokens are the MMA's rows (TMEM lanes), features its
+// Persistent, one CTA per SM, 12 warps: warp 0 TMA producer, warp 1 MMA issuer,
+// warps 4-11 the sums.  Tokens are the MMA's rows (TMEM lanes), features its
 // columns, so that a thread owns one token row and a block's factor
 // s_a * s_w is one number a thread: a weight block is 128 features wide and a
 // warp's columns lie in one.  The 128 products of a block are summed on the
 // tensor core (fp32 in tensor memory, accumulation off at the block's first
 // MMA); the warps read the block's sums, hand the buffer back, and add them, times the
-// factor, onto fp32 registers, two a time.  Two buffers: a block's MMAs run
-// while the block before is read.
+// factor, onto fp32 registers, 32 columns while the next 32 come out of tensor
+// memory.  That is full of buffers (two of 256 columns, or four of 128): a block's
+// MMAs run while the block before is read.
 //
 // Large problems: pairs of CTAs (cta_group::2), 256 x 256 a pair, every CTA
-// staging half of each operand.  Others: 128 x 128 a CTA; where those are fewer
-// than the SMs, clusters of CTAs share a tile's blocks and add their sums through
-// distributed shared memory in a fixed order.
+// staging half of each operand; 256 x 128 or one CTA's 128 x 128 where that leaves
+// fewer SMs without a tile (launch_gemm_fp8).  Where the tiles are fewer than the
+// SMs, clusters of CTAs share a tile's blocks: each pushes its partial sums to the
+// CTAs that own their rows, which add them in rank order.
+//
+// What bounds it: the way of a block's sums.  512 clocks of MMAs, but 850 to 950 a
+// block (256 x 256): 300 of FMAs a scheduler, the first columns' 130 from tensor
+// memory, 100 to 150 for each question to a barrier beside the MMAs' operand
+// reads, which take all of shared memory's width at full rate.  Two values an FMA
+// instruction were slower (as many moves to pair them).  4608 x 12288 -> 4096: 238 us,
+// 1950 TFLOP/s; 65520 x 5120 -> 13824: 4.87 ms, 1905 TFLOP/s under the power cap (1480
+// to 1530 MHz); one row of 5120 x 5120: 9.4 us, 2.8 TB/s.
 #include <string.h>
 
 #include <atomic>
-
 #include <type_traits>
 
 namespace ic {
@@ -167,7 +176,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const bool leader = !PAIR || rank == 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NST; ++i) {
-      mbar_init(full + i, 1);   // (warp 0's; the bytes of both operands)
+      mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < NB; ++i) {
@@ -230,37 +239,44 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   // registers with 128 columns a thread: 384 threads x 168 = 128 x 40 + 256 x 232
   if (warp < 4) {
     if constexpr (CPT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 || warp == 2) {
-      // ----------------------------------------- producers: 0 for x, 2 for w
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
       if (lane == 0) {
-        const bool of_x = warp == 0;
-        const CUtensorMap* tm = of_x ? &tm_x : &tm_w;
         uint32_t it = 0;
         bool ok = true, early = false;
         for (int t = first; ok && t < tiles; t += step) {
           int mt, nt;
           f8_tile(a, t, mt, nt);
-          const int row = of_x ? mt * TILE_M + m_off : nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
+          const int row = mt * TILE_M + m_off, col = nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const uint32_t s = it % NST, ph = (it / NST) & 1u;
             if (!early && !mbar_wait(empty + s, ph ^ 1u, abort_flag)) { ok = false; break; }
-            uint8_t* st = smem + s * C::STAGE + (of_x ? 0 : C::A_BYTES);
+            uint8_t* st = smem + s * C::STAGE;
             if constexpr (PAIR) {
               // both halves count on the leader's barrier
-              if (of_x && leader) mbar_arrive_expect_tx(full + s, 2 * (a.a_rows * 128 + C::B_ROWS * 128));
-              tma_load_2d_pair(st, tm, mapa_u32(smem_u32(full + s), 0u), kb * 128, row);
+              if (leader) mbar_arrive_expect_tx(full + s, 2 * (a.a_rows * 128 + C::B_ROWS * 128));
+              const uint32_t bar = mapa_u32(smem_u32(full + s), 0u);
+              tma_load_2d_pair(st, &tm_x, bar, kb * 128, row);
+              tma_load_2d_pair(st + C::A_BYTES, &tm_w, bar, kb * 128, col);
             } else {
-              if (of_x) mbar_arrive_expect_tx(full + s, a.a_rows * 128 + C::B_ROWS * 128);
-              tma_load_2d(st, tm, full + s, kb * 128, row);
+              mbar_arrive_expect_tx(full + s, a.a_rows * 128 + C::B_ROWS * 128);
+              tma_load_2d(st, &tm_x, full + s, kb * 128, row);
+              tma_load_2d(st + C::A_BYTES, &tm_w, full + s, kb * 128, col);
             }
             early = f8_test(empty + (it + 1) % NST, (((it + 1) / NST) & 1u) ^ 1u);
           }
         }
-        // every copy issued lands before the CTA may leave, whoever gave up
-        // (a pair's count on the leader's barriers: the leader waits for both)
-        if (leader && of_x) {
+        // every copy issued lands before the CTA may leave, whoever gave up.  A
+        // pair's count on the leader's barriers, and where one of the two gave up
+        // before the other not all of them can be waited for there: those land in a
+        // millisecond, as they do in microseconds.
+        if (leader) {
           volatile int never = 0;
           for (uint32_t u = it > NST ? it - NST : 0; u < it; ++u) mbar_wait(full + u % NST, (u / NST) & 1u, &never);
+        }
+        if (PAIR && (!ok || *abort_flag)) {
+          const uint64_t t0 = globaltimer();
+          while (globaltimer() - t0 < 1000000) {}
         }
       }
     } else if (warp == 1 && leader) {
@@ -342,7 +358,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       fa[1] = __ldg(sa);
       fw[1] = __ldg(sw);
       // 32 columns at a time, the next ones on their way from tensor memory while
-      // these are added; a block's last 32 are added under the next block's first
+      // these are added; a block's last 32 after its buffer is handed back
       uint32_t r[2][32];
       constexpr int NC = CPT / 32;
       for (int kb2 = kb0; ok && kb2 < kb1; kb2 += 2) {

@@ -19,6 +19,11 @@
 // launches: statistics of runs of rows, a cluster's worth each, into a
 // workspace, then the norm; the second takes the rows from the end, which the first
 // read last, so that L2 still holds some of them.
+//
+// 2 x 256 x 1280 with SiLU: 6.9 us, most of it code that runs once.  1024 x 1024 x 128
+// with SiLU: 151 us, where 805 MB (x twice, y) at 6.55 TB/s are 123: the statistics
+// take 48 us on average and 60 with the CTAs that read from far memory, the norm 78,
+// at two thirds of the instruction slots and half of the special functions'.
 #include <atomic>
 #include <type_traits>
 

@@ -3,6 +3,10 @@
 //   s = RN32(max(max |x|, 1e-8) / 448),  q = RN_e4m3(RN32(x / s))
 // A NaN makes its block's scale NaN, an infinity infinite (its own value NaN,
 // the others 0), so that neither is lost in a product.
+//
+// One pass; HBM bounds it.  65520 x 5120 bf16: 170 us, 6.0 TB/s (92% of a copy);
+// weights 13824 x 5120: 47.6 us, 4.5 TB/s (a CTA's loads, its maximum and its stores
+// follow one another; four CTAs an SM cover for each other in part).
 #include <type_traits>
 
 namespace ic {

@@ -578,3 +578,42 @@ def test_group_norm_widest(C, groups, L):
     x = normal(g, 1, L, C, dtype=torch.bfloat16)
     check_norm(rt.group_norm(x, groups), x, groups, None, None, 1e-5, 0)
     check_norm_quantized(*rt.fused_groupnorm_quantize(x, groups), x, groups, None, None, 1e-5, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", [9, 33, 100, 121, 128])
+@pytest.mark.parametrize("K,N", [(2048, 1800), (5120, 2560), (4000, 3200), (2040, 4100), (1030, 6000), (8192, 100)])
+def test_product_shared_by_clusters(K, N, M, dtype):
+    """Few tiles: clusters of two to eight CTAs share the blocks; rows that a tile
+    lacks are not staged."""
+    g = gen(K + M)
+    (x, s_a), (w, s_w) = operands(g, M, K, N)
+    b = normal(g, N, dtype=torch.float16)
+    y = rt.gemm_fp8_block(x, w, s_w, s_a, bias=b, out_dtype=dtype)
+    want, size = product_reference(x, w, s_w, s_a, b)
+    check(y, want, product_tolerance(want, size, K, dtype))
+    assert torch.equal(y, rt.gemm_fp8_block(x, w, s_w, s_a, bias=b, out_dtype=dtype))
+    assert rt.device_error() == 0
+
+
+@pytest.mark.parametrize("B,L,C,groups", [(300, 7, 64, 8), (150, 6000, 32, 2), (2, 40000, 136, 17), (700, 1, 16, 16)])
+def test_group_norm_of_many_samples(B, L, C, groups):
+    g = gen(36)
+    x = normal(g, B, L, C, dtype=torch.float16) + normal(g, B, 1, C, dtype=torch.float16)
+    weight, bias = normal(g, C), normal(g, C)
+    check_norm(rt.group_norm(x, groups, weight, bias, activation=1), x, groups, weight, bias, 1e-5, 1)
+    check_norm_quantized(*rt.fused_groupnorm_quantize(x, groups, weight, bias), x, groups, weight, bias, 1e-5, 0)
+
+
+def test_group_norm_one_sample_does_not_see_another():
+    """A sample gives the same bits alone, in a batch and between others."""
+    g = gen(37)
+    x = normal(g, 3, 30000, 64, dtype=torch.bfloat16)
+    y = rt.group_norm(x, 4, activation=3)
+    z = x.clone()
+    z[0], z[2] = 100, math.inf
+    assert torch.equal(rt.group_norm(z, 4, activation=3)[1], y[1])
+
+
+def test_wait_that_runs_out_is_not_set_by_these_calls():
+    assert rt.device_error() == 0
