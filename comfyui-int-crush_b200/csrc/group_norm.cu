@@ -320,7 +320,7 @@ __device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, c
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
     const float amax = __uint_as_float(__reduce_max_sync(0xffffu << (threadIdx.x & 16), top));
     const F8Scale of448 = {kF8Max, 1.f / kF8Max};
-    const float s = amax <= 3e38f ? f8_quotient(fmaxf(amax, kF8AmaxMin), of448) : amax;
+    const float s = amax <= 3.4028235e38f ? f8_quotient(fmaxf(amax, kF8AmaxMin), of448) : amax;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     if (inv > 0.f) inv = fmaf(inv, fmaf(-s, inv, 1.f), inv);   // (a NaN stays, a 0 too)

@@ -406,6 +406,18 @@ def test_group_norm_constant_groups_and_none(space):
 
 
 @pytest.mark.parametrize("space", [(40,), (150, 150)])
+def test_group_norm_quantized_near_the_largest_value(space):
+    x = torch.ones(1, *space, 256, device="cuda", dtype=torch.bfloat16)
+    x[..., ::2] = -1                                             # mean 0, variance 1: y = +-weight / sqrt(1 + eps)
+    weight = torch.full((256,), 3.3e38, device="cuda", dtype=torch.bfloat16)
+    weight[128:] = 2.9e38
+    q, s = rt.fused_groupnorm_quantize(x, 8, weight, eps=1e-5)
+    want = weight.double()[::128] / (1 + 1e-5) ** 0.5 / 448
+    assert ((s.double() - want).abs() <= 2.0 ** -20 * want).all()   # fewer than eight roundings of 2^-24 and an rsqrt of 2^-22
+    assert torch.equal(q.float(), 448 * x.reshape(q.shape).float())
+
+
+@pytest.mark.parametrize("space", [(40,), (150, 150)])
 def test_group_norm_not_finite(space):
     """A NaN or an infinity makes its group of its sample NaN, and no other."""
     g = gen(22)
