@@ -5,8 +5,8 @@
 // the others 0), so that neither is lost in a product.
 //
 // One pass; HBM bounds it.  65520 x 5120 bf16: 170 us, 6.0 TB/s (92% of a copy);
-// weights 13824 x 5120: 47.6 us, 4.5 TB/s (a CTA's loads, its maximum and its stores
-// follow one another; four CTAs an SM cover for each other in part).
+// weights 13824 x 5120: 44.7 us, 4.7 TB/s (a CTA's loads, its maximum and its stores
+// follow one another; an SM's CTAs cover for each other in part).
 #include <type_traits>
 
 namespace ic {
@@ -179,17 +179,23 @@ __global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const F8QuantArgs a
   }
 }
 
-// Weights: a CTA per 128 x 128 block, 64 values a thread in registers.
+// Weights: a CTA per 128 x 128 block, its values in registers: 32 a thread of 16 warps
+// for 16-bit types (13824 x 5120: 44.5 us, 47.3 with 64 of 8 warps), 64 of 8 warps for
+// fp32 (62.5 us, 64.4 with 32 of 16 warps).
 template <typename T>
-__global__ void __launch_bounds__(256) quant_fp8_square_kernel(const F8QuantArgs a) {
-  __shared__ uint32_t tops[8];
+constexpr int kF8SquareWarps = sizeof(T) == 2 ? 16 : 8;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kF8SquareWarps<T>) quant_fp8_square_kernel(const F8QuantArgs a) {
+  constexpr int W = kF8SquareWarps<T>, R = 32 / W;   // warps, rows a thread
+  __shared__ uint32_t tops[W];
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long m0 = (long long)blockIdx.y * 128 + warp * 16 + (lane >> 3);
+  const long long m0 = (long long)blockIdx.y * 128 + warp * (4 * R) + (lane >> 3);
   const int k = b * 128 + (lane & 7) * 16;
-  F8In<T> in[4];
+  F8In<T> in[R];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     const long long m = m0 + 4 * i;
     const int n = m < a.M ? max(0, min(16, a.K - k)) : 0;
     in[i].load(reinterpret_cast<const T*>(a.x) + (n > 0 ? m * a.ldx + k : 0), n, a.vec != 0);
@@ -199,10 +205,10 @@ __global__ void __launch_bounds__(256) quant_fp8_square_kernel(const F8QuantArgs
   if (lane == 0) tops[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+  for (int i = 0; i < W; ++i) top = max(top, tops[i]);
   const F8Scale f = f8_scale(F8In<T>::top_value(top));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     const long long m = m0 + 4 * i;
     if (m < a.M && k < a.width) *reinterpret_cast<uint4*>(a.q + m * a.ldq + k) = f8_bytes<T>(in[i], f);
   }
@@ -212,7 +218,7 @@ __global__ void __launch_bounds__(256) quant_fp8_square_kernel(const F8QuantArgs
 template <typename T>
 static cudaError_t f8_quant_launch(const F8QuantArgs& a, int rows, cudaStream_t st) {
   if (rows == 128) {
-    quant_fp8_square_kernel<T><<<dim3(a.kb, (unsigned)((a.M + 127) / 128)), 256, 0, st>>>(a);
+    quant_fp8_square_kernel<T><<<dim3(a.kb, (unsigned)((a.M + 127) / 128)), 32 * kF8SquareWarps<T>, 0, st>>>(a);
   } else if ((a.M + 15) / 16 * a.kb >= 8LL * num_sms()) {
     quant_fp8_rows_kernel<T, 4><<<(unsigned)(((a.M + 15) / 16 * a.kb + 7) / 8), 256, 0, st>>>(a);
   } else {
