@@ -72,12 +72,24 @@ __device__ __forceinline__ uint64_t gn_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
+__device__ __forceinline__ uint64_t gn_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t gn_fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t v;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
   return v;
 }
 __device__ __forceinline__ uint64_t gn_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+
+// the largest magnitude of three, a NaN (positive) if one is
+__device__ __forceinline__ float gn_top3(float a, float b, float c) {
+  float v;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
 
 constexpr int kGnRing = 8;   // rows of a thread on their way to shared memory
 constexpr int kGnLaneRuns = 5;   // runs of a part that a lane of the second launch joins, at most
@@ -308,24 +320,33 @@ __device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, c
   if constexpr (!F8) {
     gn_store(o.y, y, n, g.vec != 0);
   } else {
-    // The scale as it is defined (quant_fp8.cu, with the quotient's correction in
-    // place of a division), the quotients as products with its reciprocal to a unit:
-    // y is no nearer to its exact value.  (An infinity's reciprocal is 0, a NaN's NaN.)
+    // Scale and quotients as they are defined (quant_fp8.cu), the quotients from a
+    // reciprocal to a unit (300000 x 128 with SiLU: 66.4 us, 65.7 without their
+    // correction, 71.9 a value at a time).  A scale that is infinite has 0 for its
+    // reciprocal, a NaN a NaN; both correct against 0, so that the block's finite
+    // values become 0, or NaN.
     if (n < 8) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = i < n ? y[i] : 0.f;
     }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-    const float amax = __uint_as_float(__reduce_max_sync(0xffffu << (threadIdx.x & 16), top));
+    const float top = gn_top3(gn_top3(gn_top3(y[0], y[1], y[2]), y[3], y[4]), gn_top3(y[5], y[6], y[7]), 0.f);
+    const float amax = __uint_as_float(__reduce_max_sync(0xffffu << (threadIdx.x & 16), __float_as_uint(top)));
     const F8Scale of448 = {kF8Max, 1.f / kF8Max};
     const float s = amax <= 3.4028235e38f ? f8_quotient(fmaxf(amax, kF8AmaxMin), of448) : amax;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     if (inv > 0.f) inv = fmaf(inv, fmaf(-s, inv, 1.f), inv);   // (a NaN stays, a 0 too)
-    const uint2 w = make_uint2(f8_pair(y[0] * inv, y[1] * inv) | f8_pair(y[2] * inv, y[3] * inv) << 16,
-                               f8_pair(y[4] * inv, y[5] * inv) | f8_pair(y[6] * inv, y[7] * inv) << 16);
+    const float minus = inv > 0.f ? -s : 0.f;
+    const uint64_t by = gn_two(inv, inv), less = gn_two(minus, minus);
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t z = gn_two(y[2 * i], y[2 * i + 1]), r = gn_mul2(z, by);
+      float lo, hi;
+      gn_untwo(gn_fma2(gn_fma2(r, less, z), by, r), lo, hi);
+      p[i] = f8_pair(lo, hi);
+    }
+    const uint2 w = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
     if (8 * v < g.width) *reinterpret_cast<uint2*>(o.q) = w;
     if ((v & 15) == 0 && n > 0) *o.s = s;
   }
