@@ -1,0 +1,81 @@
+"""The 8-bit floating point linear and its norm at values far out: activations of
+very negative values, zeros with a sign, blocks that are not finite.
+
+Inputs of the norm alternate between 1 and -1 from row to row, so that y = +-weight
+/ sqrt(1 + eps); statistics, factors and their products are fewer than eight
+roundings of 2^-24 and an rsqrt of 2^-22, y is within D = 2^-20 of itself.  An
+activation whose logarithm changes by S for a change of 1 in that of y is then
+within (1 + S) D of its exact value, and its own exponent, of a few roundings of 2^-24,
+half of that again; 2^-19 covers the approximate functions behind it.  What lies
+below 2^-118 (SiLU of -86.6) may be any such value."""
+
+import math
+
+import pytest
+import torch
+
+from _pkg import load
+
+pytestmark = pytest.mark.gpu
+rt = load("_b200_runtime") if torch.cuda.is_available() else None
+
+f64 = torch.float64
+E4M3 = torch.float8_e4m3fn
+HALF = [torch.float16, torch.bfloat16]
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+SPACES = [(40,), (1000, 1002)]     # one launch, two
+
+
+def alternating(space, C, dtype):
+    x = torch.ones(1, math.prod(space), C, device="cuda", dtype=dtype)
+    x[:, 1::2] = -1
+    return x.view(1, *space, C)
+
+
+def exact(y, act):
+    """Value, and how much its logarithm changes with that of y (for y < 0)."""
+    u = math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3)
+    if act == 1:
+        return y * torch.sigmoid(y), y.abs()
+    if act == 2:
+        return y * 0.5 * torch.special.erfc(-y * math.sqrt(0.5)), y * y
+    return y * torch.sigmoid(2 * u), 2 * math.sqrt(2 / math.pi) * (y.abs() + 3 * 0.044715 * y.abs() ** 3)
+
+
+def check_tails(act, space, dtype):
+    far = [1e15, 1e20, 1e30, 3e38] if dtype == torch.bfloat16 else [100.0, 3e4, 6e4]
+    weight = torch.cat([torch.linspace(0.01, 14, 205), torch.linspace(14, 110, 97), torch.tensor(far + [1e4] * (18 - len(far)))]).cuda()
+    x = alternating(space, 320, dtype)
+    got = rt.group_norm(x, 1, weight, activation=act)
+    assert torch.equal(got.view(-1, 320)[2:], got.view(-1, 320)[:-2])
+    got = got.view(-1, 320)[:2].double()
+    y = torch.stack([weight, -weight]).to(f64) / math.sqrt(1 + 1e-5)
+    want, slope = exact(y, act)
+    slope = torch.where(y < 0, slope, torch.full_like(y, 0.2)).clamp(max=1e6)
+    off = want.abs() * (1.5 * (1 + slope) * 2.0 ** -20 + 2.0 ** -19) + 2.0 ** -118
+    tol = U[dtype] * (want.abs() + off) + off + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert torch.isfinite(got).all()
+    over = (got - want).abs() - tol
+    assert over.max().item() <= 0, f"y = {y.flatten()[over.argmax()]}: {got.flatten()[over.argmax()]}, not {want.flatten()[over.argmax()]}"
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("space", SPACES)
+@pytest.mark.parametrize("act", [1, 3])
+def test_activation_of_very_negative_values(act, space, dtype):
+    check_tails(act, space, dtype)
+
+
+@pytest.mark.parametrize("space", SPACES)
+@pytest.mark.parametrize("act", [1, 2, 3])
+def test_quantized_activation_of_very_negative_values(act, space):
+    """Nothing is left of a block far below 0: its scale is the least one."""
+    x = alternating(space, 384, torch.bfloat16)
+    weight = torch.full((384,), 1e20, device="cuda")
+    weight[128:256] = 50
+    q, s = rt.fused_groupnorm_quantize(x, 1, weight, activation=act)
+    q, s = q.view(-1, 384), s.view(-1, 3)
+    least = torch.tensor(1e-8, dtype=torch.float32) / torch.tensor(448.0)
+    assert (s[1::2] == least.item()).all() and (q[1::2].float() == 0).all()
+    want = weight[::128].double() / math.sqrt(1 + 1e-5) / 448
+    assert ((s[::2].double() - want).abs() <= 2.0 ** -18 * want).all() and (q[::2].float() == 448).all()
