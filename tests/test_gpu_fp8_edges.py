@@ -66,6 +66,13 @@ def test_activation_of_very_negative_values(act, space, dtype):
     check_tails(act, space, dtype)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("space", SPACES)
+def test_gelu_of_negative_values(space, dtype):
+    """Relative to the value, also where 1 + erf has no digits left."""
+    check_tails(2, space, dtype)
+
+
 @pytest.mark.parametrize("space", SPACES)
 @pytest.mark.parametrize("act", [1, 2, 3])
 def test_quantized_activation_of_very_negative_values(act, space):
