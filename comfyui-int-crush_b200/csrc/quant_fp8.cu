@@ -27,10 +27,11 @@ __device__ __forceinline__ F8Scale f8_scale(float amax) {
 // reciprocal, corrected by its remainder (Markstein, "Computation of elementary
 // functions on the IBM RISC System/6000 processor", 1990): 3 instructions where
 // the division takes about ten.  Where the remainder is below the subnormals
-// the quotient is far below e4m3's least value.
+// the quotient is far below e4m3's least value.  (The remainder is taken
+// negative: so the quotient of -0 is -0.)
 __device__ __forceinline__ float f8_quotient(float x, const F8Scale& f) {
   const float q = x * f.inv;
-  return fmaf(fmaf(-q, f.s, x), f.inv, q);
+  return fmaf(-fmaf(q, f.s, -x), f.inv, q);
 }
 // two values to e4m3, ties to even, the first in the low byte
 __device__ __forceinline__ uint32_t f8_pair(float lo, float hi) {

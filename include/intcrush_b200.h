@@ -438,7 +438,8 @@ int ic_gemm_fp8_block(const void* x, const void* w, const float* s_a, const floa
  *   activation   0 none, 1 SiLU, 2 GELU (erf), 3 GELU (tanh)
  *   y     [B, L, C] in dtype (may be x itself), or NULL for
  *   q, s  the result as e4m3 rows [B * L, ldq] with scales for blocks of 128
- *         channels, from the fp32 values (layout: ic_quantize_fp8_block)
+ *         channels, from the fp32 values (layout: ic_quantize_fp8_block); y = -0
+ *         is stored as +0
  *   workspace  ic_group_norm_workspace(...) floats (`floats` is what there is),
  *         16-byte aligned, contents arbitrary, in use until the call's work has run
  * C up to 8192.  Any alignment works; 16-byte aligned rows (C and strides

@@ -86,3 +86,34 @@ def test_quantized_activation_of_very_negative_values(act, space):
     assert (s[1::2] == least.item()).all() and (q[1::2].float() == 0).all()
     want = weight[::128].double() / math.sqrt(1 + 1e-5) / 448
     assert ((s[::2].double() - want).abs() <= 2.0 ** -18 * want).all() and (q[::2].float() == 448).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_quantize_every_quotient_to_its_byte(dtype):
+    """Values of both signs down to a quarter of the border between 0 and the least
+    e4m3 value (2^-10 scales), zeros of both signs, over the scales of every
+    significand that a block's largest value can have: the bytes of e4m3(x / s)."""
+    every = torch.arange(2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype).cuda()
+    every = every[torch.isfinite(every)]
+    tops = every[(every >= 1) & (every < 2)]
+    small = every[(every < 2) & (every > 2.0 ** -21)]
+    small = torch.cat([small, -small, small.new_tensor([0.0, -0.0])])
+    small = torch.cat([small, small.new_full((-len(small) % 127,), -0.0)]).view(-1, 127)
+    for top in tops.split(32):
+        t = top[:, None, None]
+        x = torch.cat([torch.maximum(torch.minimum(small[None].expand(len(top), -1, -1), t), -t), t.expand(-1, small.shape[0], 1)], -1)
+        x = x.reshape(-1, 128)
+        q, s = rt.quantize_fp8_block(x)
+        want_s = x.float().amax(1, keepdim=True) / torch.full((len(x), 1), 448.0, device="cuda")
+        assert torch.equal(s, want_s)
+        assert torch.equal(q.view(torch.uint8), (x.float() / want_s).to(E4M3).view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize_keeps_a_zeros_sign(rows, dtype):
+    x = torch.randn(128, 300, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    x[:, ::3] = -0.0
+    x[:, 1::3] = 0.0
+    q, _ = rt.quantize_fp8_block(x, rows=rows)
+    assert (q[:, ::3].view(torch.uint8) == 0x80).all() and (q[:, 1::3].view(torch.uint8) == 0).all()
