@@ -31,6 +31,8 @@ from . import _quant_utils as _qu
 
 __all__ = ["ConvLinear4bit", "ConvLinear8bit", "ConvLinearFP8"]
 
+_INTEGERS = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}   # by size
+
 
 def _rotated_weight(linear: nn.Linear, rot_need: bool, rot_size: int, perm: torch.Tensor | None) -> torch.Tensor:
     """The float32 weight in the rotated (and permuted) input basis the
@@ -149,10 +151,17 @@ class ConvLinearFP8(_QuantLinearBase):
 
     def _apply(self, fn, recurse=True):
         # a cast of the model's floating point tensors is not one of e4m3 values
-        # or of their scales
-        weight, scale = self.weight, self.scale
-        super()._apply(fn, recurse)
-        self.weight, self.scale = weight.to(self.weight.device), scale.to(self.scale.device)
+        # or of their scales: they go through it as integers
+        kept = {name: self._buffers[name] for name in ("weight", "scale")}
+        for name, t in kept.items():
+            self._buffers[name] = t.view(_INTEGERS[t.element_size()])
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            for name, t in kept.items():
+                now = self._buffers[name]
+                # (`type` casts integers too: then only the device is taken over)
+                self._buffers[name] = now.view(t.dtype) if now.dtype is _INTEGERS[t.element_size()] else t.to(now.device)
         return self
 
     def forward(self, x):
