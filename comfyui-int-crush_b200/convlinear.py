@@ -139,15 +139,32 @@ class ConvLinearFP8(_QuantLinearBase):
     """W8A8 linear in e4m3: weights with a scale for each 128 x 128 block,
     activations quantised 1 x 128 in ``forward``; optional rotation.  B200
     kernels only (CUDA fp16 / bf16 activations).  ``weight`` [N, K] is kept with
-    its rows filled up to a multiple of 16 bytes, as the kernel reads them."""
+    its rows filled up to a multiple of 16 bytes, as the kernel reads them; a
+    state dict holds [N, K], and one with filled rows loads too."""
 
     def __init__(self, weight, scale, rot_need=False, bias=None, rot_size=256, in_features=None):
         K = weight.shape[-1] if in_features is None else in_features
         if weight.shape[-1] % 16:
-            rows = torch.zeros(weight.shape[0], -(-K // 16) * 16, dtype=torch.uint8, device=weight.device)
-            rows[:, :K] = weight[:, :K].contiguous().view(torch.uint8)
-            weight = rows.view(weight.dtype)
+            weight = self._filled(weight, K, -(-K // 16) * 16)
         super().__init__(weight, scale, rot_need, bias, rot_size, in_features=K)
+
+    @staticmethod
+    def _filled(weight, K, width):
+        """The K columns of ``weight`` in rows of ``width``, zeros behind them."""
+        rows = torch.zeros(weight.shape[0], width, dtype=torch.uint8, device=weight.device)
+        rows[:, :K] = weight[:, :K].contiguous().view(torch.uint8)
+        return rows.view(weight.dtype)
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self.weight.shape[1] != self.in_features:
+            destination[prefix + "weight"] = destination[prefix + "weight"][:, :self.in_features].contiguous()
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        w = state_dict.get(prefix + "weight")
+        if w is not None and w.shape == (self.out_features, self.in_features) != self.weight.shape:
+            state_dict = {**state_dict, prefix + "weight": self._filled(w.to(self.weight.dtype), self.in_features, self.weight.shape[1])}
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
     def _apply(self, fn, recurse=True):
         # a cast of the model's floating point tensors is not one of e4m3 values

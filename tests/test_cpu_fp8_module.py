@@ -64,3 +64,30 @@ def test_a_failing_move_leaves_the_module_as_it_was():
     with pytest.raises(RuntimeError, match="no memory"):
         m._apply(fail)
     assert m.weight.dtype is E4M3 and same(m, want)
+
+
+@pytest.mark.parametrize("assign", [False, True])
+@pytest.mark.parametrize("K", [1, 256, 300])
+def test_state_dict_holds_the_weight_as_checkpoints_do(K, assign):
+    m = module(K)
+    state = {k: v.clone() for k, v in torch.nn.Sequential(m).state_dict().items()}
+    assert state["0.weight"].shape == (200, K) and state["0.weight"].dtype is E4M3 and state["0.weight"].is_contiguous()
+    before = dict(state)
+    for deferred in (False, True):
+        other = conv.ConvLinearFP8.from_float(torch.nn.Linear(K, 200))
+        holder = torch.nn.Sequential(other.to("meta") if deferred and assign else other)
+        assert not any(holder.load_state_dict(state, assign=assign))
+        assert holder[0].weight.stride() == (-(-K // 16) * 16, 1) and same(holder[0], m)
+    assert all(state[k] is before[k] for k in state)
+    filled = dict(state)                       # as the module holds it
+    filled["0.weight"] = m.weight
+    other = conv.ConvLinearFP8.from_float(torch.nn.Linear(K, 200))
+    torch.nn.Sequential(other).load_state_dict(filled, assign=assign)
+    assert same(other, m)
+
+
+def test_a_weight_of_another_shape_does_not_load():
+    for shape in [(200, 299), (199, 300), (200, 300, 1)]:
+        state = {**module(300).state_dict(), "weight": torch.zeros(shape, dtype=torch.uint8).view(E4M3)}
+        with pytest.raises(RuntimeError, match="size mismatch"):
+            module(300).load_state_dict(state)
