@@ -1278,6 +1278,23 @@ def _rows_of(shape, stride):
     return None if L > 1 and row < C else (L, stride[0], row)
 
 
+def _overlap(n: int, far: int, m: int, near: int, width: int) -> bool:
+    """Whether two of n x m runs of ``width`` elements, ``far`` and ``near`` apart,
+    share one."""
+    if n == 1 or m == 1:
+        return (n > 1 and far < width) or (m > 1 and near < width)
+    if near > far:
+        n, far, m, near = m, near, n, far
+    if near < width:
+        return True
+    last = (m - 1) * near
+    for j in range(1, min(n, (last + width - 1) // far + 1)):
+        i, r = divmod(j * far, near)     # the runs before and behind the j-th of the others
+        if (i < m and r < width) or (i + 1 < m and near - r < width):
+            return True
+    return False
+
+
 @functools.lru_cache(maxsize=4096)
 def _norm_form(what, index, x, groups, weight, bias, activation, out, quantize):
     """x, weight, bias and out as (dtype, shape, stride) or None: what to copy first
@@ -1313,7 +1330,7 @@ def _norm_form(what, index, x, groups, weight, bias, activation, out, quantize):
     y_batch, y_row = T * C, C
     if out is not None:
         rows = _rows_of(shape, out[2])
-        if rows is None or (B > 1 and rows[1] < C):
+        if rows is None or _overlap(B, rows[1], T, rows[2], C):
             raise ValueError(f"{what}: out must be channels last with rows that do not overlap, got strides {out[2]}")
         _, y_batch, y_row = rows
     n = _workspace("ic_group_norm_workspace", index, B, T, C, groups, int(quantize))
@@ -1367,7 +1384,8 @@ def group_norm(
     ``x.permute(0, 2, 3, 1)``, without a copy.  ``weight`` and ``bias`` [C] are
     fp16, bf16 or fp32 (None: ones, zeros), ``activation`` 0 none, 1 SiLU, 2 GELU
     (erf), 3 GELU (tanh) as in :func:`gemm_a8`.  Returns a contiguous tensor;
-    ``out`` may be ``x`` itself.  Up to 8192 channels.
+    ``out`` may be ``x`` itself, but overlap it in no other way.  Up to 8192
+    channels.
     """
     return _group_norm("group_norm", x, groups, weight, bias, eps, activation, out, False)
 

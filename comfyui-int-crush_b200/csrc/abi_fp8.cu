@@ -3,6 +3,8 @@
 // caller's stream and returns a status code; no exception crosses the ABI.
 #include <string.h>
 
+#include <utility>
+
 namespace ic {
 
 cudaError_t fp8_device_error(int* word, bool store) {
@@ -96,6 +98,22 @@ static int gn_sizes(const char* me, int64_t B, int64_t L, int64_t C, int64_t gro
   return IC_OK;
 }
 
+// Whether two of n x m runs of `width` elements, `far` and `near` apart, share one.
+static bool gn_overlap(int64_t n, int64_t far, int64_t m, int64_t near, int64_t width) {
+  if (n == 1 || m == 1) return (n > 1 && far < width) || (m > 1 && near < width);
+  if (near > far) {
+    std::swap(n, m);
+    std::swap(far, near);
+  }
+  if (near < width) return true;
+  const __int128 last = (__int128)(m - 1) * near;   // (any strides are let in here)
+  for (int64_t j = 1; j < n && (__int128)j * far < last + width; ++j) {
+    const __int128 at = (__int128)j * far, i = at / near, r = at - i * near;
+    if ((i < m && r < width) || (i + 1 < m && near - r < width)) return true;
+  }
+  return false;
+}
+
 int64_t ic_group_norm_workspace(int64_t B, int64_t L, int64_t C, int64_t groups, int quantize) {
   if (gn_sizes("ic_group_norm_workspace", B, L, C, groups) != IC_OK) return -1;
   return B && L ? ic::gn_plan(B, L, C, groups, quantize != 0).floats : 0;
@@ -135,6 +153,7 @@ int ic_group_norm(const void* x, const void* gamma, const void* beta, float eps,
   if (p.floats && (!workspace || !f8_at16(workspace) || workspace_elems < p.floats))
     return set_error(IC_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld floats, got %lld", me, (long long)p.floats,
                      (long long)workspace_elems);
+  if (y && gn_overlap(B, y_batch, L, y_row, C)) return set_error(IC_ERR_ARG, "%s: y overlaps itself", me);
   GnArgs a;
   memset(&a, 0, sizeof(a));
   a.x = x; a.L = L; a.C = (int)C; a.G = (int)groups; a.Cg = (int)(C / groups);

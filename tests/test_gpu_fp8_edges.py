@@ -117,3 +117,16 @@ def test_quantize_keeps_a_zeros_sign(rows, dtype):
     x[:, 1::3] = 0.0
     q, _ = rt.quantize_fp8_block(x, rows=rows)
     assert (q[:, ::3].view(torch.uint8) == 0x80).all() and (q[:, 1::3].view(torch.uint8) == 0).all()
+
+
+@pytest.mark.parametrize("space", [7, 80000])
+@pytest.mark.parametrize("layout", ["samples_between_rows", "rows_of_others_between"])
+def test_group_norm_into_rows_that_interleave(layout, space):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(2, space, 64, device="cuda", generator=g).half()
+    buf = torch.full((space * 128 + 512,), -7.0, dtype=torch.float16, device="cuda")
+    strides = (64, 128, 1) if layout == "samples_between_rows" else (192, 128, 1)
+    out = buf.as_strided((2, space, 64), strides)
+    y = rt.group_norm(x, 4, activation=1)
+    assert rt.group_norm(x, 4, activation=1, out=out) is out and torch.equal(out, y)
+    assert (buf == -7).sum() == len(buf) - y.numel()
