@@ -16,11 +16,11 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libintcrush_b200.so")
 # translation unit -> the sources it includes
 UNITS = {
-    "intcrush_b200.cu": ["ic_common.cuh", "prep_common.cuh", "prep.cu", "prep_tile.cu", "gemm_tc.cu", "skinny.cu",
-                         "weights.cu", "abi.cu"],
-    "attention_b200.cu": ["ic_common.cuh", "qk_norm_rope.cu", "lora_batched.cu", "lora_stream.cu", "lora_feed.h",
+    "intcrush_b200.cu": ["ic_common.cuh", "register_split.h", "prep_common.cuh", "prep.cu", "prep_tile.cu", "gemm_tc.cu",
+                         "skinny.cu", "weights.cu", "abi.cu"],
+    "attention_b200.cu": ["ic_common.cuh", "register_split.h", "qk_norm_rope.cu", "lora_batched.cu", "lora_stream.cu", "lora_feed.h",
                           "cross_attention.cuh", "cross_attention.cu", "cross_attention_tc.cu", "abi_attention.cu"],
-    "fp8_b200.cu": ["ic_common.cuh", "quant_fp8.cu", "gemm_fp8.cu", "group_norm.cu", "abi_fp8.cu"],
+    "fp8_b200.cu": ["ic_common.cuh", "register_split.h", "quant_fp8.cu", "gemm_fp8.cu", "group_norm.cu", "abi_fp8.cu"],
 }
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
          "-diag-suppress", "20044"]

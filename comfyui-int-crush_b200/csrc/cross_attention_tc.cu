@@ -51,6 +51,8 @@ struct XtCfg {
   static constexpr int OFF_BAR = OFF_ML + 2048;
   static constexpr int SMEM = OFF_BAR + 512;
   static constexpr int THREADS = 512;
+  // 512 x 128 registers; the many where a thread holds a row of S
+  static constexpr RegisterSplit REGS = {256, 72, 256, 184};
 };
 
 // n / d for 0 <= n < 2^30 by a multiplication: m = ceil(2^(30 + l) / d) with
@@ -278,10 +280,8 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     return false;
   };
 
-  // registers: 512 threads x 128 = 256 x 72 here + 256 x 184 below, where a
-  // thread holds a row of S
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XtCfg<DP>::REGS.few));
     if (warp == 8) {
       // ------------------------------------------------------------ producer
       if (lane == 0) {
@@ -569,7 +569,7 @@ xattn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XtCfg<DP>::REGS.many));
     // ------------------------------------------------------------- softmax
     const int s = warp >> 2, w = warp & 3;
     const uint32_t lane_base = (uint32_t)(w * 32) << 16;
@@ -748,7 +748,9 @@ static bool xt_map(CUtensorMap* m, bool bf, const void* p, const int64_t* st, in
 template <typename T, int DP, bool BIAS>
 static cudaError_t launch_xt(const CUtensorMap (&m)[3], const XtArgs& a, cudaStream_t st) {
   auto kern = xattn_tc_kernel<T, DP, BIAS>;
-  const cudaError_t e = set_smem_once(kern, XtCfg<DP>::SMEM);
+  static std::atomic<unsigned long long> devices{0};
+  cudaError_t e = set_smem_once(kern, XtCfg<DP>::SMEM);
+  if (e == cudaSuccess) e = split_fits_once(kern, XtCfg<DP>::REGS, devices);
   if (e != cudaSuccess) return e;
   const int grid = a.items < num_sms() ? a.items : num_sms();
   kern<<<grid, XtCfg<DP>::THREADS, XtCfg<DP>::SMEM, st>>>(m[0], m[1], m[2], a);

@@ -51,6 +51,8 @@ struct F8Cfg {
   static constexpr int OFF_BAR = OFF_STG + (PARTS > 8 * 4096 ? PARTS : 8 * 4096);
   static constexpr int SMEM = OFF_BAR + 256;
   static constexpr int THREADS = 384;
+  // with 128 columns a thread: 384 x 168 registers
+  static constexpr RegisterSplit REGS = {128, 40, 256, 232};
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -236,9 +238,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const int m_off = PAIR ? (int)rank * 128 : 0;
   const uint32_t ring = smem_u32(smem);
 
-  // registers with 128 columns a thread: 384 threads x 168 = 128 x 40 + 256 x 232
   if (warp < 4) {
-    if constexpr (CPT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if constexpr (CPT == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS.few));
     if (warp == 0) {
       // ------------------------------------------------------------ producer
       if (lane == 0) {
@@ -324,7 +325,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
   } else {
     // ------------------------------------------------------------------ sums
-    if constexpr (CPT == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if constexpr (CPT == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS.many));
     const int e = warp - 4, q = e & 3, half = e >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * CPT);
     uint8_t* stg = smem + C::OFF_STG + e * 4096;
@@ -591,6 +592,10 @@ static cudaError_t f8_launch(const F8Operands& o, F8Args a, int splits, cudaStre
     return cudaErrorInvalidValue;
   auto kern = gemm_fp8_kernel<C>;
   cudaError_t e = set_smem_once(kern, C::SMEM);
+  if constexpr (C::CPT == 128) {
+    static std::atomic<unsigned long long> devices{0};
+    if (e == cudaSuccess) e = split_fits_once(kern, C::REGS, devices);
+  }
   if (e != cudaSuccess) return e;
   const long long tiles = (long long)a.m_tiles * a.n_tiles;
   const int cluster = C::PAIR ? 2 : splits;

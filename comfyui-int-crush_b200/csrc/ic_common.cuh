@@ -15,9 +15,11 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "../../include/intcrush_b200.h"
+#include "register_split.h"
 
 #ifndef IC_WAIT_NS
 #define IC_WAIT_NS 2000000000ull   // 2 s per wait, far above any legitimate wait
@@ -73,6 +75,21 @@ inline cudaError_t set_smem_once(const void* kern, int bytes, int carveout = -1)
 template <typename K>
 inline cudaError_t set_smem_once(K* kern, int bytes, int carveout = -1) {
   return set_smem_once(reinterpret_cast<const void*>(kern), bytes, carveout);
+}
+
+// Whether a kernel has the registers that its warps share out: asked once a device,
+// the answer kept in `devices`, which is this kernel's alone.
+template <typename K>
+inline cudaError_t split_fits_once(K* kern, const RegisterSplit& split, std::atomic<unsigned long long>& devices) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (devices.load() >> (dev & 63) & 1) return cudaSuccess;
+  cudaFuncAttributes attr;
+  const cudaError_t e = cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(kern));
+  if (e != cudaSuccess) return e;
+  if (!split.fits(attr.numRegs)) return cudaErrorLaunchOutOfResources;
+  devices.fetch_or(1ull << (dev & 63));
+  return cudaSuccess;
 }
 
 __device__ __forceinline__ uint64_t globaltimer() {
