@@ -527,6 +527,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_stats_kernel(const GnArgs g)
     }
     if (lane == 0) own[i] = make_float2(mean, dev);
   }
+  __syncwarp();
   if (g.cluster > 1) cluster_sync_all();
   else __syncthreads();
   // the cluster's CTAs, a lane each
@@ -567,7 +568,10 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_stats_kernel(const GnArgs g)
       }
     }
   }
-  if (g.cluster > 1) cluster_sync_all();   // nobody leaves while another CTA may read its shared memory
+  // nobody leaves while another CTA may read its shared memory (threads without a
+  // row come here before the others of their warp)
+  __syncwarp();
+  if (g.cluster > 1) cluster_sync_all();
 }
 
 // The norm from the workspace's statistics, tile by tile from the last row on.  A

@@ -193,8 +193,10 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t smem_addr, uint32_t rank) 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
-// Cluster-wide barrier; only used at kernel start, right after the barrier
-// initialisation, where both CTAs of a pair are resident by construction.
+// Cluster-wide barrier (release and acquire): at a kernel's start, behind the
+// initialisation of its mbarriers; between writes to another CTA's shared memory and
+// their reads; before a CTA leaves whose shared memory others read.  Every thread of
+// the cluster comes here once, those of a warp together (.aligned).
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
