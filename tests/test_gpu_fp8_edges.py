@@ -14,6 +14,7 @@ import math
 import pytest
 import torch
 
+import test_gpu_fp8_ops as ops
 from _pkg import load
 
 pytestmark = pytest.mark.gpu
@@ -130,3 +131,41 @@ def test_group_norm_into_rows_that_interleave(layout, space):
     y = rt.group_norm(x, 4, activation=1)
     assert rt.group_norm(x, 4, activation=1, out=out) is out and torch.equal(out, y)
     assert (buf == -7).sum() == len(buf) - y.numel()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("act", [2, 3])
+@pytest.mark.parametrize("B,space,C,groups", ops.SIZES)
+def test_group_norm_quantized_behind_gelu(B, space, C, groups, act, dtype):
+    g = ops.gen(C + act + 2)
+    x = ops.normal(g, B, *space, C, dtype=dtype, std=1.5)
+    weight, bias = ops.normal(g, C), ops.normal(g, C, dtype=dtype)
+    q, s = rt.fused_groupnorm_quantize(x, groups, weight, bias, eps=1e-6, activation=act)
+    ops.check_norm_quantized(q, s, x, groups, weight, bias, 1e-6, act)
+    again = rt.fused_groupnorm_quantize(x, groups, weight, bias, eps=1e-6, activation=act)
+    assert torch.equal(q.view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(s, again[1])
+
+
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("space", [50, 100000])
+def test_quantized_norm_of_what_is_not_finite(space, act):
+    """A NaN makes the scales and values of its blocks NaN; an infinity its block's
+    scale infinite, its own value NaN and the others 0.  Other blocks and samples
+    keep their bits."""
+    x = ops.normal(ops.gen(3), 3, space, 256, dtype=torch.float16)
+    beta = torch.zeros(256, device="cuda")
+    q0, s0 = rt.fused_groupnorm_quantize(x, 8, None, beta, activation=act)
+    assert torch.isfinite(s0).all() and torch.isfinite(q0.float()).all()
+
+    x[0, space // 3, 40] = math.nan            # group 1 of sample 0: its channels lie in block 0
+    q, s = rt.fused_groupnorm_quantize(x, 8, None, beta, activation=act)
+    assert s[0, :, 0].isnan().all() and q[0, :, :128].float().isnan().all()
+    assert torch.equal(s[0, :, 1], s0[0, :, 1]) and torch.equal(q[0, :, 128:].float(), q0[0, :, 128:].float())
+    assert torch.equal(s[1:], s0[1:]) and torch.equal(q[1:].float(), q0[1:].float())
+
+    beta[200] = math.inf                       # a channel of block 1, in every sample
+    q, s = rt.fused_groupnorm_quantize(x, 8, None, beta, activation=act)
+    assert (s[..., 1] == math.inf).all() and q[..., 200].float().isnan().all()
+    others = torch.cat([q[..., 128:200], q[..., 201:]], -1).float()
+    assert (others == 0).all()
+    assert torch.equal(s[1:, :, 0], s0[1:, :, 0]) and torch.equal(q[1:, :, :128].float(), q0[1:, :, :128].float())
