@@ -483,8 +483,11 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_stats_kernel(const GnArgs g)
         gn_untwo(x0[i], z[0], z[1]);
 #pragma unroll
         for (int j = 2 * i; j < 2 * i + 2; ++j) {
-          q[j] = fmaxf(0.f, q[j] - s[j] * s[j] * inv);
-          s[j] = fmaf(s[j], inv, -z[j & 1]);
+          // (squares beyond fp32's range: infinite, and not NaN, of which the maximum
+          // would make 0)
+          const float d = s[j] * inv;
+          q[j] = q[j] <= 3.4028235e38f ? fmaxf(0.f, fmaf(-s[j], d, q[j])) : q[j];
+          s[j] = d - z[j & 1];
         }
       }
       // channels of one group, two by two

@@ -432,7 +432,8 @@ int ic_gemm_fp8_block(const void* x, const void* w, const float* s_a, const floa
 /* Group norm with an activation, channels last:
  *   y = act((x - mean) / sqrt(var + eps) * gamma + beta)
  * over the L rows and C / groups channels of each group of each sample (var
- * biased), in fp32.
+ * biased), in fp32; where the sum of a group's squared differences is beyond its
+ * range, the variance counts as infinite.
  *   x     [B, L, C] of `dtype` (f16 / bf16), sample stride x_batch, row stride x_row
  *   gamma, beta  [C] f16 / bf16 / f32 or NULL (ones, zeros)
  *   activation   0 none, 1 SiLU, 2 GELU (erf), 3 GELU (tanh)

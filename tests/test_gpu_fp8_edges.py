@@ -169,3 +169,20 @@ def test_quantized_norm_of_what_is_not_finite(space, act):
     others = torch.cat([q[..., 128:200], q[..., 201:]], -1).float()
     assert (others == 0).all()
     assert torch.equal(s[1:, :, 0], s0[1:, :, 0]) and torch.equal(q[1:, :, :128].float(), q0[1:, :, :128].float())
+
+
+@pytest.mark.parametrize("C,groups", [(56, 7), (64, 4)])
+@pytest.mark.parametrize("rows", [2, 146, 2 * 73 * 16, 73 * 5 * 32, 73 * 16 * 296])
+def test_group_norm_of_squares_beyond_the_range(rows, C, groups):
+    """The variance is infinite, so that all that is left is the bias; not 0, which
+    would make large numbers of the values."""
+    x = alternating((rows,), C, torch.bfloat16) * 2e19
+    bias = torch.arange(C, device="cuda", dtype=torch.float32)
+    y = rt.group_norm(x, groups, None, bias)
+    assert (y == bias.bfloat16()).all()
+    # and about its end: the sum over a group is rows * C / groups * 2^110, which 32 bits
+    # hold below 2^128; eps is nothing beside it
+    x = alternating((rows,), C, torch.bfloat16) * 2.0 ** 55
+    y = rt.group_norm(x, groups)
+    inside = rows * C // groups < 2 ** 18
+    assert (y.double() - inside * alternating((rows,), C, f64)).abs().max() <= 2.0 ** -8
