@@ -1381,7 +1381,7 @@ def group_norm(
 
     ``x`` [B, ..., C] (fp16 / bf16) has its channels last, e.g. [B, H, W, C] or
     [B, L, C]; a [B, C, H, W] tensor in ``torch.channels_last`` format comes as
-    ``x.permute(0, 2, 3, 1)``, without a copy.  ``weight`` and ``bias`` [C] are
+    ``x.permute(0, 2, 3, 1)``, without a copy; one with channels first is copied.  ``weight`` and ``bias`` [C] are
     fp16, bf16 or fp32 (None: ones, zeros), ``activation`` 0 none, 1 SiLU, 2 GELU
     (erf), 3 GELU (tanh) as in :func:`gemm_a8`.  Returns a contiguous tensor;
     ``out`` may be ``x`` itself, but overlap it in no other way.  Up to 8192

@@ -652,8 +652,9 @@ static long long f8_clusters(int splits) {
 // to 1900 MHz): a block of 128 along K takes 560 in a pair's 256 x 256, 375 in its
 // 256 x 128, 400 in one CTA's 128 x 128; a tile's output 1000 to 1500; a cluster's
 // exchange 2500.  Tiles beyond whole rounds wait for a round of their own.
-// (4608 x 12288 -> 4096: 240, 298 and 316 us; 768 x 2048 -> 8192: 23.3, 21.7 and 22.0;
-// 256 x 8192 -> 4096: 32.7, 29.9 and 28.6, in clusters of two 20.9.)
+// (4608 x 12288 -> 4096: 240, 298 and 316 us; 256 x 8192 -> 4096: 32.7, 29.9 and 28.6, in
+// clusters of two 20.9.  The first is a tenth too cheap here: of 768 x 2048 -> 8192, in
+// 23.3, 21.7 and 22.0, it is taken, by 20.9 against 21.0.)
 cudaError_t launch_gemm_fp8(const F8Operands& o, const F8Args& a, cudaStream_t st) {
   const long long sms = num_sms();
   const auto rounds = [](long long tiles, long long places) { return (double)((tiles + places - 1) / places); };

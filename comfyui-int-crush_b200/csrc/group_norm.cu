@@ -23,7 +23,7 @@
 // 2 x 256 x 1280 with SiLU: 6.9 us, most of it code that runs once.  1024 x 1024 x 128
 // with SiLU: 151 us, where 805 MB (x twice, y) at 6.55 TB/s are 123: the statistics
 // take 48 us on average and 60 with the CTAs that read from far memory, the norm 78,
-// at two thirds of the instruction slots and half of the special functions'.
+// at three quarters of the instruction slots and half of the special functions'.
 #include <atomic>
 #include <type_traits>
 
@@ -360,7 +360,7 @@ __device__ __forceinline__ void gn_finish(const GnArgs& g, const GnFactors& f, c
     gn_store(o.y, y, n, g.vec != 0);
   } else {
     // Scale and quotients as they are defined (quant_fp8.cu), the quotients from a
-    // reciprocal to a unit (300000 x 128 with SiLU: 66.4 us, 65.7 without their
+    // reciprocal to a unit (300000 x 128 with SiLU: 66.5 us, 65.7 without their
     // correction, 71.9 a value at a time).  A scale that is infinite has 0 for its
     // reciprocal, a NaN a NaN; both correct against 0, so that the block's finite
     // values become 0, or NaN.  (y = -0 becomes +0: its sign would cost 1%.)

@@ -414,7 +414,7 @@ int ic_quantize_fp8_block(const void* x, void* q, float* s, const ic_quantize_fp
 /* Product of two e4m3 matrices with scales for blocks of 128, on tcgen05
  * (kind::f8f6f4):
  *   out[m, n] = T(sum_b s_a[m, b] * s_w[n / 128, b] * sum_{k in b} x[m, k] * w[n, k] + bias[n])
- * with fp32 sums and one rounding.
+ * with fp32 sums and one rounding; s_a * s_w is a product in fp32.
  *   x, w  e4m3 [M, K] and [N, K], 16-byte aligned, row strides % 16 == 0 (bytes);
  *         what lies behind a row's K values does not matter
  *   s_a   fp32, of row m and block b at s_a[m * sa_row + b * sa_block]; s_w
