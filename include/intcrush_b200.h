@@ -436,7 +436,8 @@ int ic_gemm_fp8_block(const void* x, const void* w, const float* s_a, const floa
  * range, the variance counts as infinite.
  *   x     [B, L, C] of `dtype` (f16 / bf16), sample stride x_batch, row stride x_row
  *   gamma, beta  [C] f16 / bf16 / f32 or NULL (ones, zeros)
- *   activation   0 none, 1 SiLU, 2 GELU (erf), 3 GELU (tanh)
+ *   activation   0 none, 1 SiLU (to y: below -86.6, -infinity too, as of -86.6,
+ *         which is -2e-36), 2 GELU (erf), 3 GELU (tanh)
  *   y     [B, L, C] in dtype (may be x itself, but overlap it in no other way;
  *         rows that share elements are refused), or NULL for
  *   q, s  the result as e4m3 rows [B * L, ldq] with scales for blocks of 128
